@@ -17,7 +17,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from typing import Optional, Sequence, Tuple
+from typing import NamedTuple, Optional, Sequence, Tuple
 
 import torch
 
@@ -2404,6 +2404,181 @@ def map_difference(a: torch.Tensor, out: torch.Tensor, *, heads: int, lam: float
     code = _streams_lib().msgl_map_difference(_ptr(a), int(a.dtype == torch.float32), _ptr(out), o_stride, float(lam), float(eps), float(scale),
                                               T, heads, dv, _dt(out), _stream())
     _check(code, f"map_difference (value size {dv})")
+
+
+# ---------------------------------------------------------------------------------------
+# drafted tokens: the fields of a step that verifies them, the path that the model agrees with, log probabilities
+# (csrc/drafts.cu, csrc/logprobs.cu)
+# ---------------------------------------------------------------------------------------
+_drafts = None
+MAX_DRAFTS = 256                  # drafts of one request
+MAX_TOP = 32                      # alternatives of a token that `token_logprobs` gives
+_ACCEPT_CACHES = 128              # caches of one launch of draft_accept
+_ACCEPT_BLOCK_COLUMNS = 256       # 16-byte columns that a block of it moves at a time
+
+
+def _draft_lib():
+    global _drafts
+    if _drafts is None:
+        lib = _build.drafts_library()
+        lib.msgl_draft_plan.argtypes = [c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p] + [c_int] * 5 + [c_void_p] * 7
+        lib.msgl_draft_accept.argtypes = [c_void_p] * 4 + [c_int] * 3 + [c_void_p] * 5 + [c_int] * 3 + [c_ll, c_int, c_int, c_void_p, c_int, c_int, c_void_p]
+        lib.msgl_token_logprobs.argtypes = [c_void_p, c_int, c_int, c_ll, c_void_p, c_int] + [c_void_p] * 4 + [c_int, c_int, c_void_p]
+        _drafts = lib
+    return _drafts
+
+
+def _same_device(what: str, *tensors: Optional[torch.Tensor]) -> None:
+    """All tensors on the current CUDA device, whose stream the launch goes to."""
+    _need_cuda(*tensors)
+    dev = torch._C._cuda_getDevice()
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            raise KernelError(f"{what}: a tensor on {t.device} and the current device is cuda:{dev}")
+
+
+def _index(what: str, name: str, t: torch.Tensor, numel: Optional[int] = None) -> None:
+    if t.dtype != torch.int32 or not t.is_contiguous() or (numel is not None and t.numel() != numel):
+        raise KernelError(f"{what}: {name} is a contiguous int32 tensor" + (f" of {numel} elements" if numel is not None else "") +
+                          f"; got {t.dtype} {tuple(t.shape)}")
+
+
+def _table(what: str, t: torch.Tensor, B: int) -> None:
+    if t.dtype != torch.int32 or t.dim() != 2 or t.shape[0] != B or t.shape[1] < 1 or t.stride(1) != 1:
+        raise KernelError(f"{what}: block_table is int32 [requests, pages] with adjacent columns; got {t.dtype} {tuple(t.shape)}")
+
+
+def _draft_limit(what: str, max_draft: int) -> None:
+    if not 1 <= max_draft <= MAX_DRAFTS:
+        raise KernelError(f"{what}: max_draft {max_draft} is outside [1, {MAX_DRAFTS}]")
+
+
+class DraftPlan(NamedTuple):
+    """The fields of a step whose requests bring drafted tokens; views into one buffer."""
+    q_start: torch.Tensor         # [B + 1] first draft of every request in the step's stream of tokens
+    kv_len: torch.Tensor          # [B] tokens in the cache once the drafts are written
+    positions: torch.Tensor       # [T] cached tokens + the draft's depth in its tree
+    token_req: torch.Tensor       # [T] request of every draft
+    out_loc: torch.Tensor         # [T] cache slot (page * P + offset) of every draft
+    mask: torch.Tensor            # [T, ceil(max_draft / 32)] bit i of a row: the request's draft i is this draft or one of its ancestors
+
+
+def draft_plan(parents: torch.Tensor, draft_lens: torch.Tensor, cached: torch.Tensor, block_table: torch.Tensor, *, page_size: int,
+               max_draft: int) -> DraftPlan:
+    """The fields of a step that verifies drafted tokens, made on the device (all int32): request r brings draft_lens[r] drafts, packed
+    request after request in `parents` [T], behind cached[r] tokens whose pages stand in block_table [B, pages].  A draft's parent is the
+    index within the request of an earlier draft; anything else stands for none.  Draft i lies in the cache at place cached + i.
+    Lengths are taken within [0, max_draft] and drafts past the end of `parents` are cut; rows of `parents` behind the last draft become
+    padding: position 0 and slot 0 (the page for padding) with an empty mask.  A place beyond the block table gets slot 0 too."""
+    T, (B, width) = parents.numel(), block_table.shape
+    _index("draft_plan", "parents", parents)
+    _index("draft_plan", "draft_lens", draft_lens, B)
+    _index("draft_plan", "cached", cached, B)
+    _table("draft_plan", block_table, B)
+    _draft_limit("draft_plan", max_draft)
+    if page_size < 1:
+        raise KernelError(f"draft_plan: page_size {page_size}")
+    _same_device("draft_plan", parents, draft_lens, cached, block_table)
+    words = -(-max_draft // 32)
+    if B == 0:
+        buf = torch.zeros(1 + T * (3 + words), dtype=torch.int32, device=parents.device)
+    else:
+        buf = torch.empty(2 * B + 1 + T * (3 + words), dtype=torch.int32, device=parents.device)
+    q_start, kv_len, positions, token_req, out_loc, mask = buf.split((B + 1, B, T, T, T, T * words))
+    code = _draft_lib().msgl_draft_plan(parents.data_ptr(), T, draft_lens.data_ptr(), cached.data_ptr(), B, block_table.data_ptr(), block_table.stride(0), width,
+                                        page_size, max_draft, words, q_start.data_ptr(), kv_len.data_ptr(), positions.data_ptr(), token_req.data_ptr(),
+                                        out_loc.data_ptr(), mask.data_ptr(), _stream())
+    _check(code, "draft_plan")
+    return DraftPlan(q_start, kv_len, positions, token_req, out_loc, mask.view(T, words))
+
+
+class DraftPath(NamedTuple):
+    """What a step of drafted tokens came to; -1 behind a request's path."""
+    kept: torch.Tensor            # [B] drafts on the path, draft 0 among them (0: the request brought none)
+    path: torch.Tensor            # [B, max_draft] their indices within the request
+    tokens: torch.Tensor          # [B, max_draft] the model's token after each of them: the request's next `kept` tokens
+
+
+def draft_accept(tokens: torch.Tensor, parents: torch.Tensor, following: torch.Tensor, q_start: torch.Tensor, *, max_draft: int,
+                 kv_len: Optional[torch.Tensor] = None, block_table: Optional[torch.Tensor] = None, caches: Sequence[torch.Tensor] = ()) -> DraftPath:
+    """The path of drafts that the model agrees with, for every request (all int32): from draft 0, the newest accepted token, to its child
+    whose token is following[its parent] (the first of them), and so on.  tokens, parents and following [T] as in `draft_plan`; `following`
+    is the model's token after every draft, of `sample` say.  The keys and values of the path move to the places behind the cached
+    tokens in all `caches` ([pages, kv heads, page size, row size] of one page size, each handed over once), so that the request
+    holds kv_len - (its drafts) + kept tokens afterwards; no two requests may share the pages that their drafts lie in."""
+    T, B = tokens.numel(), q_start.numel() - 1
+    _index("draft_accept", "tokens", tokens)
+    _index("draft_accept", "parents", parents, T)
+    _index("draft_accept", "following", following, T)
+    _index("draft_accept", "q_start", q_start)
+    if B < 0:
+        raise KernelError("draft_accept: q_start has one element more than there are requests")
+    _draft_limit("draft_accept", max_draft)
+    groups = {}
+    if len(caches):
+        if kv_len is None or block_table is None:
+            raise KernelError("draft_accept: caches need kv_len and block_table")
+        _index("draft_accept", "kv_len", kv_len, B)
+        _table("draft_accept", block_table, B)
+        dev, page_size, seen = tokens.get_device(), caches[0].shape[2], set()
+        for c in caches:
+            if c.dim() != 4 or not c.is_contiguous() or c.get_device() != dev or c.shape[2] != page_size:
+                raise KernelError(f"draft_accept: a cache is a contiguous [pages, kv heads, page size, row size] on {tokens.device}, all of one page size; "
+                                  f"got {tuple(c.shape)} on {c.device}")
+            ptr = c.data_ptr()
+            if ptr in seen:                  # (keys and values in one array)
+                continue
+            seen.add(ptr)
+            groups.setdefault((c.shape, c.element_size()), []).append(ptr)
+    _same_device("draft_accept", tokens, parents, following, q_start, kv_len, block_table)
+    buf = torch.empty(B * (1 + 2 * max_draft), dtype=torch.int32, device=tokens.device)
+    kept, path, after = buf.split((B, B * max_draft, B * max_draft))
+    launches = [(shape, item, ptrs[i:i + _ACCEPT_CACHES]) for (shape, item), ptrs in groups.items() for i in range(0, len(ptrs), _ACCEPT_CACHES)]
+    out = (kept.data_ptr(), path.data_ptr(), after.data_ptr())
+    for shape, item, ptrs in launches or [((0, 1, 1, 1), 2, [])]:
+        row = shape[3] * item
+        # blocks of a request: enough to fill the SMs a few times over, no more than there are columns for
+        columns = len(ptrs) * shape[1] * -(-row // 16)
+        blocks = max(1, min(-(-columns // _ACCEPT_BLOCK_COLUMNS), -(-4 * sm_count(tokens.device) // max(B, 1))))
+        code = _draft_lib().msgl_draft_accept(tokens.data_ptr(), parents.data_ptr(), following.data_ptr(), q_start.data_ptr(), B, T, max_draft, *out,
+                                              _ptr(kv_len), _ptr(block_table), block_table.stride(0) if ptrs else 0, block_table.shape[1] if ptrs else 0, shape[2],
+                                              shape[0], shape[1], row, (c_void_p * len(ptrs))(*ptrs), len(ptrs), blocks, _stream())
+        _check(code, "draft_accept")
+        out = (None, None, None)
+    return DraftPath(kept, path.view(B, max_draft), after.view(B, max_draft))
+
+
+class TokenLogprobs(NamedTuple):
+    logprobs: torch.Tensor        # [N] log probability of the row's token
+    entropy: torch.Tensor         # [N] entropy of the row's distribution, in nats
+    top_logprobs: torch.Tensor    # [N, top] the highest log probabilities, falling
+    top_tokens: torch.Tensor      # [N, top] int32, their tokens; among equal ones the lower comes first
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> TokenLogprobs:
+    """Of softmax(logits) row by row, logits [N, V] float32 or bfloat16 with adjacent columns and rows any distance apart: the log
+    probability of tokens[n] (int32; outside the vocabulary: NaN), the entropy, and the `top` (0 to MAX_TOP) most probable tokens.
+    A row with a NaN, with +inf or without a number above -inf has NaN probabilities; a NaN logit is never among the top tokens (-1 where
+    fewer numbers are left)."""
+    if logits.dim() != 2 or logits.dtype not in _DT or logits.stride(1) != 1 and logits.shape[1] > 1:
+        raise KernelError(f"token_logprobs: logits are float32 or bfloat16 [rows, vocabulary] with adjacent columns; got {logits.dtype} {tuple(logits.shape)}")
+    N, V = logits.shape
+    _index("token_logprobs", "tokens", tokens, N)
+    if not 0 <= top <= min(MAX_TOP, V) or V < 1:
+        raise KernelError(f"token_logprobs: top {top} is outside [0, {min(MAX_TOP, V)}]")
+    _same_device("token_logprobs", logits, tokens)
+    buf = torch.empty(N * (2 + top), dtype=torch.float32, device=logits.device)
+    lp, entropy, best = buf.split((N, N, N * top))
+    ids = torch.empty((N, top), dtype=torch.int32, device=logits.device)
+    if N == 0:
+        return TokenLogprobs(lp, entropy, best.view(N, top), ids)
+    # blocks of a row: about four an SM over all rows, and none with fewer than 2,048 logits
+    want = min(4 * sm_count(logits.device) // N, V // 2048, 8)
+    blocks = 8 if want >= 8 else 4 if want >= 4 else 2 if want >= 2 else 1
+    code = _draft_lib().msgl_token_logprobs(logits.data_ptr(), N, V, logits.stride(0), tokens.data_ptr(), top, lp.data_ptr(), entropy.data_ptr(),
+                                            best.data_ptr(), ids.data_ptr(), blocks, _DT[logits.dtype], _stream())
+    _check(code, "token_logprobs")
+    return TokenLogprobs(lp, entropy, best.view(N, top), ids)
 
 
 # ---------------------------------------------------------------------------------------
