@@ -15,6 +15,7 @@ mini_sglang/layers/rotary_embedding.py, mini_sglang/layers/attn/fa3_attn_backend
 
 from __future__ import annotations
 
+import array
 import ctypes
 import os
 from typing import NamedTuple, Optional, Sequence, Tuple
@@ -2423,7 +2424,7 @@ def _draft_lib():
         lib = _build.drafts_library()
         lib.msgl_draft_plan.argtypes = [c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p] + [c_int] * 5 + [c_void_p] * 7
         lib.msgl_draft_accept.argtypes = [c_void_p] * 4 + [c_int] * 3 + [c_void_p] * 5 + [c_int] * 3 + [c_ll, c_int, c_int, c_void_p, c_int, c_int, c_void_p]
-        lib.msgl_token_logprobs.argtypes = [c_void_p, c_int, c_int, c_ll, c_void_p, c_int] + [c_void_p] * 4 + [c_int, c_int, c_void_p]
+        lib.msgl_token_logprobs.argtypes = [c_void_p, c_int, c_int, c_ll, c_void_p, c_int] + [c_void_p] * 4 + [c_int] * 3 + [c_void_p]
         _drafts = lib
     return _drafts
 
@@ -2492,6 +2493,25 @@ def draft_plan(parents: torch.Tensor, draft_lens: torch.Tensor, cached: torch.Te
     return DraftPlan(q_start, kv_len, positions, token_req, out_loc, mask.view(T, words))
 
 
+def _cache_groups(caches: Sequence[torch.Tensor], like: torch.Tensor):
+    """Addresses of the caches of draft_accept, those of one shape and element size together, each once (keys and values may be one array)."""
+    c0, dev = caches[0], like.get_device()
+    shape, dtype = c0.shape, c0.dtype
+    if c0.dim() == 4:
+        for c in caches:                     # (a model's layers are alike: looked at with few calls each)
+            if c.shape != shape or c.dtype is not dtype or c.get_device() != dev or not c.is_contiguous():
+                break
+        else:
+            return [(shape, c0.element_size(), list(dict.fromkeys([c.data_ptr() for c in caches])))]
+    groups = {}
+    for c in caches:
+        if c.dim() != 4 or not c.is_contiguous() or c.get_device() != dev or c.shape[2] != shape[2]:
+            raise KernelError(f"draft_accept: a cache is a contiguous [pages, kv heads, page size, row size] on {like.device}, all of one page size; "
+                              f"got {tuple(c.shape)} on {c.device}")
+        groups.setdefault((c.shape, c.element_size()), {})[c.data_ptr()] = None
+    return [(shape, item, list(ptrs)) for (shape, item), ptrs in groups.items()]
+
+
 class DraftPath(NamedTuple):
     """What a step of drafted tokens came to; -1 behind a request's path."""
     kept: torch.Tensor            # [B] drafts on the path, draft 0 among them (0: the request brought none)
@@ -2514,35 +2534,27 @@ def draft_accept(tokens: torch.Tensor, parents: torch.Tensor, following: torch.T
     if B < 0:
         raise KernelError("draft_accept: q_start has one element more than there are requests")
     _draft_limit("draft_accept", max_draft)
-    groups = {}
+    groups = []                              # (shape, bytes of an element, addresses) of the caches that are alike
     if len(caches):
         if kv_len is None or block_table is None:
             raise KernelError("draft_accept: caches need kv_len and block_table")
         _index("draft_accept", "kv_len", kv_len, B)
         _table("draft_accept", block_table, B)
-        dev, page_size, seen = tokens.get_device(), caches[0].shape[2], set()
-        for c in caches:
-            if c.dim() != 4 or not c.is_contiguous() or c.get_device() != dev or c.shape[2] != page_size:
-                raise KernelError(f"draft_accept: a cache is a contiguous [pages, kv heads, page size, row size] on {tokens.device}, all of one page size; "
-                                  f"got {tuple(c.shape)} on {c.device}")
-            ptr = c.data_ptr()
-            if ptr in seen:                  # (keys and values in one array)
-                continue
-            seen.add(ptr)
-            groups.setdefault((c.shape, c.element_size()), []).append(ptr)
+        groups = _cache_groups(caches, tokens)
     _same_device("draft_accept", tokens, parents, following, q_start, kv_len, block_table)
     buf = torch.empty(B * (1 + 2 * max_draft), dtype=torch.int32, device=tokens.device)
     kept, path, after = buf.split((B, B * max_draft, B * max_draft))
-    launches = [(shape, item, ptrs[i:i + _ACCEPT_CACHES]) for (shape, item), ptrs in groups.items() for i in range(0, len(ptrs), _ACCEPT_CACHES)]
+    launches = [(shape, item, ptrs[i:i + _ACCEPT_CACHES]) for shape, item, ptrs in groups for i in range(0, len(ptrs), _ACCEPT_CACHES)]
     out = (kept.data_ptr(), path.data_ptr(), after.data_ptr())
     for shape, item, ptrs in launches or [((0, 1, 1, 1), 2, [])]:
         row = shape[3] * item
         # blocks of a request: enough to fill the SMs a few times over, no more than there are columns for
         columns = len(ptrs) * shape[1] * -(-row // 16)
         blocks = max(1, min(-(-columns // _ACCEPT_BLOCK_COLUMNS), -(-4 * sm_count(tokens.device) // max(B, 1))))
+        addresses = array.array("Q", ptrs)          # (held by name until the call has read it)
         code = _draft_lib().msgl_draft_accept(tokens.data_ptr(), parents.data_ptr(), following.data_ptr(), q_start.data_ptr(), B, T, max_draft, *out,
                                               _ptr(kv_len), _ptr(block_table), block_table.stride(0) if ptrs else 0, block_table.shape[1] if ptrs else 0, shape[2],
-                                              shape[0], shape[1], row, (c_void_p * len(ptrs))(*ptrs), len(ptrs), blocks, _stream())
+                                              shape[0], shape[1], row, addresses.buffer_info()[0], len(ptrs), blocks, _stream())
         _check(code, "draft_accept")
         out = (None, None, None)
     return DraftPath(kept, path.view(B, max_draft), after.view(B, max_draft))
@@ -2576,7 +2588,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
     want = min(4 * sm_count(logits.device) // N, V // 2048, 8)
     blocks = 8 if want >= 8 else 4 if want >= 4 else 2 if want >= 2 else 1
     code = _draft_lib().msgl_token_logprobs(logits.data_ptr(), N, V, logits.stride(0), tokens.data_ptr(), top, lp.data_ptr(), entropy.data_ptr(),
-                                            best.data_ptr(), ids.data_ptr(), blocks, _DT[logits.dtype], _stream())
+                                            best.data_ptr(), ids.data_ptr(), blocks, int(N * blocks <= sm_count(logits.device)), _DT[logits.dtype], _stream())
     _check(code, "token_logprobs")
     return TokenLogprobs(lp, entropy, best.view(N, top), ids)
 

@@ -54,3 +54,31 @@ def test_logprobs_refuse():
     refused("top", f, x[:, :4], I(3), 5)
     refused("top", f, x[:, :0], I(3), 0)
     refused("CUDA device", f, x, I(3), 5)
+
+
+def test_accept_hands_over_every_cache_once(monkeypatch):
+    """What the library is called with, without a GPU: the addresses of the caches are there while the call reads them, those alike in one
+    launch, each once, and at most as many as a launch takes."""
+    import ctypes
+    calls = []
+
+    class Library:
+        @staticmethod
+        def msgl_draft_accept(*a):
+            calls.append((a[7], a[-7], a[-6], a[-5], list((ctypes.c_uint64 * a[-3]).from_address(a[-4]))))
+            return 0
+
+    monkeypatch.setattr(ops, "_drafts", Library)
+    monkeypatch.setattr(ops, "_same_device", lambda *a: None)
+    monkeypatch.setattr(ops, "sm_count", lambda d: 148)
+    monkeypatch.setattr(ops, "_stream", lambda: 0)
+    alike = [torch.zeros(5, 3, 16, 128, dtype=torch.bfloat16) for _ in range(150)]
+    other = [torch.zeros(5, 1, 16, 256, dtype=torch.bfloat16), torch.zeros(7, 1, 16, 20)]
+    more = dict(max_draft=4, kv_len=I(1), block_table=I(1, 3))
+    for given, groups in ((alike, [alike[:128], alike[128:]]), (alike[:56] + alike[:56], [alike[:56]]), (other[:1] + alike[:3] + other[1:], [other[:1], alike[:3], other[1:]])):
+        for _ in range(20):
+            calls.clear()
+            ops.draft_accept(I(8), I(8), I(8), I(2), caches=given, **more)
+            assert [c[4] for c in calls] == [[x.data_ptr() for x in g] for g in groups]
+            assert [c[0] is not None for c in calls] == [True] + [False] * (len(groups) - 1)          # the path is written by one launch
+            assert [c[1:4] for c in calls] == [(g[0].shape[0], g[0].shape[1], g[0].shape[3] * g[0].element_size()) for g in groups]
