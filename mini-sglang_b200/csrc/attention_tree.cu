@@ -1,0 +1,417 @@
+// Attention for trees of drafted tokens over the paged cache.
+//
+// Request r brings n = q_start[r + 1] - q_start[r] drafts whose keys and values are the last n of its kv_len[r] cached ones.  A draft sees
+// every key before them and of the drafts those whose bits are set in its mask row (its ancestors and itself, as draft_plan makes them, or
+// any other set):
+//
+//     o_i = sum_j p_ij v_j,   p_i = softmax over the keys that i sees of scale q_i k_j;   a draft that sees none gets 0
+//
+// What a draft does not see counts for nothing, whatever its key and value hold.  Query head h reads kv head h / G, G = n_q / n_kv.  The
+// cache is [page][kv head][slot][d]; the key at place i of request r lies in page block_table[r][i / P], slot i % P.
+//
+// Work.  A row is a (draft, head of the group) pair, so all rows of a kv head share its keys.  An item is up to ROWS rows of one request
+// under one kv head; its keys are cut into tiles of KT.  All items are laid end to end, an item as long as its tiles and TREE_HEAD
+// more (what it costs beside them), and cut into one run a block, equal but for TREE_SNAP: every block works out its run from the
+// requests' lengths by itself, so the host knows none of them and a captured launch serves any.  A block that has a whole item writes
+// its rows; of one that is cut every block leaves float32 partial sums with their maximum and sum of weights, and a second launch joins
+// them in the order of the keys.
+#include "common.cuh"
+#include <math.h>
+
+__device__ __forceinline__ unsigned smem_u32(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ float fast_exp2(float x) {          // 2^x by the special-function unit (relative error about 2^-22; -inf gives 0)
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ unsigned pack_bf16(float lo, float hi) {
+    __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<unsigned*>(&v);
+}
+
+struct TreeParams {
+    const void* q;                // [T, n_q, d]
+    void* out;
+    const void* k_cache;          // [pages, n_kv, page_size, d]
+    const void* v_cache;
+    const int* q_start;           // [B + 1]
+    const int* kv_len;            // [B]
+    const int* table;             // [B, table_width], rows table_stride apart
+    const unsigned* mask;         // [T, words]
+    float* part_o;                // [2 * blocks][ROWS][d]
+    float* part_ml;               // [2 * blocks][ROWS][2]  (maximum in log2 units, sum of the weights)
+    int4* record;                 // [blocks]: (request, item of it, pieces, rows) of the cut item whose first piece the block has; pieces 0: none
+    int B, T, n_q, n_kv, d, page_size, page_shift, table_stride, table_width, words;
+    long long pages;
+    float scale_log2;             // scale * log2(e)
+};
+
+// ---------------------------------------------------------------------------------------
+// the cut of the work
+// ---------------------------------------------------------------------------------------
+constexpr int TREE_HEAD = 1;      // what an item costs beside its tiles, in tiles
+constexpr int TREE_SNAP = 1;      // a cut this close to an item's edge, or closer, moves onto it
+constexpr int TREE_SHARE = TREE_HEAD + TREE_SNAP + 1;      // a block's run is no shorter: so no piece of an item is empty and none lies in more than its blocks
+
+struct TreeSegment {              // tiles [t_lo, t_hi) of one item
+    int r, item, kvh, row0, rows; // row0: first row of the item among the request's n * G under the kv head
+    int tok0, n, kv, base;        // the request's first draft in the stream, its drafts, its keys, those before the drafts
+    int t_lo, t_hi, tiles;
+};
+
+template <int ROWS, int KT>
+struct TreeWalk {
+    const TreeParams& p;
+    int blocks;                   // in use; none if the step has no drafts
+    long long total, x_lo, x_hi;  // the work's length, this block's run
+    int r = 0, item = 0;
+    long long start = 0;          // where the request's first item starts
+
+    __device__ __forceinline__ TreeWalk(const TreeParams& q) : p(q) {}
+    struct Request { int tok0, n, kv, tiles, items; };
+    __device__ __forceinline__ Request request(int i) const {
+        Request w;
+        w.tok0 = min(max(p.q_start[i], 0), p.T);
+        w.n = min(max(p.q_start[i + 1], w.tok0), p.T) - w.tok0;
+        w.kv = (int)min((long long)max(p.kv_len[i], 0), (long long)p.table_width * p.page_size);
+        w.tiles = max(1, (w.kv + KT - 1) / KT);
+        w.items = w.n > 0 ? p.n_kv * ((w.n * (p.n_q / p.n_kv) + ROWS - 1) / ROWS) : 0;
+        return w;
+    }
+    __device__ __forceinline__ long long cut_at(long long k) const { return total * k / blocks; }
+    // the tile that a cut at x falls on, in an item that starts at `s`
+    __device__ __forceinline__ int tile_at(long long x, long long s, int tiles) const {
+        const long long t = x - s - TREE_HEAD;
+        if (t < TREE_SNAP) return 0;
+        return tiles - t < TREE_SNAP ? tiles : (int)t;
+    }
+    // all threads of the block: the run of block j of nb; false: there is none
+    __device__ __forceinline__ bool begin(int j, int nb) {
+        __shared__ long long sums[32], found_start;
+        __shared__ int found;
+        const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n_warps = blockDim.x >> 5;
+        const int per = (p.B + blockDim.x - 1) / blockDim.x, i0 = min(p.B, tid * per), i1 = min(p.B, i0 + per);
+        long long mine = 0;
+        for (int i = i0; i < i1; ++i) { const Request w = request(i); mine += (long long)w.items * (w.tiles + TREE_HEAD); }
+        long long upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) { const long long v = __shfl_up_sync(0xffffffffu, upto, o); if (lane >= o) upto += v; }
+        if (lane == 31) sums[warp] = upto;
+        __syncthreads();
+        total = 0;
+        long long before = upto - mine;
+        for (int w = 0; w < n_warps; ++w) { if (w < warp) before += sums[w]; total += sums[w]; }
+        const long long fit = total / TREE_SHARE;
+        blocks = (int)min((long long)nb, fit > 1 ? fit : 1);
+        if (total == 0 || j >= blocks) return false;
+        x_lo = cut_at(j);
+        x_hi = cut_at(j + 1);
+        if (x_lo >= before && x_lo < before + mine) {
+            long long s = before;
+            for (int i = i0; i < i1; ++i) {
+                const Request w = request(i);
+                const long long len = (long long)w.items * (w.tiles + TREE_HEAD);
+                if (x_lo < s + len) { found = i; found_start = s; break; }
+                s += len;
+            }
+        }
+        __syncthreads();
+        r = found;
+        start = found_start;
+        const Request w = request(r);
+        item = (int)((x_lo - start) / (w.tiles + TREE_HEAD));
+        return true;
+    }
+    // the next segment of the run; false: it is done
+    __device__ __forceinline__ bool next(TreeSegment& g) {
+        while (r < p.B) {
+            const Request w = request(r);
+            const long long len = w.tiles + TREE_HEAD;
+            for (; item < w.items; ++item) {
+                const long long s = start + item * len;
+                if (s >= x_hi) return false;
+                const int lo = x_lo > s ? tile_at(x_lo, s, w.tiles) : 0, hi = x_hi < s + len ? tile_at(x_hi, s, w.tiles) : w.tiles;
+                if (lo >= hi) continue;
+                const int groups = w.items / p.n_kv, rows = w.n * (p.n_q / p.n_kv);
+                g.r = r; g.item = item; g.kvh = item / groups; g.row0 = (item - g.kvh * groups) * ROWS; g.rows = min(ROWS, rows - g.row0);
+                g.tok0 = w.tok0; g.n = w.n; g.kv = w.kv; g.base = w.kv - w.n;
+                g.t_lo = lo; g.t_hi = hi; g.tiles = w.tiles;
+                ++item;
+                return true;
+            }
+            start += w.items * len;
+            item = 0;
+            ++r;
+        }
+        return false;
+    }
+    // pieces of the item whose first piece `g` is, in block j
+    __device__ __forceinline__ int pieces(const TreeSegment& g, int j) const {
+        const long long s = start + (long long)(item - 1) * (g.tiles + TREE_HEAD), e = s + g.tiles + TREE_HEAD;
+        int k = j + 1;
+        while (k < blocks) {
+            const long long x = cut_at(k + 1);
+            ++k;
+            if (x >= e || tile_at(x, s, g.tiles) >= g.tiles) break;
+        }
+        return k - j;
+    }
+};
+
+// 32 keys from key0 on, a bit each: does the draft with mask row `row` see them?  (all before base; none from kv on)
+__device__ __forceinline__ unsigned tree_seen(const unsigned* row, int words, int key0, int base, int kv) {
+    const int d0 = key0 - base;
+    unsigned m;
+    if (d0 <= -32) m = ~0u;
+    else if (d0 < 0) m = (words > 0 ? row[0] << -d0 : 0u) | ((1u << -d0) - 1u);
+    else {
+        const int w = d0 >> 5, s = d0 & 31;
+        m = w < words ? row[w] >> s : 0u;
+        if (s > 0 && w + 1 < words) m |= row[w + 1] << (32 - s);
+    }
+    const int left = kv - key0;
+    return left >= 32 ? m : left <= 0 ? 0u : m & ((1u << left) - 1u);
+}
+
+__device__ __forceinline__ int tree_page(const TreeParams& p, int key) { return p.page_shift >= 0 ? key >> p.page_shift : key / p.page_size; }
+
+// ---------------------------------------------------------------------------------------
+// Any head size up to 512, any page size, float32 or bfloat16 data, float32 arithmetic: 32 rows a block, tiles of 32 keys.
+//
+// Warp w owns rows 4 w .. 4 w + 3.  Scores: lane = key, four rows a lane, K rows of odd 16-byte pitch, so that a warp's loads of them
+// meet no bank twice; P^T goes to shared memory (four rows a key side by side) and O is four rows x 4 CB columns a lane.  Bound by what
+// shared memory delivers (two loads for sixteen multiply-adds).  A key that a row does not see has the weight -1, which the product
+// leaves out: its value may be anything.
+// ---------------------------------------------------------------------------------------
+constexpr int TS_ROWS = 32, TS_KT = 32, TS_THREADS = 256;
+struct TreeYes { static constexpr bool value = true; };
+struct TreeNo { static constexpr bool value = false; };
+
+template <typename T, int CB>
+__global__ void __launch_bounds__(TS_THREADS) tree_simt_kernel(const TreeParams p) {
+    extern __shared__ __align__(16) float ts_smem[];
+    const int d = p.d, pitch = CB * 128 + 4, d4 = (d + 3) >> 2;
+    float* Qs = ts_smem;                             // [32][pitch]; columns from d on are zero
+    float* Ks = Qs + TS_ROWS * pitch;                // [32][pitch]
+    float* Vs = Ks + TS_KT * pitch;                  // [32][pitch]
+    float* Ps = Vs + TS_KT * pitch;                  // [8 warps][32 keys][4 rows]
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, j = blockIdx.x;
+    const int G = p.n_q / p.n_kv;
+    pdl_launch_dependents();
+    pdl_wait();
+    pdl_after_wait();
+    TreeWalk<TS_ROWS, TS_KT> walk(p);
+    int4 record = make_int4(0, 0, 0, 0);
+    TreeSegment g;
+    if (walk.begin(j, gridDim.x)) {
+        for (int i = tid; i < (TS_ROWS + 2 * TS_KT) * pitch; i += TS_THREADS) ts_smem[i] = 0.f;      // (what lies from d on stays zero)
+        while (walk.next(g)) {
+            const T* q = reinterpret_cast<const T*>(p.q);
+            __syncthreads();                         // the segment before has been read
+            for (int i = tid; i < TS_ROWS * d; i += TS_THREADS) {
+                const int row = i / d, c = i - row * d, rr = g.row0 + row;
+                Qs[row * pitch + c] = row < g.rows ? to_f32<T>(q[((size_t)(g.tok0 + rr / G) * p.n_q + (size_t)g.kvh * G + rr % G) * d + c]) : 0.f;
+            }
+            float o[4][CB][4], m_run[4], l_run[4];
+            const unsigned* row_mask[4];
+#pragma unroll
+            for (int a = 0; a < 4; ++a) {
+                m_run[a] = -INFINITY;
+                l_run[a] = 0.f;
+                const int row = min(4 * warp + a, g.rows - 1);
+                row_mask[a] = p.mask + (size_t)(g.tok0 + (g.row0 + row) / G) * p.words;
+#pragma unroll
+                for (int b = 0; b < CB; ++b) o[a][b][0] = o[a][b][1] = o[a][b][2] = o[a][b][3] = 0.f;
+            }
+            for (int t = g.t_lo; t < g.t_hi; ++t) {
+                const int key0 = t * TS_KT;
+                __syncthreads();                     // the tile before has been read (and Q written)
+                for (int i = tid; i < TS_KT * d; i += TS_THREADS) {
+                    const int row = i / d, c = i - row * d, key = key0 + row;
+                    float kv = 0.f, vv = 0.f;
+                    if (key < g.kv) {
+                        const int pi = tree_page(p, key), id = p.table[(size_t)g.r * p.table_stride + pi];
+                        if (id >= 0 && id < p.pages) {
+                            const size_t at = (((size_t)id * p.n_kv + g.kvh) * p.page_size + (key - pi * p.page_size)) * d + c;
+                            kv = to_f32<T>(reinterpret_cast<const T*>(p.k_cache)[at]);
+                            vv = to_f32<T>(reinterpret_cast<const T*>(p.v_cache)[at]);
+                        }
+                    }
+                    Ks[row * pitch + c] = kv;
+                    Vs[row * pitch + c] = vv;
+                }
+                __syncthreads();
+                if (4 * warp >= g.rows) continue;    // (no row of this warp)
+                float s[4] = {0.f, 0.f, 0.f, 0.f};
+                for (int c = 0; c < d4; ++c) {
+                    const float4 k4 = *reinterpret_cast<const float4*>(Ks + lane * pitch + 4 * c);
+#pragma unroll
+                    for (int a = 0; a < 4; ++a) {
+                        const float4 q4 = *reinterpret_cast<const float4*>(Qs + (4 * warp + a) * pitch + 4 * c);
+                        s[a] = fmaf(q4.x, k4.x, fmaf(q4.y, k4.y, fmaf(q4.z, k4.z, fmaf(q4.w, k4.w, s[a]))));
+                    }
+                }
+                const bool ends = key0 + TS_KT > g.base;
+                float w[4];
+#pragma unroll
+                for (int a = 0; a < 4; ++a) {
+                    const unsigned seen = ends ? tree_seen(row_mask[a], p.words, key0, g.base, g.kv) : ~0u;
+                    const bool in = seen >> lane & 1u;
+                    s[a] = in ? s[a] * p.scale_log2 : -INFINITY;
+                    const float mx = fmaxf(m_run[a], warp_max(s[a])), mu = mx == -INFINITY ? 0.f : mx;
+                    const float f = fast_exp2(m_run[a] - mu), e = fast_exp2(s[a] - mu);
+                    m_run[a] = mx;
+                    l_run[a] = fmaf(l_run[a], f, e);             // this lane's keys alone
+                    w[a] = in ? e : -1.f;
+#pragma unroll
+                    for (int b = 0; b < CB; ++b) { o[a][b][0] *= f; o[a][b][1] *= f; o[a][b][2] *= f; o[a][b][3] *= f; }
+                }
+                float* P = Ps + warp * TS_KT * 4;
+                *reinterpret_cast<float4*>(P + lane * 4) = make_float4(w[0], w[1], w[2], w[3]);
+                __syncwarp();
+                auto product = [&](auto guarded) {
+#pragma unroll 4
+                    for (int key = 0; key < TS_KT; ++key) {
+                        const float4 w4 = *reinterpret_cast<const float4*>(P + key * 4);
+                        const float ww[4] = {w4.x, w4.y, w4.z, w4.w};
+#pragma unroll
+                        for (int b = 0; b < CB; ++b) {
+                            const float4 v4 = *reinterpret_cast<const float4*>(Vs + key * pitch + b * 128 + lane * 4);
+#pragma unroll
+                            for (int a = 0; a < 4; ++a) {
+                                if (decltype(guarded)::value && ww[a] < 0.f) continue;
+                                o[a][b][0] = fmaf(ww[a], v4.x, o[a][b][0]); o[a][b][1] = fmaf(ww[a], v4.y, o[a][b][1]);
+                                o[a][b][2] = fmaf(ww[a], v4.z, o[a][b][2]); o[a][b][3] = fmaf(ww[a], v4.w, o[a][b][3]);
+                            }
+                        }
+                    }
+                };
+                if (ends) product(TreeYes());
+                else product(TreeNo());
+                __syncwarp();
+            }
+            const bool whole = g.t_lo == 0 && g.t_hi == g.tiles;
+            const int slot = 2 * j + (g.t_lo == 0 ? 1 : 0);
+#pragma unroll
+            for (int a = 0; a < 4; ++a) {
+                const int row = 4 * warp + a;
+                if (row >= g.rows) continue;
+                const float l = warp_sum(l_run[a]);
+                if (whole) {
+                    const int rr = g.row0 + row;
+                    const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
+                    T* dst = reinterpret_cast<T*>(p.out) + ((size_t)(g.tok0 + rr / G) * p.n_q + (size_t)g.kvh * G + rr % G) * d;
+#pragma unroll
+                    for (int b = 0; b < CB; ++b)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (b * 128 + lane * 4 + e < d) dst[b * 128 + lane * 4 + e] = from_f32<T>(o[a][b][e] * inv);
+                } else {
+                    float* dst = p.part_o + ((size_t)slot * TS_ROWS + row) * d;
+#pragma unroll
+                    for (int b = 0; b < CB; ++b)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (b * 128 + lane * 4 + e < d) dst[b * 128 + lane * 4 + e] = o[a][b][e];
+                    if (lane == 0) *reinterpret_cast<float2*>(p.part_ml + ((size_t)slot * TS_ROWS + row) * 2) = make_float2(m_run[a], l);
+                }
+            }
+            if (!whole && g.t_lo == 0) record = make_int4(g.r, g.item, walk.pieces(g, j), g.rows);
+        }
+    }
+    if (tid == 0) p.record[j] = record;
+}
+
+// ---------------------------------------------------------------------------------------
+// The pieces of cut items, joined in the order of the keys: block (j, y) takes eight rows of the item whose first piece block j has.
+// ---------------------------------------------------------------------------------------
+template <typename T, int ROWS>
+__global__ void __launch_bounds__(256) tree_join_kernel(const TreeParams p) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, j = blockIdx.x, row = blockIdx.y * 8 + warp;
+    pdl_launch_dependents();
+    pdl_wait();
+    pdl_after_wait();
+    const int4 rec = p.record[j];
+    if (rec.z == 0 || row >= rec.w) return;
+    const int G = p.n_q / p.n_kv, d = p.d, tok0 = min(max(p.q_start[rec.x], 0), p.T), n = min(max(p.q_start[rec.x + 1], tok0), p.T) - tok0;
+    const int groups = (n * G + ROWS - 1) / ROWS, kvh = rec.y / groups, rr = (rec.y - kvh * groups) * ROWS + row;
+    auto at = [&](int k) { return (size_t)(2 * (j + k) + (k == 0 ? 1 : 0)) * ROWS + row; };
+    float M = -INFINITY;
+    for (int k = lane; k < rec.z; k += 32) M = fmaxf(M, p.part_ml[at(k) * 2]);
+    M = warp_max(M);
+    const float mu = M == -INFINITY ? 0.f : M;
+    float L = 0.f;
+    T* dst = reinterpret_cast<T*>(p.out) + ((size_t)(tok0 + rr / G) * p.n_q + (size_t)kvh * G + rr % G) * d;
+    for (int c0 = 0; c0 < d; c0 += 128) {
+        float acc[4] = {0.f, 0.f, 0.f, 0.f};
+        L = 0.f;
+        for (int k0 = 0; k0 < rec.z; k0 += 32) {
+            float2 ml = make_float2(-INFINITY, 0.f);
+            if (k0 + lane < rec.z) ml = *reinterpret_cast<const float2*>(p.part_ml + at(k0 + lane) * 2);
+            const float w = fast_exp2(ml.x - mu);
+            L += w * ml.y;
+            const int m = min(rec.z - k0, 32);
+#pragma unroll 4
+            for (int k = 0; k < m; ++k) {
+                const float f = __shfl_sync(0xffffffffu, w, k);
+                const float* src = p.part_o + at(k0 + k) * d + c0 + lane * 4;
+                if ((d & 3) == 0) {
+                    if (c0 + lane * 4 < d) {
+                        const float4 v = *reinterpret_cast<const float4*>(src);
+                        acc[0] = fmaf(f, v.x, acc[0]); acc[1] = fmaf(f, v.y, acc[1]); acc[2] = fmaf(f, v.z, acc[2]); acc[3] = fmaf(f, v.w, acc[3]);
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (c0 + lane * 4 + e < d) acc[e] = fmaf(f, src[e], acc[e]);
+                }
+            }
+        }
+        L = warp_sum(L);
+        const float inv = L > 0.f ? 1.f / L : (L == L ? 0.f : L);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (c0 + lane * 4 + e < d) dst[c0 + lane * 4 + e] = from_f32<T>(acc[e] * inv);
+    }
+}
+
+static int tree_simt_blocks_per_sm(int d) { return d <= 128 ? 4 : d <= 256 ? 2 : 1; }
+static size_t tree_simt_smem(int cb) { return ((size_t)(TS_ROWS + 2 * TS_KT) * (cb * 128 + 4) + 8 * TS_KT * 4) * sizeof(float); }
+
+// Blocks of a launch and rows of an item, for the sizes of the scratch memory: part_o [2 * blocks][rows][d], part_ml [2 * blocks][rows][2] float32, record [blocks][4] int32.
+MSGL_API int msgl_tree_attention_blocks(int d) { return msgl_sm_count() * tree_simt_blocks_per_sm(d); }
+MSGL_API int msgl_tree_attention_rows() { return TS_ROWS; }
+
+template <typename T, int CB>
+static int tree_simt_launch(const TreeParams& p, int blocks, cudaStream_t stream) {
+    static MsglOncePerDevice attr_set;
+    if (attr_set.due()) {
+        if (cudaFuncSetAttribute(tree_simt_kernel<T, CB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)tree_simt_smem(CB)) != cudaSuccess) return msgl_check_launch();
+        attr_set.mark();
+    }
+    msgl_launch_pdl(tree_simt_kernel<T, CB>, dim3(blocks), dim3(TS_THREADS), tree_simt_smem(CB), stream, p);
+    msgl_launch_pdl(tree_join_kernel<T, TS_ROWS>, dim3(blocks, TS_ROWS / 8), dim3(256), 0, stream, p);
+    return msgl_check_launch();
+}
+
+MSGL_API int msgl_tree_attention(const void* q, void* out, const void* k_cache, const void* v_cache, const int* q_start, const int* kv_len, const int* table,
+                                 const void* mask, int B, int T, int n_q, int n_kv, int d, int page_size, int table_stride, int table_width, int words,
+                                 long long pages, float scale, float* part_o, float* part_ml, int* record, int blocks, int dtype, cudaStream_t stream) {
+    if (B <= 0 || T <= 0) return MSGL_OK;
+    if (n_kv <= 0 || n_q <= 0 || n_q % n_kv || d < 1 || d > 512 || page_size < 1 || table_width < 1 || words < 1 || blocks < 1 || pages < 0) return MSGL_ERR_SIZE;
+    if ((long long)table_width * page_size > 0x7fffffffLL - 1024 || (long long)T * (n_q / n_kv) > 0x7fffffffLL / 2) return MSGL_ERR_SIZE;
+    if (((uintptr_t)part_o | (uintptr_t)record) & 15 || (uintptr_t)part_ml & 7) return MSGL_ERR_ALIGN;
+    TreeParams p;
+    p.q = q; p.out = out; p.k_cache = k_cache; p.v_cache = v_cache; p.q_start = q_start; p.kv_len = kv_len; p.table = table; p.mask = (const unsigned*)mask;
+    p.part_o = part_o; p.part_ml = part_ml; p.record = (int4*)record;
+    p.B = B; p.T = T; p.n_q = n_q; p.n_kv = n_kv; p.d = d; p.page_size = page_size; p.table_stride = table_stride; p.table_width = table_width; p.words = words;
+    p.pages = pages;
+    p.page_shift = -1;
+    if ((page_size & (page_size - 1)) == 0) { int sh = 0; while ((1 << sh) < page_size) ++sh; p.page_shift = sh; }
+    p.scale_log2 = scale * 1.4426950408889634f;
+    if (dtype == MSGL_F32) return d <= 128 ? tree_simt_launch<float, 1>(p, blocks, stream) : d <= 256 ? tree_simt_launch<float, 2>(p, blocks, stream) : tree_simt_launch<float, 4>(p, blocks, stream);
+    if (dtype == MSGL_BF16)
+        return d <= 128 ? tree_simt_launch<__nv_bfloat16, 1>(p, blocks, stream) : d <= 256 ? tree_simt_launch<__nv_bfloat16, 2>(p, blocks, stream)
+                                                                                          : tree_simt_launch<__nv_bfloat16, 4>(p, blocks, stream);
+    return MSGL_ERR_DTYPE;
+}

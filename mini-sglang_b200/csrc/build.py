@@ -139,7 +139,7 @@ MIXER_SOURCES = ["mixers.cu"]
 GATED_MIXER_SOURCES = ["mixers_gated.cu"]
 DELTA_MIXER_SOURCES = ["mixers_delta.cu"]
 STREAM_MIXER_SOURCES = ["mixers_streams.cu"]
-DRAFT_SOURCES = ["drafts.cu", "logprobs.cu"]
+DRAFT_SOURCES = ["drafts.cu", "logprobs.cu", "attention_tree.cu"]
 MMA_HEAD_DIMS = tuple(range(16, 257, 16))   # head sizes the tensor-core attention kernel is built for
 
 
@@ -176,8 +176,8 @@ def stream_mixers_library() -> ctypes.CDLL:
 
 
 def drafts_library() -> ctypes.CDLL:
-    """The kernels of a step that verifies drafted tokens (csrc/drafts.cu: its fields and the accepted path) and the log
-    probabilities of tokens (csrc/logprobs.cu); built at their first use."""
+    """The kernels of a step that verifies drafted tokens (csrc/drafts.cu: its fields and the accepted path, csrc/attention_tree.cu:
+    their attention) and the log probabilities of tokens (csrc/logprobs.cu); built at their first use."""
     return load_library("drafts", DRAFT_SOURCES)
 
 

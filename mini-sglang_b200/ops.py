@@ -2424,6 +2424,7 @@ def _draft_lib():
         lib = _build.drafts_library()
         lib.msgl_draft_plan.argtypes = [c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p] + [c_int] * 5 + [c_void_p] * 7
         lib.msgl_draft_accept.argtypes = [c_void_p] * 4 + [c_int] * 3 + [c_void_p] * 5 + [c_int] * 3 + [c_ll, c_int, c_int, c_void_p, c_int, c_int, c_void_p]
+        lib.msgl_tree_attention.argtypes = [c_void_p] * 8 + [c_int] * 9 + [c_ll, c_float] + [c_void_p] * 3 + [c_int, c_int, c_void_p]
         lib.msgl_token_logprobs.argtypes = [c_void_p, c_int, c_int, c_ll, c_void_p, c_int] + [c_void_p] * 4 + [c_int] * 3 + [c_void_p]
         _drafts = lib
     return _drafts
@@ -2491,6 +2492,48 @@ def draft_plan(parents: torch.Tensor, draft_lens: torch.Tensor, cached: torch.Te
                                         out_loc.data_ptr(), mask.data_ptr(), _stream())
     _check(code, "draft_plan")
     return DraftPlan(q_start, kv_len, positions, token_req, out_loc, mask.view(T, words))
+
+
+def tree_attention(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, *, q_start: torch.Tensor, kv_len: torch.Tensor,
+                   block_table: torch.Tensor, mask: torch.Tensor, n_kv: int, page_size: int, scale: float, max_draft: int) -> None:
+    """Attention of a step whose requests bring drafted tokens: q and out [T, heads, d] float32 or bfloat16, the paged caches as for
+    `attention`, q_start, kv_len and mask as `draft_plan` makes them (any other mask will do).  A draft sees all keys of its request before
+    the drafts, and of these the ones whose bits are set in its mask row; what it does not see counts for nothing, whatever it holds, and
+    a draft that sees no key gets 0.  No request brings more than max_draft (the host's bound; it sizes the launch).  Rows of out behind the
+    last draft are left as they were.  Head sizes up to 512; bfloat16 heads of 128 on pages that TMA can fetch (a power of two from 8
+    on) go through the tensor cores.  A page number outside the cache reads as zeros."""
+    T, n_q, d = q.shape
+    B, width = block_table.shape
+    what = "tree_attention"
+    if q.dtype not in _DT or out.dtype != q.dtype or out.shape != q.shape or not q.is_contiguous() or not out.is_contiguous():
+        raise KernelError(f"{what}: q and out are contiguous [drafts, heads, head size], both float32 or both bfloat16; got {q.dtype} {tuple(q.shape)}, {out.dtype} {tuple(out.shape)}")
+    if not (k_cache.dim() == 4 and k_cache.shape == v_cache.shape and k_cache.dtype == v_cache.dtype == q.dtype and k_cache.is_contiguous() and v_cache.is_contiguous()
+            and tuple(k_cache.shape[1:]) == (n_kv, page_size, d)):
+        raise KernelError(f"{what}: the caches are contiguous [pages, {n_kv}, {page_size}, {d}] of q's type; got {tuple(k_cache.shape)}, {tuple(v_cache.shape)}")
+    if n_kv < 1 or n_q % n_kv or not 1 <= d <= 512:
+        raise KernelError(f"{what}: {n_q} query heads over {n_kv} kv heads of size {d}: whole groups, sizes up to 512")
+    _table(what, block_table, B)
+    _index(what, "q_start", q_start, B + 1)
+    _index(what, "kv_len", kv_len, B)
+    _draft_limit(what, max_draft)
+    words = mask.shape[1] if mask.dim() == 2 else 0
+    if words * 32 < max_draft:
+        raise KernelError(f"{what}: a mask row has a bit for every one of up to {max_draft} drafts; got {tuple(mask.shape)}")
+    _index(what, "mask", mask, T * words)
+    _same_device(what, q, out, k_cache, v_cache, q_start, kv_len, block_table, mask)
+    if T == 0 or B == 0:
+        return
+    lib = _draft_lib()
+    blocks, rows = lib.msgl_tree_attention_blocks(d), lib.msgl_tree_attention_rows()
+    part = torch.empty(2 * blocks * rows * (d + 2) + 4 * blocks, dtype=torch.float32, device=q.device)
+    at = part.data_ptr()
+    part_ml, record = at + 4 * 2 * blocks * rows * d, at + 4 * 2 * blocks * rows * (d + 2)
+    code = lib.msgl_tree_attention(q.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), q_start.data_ptr(), kv_len.data_ptr(), block_table.data_ptr(),
+                                   mask.data_ptr(), B, T, n_q, n_kv, d, page_size, block_table.stride(0), width, words, k_cache.shape[0], float(scale), at, part_ml, record,
+                                   blocks, _DT[q.dtype], _stream())
+    _check(code, what)
+    global LAUNCHES
+    LAUNCHES += 1                # the join of cut items is a kernel of its own
 
 
 def _cache_groups(caches: Sequence[torch.Tensor], like: torch.Tensor):

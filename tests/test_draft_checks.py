@@ -82,3 +82,28 @@ def test_accept_hands_over_every_cache_once(monkeypatch):
             assert [c[4] for c in calls] == [[x.data_ptr() for x in g] for g in groups]
             assert [c[0] is not None for c in calls] == [True] + [False] * (len(groups) - 1)          # the path is written by one launch
             assert [c[1:4] for c in calls] == [(g[0].shape[0], g[0].shape[1], g[0].shape[3] * g[0].element_size()) for g in groups]
+
+
+def test_tree_attention_refuses():
+    f = ops.tree_attention
+    q, c = torch.zeros(4, 8, 16), torch.zeros(5, 2, 16, 16)
+    ok = dict(q_start=I(2), kv_len=I(1), block_table=I(1, 3), mask=I(4, 1), n_kv=2, page_size=16, scale=1.0, max_draft=4)
+    refused("q and out", f, q, q[:3], c, c, **ok)
+    refused("q and out", f, q, q.bfloat16(), c, c, **ok)
+    refused("q and out", f, q.half(), q.half(), c, c, **ok)
+    refused("q and out", f, q.transpose(1, 2), q.transpose(1, 2), c, c, **ok)
+    refused("caches", f, q, q, c, c[:, :, :8], **ok)
+    refused("caches", f, q, q, c.bfloat16(), c.bfloat16(), **ok)
+    refused("caches", f, q, q, c, c, **dict(ok, page_size=8))
+    refused("whole groups", f, torch.zeros(4, 7, 16), torch.zeros(4, 7, 16), c, c, **ok)
+    wide = torch.zeros(5, 2, 16, 513)
+    refused("sizes up to 512", f, torch.zeros(4, 8, 513), torch.zeros(4, 8, 513), wide, wide, **ok)
+    refused("block_table", f, q, q, c, c, **dict(ok, block_table=I(1, 3).long()))
+    refused("q_start", f, q, q, c, c, **dict(ok, q_start=I(3)))
+    refused("kv_len", f, q, q, c, c, **dict(ok, kv_len=I(2)))
+    refused("max_draft", f, q, q, c, c, **dict(ok, max_draft=257))
+    refused("a mask row", f, q, q, c, c, **dict(ok, max_draft=33))
+    refused("a mask row", f, q, q, c, c, **dict(ok, mask=I(4)))
+    refused("mask", f, q, q, c, c, **dict(ok, mask=I(3, 1)))
+    refused("mask", f, q, q, c, c, **dict(ok, mask=I(4, 1).long()))
+    refused("CUDA device", f, q, q, c, c, **ok)
