@@ -375,30 +375,54 @@ __global__ void __launch_bounds__(256) tree_join_kernel(const TreeParams p) {
     }
 }
 
+#include "attention_tree_tc.cuh"
+
 static int tree_simt_blocks_per_sm(int d) { return d <= 128 ? 4 : d <= 256 ? 2 : 1; }
 static size_t tree_simt_smem(int cb) { return ((size_t)(TS_ROWS + 2 * TS_KT) * (cb * 128 + 4) + 8 * TS_KT * 4) * sizeof(float); }
 
+// Whether the tensor cores take a launch: bfloat16, head sizes 64 and 128, pages that TMA can fetch, a cache whose rows a coordinate can name.
+MSGL_API int msgl_tree_attention_tensor(int d, int page_size, long long cache_rows, int dtype) {
+    return dtype == MSGL_BF16 && (d == 64 || d == 128) && page_size >= 8 && (page_size & (page_size - 1)) == 0 && cache_rows < 0x7fffffffLL - 4096 && tc_encoder() != nullptr;
+}
 // Blocks of a launch and rows of an item, for the sizes of the scratch memory: part_o [2 * blocks][rows][d], part_ml [2 * blocks][rows][2] float32, record [blocks][4] int32.
-MSGL_API int msgl_tree_attention_blocks(int d) { return msgl_sm_count() * tree_simt_blocks_per_sm(d); }
-MSGL_API int msgl_tree_attention_rows() { return TS_ROWS; }
+MSGL_API int msgl_tree_attention_blocks(int d, int tensor) { return msgl_sm_count() * (tensor ? 1 : tree_simt_blocks_per_sm(d)); }
+MSGL_API int msgl_tree_attention_rows(int tensor) { return tensor ? TT_ROWS : TS_ROWS; }
 
 template <typename T, int CB>
-static int tree_simt_launch(const TreeParams& p, int blocks, cudaStream_t stream) {
+static int tree_simt_launch(const TreeParams& p, int blocks, int max_rows, cudaStream_t stream) {
     static MsglOncePerDevice attr_set;
     if (attr_set.due()) {
         if (cudaFuncSetAttribute(tree_simt_kernel<T, CB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)tree_simt_smem(CB)) != cudaSuccess) return msgl_check_launch();
         attr_set.mark();
     }
     msgl_launch_pdl(tree_simt_kernel<T, CB>, dim3(blocks), dim3(TS_THREADS), tree_simt_smem(CB), stream, p);
-    msgl_launch_pdl(tree_join_kernel<T, TS_ROWS>, dim3(blocks, TS_ROWS / 8), dim3(256), 0, stream, p);
+    msgl_launch_pdl(tree_join_kernel<T, TS_ROWS>, dim3(blocks, (min(max_rows, TS_ROWS) + 7) / 8), dim3(256), 0, stream, p);
     return msgl_check_launch();
 }
 
+template <int D>
+static int tree_tc_launch(const TreeParams& p, int* status, int blocks, int max_rows, cudaStream_t stream) {
+    static MsglOncePerDevice attr_set;
+    if (attr_set.due()) {
+        if (cudaFuncSetAttribute(tree_tc_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)TreeTc<D>::ALLOC) != cudaSuccess) return msgl_check_launch();
+        attr_set.mark();
+    }
+    const int box = p.page_size < 128 ? p.page_size : 128;
+    const long long rows = p.pages * p.n_kv * p.page_size;
+    CUtensorMap kmap, vmap;
+    if (!tc_matrix_map(p.k_cache, rows, D, (long long)D * 2, box, &kmap) || !tc_matrix_map(p.v_cache, rows, D, (long long)D * 2, box, &vmap)) return MSGL_ERR_SIZE;
+    msgl_launch_pdl(tree_tc_kernel<D>, dim3(blocks), dim3(TT_THREADS), TreeTc<D>::ALLOC, stream, p, status, kmap, vmap, box);
+    msgl_launch_pdl(tree_join_kernel<__nv_bfloat16, TT_ROWS>, dim3(blocks, (min(max_rows, TT_ROWS) + 7) / 8), dim3(256), 0, stream, p);
+    return msgl_check_launch();
+}
+
+// tensor: whether the tensor cores are to take it (status then points at the status word); max_rows: the most rows that a request has under a kv head.
 MSGL_API int msgl_tree_attention(const void* q, void* out, const void* k_cache, const void* v_cache, const int* q_start, const int* kv_len, const int* table,
                                  const void* mask, int B, int T, int n_q, int n_kv, int d, int page_size, int table_stride, int table_width, int words,
-                                 long long pages, float scale, float* part_o, float* part_ml, int* record, int blocks, int dtype, cudaStream_t stream) {
+                                 long long pages, float scale, float* part_o, float* part_ml, int* record, int blocks, int max_rows, int tensor, int* status,
+                                 int dtype, cudaStream_t stream) {
     if (B <= 0 || T <= 0) return MSGL_OK;
-    if (n_kv <= 0 || n_q <= 0 || n_q % n_kv || d < 1 || d > 512 || page_size < 1 || table_width < 1 || words < 1 || blocks < 1 || pages < 0) return MSGL_ERR_SIZE;
+    if (n_kv <= 0 || n_q <= 0 || n_q % n_kv || d < 1 || d > 512 || page_size < 1 || table_width < 1 || words < 1 || blocks < 1 || pages < 0 || max_rows < 1) return MSGL_ERR_SIZE;
     if ((long long)table_width * page_size > 0x7fffffffLL - 1024 || (long long)T * (n_q / n_kv) > 0x7fffffffLL / 2) return MSGL_ERR_SIZE;
     if (((uintptr_t)part_o | (uintptr_t)record) & 15 || (uintptr_t)part_ml & 7) return MSGL_ERR_ALIGN;
     TreeParams p;
@@ -409,9 +433,14 @@ MSGL_API int msgl_tree_attention(const void* q, void* out, const void* k_cache, 
     p.page_shift = -1;
     if ((page_size & (page_size - 1)) == 0) { int sh = 0; while ((1 << sh) < page_size) ++sh; p.page_shift = sh; }
     p.scale_log2 = scale * 1.4426950408889634f;
-    if (dtype == MSGL_F32) return d <= 128 ? tree_simt_launch<float, 1>(p, blocks, stream) : d <= 256 ? tree_simt_launch<float, 2>(p, blocks, stream) : tree_simt_launch<float, 4>(p, blocks, stream);
-    if (dtype == MSGL_BF16)
-        return d <= 128 ? tree_simt_launch<__nv_bfloat16, 1>(p, blocks, stream) : d <= 256 ? tree_simt_launch<__nv_bfloat16, 2>(p, blocks, stream)
-                                                                                          : tree_simt_launch<__nv_bfloat16, 4>(p, blocks, stream);
+    if (tensor) {
+        if (status == nullptr || pages < 1 || !msgl_tree_attention_tensor(d, page_size, pages * n_kv * page_size, dtype)) return MSGL_ERR_SIZE;
+        if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_cache | (uintptr_t)v_cache) & 15) return MSGL_ERR_ALIGN;
+        return d == 128 ? tree_tc_launch<128>(p, status, blocks, max_rows, stream) : tree_tc_launch<64>(p, status, blocks, max_rows, stream);
+    }
+#define MSGL_TREE(T, CB) tree_simt_launch<T, CB>(p, blocks, max_rows, stream)
+    if (dtype == MSGL_F32) return d <= 128 ? MSGL_TREE(float, 1) : d <= 256 ? MSGL_TREE(float, 2) : MSGL_TREE(float, 4);
+    if (dtype == MSGL_BF16) return d <= 128 ? MSGL_TREE(__nv_bfloat16, 1) : d <= 256 ? MSGL_TREE(__nv_bfloat16, 2) : MSGL_TREE(__nv_bfloat16, 4);
+#undef MSGL_TREE
     return MSGL_ERR_DTYPE;
 }

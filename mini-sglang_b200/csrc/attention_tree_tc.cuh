@@ -1,0 +1,441 @@
+// Attention for trees of drafted tokens on the 5th-generation tensor cores: bfloat16, head sizes 64 and 128, pages that TMA can fetch.
+//
+// A block, alone on its SM, walks its run of segments (attention_tree.cu): up to 256 rows -- (draft, head of the group) pairs of one kv head --
+// against tiles of 128 keys.
+//
+//     S = Q K^T     tcgen05.mma 128 x 128 x 16, operands in shared memory, accumulator in tensor memory
+//     softmax       thread t of a group of four warps owns row t = TMEM lane t, with the row's 128 scores in registers; P, rounded to
+//                   bfloat16 (half a step, 2^-9, of each weight; the sum of the weights is taken before), goes back over the columns of S
+//     O += P V      tcgen05.mma 128 x D x 16, P from tensor memory, V from shared memory as it lies in the cache
+//
+// The products of a tile keep the tensor core about as busy as its exponentials the special-function units, and one follows the other for
+// any one tile.  So there are always two softmax groups, A and B, with scores and accumulators of their own, and the issuer alternates
+// between them:  S_A  S_B  P V_A  S_A  P V_B  S_B ...  What differs is what they share:
+//
+//     more than 128 rows    A has rows 0 .. 127, B the others; both see every key tile
+//     up to 128 rows        both have the same rows, A the even key tiles of the segment, B the odd ones; the two results are joined at the end
+//
+// so few rows, where the stream of keys is the bound, still have two tiles in work and two on their way.
+//
+// Keys come by TMA (a page of a kv head is a run of rows of the cache taken as one matrix), a lane a page, into rings of ST tiles of keys
+// and of values; the loaders run ahead across the segments.  Of the tiles that hold drafts the values are looked at: rows behind the last
+// key are cleared (free slots may hold anything), and elements that are no numbers are cleared and remembered, since 0 x inf would reach
+// drafts that do not see them; the drafts that do see them get them back at the end.
+//
+// The exponentials' reference m need not be a row's maximum: it is found for a row's first tile and moved where a tile's sum shows that it
+// fell behind by 2^16 or the exponentials overflowed (then the tile is done again).  Whenever it moves, O is scaled in tensor memory.
+//
+// Every wait is bounded; a block that gives up sets the status word, waits for its copies, frees its tensor memory and returns.
+//
+// Warps: 0-3 softmax A, 4-7 softmax B (both also fetch Q), 8 keys, 9 values, 10 issuer, 11 idle.
+#pragma once
+#include "tc_common.cuh"
+
+constexpr int TT_ROWS = 256, TT_KT = 128, TT_THREADS = 384;
+constexpr unsigned TT_HALF = 128u * 128u;            // 128 rows of 64 columns, 128-byte swizzle: 16 KB
+constexpr int TT_BAD = 8;                            // segments whose non-numbers are remembered: more than the loaders run ahead
+
+template <int D> struct TreeTc {
+    static constexpr int H = D / 64, ST = D == 128 ? 2 : 4;                                       // halves of a row, stages of a ring
+    static constexpr unsigned TILE = H * TT_HALF;
+    static constexpr unsigned SMEM = 2u * TILE + 2u * ST * TILE;                                  // Q_A, Q_B, keys, values
+    static constexpr unsigned ALLOC = SMEM + 1024u + 4096u;                                       // barriers and scalars ahead, alignment
+};
+
+// two float32 values in one 64-bit register, for the packed float32 instructions of sm_100
+__device__ __forceinline__ unsigned long long tt_pack(float lo, float hi) {
+    unsigned long long r;
+    asm("mov.b64 %0, {%1, %2};\n" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void tt_unpack(unsigned long long v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;\n" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ unsigned long long tt_fma(unsigned long long a, unsigned long long b, unsigned long long c) {
+    unsigned long long r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ unsigned long long tt_add(unsigned long long a, unsigned long long b) {
+    unsigned long long r;
+    asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ void tt_cp_async16(unsigned s, const void* gmem, bool valid) {
+    const int n = valid ? 16 : 0;
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(s), "l"(gmem), "r"(n));
+}
+// byte offset of (row, 16-byte chunk c) in a swizzled tile
+__device__ __forceinline__ unsigned tt_off(int row, int c) {
+    return (unsigned)(c >> 3) * TT_HALF + (unsigned)row * 128u + (unsigned)(((c & 7) ^ (row & 7)) << 4);
+}
+__device__ __forceinline__ unsigned tt_nonfinite(unsigned w) {               // two bfloat16: the bits of those that are inf or NaN
+    return ((w & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) | ((w & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u);
+}
+
+// tma_box: rows of a TMA box, min(page_size, 128)
+template <int D>
+__global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const TreeParams p, int* status, const __grid_constant__ CUtensorMap kmap,
+                                                                const __grid_constant__ CUtensorMap vmap, int tma_box) {
+    using C = TreeTc<D>;
+    constexpr int ST = C::ST, H = C::H;
+    extern __shared__ __align__(16) unsigned char tt_smem[];
+    // the first 4 KB: barriers, scalars, the non-numbers' words, the rows' sums that groups A and B exchange
+    unsigned& tmem_base_s = *reinterpret_cast<unsigned*>(tt_smem + 248);
+    unsigned* bad_words = reinterpret_cast<unsigned*>(tt_smem + 256);                     // [TT_BAD][8]
+    float4* exchange = reinterpret_cast<float4*>(tt_smem + 512);                          // [128]: of the other group (two groups, one after the other: 2 KB each)
+    const unsigned smem_base = smem_u32(tt_smem);
+    const unsigned smem0 = (smem_base + 512u + 2u * 128u * 12u + 1023u) & ~1023u;
+    const unsigned q_s = smem0, k_s = q_s + 2u * C::TILE, v_s = k_s + ST * C::TILE;
+    auto bar_s = [&](int x) { return smem_base + 8u * x; };                  // S_X is in TMEM (tensor core commits)
+    auto bar_p = [&](int x) { return smem_base + 16u + 8u * x; };            // P_X is in TMEM, O_X rescaled (4 softmax warps)
+    auto bar_o = [&](int x) { return smem_base + 32u + 8u * x; };            // P V_X is done (tensor core commits)
+    const unsigned bar_q = smem_base + 48u, bar_vt = smem_base + 56u;        // the segment's Q is there (256 threads); a V tile that is looked at has come
+    auto bar_kf = [&](int st) { return smem_base + 64u + 8u * st; };         // stage holds a tile of keys (TMA bytes)
+    auto bar_kr = [&](int st) { return smem_base + 96u + 8u * st; };         // it has been read
+    auto bar_vf = [&](int st) { return smem_base + 128u + 8u * st; };
+    auto bar_vr = [&](int st) { return smem_base + 160u + 8u * st; };
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, j = blockIdx.x;
+    const int G = p.n_q / p.n_kv;
+
+    if (tid == 0) {
+        for (int x = 0; x < 2; ++x) { tc_mbar_init(bar_s(x), 1); tc_mbar_init(bar_p(x), 4); tc_mbar_init(bar_o(x), 1); }
+        for (int st = 0; st < ST; ++st) { tc_mbar_init(bar_kf(st), 1); tc_mbar_init(bar_kr(st), 1); tc_mbar_init(bar_vf(st), 1); tc_mbar_init(bar_vr(st), 1); }
+        tc_mbar_init(bar_q, 256); tc_mbar_init(bar_vt, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    }
+    if (warp == 0) {             // all 512 columns of tensor memory: S_A | S_B | O_A | O_B
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;\n" ::"r"(smem_u32(&tmem_base_s)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+    }
+    tc_fence_before();
+    pdl_launch_dependents();
+    pdl_wait();
+    pdl_after_wait();
+    TreeWalk<TT_ROWS, TT_KT> walk(p);
+    const bool stop = __syncthreads_or(*reinterpret_cast<volatile int*>(status) != 0) != 0;      // an earlier block gave up: do not pile up
+    const bool work = walk.begin(j, gridDim.x) && !stop && smem0 + C::SMEM <= smem_base + C::ALLOC;      // (a barrier of the block stands in begin)
+    __syncthreads();
+    tc_fence_after();
+    const unsigned tmem = tmem_base_s;
+    int fail = 0;
+    int4 record = make_int4(0, 0, 0, 0);
+
+    if (!work) {
+        if (tid == 0 && smem0 + C::SMEM > smem_base + C::ALLOC) atomicExch(status, 2);      // allocation not aligned as assumed
+    } else if (warp == 8 || warp == 9) {
+        // =========================== loaders: lane b brings box b
+        const bool is_k = warp == 8;
+        const CUtensorMap* map = is_k ? &kmap : &vmap;
+        const int n_box = TT_KT / tma_box;
+        unsigned vt_phase = 0, count = 0, seg = 0;
+        TreeSegment g;
+        for (; !fail && walk.next(g); ++seg) {
+            const int* bt = p.table + (size_t)g.r * p.table_stride;
+            if (!is_k) { if (lane < 8) bad_words[(seg % TT_BAD) * 8 + lane] = 0u; __syncwarp(); }
+            for (int t = g.t_lo; t < g.t_hi; ++t, ++count) {
+                const int st = count % ST, key0 = t * TT_KT, key_b = key0 + lane * tma_box;
+                int y = -1;                          // (a box that is not fetched)
+                if (lane < n_box && key_b < g.kv) {
+                    const int pi = tree_page(p, key_b), id = bt[pi];
+                    // a page outside the cache: rows ahead of the matrix, which TMA reads as zeros
+                    y = id >= 0 && id < p.pages ? (int)(((long long)id * p.n_kv + g.kvh) * p.page_size) + (key_b - pi * p.page_size) : -1024;
+                }
+                const unsigned n_act = __popc(__ballot_sync(0xffffffffu, y != -1));
+                const bool looked_at = !is_k && key0 + TT_KT > g.base;
+                if (count >= ST && __any_sync(0xffffffffu, !tc_mbar_wait(is_k ? bar_kr(st) : bar_vr(st), (count / ST - 1) & 1))) { fail = 1; break; }
+                const unsigned bar = looked_at ? bar_vt : (is_k ? bar_kf(st) : bar_vf(st)), dst_tile = (is_k ? k_s : v_s) + (unsigned)st * C::TILE;
+                if (lane == 0) tc_mbar_expect_tx(bar, n_act * H * (unsigned)tma_box * 128u);
+                __syncwarp();
+                if (y != -1) {
+                    const unsigned dst = dst_tile + (unsigned)(lane * tma_box) * 128u;
+#pragma unroll
+                    for (int h = 0; h < H; ++h) tc_tma_load(dst + h * TT_HALF, map, 64 * h, y, bar);
+                }
+                if (!looked_at) continue;
+                if (__any_sync(0xffffffffu, !tc_mbar_wait(bar_vt, vt_phase))) { fail = 1; ++count; break; }
+                vt_phase ^= 1u;
+                auto chunk_at = [&](int row, int c) { return dst_tile + tt_off(row, c); };
+                const int end = min(max(g.kv - key0, 0), TT_KT);             // rows that hold keys
+                for (int i = lane; i < (TT_KT - end) * H * 8; i += 32)
+                    asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};\n" ::"r"(chunk_at(end + i / (H * 8), i % (H * 8))), "r"(0u) : "memory");
+                const int first = min(max(g.base - key0, 0), end);           // the drafts among them
+                for (int i = lane; i < (end - first) * H * 8; i += 32) {
+                    const int row = first + i / (H * 8);
+                    const unsigned a = chunk_at(row, i % (H * 8));
+                    uint4 v;
+                    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+                    const unsigned bx = tt_nonfinite(v.x), by = tt_nonfinite(v.y), bz = tt_nonfinite(v.z), bw = tt_nonfinite(v.w);
+                    if ((bx | by | bz | bw) != 0u) {
+                        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};\n" ::"r"(a), "r"(v.x & ~bx), "r"(v.y & ~by), "r"(v.z & ~bz), "r"(v.w & ~bw) : "memory");
+                        const int draft = key0 + row - g.base;
+                        if (draft >= 0 && draft < 256) atomicOr(&bad_words[(seg % TT_BAD) * 8 + (draft >> 5)], 1u << (draft & 31));
+                    }
+                }
+                tc_fence_async_smem();
+                __syncwarp();
+                if (lane == 0) tc_mbar_arrive(bar_vf(st));
+            }
+        }
+        // nobody leaves with copies under way (values that are looked at have been waited for above)
+        for (unsigned c = count > ST ? count - ST : 0; c < count; ++c) tc_mbar_wait(is_k ? bar_kf(c % ST) : bar_vf(c % ST), (c / ST) & 1);
+    } else if (warp == 10) {
+        // =========================== issuer: one lane feeds the tensor core
+        if (lane == 0) {
+            const unsigned idesc_s = tc_idesc(false, TT_KT), idesc_o = tc_idesc(true, D);
+            unsigned long long dq[D / 16], dk[D / 16], dv[8];
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk) {
+                dq[kk] = tc_desc(q_s + (unsigned)(kk >> 2) * TT_HALF + (unsigned)(kk & 3) * 32u, 16, 1024);
+                dk[kk] = tc_desc(k_s + (unsigned)(kk >> 2) * TT_HALF + (unsigned)(kk & 3) * 32u, 16, 1024);
+            }
+#pragma unroll
+            for (int kk = 0; kk < 8; ++kk) dv[kk] = tc_desc(v_s + (unsigned)kk * 2048u, TT_HALF, 1024);
+            const unsigned long long step = (unsigned long long)(C::TILE >> 4);           // a tile further in a descriptor's address field
+            unsigned count = 0, seg = 0, phase_p[2] = {0u, 0u};                           // tiles before this segment
+            TreeSegment g;
+            bool ok = true;
+            for (; ok && walk.next(g); ++seg) {
+                const bool dual = g.rows > 128;
+                const int tiles = g.t_hi - g.t_lo, steps = dual ? 2 * tiles : tiles;
+                auto tile_of = [&](int s) { return count + (dual ? s >> 1 : s); };
+                auto issue_o = [&](int s) {                               // O_X += P_X V
+                    const int x = s & 1;
+                    const unsigned c = tile_of(s), st = c % ST;
+                    ok = tc_mbar_wait(bar_p(x), phase_p[x]);
+                    phase_p[x] ^= 1u;
+                    if (ok && (!dual || x == 0)) ok = tc_mbar_wait(bar_vf(st), (c / ST) & 1);
+                    if (!ok) return;
+                    tc_fence_async_smem(); tc_fence_after();
+#pragma unroll
+                    for (int kk = 0; kk < 8; ++kk)
+                        tc_mma_ta(tmem + 256u + (unsigned)x * 128u, tmem + (unsigned)x * 128u + kk * 8u, dv[kk] + st * step, idesc_o, (s < 2 && kk == 0) ? 0u : 1u);
+                    tc_commit(bar_o(x));
+                    if (!dual || x == 1) tc_commit(bar_vr(st));
+                };
+                ok = tc_mbar_wait(bar_q, seg & 1);
+                for (int s = 0; s < steps && ok; ++s) {
+                    const int x = s & 1;
+                    const unsigned c = tile_of(s), st = c % ST;
+                    if (!dual || x == 0) ok = tc_mbar_wait(bar_kf(st), (c / ST) & 1);
+                    if (!ok) break;
+                    tc_fence_async_smem(); tc_fence_after();
+                    const unsigned long long qx = dual && x ? step : 0ull;
+#pragma unroll
+                    for (int kk = 0; kk < D / 16; ++kk) tc_mma(tmem + (unsigned)x * 128u, dq[kk] + qx, dk[kk] + st * step, idesc_s, kk > 0 ? 1u : 0u);
+                    tc_commit(bar_s(x));
+                    if (!dual || x == 1) tc_commit(bar_kr(st));
+                    if (s >= 1) issue_o(s - 1);
+                }
+                if (ok) issue_o(steps - 1);
+                count += tiles;
+            }
+            if (!ok) fail = 1;
+        }
+    } else if (warp < 8) {
+        // =========================== softmax: group x = warp / 4; thread r of a group owns its row r
+        const int x = warp >> 2, lane_row = tid & 127;
+        const unsigned lane_sel = (unsigned)((warp & 3) * 32) << 16;
+        const unsigned ts = tmem + (unsigned)x * 128u + lane_sel, to = tmem + 256u + (unsigned)x * 128u + lane_sel;
+        unsigned phase_s = 0, phase_o = 0, seg = 0;
+        const float sc = p.scale_log2;
+        const __nv_bfloat16* qg = reinterpret_cast<const __nv_bfloat16*>(p.q);
+        TreeSegment g;
+        for (; walk.next(g); ++seg) {
+            const bool dual = g.rows > 128;
+            // ---- Q: 16-byte chunks over all 256 threads; rows without a query are zero
+            for (int i = tid; i < (dual ? 256 : 128) * H * 8; i += 256) {
+                const int row = i / (H * 8), c = i % (H * 8), rr = g.row0 + row;
+                const bool valid = row < g.rows;
+                const __nv_bfloat16* src = valid ? qg + ((size_t)(g.tok0 + rr / G) * p.n_q + (size_t)g.kvh * G + rr % G) * D + c * 8 : qg;
+                tt_cp_async16(q_s + (unsigned)(row >> 7) * C::TILE + tt_off(row & 127, c), src, valid);
+            }
+            tc_cp_async_arrive(bar_q);
+
+            const int tiles = g.t_hi - g.t_lo, n_mine = dual ? tiles : (tiles + 1 - x) >> 1;
+            const int row = dual ? x * 128 + lane_row : lane_row, rr = g.row0 + row;
+            const bool valid = row < g.rows, active = row - lane < g.rows;               // whether the row, and any of the warp's, exists
+            const size_t tok = (size_t)g.tok0 + (valid ? rr / G : 0);
+            const unsigned* row_mask = p.mask + tok * p.words;
+            float m_run = -INFINITY, l_run = 0.f, o_scale = 1.f;
+            for (int it = 0; it < n_mine && !fail; ++it) {
+                if (__any_sync(0xffffffffu, !tc_mbar_wait(bar_s(x), phase_s))) { fail = 1; break; }
+                phase_s ^= 1u;
+                tc_fence_after();
+                if (!active) {                       // P of rows that do not exist may be anything
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) tc_mbar_arrive(bar_p(x));
+                    continue;
+                }
+                const int key0 = (g.t_lo + (dual ? it : 2 * it + x)) * TT_KT;
+                float s0[32], s1[32], s2[32], s3[32];
+                tc_ld32(ts, s0); tc_ld32(ts + 32, s1); tc_ld32(ts + 64, s2); tc_ld32(ts + 96, s3);
+                tc_wait_ld(s0); tc_wait_ld(s1); tc_wait_ld(s2); tc_wait_ld(s3);
+                if (key0 + TT_KT > g.base) {
+                    auto mask = [&](float (&sv)[32], int cb) {
+                        const unsigned seen = tree_seen(row_mask, p.words, key0 + 32 * cb, g.base, g.kv);
+#pragma unroll
+                        for (int e = 0; e < 32; ++e)
+                            if (!(seen >> e & 1u)) sv[e] = -INFINITY;
+                    };
+                    mask(s0, 0); mask(s1, 1); mask(s2, 2); mask(s3, 3);
+                }
+                auto row_max = [&]() -> float {
+                    float c8[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) c8[e] = fmaxf(fmaxf(s0[e], s1[e]), fmaxf(s2[e], s3[e]));
+#pragma unroll
+                    for (int e = 8; e < 32; ++e) c8[e & 7] = fmaxf(c8[e & 7], fmaxf(fmaxf(s0[e], s1[e]), fmaxf(s2[e], s3[e])));
+                    return fmaxf(fmaxf(fmaxf(c8[0], c8[1]), fmaxf(c8[2], c8[3])), fmaxf(fmaxf(c8[4], c8[5]), fmaxf(c8[6], c8[7]))) * sc;
+                };
+                auto move_reference = [&](float m_new) {
+                    const float a = fast_exp2(m_run - m_new);                // 0 for the first
+                    m_run = m_new;
+                    l_run *= a;
+                    o_scale *= a;
+                };
+                if (__any_sync(0xffffffffu, m_run == -INFINITY)) {
+                    const float cm = row_max();
+                    if (m_run == -INFINITY && cm > -INFINITY) move_reference(cm);
+                }
+                auto rescale_o = [&]() {             // (P V of this group's tile before is done: this S was issued after it)
+                    if (it >= 1 && __any_sync(0xffffffffu, o_scale != 1.f)) {
+#pragma unroll 1
+                        for (int cb = 0; cb < D / 32; ++cb) {
+                            float v0[32];
+                            tc_ld32(to + cb * 32, v0);
+                            tc_wait_ld(v0);
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) v0[e] *= o_scale;
+                            tc_st32(to + cb * 32, v0);
+                        }
+                    }
+                    o_scale = 1.f;
+                };
+                rescale_o();
+                float tile_sum;
+                auto exponentials = [&]() {
+                    const float mu = (m_run == -INFINITY) ? 0.f : m_run;
+                    const unsigned long long sc2 = tt_pack(sc, sc), nmu2 = tt_pack(-mu, -mu);
+                    unsigned long long sum2[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) sum2[e] = 0ull;              // (0.f, 0.f)
+                    auto expo = [&](const float (&sv)[32], int cb) {
+                        unsigned pk[16];
+#pragma unroll
+                        for (int e = 0; e < 32; e += 2) {
+                            float x0, x1;
+                            tt_unpack(tt_fma(tt_pack(sv[e], sv[e + 1]), sc2, nmu2), x0, x1);
+                            const float e0 = fast_exp2(x0), e1 = fast_exp2(x1);
+                            sum2[(e >> 1) & 7] = tt_add(sum2[(e >> 1) & 7], tt_pack(e0, e1));
+                            pk[e >> 1] = pack_bf16(e0, e1);
+                        }
+                        tc_st16(ts + cb * 16, pk);
+                    };
+                    expo(s0, 0); expo(s1, 1); expo(s2, 2); expo(s3, 3);
+                    const unsigned long long t4 = tt_add(tt_add(tt_add(sum2[0], sum2[1]), tt_add(sum2[2], sum2[3])),
+                                                         tt_add(tt_add(sum2[4], sum2[5]), tt_add(sum2[6], sum2[7])));
+                    float lo, hi;
+                    tt_unpack(t4, lo, hi);
+                    tile_sum = lo + hi;
+                };
+                exponentials();
+                if (__any_sync(0xffffffffu, !(tile_sum < 1.0e30f))) {        // overflow (inf, or NaN from inf - inf): again, from the maximum
+                    const float cm = row_max();
+                    if (cm > m_run) move_reference(cm);
+                    rescale_o();
+                    tc_wait_st();
+                    exponentials();
+                }
+                l_run += tile_sum;
+                if (tile_sum > 65536.f) move_reference(m_run + log2f(tile_sum));         // takes effect with the next tile (O: before its product)
+                tc_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) tc_mbar_arrive(bar_p(x));
+            }
+            // ---- the segment's end
+            if (n_mine > 0) {
+                if (!fail && __any_sync(0xffffffffu, !tc_mbar_wait(bar_o(x), (phase_o + n_mine - 1) & 1))) fail = 1;
+                phase_o += n_mine;
+                tc_fence_after();
+            }
+            float fa = o_scale, fb = 0.f, m_all = m_run, l_all = l_run;      // factors of O_A and O_B (dual: of the group's own alone)
+            if (!dual) {                             // both groups meet here, also where one of them has given up
+                float* ex = reinterpret_cast<float*>(exchange);              // [2][3][128]
+                ex[(x * 3 + 0) * 128 + lane_row] = m_run;
+                ex[(x * 3 + 1) * 128 + lane_row] = l_run;
+                ex[(x * 3 + 2) * 128 + lane_row] = o_scale;
+                tc_fence_before();
+                asm volatile("bar.sync 1, 256;\n" ::: "memory");
+                tc_fence_after();
+                const float ma = ex[lane_row], la = ex[128 + lane_row], oa = ex[256 + lane_row], mb = ex[384 + lane_row], lb = ex[512 + lane_row], ob = ex[640 + lane_row];
+                m_all = fmaxf(ma, mb);
+                const float mu = m_all == -INFINITY ? 0.f : m_all, wa = fast_exp2(ma - mu), wb = fast_exp2(mb - mu);
+                l_all = la * wa + lb * wb;
+                fa = wa * oa;
+                fb = wb * ob;
+            }
+            if (active && !fail) {
+                const bool whole = g.t_lo == 0 && g.t_hi == g.tiles;
+                const float inv = whole ? (l_all > 0.f ? 1.f / l_all : (l_all == l_all ? 0.f : l_all)) : 1.f;
+                const unsigned* bad = bad_words + (seg % TT_BAD) * 8;
+                unsigned any_bad = 0u;
+#pragma unroll
+                for (int w = 0; w < 8; ++w) any_bad |= *reinterpret_cast<const volatile unsigned*>(bad + w);
+                const int slot = 2 * j + (g.t_lo == 0 ? 1 : 0);
+                const int cb0 = dual ? 0 : x * (D / 64), cb1 = dual ? D / 32 : cb0 + D / 64;      // blocks of 32 columns: both groups share them out
+                const bool two = !dual && tiles > 1;
+                __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(p.out) + (tok * p.n_q + (size_t)g.kvh * G + (valid ? rr % G : 0)) * D;
+                float* part = p.part_o + ((size_t)slot * TT_ROWS + row) * D;
+                const unsigned t_own = dual ? to : tmem + 256u + lane_sel, t_other = tmem + 384u + lane_sel;
+#pragma unroll 1
+                for (int cb = cb0; cb < cb1; ++cb) {
+                    float v[32];
+                    tc_ld32(t_own + cb * 32, v);
+                    tc_wait_ld(v);
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) v[e] *= fa;
+                    if (two) {
+                        float u[32];
+                        tc_ld32(t_other + cb * 32, u);
+                        tc_wait_ld(u);
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) v[e] = fmaf(u[e], fb, v[e]);
+                    }
+                    if (any_bad != 0u && valid) {    // what was taken out of the values of drafts that this row sees
+                        for (int w = 0; w < 8; ++w)
+                            for (unsigned left = w < p.words ? row_mask[w] & *reinterpret_cast<const volatile unsigned*>(bad + w) : 0u; left; left &= left - 1u) {
+                                const int key = g.base + 32 * w + __ffs(left) - 1, pi = tree_page(p, key);
+                                const __nv_bfloat16* src = reinterpret_cast<const __nv_bfloat16*>(p.v_cache) +
+                                    (((size_t)p.table[(size_t)g.r * p.table_stride + pi] * p.n_kv + g.kvh) * p.page_size + (key - pi * p.page_size)) * D + cb * 32;
+#pragma unroll
+                                for (int e = 0; e < 32; ++e) {
+                                    const float f = __bfloat162float(src[e]);
+                                    if (!(fabsf(f) < INFINITY)) v[e] += f;
+                                }
+                            }
+                    }
+                    if (valid && whole) {
+#pragma unroll
+                        for (int e = 0; e < 32; e += 8)
+                            *reinterpret_cast<uint4*>(dst + cb * 32 + e) = make_uint4(pack_bf16(v[e] * inv, v[e + 1] * inv), pack_bf16(v[e + 2] * inv, v[e + 3] * inv),
+                                                                                      pack_bf16(v[e + 4] * inv, v[e + 5] * inv), pack_bf16(v[e + 6] * inv, v[e + 7] * inv));
+                    } else if (valid) {
+#pragma unroll
+                        for (int e = 0; e < 32; e += 4) *reinterpret_cast<float4*>(part + cb * 32 + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+                    }
+                }
+                if (valid && !whole && (dual || x == 0)) *reinterpret_cast<float2*>(p.part_ml + ((size_t)slot * TT_ROWS + row) * 2) = make_float2(m_all, l_all);
+                if (tid == 0 && !whole && g.t_lo == 0) record = make_int4(g.r, g.item, walk.pieces(g, j), g.rows);
+            }
+            tc_fence_before();
+            asm volatile("bar.sync 1, 256;\n" ::: "memory");                 // Q, the exchange and both accumulators are free
+        }
+    }
+    if (tid == 0) p.record[j] = record;
+    tc_fence_before();
+    const bool failed = __syncthreads_or(fail) != 0;
+    tc_fence_after();
+    if (failed && tid == 0) atomicExch(status, 1);
+    if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;\n" ::"r"(tmem) : "memory");
+}

@@ -2424,7 +2424,8 @@ def _draft_lib():
         lib = _build.drafts_library()
         lib.msgl_draft_plan.argtypes = [c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p] + [c_int] * 5 + [c_void_p] * 7
         lib.msgl_draft_accept.argtypes = [c_void_p] * 4 + [c_int] * 3 + [c_void_p] * 5 + [c_int] * 3 + [c_ll, c_int, c_int, c_void_p, c_int, c_int, c_void_p]
-        lib.msgl_tree_attention.argtypes = [c_void_p] * 8 + [c_int] * 9 + [c_ll, c_float] + [c_void_p] * 3 + [c_int, c_int, c_void_p]
+        lib.msgl_tree_attention.argtypes = [c_void_p] * 8 + [c_int] * 9 + [c_ll, c_float] + [c_void_p] * 3 + [c_int] * 3 + [c_void_p, c_int, c_void_p]
+        lib.msgl_tree_attention_tensor.argtypes = [c_int, c_int, c_ll, c_int]
         lib.msgl_token_logprobs.argtypes = [c_void_p, c_int, c_int, c_ll, c_void_p, c_int] + [c_void_p] * 4 + [c_int] * 3 + [c_void_p]
         _drafts = lib
     return _drafts
@@ -2523,14 +2524,22 @@ def tree_attention(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_
     _same_device(what, q, out, k_cache, v_cache, q_start, kv_len, block_table, mask)
     if T == 0 or B == 0:
         return
-    lib = _draft_lib()
-    blocks, rows = lib.msgl_tree_attention_blocks(d), lib.msgl_tree_attention_rows()
-    part = torch.empty(2 * blocks * rows * (d + 2) + 4 * blocks, dtype=torch.float32, device=q.device)
-    at = part.data_ptr()
-    part_ml, record = at + 4 * 2 * blocks * rows * d, at + 4 * 2 * blocks * rows * (d + 2)
-    code = lib.msgl_tree_attention(q.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), q_start.data_ptr(), kv_len.data_ptr(), block_table.data_ptr(),
-                                   mask.data_ptr(), B, T, n_q, n_kv, d, page_size, block_table.stride(0), width, words, k_cache.shape[0], float(scale), at, part_ml, record,
-                                   blocks, _DT[q.dtype], _stream())
+    lib, pages = _draft_lib(), k_cache.shape[0]
+    max_rows = max_draft * (n_q // n_kv)
+    # (the status words are made for the first device; none in a stream capture that comes before them)
+    status = _status_words(q.device) if lib.msgl_tree_attention_tensor(d, page_size, pages * n_kv * page_size, _DT[q.dtype]) else None
+    if status is not None and (status.get_device() != q.get_device() or (q.data_ptr() | out.data_ptr() | k_cache.data_ptr() | v_cache.data_ptr()) & 15):
+        status = None
+    for tensor in (1, 0) if status is not None else (0,):
+        blocks, rows = lib.msgl_tree_attention_blocks(d, tensor), lib.msgl_tree_attention_rows(tensor)
+        part = torch.empty(2 * blocks * rows * (d + 2) + 4 * blocks, dtype=torch.float32, device=q.device)
+        at = part.data_ptr()
+        part_ml, record = at + 4 * 2 * blocks * rows * d, at + 4 * 2 * blocks * rows * (d + 2)
+        code = lib.msgl_tree_attention(q.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), q_start.data_ptr(), kv_len.data_ptr(), block_table.data_ptr(),
+                                       mask.data_ptr(), B, T, n_q, n_kv, d, page_size, block_table.stride(0), width, words, pages, float(scale), at, part_ml, record,
+                                       blocks, max_rows, tensor, _ptr(status), _DT[q.dtype], _stream())
+        if code != 2:             # (2: no tensor map of this layout)
+            break
     _check(code, what)
     global LAUNCHES
     LAUNCHES += 1                # the join of cut items is a kernel of its own
