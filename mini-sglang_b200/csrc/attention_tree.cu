@@ -59,6 +59,8 @@ struct TreeSegment {              // tiles [t_lo, t_hi) of one item
     int t_lo, t_hi, tiles;
 };
 
+struct TreeWalkState { long long total, x_lo, x_hi, start; int blocks, r, item; };      // (a walk put aside)
+
 template <int ROWS, int KT>
 struct TreeWalk {
     const TreeParams& p;
@@ -68,6 +70,8 @@ struct TreeWalk {
     long long start = 0;          // where the request's first item starts
 
     __device__ __forceinline__ TreeWalk(const TreeParams& q) : p(q) {}
+    __device__ __forceinline__ void store(TreeWalkState& s) const { s.total = total; s.x_lo = x_lo; s.x_hi = x_hi; s.start = start; s.blocks = blocks; s.r = r; s.item = item; }
+    __device__ __forceinline__ void load(const TreeWalkState& s) { total = s.total; x_lo = s.x_lo; x_hi = s.x_hi; start = s.start; blocks = s.blocks; r = s.r; item = s.item; }
     struct Request { int tok0, n, kv, tiles, items; };
     __device__ __forceinline__ Request request(int i) const {
         Request w;

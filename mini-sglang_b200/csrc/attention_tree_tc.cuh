@@ -27,11 +27,12 @@
 //
 // Every wait is bounded; a block that gives up sets the status word, waits for its copies, frees its tensor memory and returns.
 //
-// Warps: 0-3 softmax A, 4-7 softmax B (both also fetch Q), 8 keys, 9 values, 10 issuer, 11 idle.
+// Warps: 0-3 softmax A, 4-7 softmax B (both also fetch Q), 8 keys, 9 values, 10 issuer.  What the softmax warps know of their segments stands in
+// shared memory: with 128 scores a thread there is no register for it (spilled, it doubled the time of a tile).
 #pragma once
 #include "tc_common.cuh"
 
-constexpr int TT_ROWS = 256, TT_KT = 128, TT_THREADS = 384;
+constexpr int TT_ROWS = 256, TT_KT = 128, TT_THREADS = 352;
 constexpr unsigned TT_HALF = 128u * 128u;            // 128 rows of 64 columns, 128-byte swizzle: 16 KB
 constexpr int TT_BAD = 8;                            // segments whose non-numbers are remembered: more than the loaders run ahead
 
@@ -82,6 +83,9 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const TreeParams
     unsigned& tmem_base_s = *reinterpret_cast<unsigned*>(tt_smem + 248);
     unsigned* bad_words = reinterpret_cast<unsigned*>(tt_smem + 256);                     // [TT_BAD][8]
     float4* exchange = reinterpret_cast<float4*>(tt_smem + 512);                          // [128]: of the other group (two groups, one after the other: 2 KB each)
+    __shared__ TreeSegment sh_seg[2];                // the softmax groups' segment and the one after it
+    __shared__ bool sh_more[2];
+    __shared__ TreeWalkState sh_walk;
     const unsigned smem_base = smem_u32(tt_smem);
     const unsigned smem0 = (smem_base + 512u + 2u * 128u * 12u + 1023u) & ~1023u;
     const unsigned q_s = smem0, k_s = q_s + 2u * C::TILE, v_s = k_s + ST * C::TILE;
@@ -237,10 +241,23 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const TreeParams
         const unsigned ts = tmem + (unsigned)x * 128u + lane_sel, to = tmem + 256u + (unsigned)x * 128u + lane_sel;
         unsigned phase_s = 0, phase_o = 0, seg = 0;
         const float sc = p.scale_log2;
-        const __nv_bfloat16* qg = reinterpret_cast<const __nv_bfloat16*>(p.q);
-        TreeSegment g;
-        for (; walk.next(g); ++seg) {
+        auto find = [&](unsigned s) {                // (one thread)
+            walk.load(sh_walk);
+            TreeSegment w;
+            const bool more = walk.next(w);
+            if (more) sh_seg[s & 1] = w;
+            sh_more[s & 1] = more;
+            walk.store(sh_walk);
+        };
+        if (tid == 0) {
+            walk.store(sh_walk);
+            find(0);
+        }
+        asm volatile("bar.sync 1, 256;\n" ::: "memory");
+        for (; *reinterpret_cast<volatile bool*>(&sh_more[seg & 1]); ++seg) {
+            const TreeSegment& g = sh_seg[seg & 1];
             const bool dual = g.rows > 128;
+            const __nv_bfloat16* qg = reinterpret_cast<const __nv_bfloat16*>(p.q);
             // ---- Q: 16-byte chunks over all 256 threads; rows without a query are zero
             for (int i = tid; i < (dual ? 256 : 128) * H * 8; i += 256) {
                 const int row = i / (H * 8), c = i % (H * 8), rr = g.row0 + row;
@@ -249,12 +266,19 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const TreeParams
                 tt_cp_async16(q_s + (unsigned)(row >> 7) * C::TILE + tt_off(row & 127, c), src, valid);
             }
             tc_cp_async_arrive(bar_q);
+            const bool cut = g.t_lo != 0 || g.t_hi != g.tiles;
+            if (tid == 0) {
+                if (cut && g.t_lo == 0) {
+                    walk.load(sh_walk);
+                    record = make_int4(g.r, g.item, walk.pieces(g, j), g.rows);
+                }
+                find(seg + 1);                       // (the segment before the present one has been left by all)
+            }
 
             const int tiles = g.t_hi - g.t_lo, n_mine = dual ? tiles : (tiles + 1 - x) >> 1;
             const int row = dual ? x * 128 + lane_row : lane_row, rr = g.row0 + row;
             const bool valid = row < g.rows, active = row - lane < g.rows;               // whether the row, and any of the warp's, exists
             const size_t tok = (size_t)g.tok0 + (valid ? rr / G : 0);
-            const unsigned* row_mask = p.mask + tok * p.words;
             float m_run = -INFINITY, l_run = 0.f, o_scale = 1.f;
             for (int it = 0; it < n_mine && !fail; ++it) {
                 if (__any_sync(0xffffffffu, !tc_mbar_wait(bar_s(x), phase_s))) { fail = 1; break; }
@@ -271,6 +295,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const TreeParams
                 tc_ld32(ts, s0); tc_ld32(ts + 32, s1); tc_ld32(ts + 64, s2); tc_ld32(ts + 96, s3);
                 tc_wait_ld(s0); tc_wait_ld(s1); tc_wait_ld(s2); tc_wait_ld(s3);
                 if (key0 + TT_KT > g.base) {
+                    const unsigned* row_mask = p.mask + tok * p.words;
                     auto mask = [&](float (&sv)[32], int cb) {
                         const unsigned seen = tree_seen(row_mask, p.words, key0 + 32 * cb, g.base, g.kv);
 #pragma unroll
@@ -316,9 +341,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const TreeParams
                 auto exponentials = [&]() {
                     const float mu = (m_run == -INFINITY) ? 0.f : m_run;
                     const unsigned long long sc2 = tt_pack(sc, sc), nmu2 = tt_pack(-mu, -mu);
-                    unsigned long long sum2[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) sum2[e] = 0ull;              // (0.f, 0.f)
+                    unsigned long long sum2[4] = {0ull, 0ull, 0ull, 0ull};   // (0.f, 0.f)
                     auto expo = [&](const float (&sv)[32], int cb) {
                         unsigned pk[16];
 #pragma unroll
@@ -326,16 +349,14 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const TreeParams
                             float x0, x1;
                             tt_unpack(tt_fma(tt_pack(sv[e], sv[e + 1]), sc2, nmu2), x0, x1);
                             const float e0 = fast_exp2(x0), e1 = fast_exp2(x1);
-                            sum2[(e >> 1) & 7] = tt_add(sum2[(e >> 1) & 7], tt_pack(e0, e1));
+                            sum2[(e >> 1) & 3] = tt_add(sum2[(e >> 1) & 3], tt_pack(e0, e1));
                             pk[e >> 1] = pack_bf16(e0, e1);
                         }
                         tc_st16(ts + cb * 16, pk);
                     };
                     expo(s0, 0); expo(s1, 1); expo(s2, 2); expo(s3, 3);
-                    const unsigned long long t4 = tt_add(tt_add(tt_add(sum2[0], sum2[1]), tt_add(sum2[2], sum2[3])),
-                                                         tt_add(tt_add(sum2[4], sum2[5]), tt_add(sum2[6], sum2[7])));
                     float lo, hi;
-                    tt_unpack(t4, lo, hi);
+                    tt_unpack(tt_add(tt_add(sum2[0], sum2[1]), tt_add(sum2[2], sum2[3])), lo, hi);
                     tile_sum = lo + hi;
                 };
                 exponentials();
@@ -376,7 +397,8 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const TreeParams
                 fb = wb * ob;
             }
             if (active && !fail) {
-                const bool whole = g.t_lo == 0 && g.t_hi == g.tiles;
+                const bool whole = !cut;
+                const unsigned* row_mask = p.mask + tok * p.words;
                 const float inv = whole ? (l_all > 0.f ? 1.f / l_all : (l_all == l_all ? 0.f : l_all)) : 1.f;
                 const unsigned* bad = bad_words + (seg % TT_BAD) * 8;
                 unsigned any_bad = 0u;
@@ -426,7 +448,6 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const TreeParams
                     }
                 }
                 if (valid && !whole && (dual || x == 0)) *reinterpret_cast<float2*>(p.part_ml + ((size_t)slot * TT_ROWS + row) * 2) = make_float2(m_all, l_all);
-                if (tid == 0 && !whole && g.t_lo == 0) record = make_int4(g.r, g.item, walk.pieces(g, j), g.rows);
             }
             tc_fence_before();
             asm volatile("bar.sync 1, 256;\n" ::: "memory");                 // Q, the exchange and both accumulators are free
