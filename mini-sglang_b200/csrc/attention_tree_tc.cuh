@@ -4,8 +4,8 @@
 // against tiles of 128 keys.
 //
 //     S = Q K^T     tcgen05.mma 128 x 128 x 16, operands in shared memory, accumulator in tensor memory
-//     softmax       thread t of a group of four warps owns row t = TMEM lane t, with the row's 128 scores in registers; P, rounded to
-//                   bfloat16 (half a step, 2^-9, of each weight; the sum of the weights is taken before), goes back over the columns of S
+//     softmax       two threads a row (TMEM lane), 64 scores each in registers; P, rounded to bfloat16 (half a step, 2^-9, of each weight;
+//                   the sum of the weights is taken before), goes back over the columns of S
 //     O += P V      tcgen05.mma 128 x D x 16, P from tensor memory, V from shared memory as it lies in the cache
 //
 // The products of a tile keep the tensor core about as busy as its exponentials the special-function units, and one follows the other for
@@ -22,17 +22,20 @@
 // key are cleared (free slots may hold anything), and elements that are no numbers are cleared and remembered, since 0 x inf would reach
 // drafts that do not see them; the drafts that do see them get them back at the end.
 //
-// The exponentials' reference m need not be a row's maximum: it is found for a row's first tile and moved where a tile's sum shows that it
-// fell behind by 2^16 or the exponentials overflowed (then the tile is done again).  Whenever it moves, O is scaled in tensor memory.
+// The exponentials' reference m need not be a row's maximum: it moves where a tile's maximum is 2^8 above it, and O is scaled in tensor
+// memory then.  The two threads of a row meet once a tile, over the maximum, when both have their scores in registers (P of the one
+// lies over scores of the other), so they move alike.
 //
 // Every wait is bounded; a block that gives up sets the status word, waits for its copies, frees its tensor memory and returns.
 //
-// Warps: 0-3 softmax A, 4-7 softmax B (both also fetch Q), 8 keys, 9 values, 10 issuer.  What the softmax warps know of their segments stands in
-// shared memory: with 128 scores a thread there is no register for it (spilled, it doubled the time of a tile).
+// Warps: 0-7 softmax A, 8-15 softmax B (all also fetch Q), 16 keys, 17 values, 18 issuer.  A softmax warp w works on TMEM lanes 32 (w % 4) .., and
+// on the half (w / 4) % 2 of a tile's keys and of O's columns.  With one thread a row and 128 scores each a tile of 256 rows took 2.7 us, half
+// of it waiting for the next scores: the softmax of a tile is what its successor waits for, and so it is spread over twice the warps.
+// What the softmax warps know of their segments stands in shared memory: there is no register for it.
 #pragma once
 #include "tc_common.cuh"
 
-constexpr int TT_ROWS = 256, TT_KT = 128, TT_THREADS = 352;
+constexpr int TT_ROWS = 256, TT_KT = 128, TT_THREADS = 608, TT_SOFT = 512;
 constexpr unsigned TT_HALF = 128u * 128u;            // 128 rows of 64 columns, 128-byte swizzle: 16 KB
 constexpr int TT_BAD = 8;                            // segments whose non-numbers are remembered: more than the loaders run ahead
 
@@ -40,7 +43,7 @@ template <int D> struct TreeTc {
     static constexpr int H = D / 64, ST = D == 128 ? 2 : 4;                                       // halves of a row, stages of a ring
     static constexpr unsigned TILE = H * TT_HALF;
     static constexpr unsigned SMEM = 2u * TILE + 2u * ST * TILE;                                  // Q_A, Q_B, keys, values
-    static constexpr unsigned ALLOC = SMEM + 1024u + 4096u;                                       // barriers and scalars ahead, alignment
+    static constexpr unsigned ALLOC = SMEM + 1024u + 512u + 1280u * 4u;                           // barriers, scalars and exchange ahead, alignment
 };
 
 // two float32 values in one 64-bit register, for the packed float32 instructions of sm_100
@@ -72,6 +75,27 @@ __device__ __forceinline__ unsigned tt_nonfinite(unsigned w) {               // 
     return ((w & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) | ((w & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u);
 }
 
+// The products are issued by a whole warp, converged, one lane of which is elected: what they take then stands in uniform registers.  From a branch of
+// a single lane every operand had to be moved there by itself, and a 128 x 128 x 16 product (64 cycles) took 118.
+__device__ __forceinline__ unsigned tt_elect() {
+    unsigned leader;
+    asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(leader));
+    return leader;
+}
+__device__ __forceinline__ void tt_mma(unsigned leader, unsigned d_tmem, unsigned long long a_desc, unsigned long long b_desc, unsigned idesc, unsigned accumulate) {
+    asm volatile("{\n.reg .pred p, q;\nsetp.ne.b32 p, %4, 0;\nsetp.ne.b32 q, %5, 0;\n"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n"
+                 ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(leader) : "memory");
+}
+__device__ __forceinline__ void tt_mma_ta(unsigned leader, unsigned d_tmem, unsigned a_tmem, unsigned long long b_desc, unsigned idesc, unsigned accumulate) {
+    asm volatile("{\n.reg .pred p, q;\nsetp.ne.b32 p, %4, 0;\nsetp.ne.b32 q, %5, 0;\n"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n"
+                 ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(leader) : "memory");
+}
+__device__ __forceinline__ void tt_commit(unsigned leader, unsigned bar) {
+    asm volatile("{\n.reg .pred q;\nsetp.ne.b32 q, %1, 0;\n@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(bar), "r"(leader) : "memory");
+}
+
 // tma_box: rows of a TMA box, min(page_size, 128)
 template <int D>
 __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const TreeParams p, int* status, const __grid_constant__ CUtensorMap kmap,
@@ -79,20 +103,20 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const TreeParams
     using C = TreeTc<D>;
     constexpr int ST = C::ST, H = C::H;
     extern __shared__ __align__(16) unsigned char tt_smem[];
-    // the first 4 KB: barriers, scalars, the non-numbers' words, the rows' sums that groups A and B exchange
+    // ahead of the tiles: barriers, scalars, the non-numbers' words, what the rows' threads exchange
     unsigned& tmem_base_s = *reinterpret_cast<unsigned*>(tt_smem + 248);
     unsigned* bad_words = reinterpret_cast<unsigned*>(tt_smem + 256);                     // [TT_BAD][8]
-    float4* exchange = reinterpret_cast<float4*>(tt_smem + 512);                          // [128]: of the other group (two groups, one after the other: 2 KB each)
+    float* exchange = reinterpret_cast<float*>(tt_smem + 512);                            // [2 groups][2 halves][128] maxima, the same of sums, [2][128] references
     __shared__ TreeSegment sh_seg[2];                // the softmax groups' segment and the one after it
     __shared__ bool sh_more[2];
     __shared__ TreeWalkState sh_walk;
     const unsigned smem_base = smem_u32(tt_smem);
-    const unsigned smem0 = (smem_base + 512u + 2u * 128u * 12u + 1023u) & ~1023u;
+    const unsigned smem0 = (smem_base + 512u + 1280u * 4u + 1023u) & ~1023u;
     const unsigned q_s = smem0, k_s = q_s + 2u * C::TILE, v_s = k_s + ST * C::TILE;
     auto bar_s = [&](int x) { return smem_base + 8u * x; };                  // S_X is in TMEM (tensor core commits)
-    auto bar_p = [&](int x) { return smem_base + 16u + 8u * x; };            // P_X is in TMEM, O_X rescaled (4 softmax warps)
+    auto bar_p = [&](int x) { return smem_base + 16u + 8u * x; };            // P_X is in TMEM, O_X rescaled (8 softmax warps)
     auto bar_o = [&](int x) { return smem_base + 32u + 8u * x; };            // P V_X is done (tensor core commits)
-    const unsigned bar_q = smem_base + 48u, bar_vt = smem_base + 56u;        // the segment's Q is there (256 threads); a V tile that is looked at has come
+    const unsigned bar_q = smem_base + 48u, bar_vt = smem_base + 56u;        // the segment's Q is there (512 threads); a V tile that is looked at has come
     auto bar_kf = [&](int st) { return smem_base + 64u + 8u * st; };         // stage holds a tile of keys (TMA bytes)
     auto bar_kr = [&](int st) { return smem_base + 96u + 8u * st; };         // it has been read
     auto bar_vf = [&](int st) { return smem_base + 128u + 8u * st; };
@@ -101,9 +125,9 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const TreeParams
     const int G = p.n_q / p.n_kv;
 
     if (tid == 0) {
-        for (int x = 0; x < 2; ++x) { tc_mbar_init(bar_s(x), 1); tc_mbar_init(bar_p(x), 4); tc_mbar_init(bar_o(x), 1); }
+        for (int x = 0; x < 2; ++x) { tc_mbar_init(bar_s(x), 1); tc_mbar_init(bar_p(x), 8); tc_mbar_init(bar_o(x), 1); }
         for (int st = 0; st < ST; ++st) { tc_mbar_init(bar_kf(st), 1); tc_mbar_init(bar_kr(st), 1); tc_mbar_init(bar_vf(st), 1); tc_mbar_init(bar_vr(st), 1); }
-        tc_mbar_init(bar_q, 256); tc_mbar_init(bar_vt, 1);
+        tc_mbar_init(bar_q, TT_SOFT); tc_mbar_init(bar_vt, 1);
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
     if (warp == 0) {             // all 512 columns of tensor memory: S_A | S_B | O_A | O_B
@@ -125,9 +149,9 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const TreeParams
 
     if (!work) {
         if (tid == 0 && smem0 + C::SMEM > smem_base + C::ALLOC) atomicExch(status, 2);      // allocation not aligned as assumed
-    } else if (warp == 8 || warp == 9) {
+    } else if (warp == 16 || warp == 17) {
         // =========================== loaders: lane b brings box b
-        const bool is_k = warp == 8;
+        const bool is_k = warp == 16;
         const CUtensorMap* map = is_k ? &kmap : &vmap;
         const int n_box = TT_KT / tma_box;
         unsigned vt_phase = 0, count = 0, seg = 0;
@@ -181,64 +205,65 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const TreeParams
         }
         // nobody leaves with copies under way (values that are looked at have been waited for above)
         for (unsigned c = count > ST ? count - ST : 0; c < count; ++c) tc_mbar_wait(is_k ? bar_kf(c % ST) : bar_vf(c % ST), (c / ST) & 1);
-    } else if (warp == 10) {
-        // =========================== issuer: one lane feeds the tensor core
-        if (lane == 0) {
-            const unsigned idesc_s = tc_idesc(false, TT_KT), idesc_o = tc_idesc(true, D);
-            unsigned long long dq[D / 16], dk[D / 16], dv[8];
+    } else if (warp == 18) {
+        // =========================== issuer
+        const unsigned idesc_s = tc_idesc(false, TT_KT), idesc_o = tc_idesc(true, D), leader = tt_elect();
+        // descriptors of the first tiles; others are a number of 16-byte units further in the address field
+        const unsigned long long dq = tc_desc(q_s, 16, 1024), dk = tc_desc(k_s, 16, 1024), dv = tc_desc(v_s, TT_HALF, 1024);
+        constexpr unsigned step = C::TILE >> 4;
+        const unsigned tm = __shfl_sync(0xffffffffu, tmem, 0);
+        unsigned count = 0, seg = 0, phase_p[2] = {0u, 0u};                           // tiles before this segment
+        TreeSegment g;
+        auto wait = [&](unsigned bar, unsigned parity) { return __all_sync(0xffffffffu, tc_mbar_wait(bar, parity)) != 0; };
+        bool ok = true;
+        for (; ok && walk.next(g); ++seg) {
+            const bool dual = __shfl_sync(0xffffffffu, g.rows, 0) > 128;
+            const int tiles = __shfl_sync(0xffffffffu, g.t_hi - g.t_lo, 0), steps = dual ? 2 * tiles : tiles;
+            auto tile_of = [&](int s) { return count + (dual ? s >> 1 : s); };
+            auto issue_o = [&](int s) {                               // O_X += P_X V
+                const int x = s & 1;
+                const unsigned c = tile_of(s), st = c % ST;
+                ok = wait(bar_p(x), phase_p[x]);
+                phase_p[x] ^= 1u;
+                if (ok && (!dual || x == 0)) ok = wait(bar_vf(st), (c / ST) & 1);
+                if (!ok) return;
+                tc_fence_async_smem(); tc_fence_after();
+                const unsigned long long dv_st = dv + st * step;
+                const unsigned t_o = tm + 256u + (unsigned)x * 128u, t_p = tm + (unsigned)x * 128u;
 #pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk) {
-                dq[kk] = tc_desc(q_s + (unsigned)(kk >> 2) * TT_HALF + (unsigned)(kk & 3) * 32u, 16, 1024);
-                dk[kk] = tc_desc(k_s + (unsigned)(kk >> 2) * TT_HALF + (unsigned)(kk & 3) * 32u, 16, 1024);
-            }
+                for (int kk = 0; kk < 8; ++kk) tt_mma_ta(leader, t_o, t_p + kk * 8u, dv_st + kk * (2048u >> 4), idesc_o, kk > 0 ? 1u : s < 2 ? 0u : 1u);
+                tt_commit(leader, bar_o(x));
+                if (!dual || x == 1) tt_commit(leader, bar_vr(st));
+            };
+            ok = wait(bar_q, seg & 1);
+            for (int s = 0; s < steps && ok; ++s) {
+                const int x = s & 1;
+                const unsigned c = tile_of(s), st = c % ST;
+                if (!dual || x == 0) ok = wait(bar_kf(st), (c / ST) & 1);
+                if (!ok) break;
+                tc_fence_async_smem(); tc_fence_after();
+                const unsigned long long dq_x = dq + (dual && x ? step : 0u), dk_st = dk + st * step;
+                const unsigned t_s = tm + (unsigned)x * 128u;
 #pragma unroll
-            for (int kk = 0; kk < 8; ++kk) dv[kk] = tc_desc(v_s + (unsigned)kk * 2048u, TT_HALF, 1024);
-            const unsigned long long step = (unsigned long long)(C::TILE >> 4);           // a tile further in a descriptor's address field
-            unsigned count = 0, seg = 0, phase_p[2] = {0u, 0u};                           // tiles before this segment
-            TreeSegment g;
-            bool ok = true;
-            for (; ok && walk.next(g); ++seg) {
-                const bool dual = g.rows > 128;
-                const int tiles = g.t_hi - g.t_lo, steps = dual ? 2 * tiles : tiles;
-                auto tile_of = [&](int s) { return count + (dual ? s >> 1 : s); };
-                auto issue_o = [&](int s) {                               // O_X += P_X V
-                    const int x = s & 1;
-                    const unsigned c = tile_of(s), st = c % ST;
-                    ok = tc_mbar_wait(bar_p(x), phase_p[x]);
-                    phase_p[x] ^= 1u;
-                    if (ok && (!dual || x == 0)) ok = tc_mbar_wait(bar_vf(st), (c / ST) & 1);
-                    if (!ok) return;
-                    tc_fence_async_smem(); tc_fence_after();
-#pragma unroll
-                    for (int kk = 0; kk < 8; ++kk)
-                        tc_mma_ta(tmem + 256u + (unsigned)x * 128u, tmem + (unsigned)x * 128u + kk * 8u, dv[kk] + st * step, idesc_o, (s < 2 && kk == 0) ? 0u : 1u);
-                    tc_commit(bar_o(x));
-                    if (!dual || x == 1) tc_commit(bar_vr(st));
-                };
-                ok = tc_mbar_wait(bar_q, seg & 1);
-                for (int s = 0; s < steps && ok; ++s) {
-                    const int x = s & 1;
-                    const unsigned c = tile_of(s), st = c % ST;
-                    if (!dual || x == 0) ok = tc_mbar_wait(bar_kf(st), (c / ST) & 1);
-                    if (!ok) break;
-                    tc_fence_async_smem(); tc_fence_after();
-                    const unsigned long long qx = dual && x ? step : 0ull;
-#pragma unroll
-                    for (int kk = 0; kk < D / 16; ++kk) tc_mma(tmem + (unsigned)x * 128u, dq[kk] + qx, dk[kk] + st * step, idesc_s, kk > 0 ? 1u : 0u);
-                    tc_commit(bar_s(x));
-                    if (!dual || x == 1) tc_commit(bar_kr(st));
-                    if (s >= 1) issue_o(s - 1);
+                for (int kk = 0; kk < D / 16; ++kk) {
+                    const unsigned at = (kk >> 2) * (TT_HALF >> 4) + (kk & 3) * 2u;
+                    tt_mma(leader, t_s, dq_x + at, dk_st + at, idesc_s, kk > 0 ? 1u : 0u);
                 }
-                if (ok) issue_o(steps - 1);
-                count += tiles;
+                tt_commit(leader, bar_s(x));
+                if (!dual || x == 1) tt_commit(leader, bar_kr(st));
+                if (s >= 1) issue_o(s - 1);
             }
-            if (!ok) fail = 1;
+            if (ok) issue_o(steps - 1);
+            count += tiles;
         }
-    } else if (warp < 8) {
-        // =========================== softmax: group x = warp / 4; thread r of a group owns its row r
-        const int x = warp >> 2, lane_row = tid & 127;
+        if (!ok) fail = 1;
+    } else if (warp < 16) {
+        // =========================== softmax: group x, half of the columns; TMEM lane lane_row
+        const int x = warp >> 3, half = (warp >> 2) & 1, lane_row = tid & 127;
         const unsigned lane_sel = (unsigned)((warp & 3) * 32) << 16;
         const unsigned ts = tmem + (unsigned)x * 128u + lane_sel, to = tmem + 256u + (unsigned)x * 128u + lane_sel;
+        float* const ex_max = exchange + x * 256, * const ex_sum = exchange + 512, * const ex_ref = exchange + 1024;
+        const int pair = 2 + x * 4 + (warp & 3);     // the barrier of the two warps of these rows
         unsigned phase_s = 0, phase_o = 0, seg = 0;
         const float sc = p.scale_log2;
         auto find = [&](unsigned s) {                // (one thread)
@@ -253,13 +278,13 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const TreeParams
             walk.store(sh_walk);
             find(0);
         }
-        asm volatile("bar.sync 1, 256;\n" ::: "memory");
+        asm volatile("bar.sync 1, 512;\n" ::: "memory");
         for (; *reinterpret_cast<volatile bool*>(&sh_more[seg & 1]); ++seg) {
             const TreeSegment& g = sh_seg[seg & 1];
             const bool dual = g.rows > 128;
             const __nv_bfloat16* qg = reinterpret_cast<const __nv_bfloat16*>(p.q);
-            // ---- Q: 16-byte chunks over all 256 threads; rows without a query are zero
-            for (int i = tid; i < (dual ? 256 : 128) * H * 8; i += 256) {
+            // ---- Q: 16-byte chunks over all softmax threads; rows without a query are zero
+            for (int i = tid; i < (dual ? 256 : 128) * H * 8; i += TT_SOFT) {
                 const int row = i / (H * 8), c = i % (H * 8), rr = g.row0 + row;
                 const bool valid = row < g.rows;
                 const __nv_bfloat16* src = valid ? qg + ((size_t)(g.tok0 + rr / G) * p.n_q + (size_t)g.kvh * G + rr % G) * D + c * 8 : qg;
@@ -279,69 +304,55 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const TreeParams
             const int row = dual ? x * 128 + lane_row : lane_row, rr = g.row0 + row;
             const bool valid = row < g.rows, active = row - lane < g.rows;               // whether the row, and any of the warp's, exists
             const size_t tok = (size_t)g.tok0 + (valid ? rr / G : 0);
-            float m_run = -INFINITY, l_run = 0.f, o_scale = 1.f;
-            for (int it = 0; it < n_mine && !fail; ++it) {
-                if (__any_sync(0xffffffffu, !tc_mbar_wait(bar_s(x), phase_s))) { fail = 1; break; }
+            float m_run = -INFINITY, l_run = 0.f;    // of the row; of this thread's half of the keys
+            for (int it = 0; it < n_mine; ++it) {    // (a warp that gave up goes on to meet its partner)
+                if (!fail && __any_sync(0xffffffffu, !tc_mbar_wait(bar_s(x), phase_s))) fail = 1;
                 phase_s ^= 1u;
                 tc_fence_after();
-                if (!active) {                       // P of rows that do not exist may be anything
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) tc_mbar_arrive(bar_p(x));
-                    continue;
-                }
-                const int key0 = (g.t_lo + (dual ? it : 2 * it + x)) * TT_KT;
-                float s0[32], s1[32], s2[32], s3[32];
-                tc_ld32(ts, s0); tc_ld32(ts + 32, s1); tc_ld32(ts + 64, s2); tc_ld32(ts + 96, s3);
-                tc_wait_ld(s0); tc_wait_ld(s1); tc_wait_ld(s2); tc_wait_ld(s3);
-                if (key0 + TT_KT > g.base) {
-                    const unsigned* row_mask = p.mask + tok * p.words;
-                    auto mask = [&](float (&sv)[32], int cb) {
-                        const unsigned seen = tree_seen(row_mask, p.words, key0 + 32 * cb, g.base, g.kv);
+                if (active) {                        // (P of rows that do not exist may be anything)
+                    const int key0 = (g.t_lo + (dual ? it : 2 * it + x)) * TT_KT + 64 * half;
+                    float s0[32], s1[32];
+                    tc_ld32(ts + 64 * half, s0); tc_ld32(ts + 64 * half + 32, s1);
+                    tc_wait_ld(s0); tc_wait_ld(s1);
+                    if (key0 + 64 > g.base) {
+                        const unsigned* row_mask = p.mask + tok * p.words;
+                        const unsigned seen0 = tree_seen(row_mask, p.words, key0, g.base, g.kv), seen1 = tree_seen(row_mask, p.words, key0 + 32, g.base, g.kv);
 #pragma unroll
-                        for (int e = 0; e < 32; ++e)
-                            if (!(seen >> e & 1u)) sv[e] = -INFINITY;
-                    };
-                    mask(s0, 0); mask(s1, 1); mask(s2, 2); mask(s3, 3);
-                }
-                auto row_max = [&]() -> float {
-                    float c8[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) c8[e] = fmaxf(fmaxf(s0[e], s1[e]), fmaxf(s2[e], s3[e]));
-#pragma unroll
-                    for (int e = 8; e < 32; ++e) c8[e & 7] = fmaxf(c8[e & 7], fmaxf(fmaxf(s0[e], s1[e]), fmaxf(s2[e], s3[e])));
-                    return fmaxf(fmaxf(fmaxf(c8[0], c8[1]), fmaxf(c8[2], c8[3])), fmaxf(fmaxf(c8[4], c8[5]), fmaxf(c8[6], c8[7]))) * sc;
-                };
-                auto move_reference = [&](float m_new) {
-                    const float a = fast_exp2(m_run - m_new);                // 0 for the first
-                    m_run = m_new;
-                    l_run *= a;
-                    o_scale *= a;
-                };
-                if (__any_sync(0xffffffffu, m_run == -INFINITY)) {
-                    const float cm = row_max();
-                    if (m_run == -INFINITY && cm > -INFINITY) move_reference(cm);
-                }
-                auto rescale_o = [&]() {             // (P V of this group's tile before is done: this S was issued after it)
-                    if (it >= 1 && __any_sync(0xffffffffu, o_scale != 1.f)) {
-#pragma unroll 1
-                        for (int cb = 0; cb < D / 32; ++cb) {
-                            float v0[32];
-                            tc_ld32(to + cb * 32, v0);
-                            tc_wait_ld(v0);
-#pragma unroll
-                            for (int e = 0; e < 32; ++e) v0[e] *= o_scale;
-                            tc_st32(to + cb * 32, v0);
+                        for (int e = 0; e < 32; ++e) {
+                            if (!(seen0 >> e & 1u)) s0[e] = -INFINITY;
+                            if (!(seen1 >> e & 1u)) s1[e] = -INFINITY;
                         }
                     }
-                    o_scale = 1.f;
-                };
-                rescale_o();
-                float tile_sum;
-                auto exponentials = [&]() {
-                    const float mu = (m_run == -INFINITY) ? 0.f : m_run;
+                    float c4[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) c4[e] = fmaxf(s0[e], s1[e]);
+#pragma unroll
+                    for (int e = 4; e < 32; ++e) c4[e & 3] = fmaxf(c4[e & 3], fmaxf(s0[e], s1[e]));
+                    const float mine = fmaxf(fmaxf(c4[0], c4[1]), fmaxf(c4[2], c4[3])) * sc;
+                    ex_max[half * 128 + lane_row] = mine;
+                    tc_fence_before();               // (the scores have been read, for the partner's P)
+                    asm volatile("bar.sync %0, 64;\n" ::"r"(pair) : "memory");
+                    tc_fence_after();
+                    const float mx = fmaxf(mine, ex_max[(1 - half) * 128 + lane_row]);
+                    const bool move = mx > m_run + 8.f || (m_run == -INFINITY && mx > -INFINITY);
+                    if (__any_sync(0xffffffffu, move)) {
+                        const float a = move ? fast_exp2(m_run - mx) : 1.f;              // 0 for the first
+                        if (move) { m_run = mx; l_run *= a; }
+                        if (it >= 1) {               // (P V of this group's tile before is done: this S was issued after it)
+#pragma unroll 1
+                            for (int cb = half * (D / 32); cb < (half + 1) * (D / 32); ++cb) {
+                                unsigned v0[16];
+                                tc_ld16(to + cb * 16, v0);
+                                tc_wait_ld16(v0);
+#pragma unroll
+                                for (int e = 0; e < 16; ++e) v0[e] = __float_as_uint(__uint_as_float(v0[e]) * a);
+                                tc_st16(to + cb * 16, v0);
+                            }
+                        }
+                    }
+                    const float mu = m_run == -INFINITY ? 0.f : m_run;
                     const unsigned long long sc2 = tt_pack(sc, sc), nmu2 = tt_pack(-mu, -mu);
-                    unsigned long long sum2[4] = {0ull, 0ull, 0ull, 0ull};   // (0.f, 0.f)
+                    unsigned long long sum2[4] = {0ull, 0ull, 0ull, 0ull};               // (0.f, 0.f)
                     auto expo = [&](const float (&sv)[32], int cb) {
                         unsigned pk[16];
 #pragma unroll
@@ -352,24 +363,14 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const TreeParams
                             sum2[(e >> 1) & 3] = tt_add(sum2[(e >> 1) & 3], tt_pack(e0, e1));
                             pk[e >> 1] = pack_bf16(e0, e1);
                         }
-                        tc_st16(ts + cb * 16, pk);
+                        tc_st16(ts + 32 * half + cb * 16, pk);
                     };
-                    expo(s0, 0); expo(s1, 1); expo(s2, 2); expo(s3, 3);
+                    expo(s0, 0); expo(s1, 1);
                     float lo, hi;
                     tt_unpack(tt_add(tt_add(sum2[0], sum2[1]), tt_add(sum2[2], sum2[3])), lo, hi);
-                    tile_sum = lo + hi;
-                };
-                exponentials();
-                if (__any_sync(0xffffffffu, !(tile_sum < 1.0e30f))) {        // overflow (inf, or NaN from inf - inf): again, from the maximum
-                    const float cm = row_max();
-                    if (cm > m_run) move_reference(cm);
-                    rescale_o();
+                    l_run += lo + hi;
                     tc_wait_st();
-                    exponentials();
                 }
-                l_run += tile_sum;
-                if (tile_sum > 65536.f) move_reference(m_run + log2f(tile_sum));         // takes effect with the next tile (O: before its product)
-                tc_wait_st();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) tc_mbar_arrive(bar_p(x));
@@ -380,21 +381,22 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const TreeParams
                 phase_o += n_mine;
                 tc_fence_after();
             }
-            float fa = o_scale, fb = 0.f, m_all = m_run, l_all = l_run;      // factors of O_A and O_B (dual: of the group's own alone)
-            if (!dual) {                             // both groups meet here, also where one of them has given up
-                float* ex = reinterpret_cast<float*>(exchange);              // [2][3][128]
-                ex[(x * 3 + 0) * 128 + lane_row] = m_run;
-                ex[(x * 3 + 1) * 128 + lane_row] = l_run;
-                ex[(x * 3 + 2) * 128 + lane_row] = o_scale;
-                tc_fence_before();
-                asm volatile("bar.sync 1, 256;\n" ::: "memory");
-                tc_fence_after();
-                const float ma = ex[lane_row], la = ex[128 + lane_row], oa = ex[256 + lane_row], mb = ex[384 + lane_row], lb = ex[512 + lane_row], ob = ex[640 + lane_row];
+            // the row's halves and, where both groups have it, the groups' results; both groups meet here, also where one of them has given up
+            ex_sum[(x * 2 + half) * 128 + lane_row] = l_run;
+            if (half == 0) ex_ref[x * 128 + lane_row] = m_run;
+            tc_fence_before();
+            asm volatile("bar.sync 1, 512;\n" ::: "memory");
+            tc_fence_after();
+            float fa = 1.f, fb = 0.f, m_all = m_run, l_all;                              // factors of O_A and O_B (dual: of the group's own alone)
+            if (dual) {
+                l_all = ex_sum[x * 256 + lane_row] + ex_sum[x * 256 + 128 + lane_row];
+            } else {
+                const float ma = ex_ref[lane_row], mb = ex_ref[128 + lane_row];
                 m_all = fmaxf(ma, mb);
-                const float mu = m_all == -INFINITY ? 0.f : m_all, wa = fast_exp2(ma - mu), wb = fast_exp2(mb - mu);
-                l_all = la * wa + lb * wb;
-                fa = wa * oa;
-                fb = wb * ob;
+                const float mu = m_all == -INFINITY ? 0.f : m_all;
+                fa = fast_exp2(ma - mu);
+                fb = fast_exp2(mb - mu);
+                l_all = (ex_sum[lane_row] + ex_sum[128 + lane_row]) * fa + (ex_sum[256 + lane_row] + ex_sum[384 + lane_row]) * fb;
             }
             if (active && !fail) {
                 const bool whole = !cut;
@@ -405,7 +407,8 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const TreeParams
 #pragma unroll
                 for (int w = 0; w < 8; ++w) any_bad |= *reinterpret_cast<const volatile unsigned*>(bad + w);
                 const int slot = 2 * j + (g.t_lo == 0 ? 1 : 0);
-                const int cb0 = dual ? 0 : x * (D / 64), cb1 = dual ? D / 32 : cb0 + D / 64;      // blocks of 32 columns: both groups share them out
+                // blocks of 32 columns: two threads a row share them out, or four
+                const int cb0 = dual ? half * (D / 64) : D == 128 ? 2 * x + half : x, cb1 = dual ? cb0 + D / 64 : D == 128 || half == 0 ? cb0 + 1 : cb0;
                 const bool two = !dual && tiles > 1;
                 __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(p.out) + (tok * p.n_q + (size_t)g.kvh * G + (valid ? rr % G : 0)) * D;
                 float* part = p.part_o + ((size_t)slot * TT_ROWS + row) * D;
@@ -447,10 +450,10 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const TreeParams
                         for (int e = 0; e < 32; e += 4) *reinterpret_cast<float4*>(part + cb * 32 + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
                     }
                 }
-                if (valid && !whole && (dual || x == 0)) *reinterpret_cast<float2*>(p.part_ml + ((size_t)slot * TT_ROWS + row) * 2) = make_float2(m_all, l_all);
+                if (valid && !whole && half == 0 && (dual || x == 0)) *reinterpret_cast<float2*>(p.part_ml + ((size_t)slot * TT_ROWS + row) * 2) = make_float2(m_all, l_all);
             }
             tc_fence_before();
-            asm volatile("bar.sync 1, 256;\n" ::: "memory");                 // Q, the exchange and both accumulators are free
+            asm volatile("bar.sync 1, 512;\n" ::: "memory");                 // Q, the exchange and both accumulators are free
         }
     }
     if (tid == 0) p.record[j] = record;

@@ -17,6 +17,7 @@ from __future__ import annotations
 
 import array
 import ctypes
+import math
 import os
 from typing import NamedTuple, Optional, Sequence, Tuple
 
@@ -2513,6 +2514,8 @@ def tree_attention(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_
         raise KernelError(f"{what}: the caches are contiguous [pages, {n_kv}, {page_size}, {d}] of q's type; got {tuple(k_cache.shape)}, {tuple(v_cache.shape)}")
     if n_kv < 1 or n_q % n_kv or not 1 <= d <= 512:
         raise KernelError(f"{what}: {n_q} query heads over {n_kv} kv heads of size {d}: whole groups, sizes up to 512")
+    if not 0.0 < scale < math.inf:
+        raise KernelError(f"{what}: scale {scale} is not above 0")
     _table(what, block_table, B)
     _index(what, "q_start", q_start, B + 1)
     _index(what, "kv_len", kv_len, B)

@@ -102,6 +102,8 @@ def test_tree_attention_refuses():
     refused("q_start", f, q, q, c, c, **dict(ok, q_start=I(3)))
     refused("kv_len", f, q, q, c, c, **dict(ok, kv_len=I(2)))
     refused("max_draft", f, q, q, c, c, **dict(ok, max_draft=257))
+    for scale in (0.0, -1.0, float("nan"), float("inf")):
+        refused("scale", f, q, q, c, c, **dict(ok, scale=scale))
     refused("a mask row", f, q, q, c, c, **dict(ok, max_draft=33))
     refused("a mask row", f, q, q, c, c, **dict(ok, mask=I(4)))
     refused("mask", f, q, q, c, c, **dict(ok, mask=I(3, 1)))
