@@ -29,6 +29,12 @@ __device__ __forceinline__ unsigned pack_bf16(float lo, float hi) {
     return *reinterpret_cast<unsigned*>(&v);
 }
 
+struct TreeRecord {               // the cut item whose first piece a block has
+    int pieces;                   // 0: it has none
+    int rows, tok0, row0, kvh;    // rows of the item, the first of them among the request's under the kv head, the request's first draft
+    int pad[3];
+};
+
 struct TreeParams {
     const void* q;                // [T, n_q, d]
     void* out;
@@ -38,9 +44,11 @@ struct TreeParams {
     const int* kv_len;            // [B]
     const int* table;             // [B, table_width], rows table_stride apart
     const unsigned* mask;         // [T, words]
-    float* part_o;                // [2 * blocks][ROWS][d]
+    // Partial results, by four columns and then by rows: what a warp's 32 rows write or read of one column lies side by side (row by row, 64 drafts of
+    // one request behind 4,096 keys spent 6 us on writing them and 7 on the join).
+    float* part_o;                // [2 * blocks][ceil(d / 4)][ROWS][4]
     float* part_ml;               // [2 * blocks][ROWS][2]  (maximum in log2 units, sum of the weights)
-    int4* record;                 // [blocks]: (request, item of it, pieces, rows) of the cut item whose first piece the block has; pieces 0: none
+    struct TreeRecord* record;    // [blocks]
     int B, T, n_q, n_kv, d, page_size, page_shift, table_stride, table_width, words;
     long long pages;
     float scale_log2;             // scale * log2(e)
@@ -59,15 +67,20 @@ struct TreeSegment {              // tiles [t_lo, t_hi) of one item
     int t_lo, t_hi, tiles;
 };
 
-struct TreeWalkState { long long total, x_lo, x_hi, start; int blocks, r, item; };      // (a walk put aside)
+struct TreeWalkState { int total, x_lo, x_hi, start, blocks, r, item; };      // (a walk put aside)
+struct TreeStart {                // what the block's walkers start with: the first segment, and the walk behind it
+    TreeWalkState walk;
+    TreeSegment first;
+    int work;
+};
 
 template <int ROWS, int KT>
 struct TreeWalk {
     const TreeParams& p;
-    int blocks;                   // in use; none if the step has no drafts
-    long long total, x_lo, x_hi;  // the work's length, this block's run
+    int blocks;                   // in use
+    int total, x_lo, x_hi;        // the work's length (the host has seen to it that it fits), this block's run
     int r = 0, item = 0;
-    long long start = 0;          // where the request's first item starts
+    int start = 0;                // where the request's first item starts
 
     __device__ __forceinline__ TreeWalk(const TreeParams& q) : p(q) {}
     __device__ __forceinline__ void store(TreeWalkState& s) const { s.total = total; s.x_lo = x_lo; s.x_hi = x_hi; s.start = start; s.blocks = blocks; s.r = r; s.item = item; }
@@ -82,57 +95,57 @@ struct TreeWalk {
         w.items = w.n > 0 ? p.n_kv * ((w.n * (p.n_q / p.n_kv) + ROWS - 1) / ROWS) : 0;
         return w;
     }
-    __device__ __forceinline__ long long cut_at(long long k) const { return total * k / blocks; }
+    __device__ __forceinline__ int cut_at(int k) const { const int q = total / blocks; return q * k + (total - q * blocks) * k / blocks; }      // floor(total k / blocks)
     // the tile that a cut at x falls on, in an item that starts at `s`
-    __device__ __forceinline__ int tile_at(long long x, long long s, int tiles) const {
-        const long long t = x - s - TREE_HEAD;
+    __device__ __forceinline__ int tile_at(int x, int s, int tiles) const {
+        const int t = x - s - TREE_HEAD;
         if (t < TREE_SNAP) return 0;
-        return tiles - t < TREE_SNAP ? tiles : (int)t;
+        return tiles - t < TREE_SNAP ? tiles : t;
     }
-    // all threads of the block: the run of block j of nb; false: there is none
-    __device__ __forceinline__ bool begin(int j, int nb) {
-        __shared__ long long sums[32], found_start;
-        __shared__ int found;
+    // All threads of the block: the run of block j of nb; false: it has none.  The thread whose request the run starts in finds the first segment for all:
+    // every further look at the lengths would be a wait for memory (walking from its start each by itself took the warps 2 us longer).
+    __device__ __forceinline__ bool begin(int j, int nb, TreeStart& to) {
+        __shared__ int sums[32];
         const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n_warps = blockDim.x >> 5;
         const int per = (p.B + blockDim.x - 1) / blockDim.x, i0 = min(p.B, tid * per), i1 = min(p.B, i0 + per);
-        long long mine = 0;
-        for (int i = i0; i < i1; ++i) { const Request w = request(i); mine += (long long)w.items * (w.tiles + TREE_HEAD); }
-        long long upto = mine;
+        int mine = 0;
+        for (int i = i0; i < i1; ++i) { const Request w = request(i); mine += w.items * (w.tiles + TREE_HEAD); }
+        int upto = mine;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) { const long long v = __shfl_up_sync(0xffffffffu, upto, o); if (lane >= o) upto += v; }
+        for (int o = 1; o < 32; o <<= 1) { const int v = __shfl_up_sync(0xffffffffu, upto, o); if (lane >= o) upto += v; }
         if (lane == 31) sums[warp] = upto;
+        if (tid == 0) to.work = 0;
         __syncthreads();
         total = 0;
-        long long before = upto - mine;
+        int before = upto - mine;
         for (int w = 0; w < n_warps; ++w) { if (w < warp) before += sums[w]; total += sums[w]; }
-        const long long fit = total / TREE_SHARE;
-        blocks = (int)min((long long)nb, fit > 1 ? fit : 1);
+        blocks = max(1, min(nb, total / TREE_SHARE));
         if (total == 0 || j >= blocks) return false;
         x_lo = cut_at(j);
         x_hi = cut_at(j + 1);
         if (x_lo >= before && x_lo < before + mine) {
-            long long s = before;
-            for (int i = i0; i < i1; ++i) {
-                const Request w = request(i);
-                const long long len = (long long)w.items * (w.tiles + TREE_HEAD);
-                if (x_lo < s + len) { found = i; found_start = s; break; }
-                s += len;
+            start = before;
+            for (r = i0; r < i1; ++r) {
+                const Request w = request(r);
+                const int len = w.items * (w.tiles + TREE_HEAD);
+                if (x_lo < start + len) { item = (x_lo - start) / (w.tiles + TREE_HEAD); break; }
+                start += len;
             }
+            TreeSegment g;
+            if (next(g)) { to.first = g; to.work = 1; }
+            store(to.walk);
         }
         __syncthreads();
-        r = found;
-        start = found_start;
-        const Request w = request(r);
-        item = (int)((x_lo - start) / (w.tiles + TREE_HEAD));
-        return true;
+        load(to.walk);
+        return to.work != 0;
     }
     // the next segment of the run; false: it is done
     __device__ __forceinline__ bool next(TreeSegment& g) {
         while (r < p.B) {
             const Request w = request(r);
-            const long long len = w.tiles + TREE_HEAD;
+            const int len = w.tiles + TREE_HEAD;
             for (; item < w.items; ++item) {
-                const long long s = start + item * len;
+                const int s = start + item * len;
                 if (s >= x_hi) return false;
                 const int lo = x_lo > s ? tile_at(x_lo, s, w.tiles) : 0, hi = x_hi < s + len ? tile_at(x_hi, s, w.tiles) : w.tiles;
                 if (lo >= hi) continue;
@@ -151,10 +164,10 @@ struct TreeWalk {
     }
     // pieces of the item whose first piece `g` is, in block j
     __device__ __forceinline__ int pieces(const TreeSegment& g, int j) const {
-        const long long s = start + (long long)(item - 1) * (g.tiles + TREE_HEAD), e = s + g.tiles + TREE_HEAD;
+        const int s = start + (item - 1) * (g.tiles + TREE_HEAD), e = s + g.tiles + TREE_HEAD;
         int k = j + 1;
         while (k < blocks) {
-            const long long x = cut_at(k + 1);
+            const int x = cut_at(k + 1);
             ++k;
             if (x >= e || tile_at(x, s, g.tiles) >= g.tiles) break;
         }
@@ -205,11 +218,12 @@ __global__ void __launch_bounds__(TS_THREADS) tree_simt_kernel(const TreeParams 
     pdl_wait();
     pdl_after_wait();
     TreeWalk<TS_ROWS, TS_KT> walk(p);
-    int4 record = make_int4(0, 0, 0, 0);
-    TreeSegment g;
-    if (walk.begin(j, gridDim.x)) {
+    TreeRecord record = {};
+    __shared__ TreeStart begun;
+    if (walk.begin(j, gridDim.x, begun)) {
         for (int i = tid; i < (TS_ROWS + 2 * TS_KT) * pitch; i += TS_THREADS) ts_smem[i] = 0.f;      // (what lies from d on stays zero)
-        while (walk.next(g)) {
+        TreeSegment g = begun.first;
+        for (bool more = true; more; more = walk.next(g)) {
             const T* q = reinterpret_cast<const T*>(p.q);
             __syncthreads();                         // the segment before has been read
             for (int i = tid; i < TS_ROWS * d; i += TS_THREADS) {
@@ -311,72 +325,93 @@ __global__ void __launch_bounds__(TS_THREADS) tree_simt_kernel(const TreeParams 
                         for (int e = 0; e < 4; ++e)
                             if (b * 128 + lane * 4 + e < d) dst[b * 128 + lane * 4 + e] = from_f32<T>(o[a][b][e] * inv);
                 } else {
-                    float* dst = p.part_o + ((size_t)slot * TS_ROWS + row) * d;
+                    float4* dst = reinterpret_cast<float4*>(p.part_o) + (size_t)slot * d4 * TS_ROWS + row;
 #pragma unroll
                     for (int b = 0; b < CB; ++b)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (b * 128 + lane * 4 + e < d) dst[b * 128 + lane * 4 + e] = o[a][b][e];
+                        if (b * 32 + lane < d4) dst[(b * 32 + lane) * TS_ROWS] = make_float4(o[a][b][0], o[a][b][1], o[a][b][2], o[a][b][3]);
                     if (lane == 0) *reinterpret_cast<float2*>(p.part_ml + ((size_t)slot * TS_ROWS + row) * 2) = make_float2(m_run[a], l);
                 }
             }
-            if (!whole && g.t_lo == 0) record = make_int4(g.r, g.item, walk.pieces(g, j), g.rows);
+            if (!whole && g.t_lo == 0) record = TreeRecord{walk.pieces(g, j), g.rows, g.tok0, g.row0, g.kvh, {0, 0, 0}};
         }
     }
     if (tid == 0) p.record[j] = record;
 }
 
 // ---------------------------------------------------------------------------------------
-// The pieces of cut items, joined in the order of the keys: block (j, y) takes eight rows of the item whose first piece block j has.
+// The pieces of cut items, joined in the order of the keys.  A warp takes 32 rows, a lane each, and 16 columns of the item whose first piece block j
+// has.  Bound by latency: a record, the pieces' maxima, then their rows, 24 loads of 512 bytes of a warp at a time.
 // ---------------------------------------------------------------------------------------
+constexpr int TJ_WARPS = 4, TJ_C = 4, TJ_K = 6;       // warps of a block, fours of columns of a warp, pieces at a time
+
 template <typename T, int ROWS>
-__global__ void __launch_bounds__(256) tree_join_kernel(const TreeParams p) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, j = blockIdx.x, row = blockIdx.y * 8 + warp;
-    pdl_launch_dependents();
+__global__ void __launch_bounds__(TJ_WARPS * 32) tree_join_kernel(const TreeParams p) {
+    const int lane = threadIdx.x & 31, j = blockIdx.x, d4 = (p.d + 3) >> 2, n_cols = (d4 + TJ_C - 1) / TJ_C, task = blockIdx.y * TJ_WARPS + (threadIdx.x >> 5);
+    const int row = task / n_cols * 32 + lane, c0 = task % n_cols * TJ_C;       // of the item; in fours of columns
     pdl_wait();
-    pdl_after_wait();
-    const int4 rec = p.record[j];
-    if (rec.z == 0 || row >= rec.w) return;
-    const int G = p.n_q / p.n_kv, d = p.d, tok0 = min(max(p.q_start[rec.x], 0), p.T), n = min(max(p.q_start[rec.x + 1], tok0), p.T) - tok0;
-    const int groups = (n * G + ROWS - 1) / ROWS, kvh = rec.y / groups, rr = (rec.y - kvh * groups) * ROWS + row;
-    auto at = [&](int k) { return (size_t)(2 * (j + k) + (k == 0 ? 1 : 0)) * ROWS + row; };
-    float M = -INFINITY;
-    for (int k = lane; k < rec.z; k += 32) M = fmaxf(M, p.part_ml[at(k) * 2]);
-    M = warp_max(M);
-    const float mu = M == -INFINITY ? 0.f : M;
-    float L = 0.f;
-    T* dst = reinterpret_cast<T*>(p.out) + ((size_t)(tok0 + rr / G) * p.n_q + (size_t)kvh * G + rr % G) * d;
-    for (int c0 = 0; c0 < d; c0 += 128) {
-        float acc[4] = {0.f, 0.f, 0.f, 0.f};
-        L = 0.f;
-        for (int k0 = 0; k0 < rec.z; k0 += 32) {
-            float2 ml = make_float2(-INFINITY, 0.f);
-            if (k0 + lane < rec.z) ml = *reinterpret_cast<const float2*>(p.part_ml + at(k0 + lane) * 2);
-            const float w = fast_exp2(ml.x - mu);
-            L += w * ml.y;
-            const int m = min(rec.z - k0, 32);
-#pragma unroll 4
-            for (int k = 0; k < m; ++k) {
-                const float f = __shfl_sync(0xffffffffu, w, k);
-                const float* src = p.part_o + at(k0 + k) * d + c0 + lane * 4;
-                if ((d & 3) == 0) {
-                    if (c0 + lane * 4 < d) {
-                        const float4 v = *reinterpret_cast<const float4*>(src);
-                        acc[0] = fmaf(f, v.x, acc[0]); acc[1] = fmaf(f, v.y, acc[1]); acc[2] = fmaf(f, v.z, acc[2]); acc[3] = fmaf(f, v.w, acc[3]);
-                    }
-                } else {
+    pdl_small();
+    const int4 rec = *reinterpret_cast<const int4*>(p.record + j);           // pieces, rows, first draft, first row
+    const int pieces = rec.x, kvh = p.record[j].kvh;
+    if (pieces == 0 || row >= rec.y) return;
+    const int G = p.n_q / p.n_kv, d = p.d, rr = rec.w + row, tok0 = rec.z;
+    auto slot = [&](int k) { return (size_t)(2 * (j + k) + (k == 0 ? 1 : 0)); };
+    auto ml_of = [&](int k) { return *reinterpret_cast<const float2*>(p.part_ml + (slot(k) * ROWS + row) * 2); };
+    float M = -INFINITY, L = 0.f;
+    float4 acc[TJ_C];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (c0 + lane * 4 + e < d) acc[e] = fmaf(f, src[e], acc[e]);
-                }
+    for (int c = 0; c < TJ_C; ++c) acc[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k0 = 0; k0 < pieces; k0 += TJ_K) {      // TJ_K pieces at a time: their maxima and rows are all asked for at once
+        float2 ml[TJ_K];
+        float4 v[TJ_K][TJ_C];
+#pragma unroll
+        for (int k = 0; k < TJ_K; ++k) {
+            const bool there = k0 + k < pieces;
+            ml[k] = there ? ml_of(k0 + k) : make_float2(-INFINITY, 0.f);
+            const float4* src = reinterpret_cast<const float4*>(p.part_o) + slot(k0 + k) * d4 * ROWS + row;
+#pragma unroll
+            for (int c = 0; c < TJ_C; ++c) v[k][c] = there && c0 + c < d4 ? src[(c0 + c) * ROWS] : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        float mx = M;
+#pragma unroll
+        for (int k = 0; k < TJ_K; ++k) mx = fmaxf(mx, ml[k].x);
+        const float mu = mx == -INFINITY ? 0.f : mx, f = fast_exp2(M - mu);
+        M = mx;
+        L *= f;
+#pragma unroll
+        for (int c = 0; c < TJ_C; ++c) { acc[c].x *= f; acc[c].y *= f; acc[c].z *= f; acc[c].w *= f; }
+#pragma unroll
+        for (int k = 0; k < TJ_K; ++k) {
+            const float w = fast_exp2(ml[k].x - mu);
+            L = fmaf(w, ml[k].y, L);
+#pragma unroll
+            for (int c = 0; c < TJ_C; ++c) {
+                acc[c].x = fmaf(w, v[k][c].x, acc[c].x); acc[c].y = fmaf(w, v[k][c].y, acc[c].y);
+                acc[c].z = fmaf(w, v[k][c].z, acc[c].z); acc[c].w = fmaf(w, v[k][c].w, acc[c].w);
             }
         }
-        L = warp_sum(L);
-        const float inv = L > 0.f ? 1.f / L : (L == L ? 0.f : L);
+    }
+    const float inv = L > 0.f ? 1.f / L : (L == L ? 0.f : L);
+    T* dst = reinterpret_cast<T*>(p.out) + ((size_t)(tok0 + rr / G) * p.n_q + (size_t)kvh * G + rr % G) * d + c0 * 4;
+    if (sizeof(T) == 2 && (d & 7) == 0 && ((uintptr_t)p.out & 15) == 0) {
+#pragma unroll
+        for (int c = 0; c < TJ_C; c += 2)
+            if (c0 + c < d4)
+                *reinterpret_cast<uint4*>(dst + c * 4) = make_uint4(pack_bf16(acc[c].x * inv, acc[c].y * inv), pack_bf16(acc[c].z * inv, acc[c].w * inv),
+                                                                    pack_bf16(acc[c + 1].x * inv, acc[c + 1].y * inv), pack_bf16(acc[c + 1].z * inv, acc[c + 1].w * inv));
+        return;
+    }
+#pragma unroll
+    for (int c = 0; c < TJ_C; ++c) {
+        const float x[4] = {acc[c].x, acc[c].y, acc[c].z, acc[c].w};
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-            if (c0 + lane * 4 + e < d) dst[c0 + lane * 4 + e] = from_f32<T>(acc[e] * inv);
+            if ((c0 + c) * 4 + e < d) dst[c * 4 + e] = from_f32<T>(x[e] * inv);
     }
+}
+template <typename T, int ROWS>
+static void tree_join(const TreeParams& p, int blocks, int max_rows, cudaStream_t stream) {
+    const int tasks = ((max_rows < ROWS ? max_rows : ROWS) + 31) / 32 * (((p.d + 3) / 4 + TJ_C - 1) / TJ_C);
+    msgl_launch_pdl(tree_join_kernel<T, ROWS>, dim3(blocks, (tasks + TJ_WARPS - 1) / TJ_WARPS), dim3(TJ_WARPS * 32), 0, stream, p);
 }
 
 #include "attention_tree_tc.cuh"
@@ -388,7 +423,7 @@ static size_t tree_simt_smem(int cb) { return ((size_t)(TS_ROWS + 2 * TS_KT) * (
 MSGL_API int msgl_tree_attention_tensor(int d, int page_size, long long cache_rows, int dtype) {
     return dtype == MSGL_BF16 && (d == 64 || d == 128) && page_size >= 8 && (page_size & (page_size - 1)) == 0 && cache_rows < 0x7fffffffLL - 4096 && tc_encoder() != nullptr;
 }
-// Blocks of a launch and rows of an item, for the sizes of the scratch memory: part_o [2 * blocks][rows][d], part_ml [2 * blocks][rows][2] float32, record [blocks][4] int32.
+// Blocks of a launch and rows of an item, for the sizes of the scratch memory: part_o [2 * blocks][ceil(d / 4)][rows][4], part_ml [2 * blocks][rows][2] float32, record [blocks][8] int32.
 MSGL_API int msgl_tree_attention_blocks(int d, int tensor) { return msgl_sm_count() * (tensor ? 1 : tree_simt_blocks_per_sm(d)); }
 MSGL_API int msgl_tree_attention_rows(int tensor) { return tensor ? TT_ROWS : TS_ROWS; }
 
@@ -400,7 +435,7 @@ static int tree_simt_launch(const TreeParams& p, int blocks, int max_rows, cudaS
         attr_set.mark();
     }
     msgl_launch_pdl(tree_simt_kernel<T, CB>, dim3(blocks), dim3(TS_THREADS), tree_simt_smem(CB), stream, p);
-    msgl_launch_pdl(tree_join_kernel<T, TS_ROWS>, dim3(blocks, (min(max_rows, TS_ROWS) + 7) / 8), dim3(256), 0, stream, p);
+    tree_join<T, TS_ROWS>(p, blocks, max_rows, stream);
     return msgl_check_launch();
 }
 
@@ -416,7 +451,7 @@ static int tree_tc_launch(const TreeParams& p, int* status, int blocks, int max_
     CUtensorMap kmap, vmap;
     if (!tc_matrix_map(p.k_cache, rows, D, (long long)D * 2, box, &kmap) || !tc_matrix_map(p.v_cache, rows, D, (long long)D * 2, box, &vmap)) return MSGL_ERR_SIZE;
     msgl_launch_pdl(tree_tc_kernel<D>, dim3(blocks), dim3(TT_THREADS), TreeTc<D>::ALLOC, stream, p, status, kmap, vmap, box);
-    msgl_launch_pdl(tree_join_kernel<__nv_bfloat16, TT_ROWS>, dim3(blocks, (min(max_rows, TT_ROWS) + 7) / 8), dim3(256), 0, stream, p);
+    tree_join<__nv_bfloat16, TT_ROWS>(p, blocks, max_rows, stream);
     return msgl_check_launch();
 }
 
@@ -428,10 +463,12 @@ MSGL_API int msgl_tree_attention(const void* q, void* out, const void* k_cache, 
     if (B <= 0 || T <= 0) return MSGL_OK;
     if (n_kv <= 0 || n_q <= 0 || n_q % n_kv || d < 1 || d > 512 || page_size < 1 || table_width < 1 || words < 1 || blocks < 1 || pages < 0 || max_rows < 1) return MSGL_ERR_SIZE;
     if ((long long)table_width * page_size > 0x7fffffffLL - 1024 || (long long)T * (n_q / n_kv) > 0x7fffffffLL / 2) return MSGL_ERR_SIZE;
+    // the length of the work, in whole numbers of 32 bits: at most this many tiles and heads of items
+    if ((long long)B * n_kv * ((long long)max_rows / TS_ROWS + 1) * ((long long)table_width * page_size / TS_KT + 1 + TREE_HEAD) > 0x7fffffffLL) return MSGL_ERR_SIZE;
     if (((uintptr_t)part_o | (uintptr_t)record) & 15 || (uintptr_t)part_ml & 7) return MSGL_ERR_ALIGN;
     TreeParams p;
     p.q = q; p.out = out; p.k_cache = k_cache; p.v_cache = v_cache; p.q_start = q_start; p.kv_len = kv_len; p.table = table; p.mask = (const unsigned*)mask;
-    p.part_o = part_o; p.part_ml = part_ml; p.record = (int4*)record;
+    p.part_o = part_o; p.part_ml = part_ml; p.record = (TreeRecord*)record;
     p.B = B; p.T = T; p.n_q = n_q; p.n_kv = n_kv; p.d = d; p.page_size = page_size; p.table_stride = table_stride; p.table_width = table_width; p.words = words;
     p.pages = pages;
     p.page_shift = -1;

@@ -109,7 +109,8 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const TreeParams
     float* exchange = reinterpret_cast<float*>(tt_smem + 512);                            // [2 groups][2 halves][128] maxima, the same of sums, [2][128] references
     __shared__ TreeSegment sh_seg[2];                // the softmax groups' segment and the one after it
     __shared__ bool sh_more[2];
-    __shared__ TreeWalkState sh_walk;
+    __shared__ TreeWalkState sh_walk;                 // their walk
+    __shared__ TreeStart begun;
     const unsigned smem_base = smem_u32(tt_smem);
     const unsigned smem0 = (smem_base + 512u + 1280u * 4u + 1023u) & ~1023u;
     const unsigned q_s = smem0, k_s = q_s + 2u * C::TILE, v_s = k_s + ST * C::TILE;
@@ -140,12 +141,12 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const TreeParams
     pdl_after_wait();
     TreeWalk<TT_ROWS, TT_KT> walk(p);
     const bool stop = __syncthreads_or(*reinterpret_cast<volatile int*>(status) != 0) != 0;      // an earlier block gave up: do not pile up
-    const bool work = walk.begin(j, gridDim.x) && !stop && smem0 + C::SMEM <= smem_base + C::ALLOC;      // (a barrier of the block stands in begin)
+    const bool work = walk.begin(j, gridDim.x, begun) && !stop && smem0 + C::SMEM <= smem_base + C::ALLOC;      // (a barrier of the block stands in begin)
     __syncthreads();
     tc_fence_after();
     const unsigned tmem = tmem_base_s;
     int fail = 0;
-    int4 record = make_int4(0, 0, 0, 0);
+    TreeRecord record = {};
 
     if (!work) {
         if (tid == 0 && smem0 + C::SMEM > smem_base + C::ALLOC) atomicExch(status, 2);      // allocation not aligned as assumed
@@ -155,8 +156,8 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const TreeParams
         const CUtensorMap* map = is_k ? &kmap : &vmap;
         const int n_box = TT_KT / tma_box;
         unsigned vt_phase = 0, count = 0, seg = 0;
-        TreeSegment g;
-        for (; !fail && walk.next(g); ++seg) {
+        TreeSegment g = begun.first;
+        for (bool more = true; !fail && more; more = walk.next(g), ++seg) {
             const int* bt = p.table + (size_t)g.r * p.table_stride;
             if (!is_k) { if (lane < 8) bad_words[(seg % TT_BAD) * 8 + lane] = 0u; __syncwarp(); }
             for (int t = g.t_lo; t < g.t_hi; ++t, ++count) {
@@ -213,10 +214,10 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const TreeParams
         constexpr unsigned step = C::TILE >> 4;
         const unsigned tm = __shfl_sync(0xffffffffu, tmem, 0);
         unsigned count = 0, seg = 0, phase_p[2] = {0u, 0u};                           // tiles before this segment
-        TreeSegment g;
+        TreeSegment g = begun.first;
         auto wait = [&](unsigned bar, unsigned parity) { return __all_sync(0xffffffffu, tc_mbar_wait(bar, parity)) != 0; };
         bool ok = true;
-        for (; ok && walk.next(g); ++seg) {
+        for (bool more = true; ok && more; more = walk.next(g), ++seg) {
             const bool dual = __shfl_sync(0xffffffffu, g.rows, 0) > 128;
             const int tiles = __shfl_sync(0xffffffffu, g.t_hi - g.t_lo, 0), steps = dual ? 2 * tiles : tiles;
             auto tile_of = [&](int s) { return count + (dual ? s >> 1 : s); };
@@ -274,28 +275,27 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const TreeParams
             sh_more[s & 1] = more;
             walk.store(sh_walk);
         };
-        if (tid == 0) {
-            walk.store(sh_walk);
-            find(0);
-        }
+        auto load_q = [&](const TreeSegment& w) {    // 16-byte chunks over all softmax threads; rows without a query are zero
+            const __nv_bfloat16* qg = reinterpret_cast<const __nv_bfloat16*>(p.q);
+            for (int i = tid; i < (w.rows > 128 ? 256 : 128) * H * 8; i += TT_SOFT) {
+                const int row = i / (H * 8), c = i % (H * 8), rr = w.row0 + row;
+                const bool valid = row < w.rows;
+                const __nv_bfloat16* src = valid ? qg + ((size_t)(w.tok0 + rr / G) * p.n_q + (size_t)w.kvh * G + rr % G) * D + c * 8 : qg;
+                tt_cp_async16(q_s + (unsigned)(row >> 7) * C::TILE + tt_off(row & 127, c), src, valid);
+            }
+            tc_cp_async_arrive(bar_q);
+        };
+        load_q(begun.first);
+        if (tid == 0) { sh_seg[0] = begun.first; sh_more[0] = true; sh_walk = begun.walk; }
         asm volatile("bar.sync 1, 512;\n" ::: "memory");
         for (; *reinterpret_cast<volatile bool*>(&sh_more[seg & 1]); ++seg) {
             const TreeSegment& g = sh_seg[seg & 1];
             const bool dual = g.rows > 128;
-            const __nv_bfloat16* qg = reinterpret_cast<const __nv_bfloat16*>(p.q);
-            // ---- Q: 16-byte chunks over all softmax threads; rows without a query are zero
-            for (int i = tid; i < (dual ? 256 : 128) * H * 8; i += TT_SOFT) {
-                const int row = i / (H * 8), c = i % (H * 8), rr = g.row0 + row;
-                const bool valid = row < g.rows;
-                const __nv_bfloat16* src = valid ? qg + ((size_t)(g.tok0 + rr / G) * p.n_q + (size_t)g.kvh * G + rr % G) * D + c * 8 : qg;
-                tt_cp_async16(q_s + (unsigned)(row >> 7) * C::TILE + tt_off(row & 127, c), src, valid);
-            }
-            tc_cp_async_arrive(bar_q);
             const bool cut = g.t_lo != 0 || g.t_hi != g.tiles;
             if (tid == 0) {
                 if (cut && g.t_lo == 0) {
                     walk.load(sh_walk);
-                    record = make_int4(g.r, g.item, walk.pieces(g, j), g.rows);
+                    record = TreeRecord{walk.pieces(g, j), g.rows, g.tok0, g.row0, g.kvh, {0, 0, 0}};
                 }
                 find(seg + 1);                       // (the segment before the present one has been left by all)
             }
@@ -387,6 +387,9 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const TreeParams
             tc_fence_before();
             asm volatile("bar.sync 1, 512;\n" ::: "memory");
             tc_fence_after();
+            // both groups have seen the last of this segment's scores, so Q is free: the next segment's comes while this one's rows are written, and its first
+            // scores are made meanwhile
+            if (*reinterpret_cast<volatile bool*>(&sh_more[(seg + 1) & 1])) load_q(sh_seg[(seg + 1) & 1]);
             float fa = 1.f, fb = 0.f, m_all = m_run, l_all;                              // factors of O_A and O_B (dual: of the group's own alone)
             if (dual) {
                 l_all = ex_sum[x * 256 + lane_row] + ex_sum[x * 256 + 128 + lane_row];
@@ -411,7 +414,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const TreeParams
                 const int cb0 = dual ? half * (D / 64) : D == 128 ? 2 * x + half : x, cb1 = dual ? cb0 + D / 64 : D == 128 || half == 0 ? cb0 + 1 : cb0;
                 const bool two = !dual && tiles > 1;
                 __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(p.out) + (tok * p.n_q + (size_t)g.kvh * G + (valid ? rr % G : 0)) * D;
-                float* part = p.part_o + ((size_t)slot * TT_ROWS + row) * D;
+                float4* part = reinterpret_cast<float4*>(p.part_o) + (size_t)slot * (D / 4) * TT_ROWS + row;
                 const unsigned t_own = dual ? to : tmem + 256u + lane_sel, t_other = tmem + 384u + lane_sel;
 #pragma unroll 1
                 for (int cb = cb0; cb < cb1; ++cb) {
@@ -447,16 +450,17 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const TreeParams
                                                                                       pack_bf16(v[e + 4] * inv, v[e + 5] * inv), pack_bf16(v[e + 6] * inv, v[e + 7] * inv));
                     } else if (valid) {
 #pragma unroll
-                        for (int e = 0; e < 32; e += 4) *reinterpret_cast<float4*>(part + cb * 32 + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+                        for (int e = 0; e < 32; e += 4) part[(cb * 8 + e / 4) * TT_ROWS] = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
                     }
                 }
                 if (valid && !whole && half == 0 && (dual || x == 0)) *reinterpret_cast<float2*>(p.part_ml + ((size_t)slot * TT_ROWS + row) * 2) = make_float2(m_all, l_all);
             }
             tc_fence_before();
-            asm volatile("bar.sync 1, 512;\n" ::: "memory");                 // Q, the exchange and both accumulators are free
+            asm volatile("bar.sync 1, 512;\n" ::: "memory");                 // the exchange and both accumulators are free
         }
     }
     if (tid == 0) p.record[j] = record;
+    pdl_late();
     tc_fence_before();
     const bool failed = __syncthreads_or(fail) != 0;
     tc_fence_after();

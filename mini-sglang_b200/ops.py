@@ -2474,9 +2474,9 @@ def draft_plan(parents: torch.Tensor, draft_lens: torch.Tensor, cached: torch.Te
     index within the request of an earlier draft; anything else stands for none.  Draft i lies in the cache at place cached + i.
     Lengths are taken within [0, max_draft] and drafts past the end of `parents` are cut; rows of `parents` behind the last draft become
     padding: position 0 and slot 0 (the page for padding) with an empty mask.  A place beyond the block table gets slot 0 too."""
-    T, (B, width) = parents.numel(), block_table.shape
+    T, B, width = parents.numel(), draft_lens.numel(), block_table.shape[-1] if block_table.dim() else 0
     _index("draft_plan", "parents", parents)
-    _index("draft_plan", "draft_lens", draft_lens, B)
+    _index("draft_plan", "draft_lens", draft_lens)
     _index("draft_plan", "cached", cached, B)
     _table("draft_plan", block_table, B)
     _draft_limit("draft_plan", max_draft)
@@ -2489,9 +2489,10 @@ def draft_plan(parents: torch.Tensor, draft_lens: torch.Tensor, cached: torch.Te
     else:
         buf = torch.empty(2 * B + 1 + T * (3 + words), dtype=torch.int32, device=parents.device)
     q_start, kv_len, positions, token_req, out_loc, mask = buf.split((B + 1, B, T, T, T, T * words))
+    at = buf.data_ptr()
+    rows = at + 4 * (2 * B + 1)
     code = _draft_lib().msgl_draft_plan(parents.data_ptr(), T, draft_lens.data_ptr(), cached.data_ptr(), B, block_table.data_ptr(), block_table.stride(0), width,
-                                        page_size, max_draft, words, q_start.data_ptr(), kv_len.data_ptr(), positions.data_ptr(), token_req.data_ptr(),
-                                        out_loc.data_ptr(), mask.data_ptr(), _stream())
+                                        page_size, max_draft, words, at, at + 4 * (B + 1), rows, rows + 4 * T, rows + 8 * T, rows + 12 * T, _stream())
     _check(code, "draft_plan")
     return DraftPlan(q_start, kv_len, positions, token_req, out_loc, mask.view(T, words))
 
@@ -2504,18 +2505,70 @@ def tree_attention(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_
     a draft that sees no key gets 0.  No request brings more than max_draft (the host's bound; it sizes the launch).  Rows of out behind the
     last draft are left as they were.  Head sizes up to 512; bfloat16 heads of 128 on pages that TMA can fetch (a power of two from 8
     on) go through the tensor cores.  A page number outside the cache reads as zeros."""
+    i32, dt, dev = torch.int32, q.dtype, q.get_device()
+    k_shape, words = k_cache.shape, mask.shape[-1] if mask.dim() else 0
+    # every argument is looked at in one go, and told apart only where something is wrong: small steps wait for the host
+    if not (q.dim() == 3 and dt in _DT and out.dtype is dt and out.shape == q.shape and q.is_contiguous() and out.is_contiguous()
+            and k_cache.dtype is dt and v_cache.dtype is dt and k_shape == v_cache.shape and k_shape[1:] == (n_kv, page_size, q.shape[2]) and k_cache.is_contiguous()
+            and v_cache.is_contiguous() and n_kv >= 1 and q.shape[1] % n_kv == 0 and 1 <= q.shape[2] <= 512 and 0.0 < scale < math.inf
+            and block_table.dtype is i32 and block_table.dim() == 2 and block_table.shape[1] >= 1 and block_table.stride(1) == 1
+            and q_start.dtype is i32 and q_start.numel() == block_table.shape[0] + 1 and q_start.is_contiguous()
+            and kv_len.dtype is i32 and kv_len.numel() == block_table.shape[0] and kv_len.is_contiguous()
+            and 1 <= max_draft <= MAX_DRAFTS and max_draft <= 32 * words and mask.dtype is i32 and mask.dim() == 2 and mask.shape[0] == q.shape[0] and mask.is_contiguous()
+            and out.get_device() == k_cache.get_device() == v_cache.get_device() == q_start.get_device() == kv_len.get_device() == block_table.get_device()
+            == mask.get_device() == dev >= 0 and dev == torch._C._cuda_getDevice()):
+        _refuse_tree_attention(q, out, k_cache, v_cache, q_start, kv_len, block_table, mask, n_kv, page_size, scale, max_draft)
     T, n_q, d = q.shape
     B, width = block_table.shape
+    if T == 0 or B == 0:
+        return
+    lib = _draft_lib()
+    facts = _tree_facts.get((dev, d, page_size, dt))
+    if facts is None:
+        sizes = [(lib.msgl_tree_attention_blocks(d, t), lib.msgl_tree_attention_rows(t)) for t in (0, 1)]
+        facts = (lib.msgl_tree_attention_tensor(d, page_size, 1, _DT[dt]), sizes)
+        _tree_facts[(dev, d, page_size, dt)] = facts
+    at_q, at_out, at_k, at_v, pages = q.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_shape[0]
+    tensor, status = int(facts[0] and pages > 0 and pages * n_kv * page_size < _TREE_ROWS_MAX and not (at_q | at_out | at_k | at_v) & 15), None
+    if tensor:
+        # the status words lie on the first device that asked for them, and are not made in a stream capture: elsewhere the kernel that has no waits
+        status = _status if _status is not None else _status_words(q.device)
+        tensor = int(status is not None and status.get_device() == dev)
+    while True:
+        blocks, rows = facts[1][tensor]
+        n_part = 2 * blocks * rows
+        d4 = d + 3 & ~3
+        part = torch.empty(n_part * (d4 + 2) + 8 * blocks, dtype=torch.float32, device=q.device)
+        at = part.data_ptr()
+        code = lib.msgl_tree_attention(at_q, at_out, at_k, at_v, q_start.data_ptr(), kv_len.data_ptr(), block_table.data_ptr(), mask.data_ptr(), B, T, n_q, n_kv, d,
+                                       page_size, block_table.stride(0), width, words, pages, scale, at, at + 4 * n_part * d4, at + 4 * n_part * (d4 + 2), blocks,
+                                       max_draft * (n_q // n_kv), tensor, status.data_ptr() if tensor else None, _DT[dt], _stream())
+        if code != 2 or not tensor:
+            break
+        tensor = 0                # (no tensor map of this layout)
+    _check(code, "tree_attention")
+    global LAUNCHES
+    LAUNCHES += 1                # the join of cut items is a kernel of its own
+
+
+_tree_facts = {}                  # (device, head size, page size, type): whether the tensor cores take it, (blocks, rows of an item) without and with them
+_TREE_ROWS_MAX = 0x7fffffff - 4096          # rows of a cache that a TMA coordinate can name
+
+
+def _refuse_tree_attention(q, out, k_cache, v_cache, q_start, kv_len, block_table, mask, n_kv, page_size, scale, max_draft) -> None:
+    """What is wrong with the arguments of tree_attention."""
     what = "tree_attention"
-    if q.dtype not in _DT or out.dtype != q.dtype or out.shape != q.shape or not q.is_contiguous() or not out.is_contiguous():
+    if q.dim() != 3 or q.dtype not in _DT or out.dtype != q.dtype or out.shape != q.shape or not q.is_contiguous() or not out.is_contiguous():
         raise KernelError(f"{what}: q and out are contiguous [drafts, heads, head size], both float32 or both bfloat16; got {q.dtype} {tuple(q.shape)}, {out.dtype} {tuple(out.shape)}")
-    if not (k_cache.dim() == 4 and k_cache.shape == v_cache.shape and k_cache.dtype == v_cache.dtype == q.dtype and k_cache.is_contiguous() and v_cache.is_contiguous()
+    T, n_q, d = q.shape
+    if not (k_cache.shape == v_cache.shape and k_cache.dtype == v_cache.dtype == q.dtype and k_cache.is_contiguous() and v_cache.is_contiguous()
             and tuple(k_cache.shape[1:]) == (n_kv, page_size, d)):
         raise KernelError(f"{what}: the caches are contiguous [pages, {n_kv}, {page_size}, {d}] of q's type; got {tuple(k_cache.shape)}, {tuple(v_cache.shape)}")
     if n_kv < 1 or n_q % n_kv or not 1 <= d <= 512:
         raise KernelError(f"{what}: {n_q} query heads over {n_kv} kv heads of size {d}: whole groups, sizes up to 512")
     if not 0.0 < scale < math.inf:
         raise KernelError(f"{what}: scale {scale} is not above 0")
+    B = block_table.shape[0] if block_table.dim() == 2 else -1
     _table(what, block_table, B)
     _index(what, "q_start", q_start, B + 1)
     _index(what, "kv_len", kv_len, B)
@@ -2525,27 +2578,7 @@ def tree_attention(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_
         raise KernelError(f"{what}: a mask row has a bit for every one of up to {max_draft} drafts; got {tuple(mask.shape)}")
     _index(what, "mask", mask, T * words)
     _same_device(what, q, out, k_cache, v_cache, q_start, kv_len, block_table, mask)
-    if T == 0 or B == 0:
-        return
-    lib, pages = _draft_lib(), k_cache.shape[0]
-    max_rows = max_draft * (n_q // n_kv)
-    # (the status words are made for the first device; none in a stream capture that comes before them)
-    status = _status_words(q.device) if lib.msgl_tree_attention_tensor(d, page_size, pages * n_kv * page_size, _DT[q.dtype]) else None
-    if status is not None and (status.get_device() != q.get_device() or (q.data_ptr() | out.data_ptr() | k_cache.data_ptr() | v_cache.data_ptr()) & 15):
-        status = None
-    for tensor in (1, 0) if status is not None else (0,):
-        blocks, rows = lib.msgl_tree_attention_blocks(d, tensor), lib.msgl_tree_attention_rows(tensor)
-        part = torch.empty(2 * blocks * rows * (d + 2) + 4 * blocks, dtype=torch.float32, device=q.device)
-        at = part.data_ptr()
-        part_ml, record = at + 4 * 2 * blocks * rows * d, at + 4 * 2 * blocks * rows * (d + 2)
-        code = lib.msgl_tree_attention(q.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), q_start.data_ptr(), kv_len.data_ptr(), block_table.data_ptr(),
-                                       mask.data_ptr(), B, T, n_q, n_kv, d, page_size, block_table.stride(0), width, words, pages, float(scale), at, part_ml, record,
-                                       blocks, max_rows, tensor, _ptr(status), _DT[q.dtype], _stream())
-        if code != 2:             # (2: no tensor map of this layout)
-            break
-    _check(code, what)
-    global LAUNCHES
-    LAUNCHES += 1                # the join of cut items is a kernel of its own
+    raise KernelError(f"{what}: arguments that do not go together")
 
 
 def _cache_groups(caches: Sequence[torch.Tensor], like: torch.Tensor):

@@ -15,7 +15,10 @@ def refused(match, call, *args, **kw):
 def test_plan_refuses():
     ok = dict(page_size=16, max_draft=8)
     refused("parents", ops.draft_plan, I(4).long(), I(2), I(2), I(2, 3), **ok)
-    refused("draft_lens", ops.draft_plan, I(4), I(3), I(2), I(2, 3), **ok)
+    refused("draft_lens", ops.draft_plan, I(4), I(2).long(), I(2), I(2, 3), **ok)
+    refused("cached", ops.draft_plan, I(4), I(3), I(2), I(2, 3), **ok)
+    refused("block_table", ops.draft_plan, I(4), I(3), I(3), I(2, 3), **ok)
+    refused("block_table", ops.draft_plan, I(4), I(3), I(3), I(3), **ok)
     refused("cached", ops.draft_plan, I(4), I(2), I(4)[::2], I(2, 3), **ok)
     refused("block_table", ops.draft_plan, I(4), I(2), I(2), I(3, 2).t(), **ok)
     refused("block_table", ops.draft_plan, I(4), I(2), I(2), I(2, 0), **ok)
@@ -92,7 +95,10 @@ def test_tree_attention_refuses():
     refused("q and out", f, q, q.bfloat16(), c, c, **ok)
     refused("q and out", f, q.half(), q.half(), c, c, **ok)
     refused("q and out", f, q.transpose(1, 2), q.transpose(1, 2), c, c, **ok)
+    refused("q and out", f, q[0], q[0], c, c, **ok)
     refused("caches", f, q, q, c, c[:, :, :8], **ok)
+    refused("caches", f, q, q, c[0], c[0], **ok)
+    refused("block_table", f, q, q, c, c, **dict(ok, block_table=I(3)))
     refused("caches", f, q, q, c.bfloat16(), c.bfloat16(), **ok)
     refused("caches", f, q, q, c, c, **dict(ok, page_size=8))
     refused("whole groups", f, torch.zeros(4, 7, 16), torch.zeros(4, 7, 16), c, c, **ok)
