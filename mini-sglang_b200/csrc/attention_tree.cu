@@ -49,9 +49,10 @@ struct TreeParams {
     float* part_o;                // [2 * blocks][ceil(d / 4)][ROWS][4]
     float* part_ml;               // [2 * blocks][ROWS][2]  (maximum in log2 units, sum of the weights)
     struct TreeRecord* record;    // [blocks]
-    int B, T, n_q, n_kv, d, page_size, page_shift, table_stride, table_width, words;
+    int B, T, n_q, n_kv, G, d, page_size, page_shift, table_stride, table_width, words;
     long long pages;
     float scale_log2;             // scale * log2(e)
+    int vectors;                  // rows of the caches are whole 16 bytes, on 16-byte boundaries
 };
 
 // ---------------------------------------------------------------------------------------
@@ -62,12 +63,12 @@ constexpr int TREE_SNAP = 1;      // a cut this close to an item's edge, or clos
 constexpr int TREE_SHARE = TREE_HEAD + TREE_SNAP + 1;      // a block's run is no shorter: so no piece of an item is empty and none lies in more than its blocks
 
 struct TreeSegment {              // tiles [t_lo, t_hi) of one item
-    int r, item, kvh, row0, rows; // row0: first row of the item among the request's n * G under the kv head
+    int r, kvh, row0, rows;       // row0: first row of the item among the request's n * G under the kv head
     int tok0, n, kv, base;        // the request's first draft in the stream, its drafts, its keys, those before the drafts
     int t_lo, t_hi, tiles;
 };
 
-struct TreeWalkState { int total, x_lo, x_hi, start, blocks, r, item; };      // (a walk put aside)
+struct TreeWalkState { int whole, rest, x_lo, x_hi, start, blocks, r, item; };      // (a walk put aside)
 struct TreeStart {                // what the block's walkers start with: the first segment, and the walk behind it
     TreeWalkState walk;
     TreeSegment first;
@@ -78,24 +79,32 @@ template <int ROWS, int KT>
 struct TreeWalk {
     const TreeParams& p;
     int blocks;                   // in use
-    int total, x_lo, x_hi;        // the work's length (the host has seen to it that it fits), this block's run
+    int whole, rest;              // the work's length (the host has seen to it that it fits) over them, and what is left
+    int x_lo, x_hi;               // this block's run
     int r = 0, item = 0;
     int start = 0;                // where the request's first item starts
 
     __device__ __forceinline__ TreeWalk(const TreeParams& q) : p(q) {}
-    __device__ __forceinline__ void store(TreeWalkState& s) const { s.total = total; s.x_lo = x_lo; s.x_hi = x_hi; s.start = start; s.blocks = blocks; s.r = r; s.item = item; }
-    __device__ __forceinline__ void load(const TreeWalkState& s) { total = s.total; x_lo = s.x_lo; x_hi = s.x_hi; start = s.start; blocks = s.blocks; r = s.r; item = s.item; }
-    struct Request { int tok0, n, kv, tiles, items; };
+    __device__ __forceinline__ void store(TreeWalkState& s) const { s.whole = whole; s.rest = rest; s.x_lo = x_lo; s.x_hi = x_hi; s.start = start; s.blocks = blocks; s.r = r; s.item = item; }
+    __device__ __forceinline__ void load(const TreeWalkState& s) { whole = s.whole; rest = s.rest; x_lo = s.x_lo; x_hi = s.x_hi; start = s.start; blocks = s.blocks; r = s.r; item = s.item; }
+    struct Request { int tok0, n, kv, tiles, groups, items; };      // groups: items under a kv head
     __device__ __forceinline__ Request request(int i) const {
         Request w;
         w.tok0 = min(max(p.q_start[i], 0), p.T);
         w.n = min(max(p.q_start[i + 1], w.tok0), p.T) - w.tok0;
         w.kv = (int)min((long long)max(p.kv_len[i], 0), (long long)p.table_width * p.page_size);
         w.tiles = max(1, (w.kv + KT - 1) / KT);
-        w.items = w.n > 0 ? p.n_kv * ((w.n * (p.n_q / p.n_kv) + ROWS - 1) / ROWS) : 0;
+        w.groups = (w.n * p.G + ROWS - 1) / ROWS;
+        w.items = p.n_kv * w.groups;
         return w;
     }
-    __device__ __forceinline__ int cut_at(int k) const { const int q = total / blocks; return q * k + (total - q * blocks) * k / blocks; }      // floor(total k / blocks)
+    // floor(a / b) of whole numbers below 2^24, by the reciprocal: one thread finds the first segment for all, and waits for every division
+    static __device__ __forceinline__ int quotient(int a, int b) {
+        int q = (int)(__fdividef((float)a, (float)b));
+        q -= q * b > a ? 1 : 0;
+        return q + (a - q * b >= b ? 1 : 0);
+    }
+    __device__ __forceinline__ int cut_at(int k) const { return whole * k + quotient(rest * k, blocks); }      // floor(total k / blocks); (k and rest: some hundreds)
     // the tile that a cut at x falls on, in an item that starts at `s`
     __device__ __forceinline__ int tile_at(int x, int s, int tiles) const {
         const int t = x - s - TREE_HEAD;
@@ -116,11 +125,12 @@ struct TreeWalk {
         if (lane == 31) sums[warp] = upto;
         if (tid == 0) to.work = 0;
         __syncthreads();
-        total = 0;
-        int before = upto - mine;
+        int before = upto - mine, total = 0;
         for (int w = 0; w < n_warps; ++w) { if (w < warp) before += sums[w]; total += sums[w]; }
         blocks = max(1, min(nb, total / TREE_SHARE));
         if (total == 0 || j >= blocks) return false;
+        whole = total / blocks;
+        rest = total - whole * blocks;
         x_lo = cut_at(j);
         x_hi = cut_at(j + 1);
         if (x_lo >= before && x_lo < before + mine) {
@@ -149,8 +159,10 @@ struct TreeWalk {
                 if (s >= x_hi) return false;
                 const int lo = x_lo > s ? tile_at(x_lo, s, w.tiles) : 0, hi = x_hi < s + len ? tile_at(x_hi, s, w.tiles) : w.tiles;
                 if (lo >= hi) continue;
-                const int groups = w.items / p.n_kv, rows = w.n * (p.n_q / p.n_kv);
-                g.r = r; g.item = item; g.kvh = item / groups; g.row0 = (item - g.kvh * groups) * ROWS; g.rows = min(ROWS, rows - g.row0);
+                g.r = r;
+                g.kvh = w.groups == 1 ? item : item / w.groups;
+                g.row0 = (item - g.kvh * w.groups) * ROWS;
+                g.rows = min(ROWS, w.n * p.G - g.row0);
                 g.tok0 = w.tok0; g.n = w.n; g.kv = w.kv; g.base = w.kv - w.n;
                 g.t_lo = lo; g.t_hi = hi; g.tiles = w.tiles;
                 ++item;
@@ -204,8 +216,21 @@ constexpr int TS_ROWS = 32, TS_KT = 32, TS_THREADS = 256;
 struct TreeYes { static constexpr bool value = true; };
 struct TreeNo { static constexpr bool value = false; };
 
+template <typename T> struct TsVec;                  // 16 bytes of a row; MOST: of them a thread has for 128 columns
+template <> struct TsVec<float> {
+    static constexpr int N = 4, MOST = 4;
+    static __device__ __forceinline__ void store(float* to, const uint4& v) { *reinterpret_cast<uint4*>(to) = v; }
+};
+template <> struct TsVec<__nv_bfloat16> {
+    static constexpr int N = 8, MOST = 2;
+    static __device__ __forceinline__ void store(float* to, const uint4& v) {
+        *reinterpret_cast<uint4*>(to) = make_uint4(v.x << 16, v.x & 0xffff0000u, v.y << 16, v.y & 0xffff0000u);
+        *reinterpret_cast<uint4*>(to + 4) = make_uint4(v.z << 16, v.z & 0xffff0000u, v.w << 16, v.w & 0xffff0000u);
+    }
+};
+
 template <typename T, int CB>
-__global__ void __launch_bounds__(TS_THREADS) tree_simt_kernel(const TreeParams p) {
+__global__ void __launch_bounds__(TS_THREADS, CB <= 2 ? 2 : 1) tree_simt_kernel(const TreeParams p) {
     extern __shared__ __align__(16) float ts_smem[];
     const int d = p.d, pitch = CB * 128 + 4, d4 = (d + 3) >> 2;
     float* Qs = ts_smem;                             // [32][pitch]; columns from d on are zero
@@ -213,7 +238,7 @@ __global__ void __launch_bounds__(TS_THREADS) tree_simt_kernel(const TreeParams 
     float* Vs = Ks + TS_KT * pitch;                  // [32][pitch]
     float* Ps = Vs + TS_KT * pitch;                  // [8 warps][32 keys][4 rows]
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, j = blockIdx.x;
-    const int G = p.n_q / p.n_kv;
+    const int G = p.G;
     pdl_launch_dependents();
     pdl_wait();
     pdl_after_wait();
@@ -226,9 +251,10 @@ __global__ void __launch_bounds__(TS_THREADS) tree_simt_kernel(const TreeParams 
         for (bool more = true; more; more = walk.next(g)) {
             const T* q = reinterpret_cast<const T*>(p.q);
             __syncthreads();                         // the segment before has been read
-            for (int i = tid; i < TS_ROWS * d; i += TS_THREADS) {
-                const int row = i / d, c = i - row * d, rr = g.row0 + row;
-                Qs[row * pitch + c] = row < g.rows ? to_f32<T>(q[((size_t)(g.tok0 + rr / G) * p.n_q + (size_t)g.kvh * G + rr % G) * d + c]) : 0.f;
+            {
+                const int row = tid >> 3, rr = g.row0 + row;
+                const T* src = q + ((size_t)(g.tok0 + rr / G) * p.n_q + (size_t)g.kvh * G + rr % G) * d;
+                for (int c = tid & 7; c < d; c += 8) Qs[row * pitch + c] = row < g.rows ? to_f32<T>(src[c]) : 0.f;
             }
             float o[4][CB][4], m_run[4], l_run[4];
             const unsigned* row_mask[4];
@@ -241,24 +267,50 @@ __global__ void __launch_bounds__(TS_THREADS) tree_simt_kernel(const TreeParams 
 #pragma unroll
                 for (int b = 0; b < CB; ++b) o[a][b][0] = o[a][b][1] = o[a][b][2] = o[a][b][3] = 0.f;
             }
+            // a thread fetches pieces of one key and its value, eight threads a key: 16 bytes at a time where the rows are made of them, the next tile's while
+            // this one is worked on (head sizes up to 128)
+            const int my_key = tid >> 3, sub = tid & 7;
+            uint4 raw_k[TsVec<T>::MOST * CB], raw_v[TsVec<T>::MOST * CB];
+            auto place = [&](int key) -> long long {         // element offset of the key's row, or -1
+                if (key >= g.kv) return -1;
+                const int pi = tree_page(p, key), id = p.table[(size_t)g.r * p.table_stride + pi];
+                return id >= 0 && id < p.pages ? (((long long)id * p.n_kv + g.kvh) * p.page_size + (key - pi * p.page_size)) * d : -1;
+            };
+            auto fetch = [&](int t) {
+                const long long at = place(t * TS_KT + my_key);
+#pragma unroll
+                for (int i = 0; i < TsVec<T>::MOST * CB; ++i) {
+                    const int c = (sub + 8 * i) * TsVec<T>::N;
+                    const bool there = at >= 0 && c < d;
+                    raw_k[i] = there ? *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.k_cache) + at + c) : make_uint4(0u, 0u, 0u, 0u);
+                    raw_v[i] = there ? *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.v_cache) + at + c) : make_uint4(0u, 0u, 0u, 0u);
+                }
+            };
+            auto put_down = [&]() {
+#pragma unroll
+                for (int i = 0; i < TsVec<T>::MOST * CB; ++i) {
+                    const int c = (sub + 8 * i) * TsVec<T>::N;
+                    if (c >= d) continue;
+                    TsVec<T>::store(Ks + my_key * pitch + c, raw_k[i]);
+                    TsVec<T>::store(Vs + my_key * pitch + c, raw_v[i]);
+                }
+            };
+            if (p.vectors && CB == 1) fetch(g.t_lo);
             for (int t = g.t_lo; t < g.t_hi; ++t) {
                 const int key0 = t * TS_KT;
                 __syncthreads();                     // the tile before has been read (and Q written)
-                for (int i = tid; i < TS_KT * d; i += TS_THREADS) {
-                    const int row = i / d, c = i - row * d, key = key0 + row;
-                    float kv = 0.f, vv = 0.f;
-                    if (key < g.kv) {
-                        const int pi = tree_page(p, key), id = p.table[(size_t)g.r * p.table_stride + pi];
-                        if (id >= 0 && id < p.pages) {
-                            const size_t at = (((size_t)id * p.n_kv + g.kvh) * p.page_size + (key - pi * p.page_size)) * d + c;
-                            kv = to_f32<T>(reinterpret_cast<const T*>(p.k_cache)[at]);
-                            vv = to_f32<T>(reinterpret_cast<const T*>(p.v_cache)[at]);
-                        }
+                if (p.vectors) {
+                    if (CB > 1) fetch(t);
+                    put_down();
+                } else {
+                    const long long at = place(key0 + my_key);
+                    for (int c = sub; c < d; c += 8) {
+                        Ks[my_key * pitch + c] = at >= 0 ? to_f32<T>(reinterpret_cast<const T*>(p.k_cache)[at + c]) : 0.f;
+                        Vs[my_key * pitch + c] = at >= 0 ? to_f32<T>(reinterpret_cast<const T*>(p.v_cache)[at + c]) : 0.f;
                     }
-                    Ks[row * pitch + c] = kv;
-                    Vs[row * pitch + c] = vv;
                 }
                 __syncthreads();
+                if (p.vectors && CB == 1 && t + 1 < g.t_hi) fetch(t + 1);
                 if (4 * warp >= g.rows) continue;    // (no row of this warp)
                 float s[4] = {0.f, 0.f, 0.f, 0.f};
                 for (int c = 0; c < d4; ++c) {
@@ -353,7 +405,7 @@ __global__ void __launch_bounds__(TJ_WARPS * 32) tree_join_kernel(const TreePara
     const int4 rec = *reinterpret_cast<const int4*>(p.record + j);           // pieces, rows, first draft, first row
     const int pieces = rec.x, kvh = p.record[j].kvh;
     if (pieces == 0 || row >= rec.y) return;
-    const int G = p.n_q / p.n_kv, d = p.d, rr = rec.w + row, tok0 = rec.z;
+    const int G = p.G, d = p.d, rr = rec.w + row, tok0 = rec.z;
     auto slot = [&](int k) { return (size_t)(2 * (j + k) + (k == 0 ? 1 : 0)); };
     auto ml_of = [&](int k) { return *reinterpret_cast<const float2*>(p.part_ml + (slot(k) * ROWS + row) * 2); };
     float M = -INFINITY, L = 0.f;
@@ -416,7 +468,7 @@ static void tree_join(const TreeParams& p, int blocks, int max_rows, cudaStream_
 
 #include "attention_tree_tc.cuh"
 
-static int tree_simt_blocks_per_sm(int d) { return d <= 128 ? 4 : d <= 256 ? 2 : 1; }
+static int tree_simt_blocks_per_sm(int d) { return d <= 256 ? 2 : 1; }
 static size_t tree_simt_smem(int cb) { return ((size_t)(TS_ROWS + 2 * TS_KT) * (cb * 128 + 4) + 8 * TS_KT * 4) * sizeof(float); }
 
 // Whether the tensor cores take a launch: bfloat16, head sizes 64 and 128, pages that TMA can fetch, a cache whose rows a coordinate can name.
@@ -469,11 +521,12 @@ MSGL_API int msgl_tree_attention(const void* q, void* out, const void* k_cache, 
     TreeParams p;
     p.q = q; p.out = out; p.k_cache = k_cache; p.v_cache = v_cache; p.q_start = q_start; p.kv_len = kv_len; p.table = table; p.mask = (const unsigned*)mask;
     p.part_o = part_o; p.part_ml = part_ml; p.record = (TreeRecord*)record;
-    p.B = B; p.T = T; p.n_q = n_q; p.n_kv = n_kv; p.d = d; p.page_size = page_size; p.table_stride = table_stride; p.table_width = table_width; p.words = words;
+    p.B = B; p.T = T; p.n_q = n_q; p.n_kv = n_kv; p.G = n_q / n_kv; p.d = d; p.page_size = page_size; p.table_stride = table_stride; p.table_width = table_width; p.words = words;
     p.pages = pages;
     p.page_shift = -1;
     if ((page_size & (page_size - 1)) == 0) { int sh = 0; while ((1 << sh) < page_size) ++sh; p.page_shift = sh; }
     p.scale_log2 = scale * 1.4426950408889634f;
+    p.vectors = (((uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)(d * (dtype == MSGL_F32 ? 4 : 2))) & 15) == 0;
     if (tensor) {
         if (status == nullptr || pages < 1 || !msgl_tree_attention_tensor(d, page_size, pages * n_kv * page_size, dtype)) return MSGL_ERR_SIZE;
         if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_cache | (uintptr_t)v_cache) & 15) return MSGL_ERR_ALIGN;

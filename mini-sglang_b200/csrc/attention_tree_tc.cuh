@@ -123,7 +123,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const TreeParams
     auto bar_vf = [&](int st) { return smem_base + 128u + 8u * st; };
     auto bar_vr = [&](int st) { return smem_base + 160u + 8u * st; };
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, j = blockIdx.x;
-    const int G = p.n_q / p.n_kv;
+    const int G = p.G;
 
     if (tid == 0) {
         for (int x = 0; x < 2; ++x) { tc_mbar_init(bar_s(x), 1); tc_mbar_init(bar_p(x), 8); tc_mbar_init(bar_o(x), 1); }
