@@ -1,5 +1,5 @@
 from .args import EngineArgs, ServerArgs
-from .step import ModelRunner, StepEntry
+from .step import DraftEntry, ModelRunner, StepEntry
 
 
 def __getattr__(name):

@@ -30,6 +30,7 @@ def main(argv=None) -> int:
     ap.add_argument("--temperature", type=float, default=0.0)
     ap.add_argument("--max_new_tokens", type=int, default=64)
     ap.add_argument("--ignore_eos", action="store_true")
+    ap.add_argument("--logprobs", type=int, default=None, help="With every token its log probability, the entropy of its distribution and that many most probable tokens.")
     ns = ap.parse_args(argv)
     args = EngineArgs.from_cli_args(ns)
 
@@ -48,7 +49,8 @@ def main(argv=None) -> int:
     from .engine import Engine
 
     engine = Engine(args)
-    sp = {"temperature": ns.temperature, "max_new_tokens": ns.max_new_tokens, "ignore_eos": ns.ignore_eos}
+    sp = {"temperature": ns.temperature, "max_new_tokens": ns.max_new_tokens, "ignore_eos": ns.ignore_eos,
+          "logprobs": ns.logprobs}
     reqs = [engine.add_request(prompt=p if kind == "text" else None, sampling_params=sp,
                                input_ids=p if kind == "ids" else None) for kind, p in prompts]
     import time

@@ -96,6 +96,7 @@ class Engine:
         import dataclasses as _dc
         params = (_dc.replace(sampling_params) if isinstance(sampling_params, SamplingParams)
                   else SamplingParams.init_from_dict(sampling_params))
+        params.check_logprobs()       # (refused here as well, for parameters that were not made from a dict)
         return Req(uuid.uuid4().hex, input_ids, params, self.spec.eos_token_ids)
 
     def add_request(self, prompt=None, sampling_params=None, input_ids=None) -> Req:
@@ -158,10 +159,14 @@ class Engine:
     def _result(self, req: Req, t_start: float) -> Dict:
         out = req.output
         text = self.tokenizer.decode(out) if self.tokenizer is not None else None
-        return {"text": text, "token_ids": list(out),
-                "meta_info": {"id": req.rid, "finish_reason": req.finish_reason.to_json() if req.finish_reason else None,
-                              "prompt_tokens": req.n_prompt, "completion_tokens": len(out),
-                              "cached_tokens": req.cached_tokens, "e2e_latency": time.time() - t_start}}
+        res = {"text": text, "token_ids": list(out),
+               "meta_info": {"id": req.rid, "finish_reason": req.finish_reason.to_json() if req.finish_reason else None,
+                             "prompt_tokens": req.n_prompt, "completion_tokens": len(out),
+                             "cached_tokens": req.cached_tokens, "e2e_latency": time.time() - t_start}}
+        if req.params.logprobs is not None:          # one entry a generated token
+            res["logprobs"] = [{"token": t, "logprob": lp, "entropy": entropy, "top": [{"token": a, "logprob": b} for a, b in top]}
+                               for t, (lp, entropy, top) in zip(out, req.logprobs)]
+        return res
 
     def generate(self, prompt: Union[None, str, List[str]] = None, sampling_params: Union[None, Dict, List[Dict]] = None,
                  input_ids: Union[None, List[int], List[List[int]]] = None, stream: bool = False):

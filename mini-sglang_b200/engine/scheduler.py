@@ -86,6 +86,8 @@ class Req:
         # seed, or else its number among the requests that its scheduler was given (set there), so that an engine with
         # the same seed and the same requests in the same order draws the same numbers whatever else ran in the process
         self.rng_key: Optional[int] = params.seed
+        # with params.logprobs, for every generated token that the host has seen: (log probability, entropy, [(token, its log probability), ...])
+        self.logprobs: List[Tuple[float, float, List[Tuple[int, float]]]] = []
         self.retractions = 0
         self.t_arrive = time.time()
         self.t_first_token: Optional[float] = None
@@ -121,11 +123,12 @@ class Req:
 class _InFlight:
     """A launched step whose sampled tokens have not been read yet."""
 
-    def __init__(self, reqs, ids, host, event):
+    def __init__(self, reqs, ids, host, event, scores=None):
         self.reqs: List[Req] = reqs           # the requests sampled in that step, in row order
         self.ids = ids                        # their tokens: device tensor (or anything with tolist())
         self.host = host                      # pinned mirror the copy goes to (None: read `ids` itself)
         self.event = event
+        self.scores = scores                  # (rows with log probabilities, TokenLogprobs of them: pinned mirrors where there is an event)
         self.placeholder: Dict[str, int] = {}  # rid -> index in req.tokens that stands for this step's token
         self.dead: set = set()                # rids whose token of this step is dropped
 
@@ -590,6 +593,10 @@ class Scheduler:
             return None
         ids = self.sampler.sample(logits, [r.params.temperature for r in sampled],
                                   [r.rng_key for r in sampled], [r.n_output for r in sampled])
+        scored = [i for i, r in enumerate(sampled) if r.params.logprobs is not None]
+        scores = None
+        if scored:
+            scores = (scored, self.sampler.logprobs(logits, ids, scored, max(sampled[i].params.logprobs for i in scored)))
         host = event = None
         if self.lookahead and getattr(ids, "is_cuda", False):
             import torch
@@ -599,9 +606,11 @@ class Scheduler:
                 self._host_ids[k] = torch.empty(max(1024, len(sampled)), dtype=ids.dtype, pin_memory=True)
             host = self._host_ids[k][:len(sampled)]
             host.copy_(ids, non_blocking=True)
+            if scores is not None:
+                scores = (scored, type(scores[1])(*(torch.empty(t.shape, dtype=t.dtype, pin_memory=True).copy_(t, non_blocking=True) for t in scores[1])))
             event = torch.cuda.Event()
             event.record()
-        return _InFlight(sampled, ids, host, event)
+        return _InFlight(sampled, ids, host, event, scores)
 
     def _collect(self, flight: _InFlight, successor: Optional[_InFlight]) -> List[StepOutput]:
         """Read a launched step's tokens and do what follows from them: append, finish, free.
@@ -614,10 +623,18 @@ class Scheduler:
         else:
             ids = flight.ids.tolist() if hasattr(flight.ids, "tolist") else list(flight.ids)
         now = time.time()
-        for r, tok in zip(flight.reqs, ids):
+        scores = {}
+        if flight.scores is not None:
+            rows, s = flight.scores
+            scores = {row: entry for row, *entry in zip(rows, s.logprobs.tolist(), s.entropy.tolist(), s.top_tokens.tolist(), s.top_logprobs.tolist())}
+        for row, (r, tok) in enumerate(zip(flight.reqs, ids)):
             if r.rid in flight.dead or r.finished:
                 continue
             tok = int(tok)
+            if row in scores:
+                lp, entropy, top_ids, top_lps = scores[row]
+                n = r.params.logprobs
+                r.logprobs.append((lp, entropy, list(zip(top_ids[:n], top_lps[:n]))))
             at = flight.placeholder.get(r.rid)
             if at is None:
                 r.tokens.append(tok)

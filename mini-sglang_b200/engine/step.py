@@ -28,7 +28,7 @@ import torch
 from .. import ops
 from ..cache import CacheManager, OutOfPages, PagedKVNeed, StateNeed, keys_seen
 from ..config import ModelSpec, load_config
-from ..parts import BuildEnv, DecoderModel, GroupContext, KVCacheView, StateCacheView, StepContext, Workspace
+from ..parts import BuildEnv, DecoderModel, DraftContext, GroupContext, KVCacheView, StateCacheView, StepContext, Workspace
 from ..weights import CheckpointSource, RandomSource
 
 DTYPES = {"bfloat16": torch.bfloat16, "bf16": torch.bfloat16, "float32": torch.float32, "fp32": torch.float32}
@@ -51,6 +51,15 @@ class StepEntry:
     slot: int
     tokens: Sequence[int]
     want: Sequence[int] = ()          # places among `tokens` whose logits are wanted
+
+
+@dataclasses.dataclass
+class DraftEntry:
+    """A tree of drafted tokens of one request.  tokens[0] is its newest token, which is not in the cache yet; parents[i] is the index of
+    the token that tokens[i] follows (an earlier one; parents[0] is -1).  None: each follows the one before it."""
+    slot: int
+    tokens: Sequence[int]
+    parents: Optional[Sequence[int]] = None
 
 
 def _align4(n: int) -> int:
@@ -622,6 +631,103 @@ class ModelRunner:
         for e in entries:
             self.mgr.commit(e.slot, len(e.tokens))
         return logits
+
+    # -- drafted tokens ------------------------------------------------------------------------
+    def drafts_supported(self) -> bool:
+        """Whether `verify` takes this model: every mixer attends to all keys of a paged cache (no windows, chunks or per-request states)."""
+        return bool(self.mgr.groups) and not self.mgr.state_ids and all(g.span is None for g in self.mgr.groups) and \
+            all(n.library == "attention" and (n.v_head_dim or n.head_dim) == n.head_dim <= 512 for n in self.mgr.needs.values())
+
+    @torch.no_grad()
+    def verify(self, entries: Sequence[DraftEntry], sampler, temperatures: Optional[Sequence[float]] = None, row_keys: Optional[Sequence[int]] = None,
+               steps: Optional[Sequence[int]] = None) -> List[List[int]]:
+        """Run a batch of drafted trees through the model and keep, of each, the longest path from its first token whose every token is the one that
+        the model put after its parent -> per entry the model's tokens after those of the path: its next one to len(tokens) tokens, the last of which no draft foresaw.
+
+        `sampler` (a Sampler) draws the model's token after every draft as it would after the same tokens fed one by one: with the entry's
+        temperature (default 0), its key and, for a draft of depth d, step + d (default 0).  So the tokens are those of plain decoding, drawn
+        with the same noise.  The path's keys and values are in the cache afterwards, in order; the rest is forgotten."""
+        if not self.drafts_supported():
+            raise ValueError("drafted tokens need a model whose layers attend to all keys of a paged cache")
+        entries = list(entries)
+        if not entries:
+            return []
+        V, lens, parents, depths = self.vocab_size, [], [], []
+        if len({e.slot for e in entries}) != len(entries):
+            raise ValueError("a request can bring one tree a step")
+        for e in entries:
+            n = len(e.tokens)
+            up = list(e.parents) if e.parents is not None else list(range(-1, n - 1))
+            if not 1 <= n <= ops.MAX_DRAFTS or len(up) != n:
+                raise ValueError(f"slot {e.slot}: 1 to {ops.MAX_DRAFTS} drafted tokens with a parent each")
+            if up[0] != -1 or any(not 0 <= p < i for i, p in enumerate(up) if i):
+                raise ValueError(f"slot {e.slot}: the first draft has parent -1, every other an earlier draft")
+            if min(e.tokens) < 0 or max(e.tokens) >= V:
+                raise ValueError(f"token id outside [0, {V}) in the drafts of slot {e.slot}")
+            depth = [0] * n
+            for i in range(1, n):
+                depth[i] = depth[up[i]] + 1
+            lens.append(n)
+            parents.append(up)
+            depths.append(depth)
+        short = [max(0, n - g.pool.available) for n, g in zip(map(sum, zip(*(self.mgr.pages_needed(e.slot, n) for e, n in zip(entries, lens)))), self.mgr.groups)]
+        if any(short):
+            raise OutOfPages(f"the step needs {short} more pages than are free (per group)")
+        reserved: List[int] = []
+        try:
+            for e, n in zip(entries, lens):
+                self.mgr.reserve(e.slot, n)
+                reserved.append(e.slot)
+            kept, tokens = self._verify(entries, lens, parents, depths, sampler, temperatures, row_keys, steps)
+            for e, k in zip(entries, kept):
+                self.mgr.commit(e.slot, k)
+        finally:
+            for slot in reserved:
+                self.mgr.unreserve(slot)
+        return [row[:k] for row, k in zip(tokens, kept)]
+
+    def _verify(self, entries, lens, parents, depths, sampler, temperatures, row_keys, steps):
+        B, T, most, P = len(entries), sum(lens), max(lens), self.page_size
+        cached = [int(self.mgr.length[e.slot]) for e in entries]
+        group = self.mgr.groups[0]
+        mp = max(int(group.n_pages[e.slot]) for e in entries)
+        # one staging copy: tokens, parents, lengths, cached lengths, slots, block-table rows
+        size = 2 * T + 3 * B + B * mp
+        host_t, idx = self._pinned_buffer(size)
+        host = host_t.numpy()
+        host[:T] = [t for e in entries for t in e.tokens]
+        host[T:2 * T] = [p for up in parents for p in up]
+        off = 2 * T
+        host[off:off + B], host[off + B:off + 2 * B], host[off + 2 * B:off + 3 * B] = lens, cached, [e.slot for e in entries]
+        rows = host[off + 3 * B:size].reshape(B, mp)
+        rows[:] = 0
+        for r, e in enumerate(entries):
+            row = self.mgr.block_table_row(0, e.slot)
+            rows[r, :len(row)] = row
+        dev = torch.empty(size, dtype=torch.int32, device=self.device)
+        dev.copy_(host_t[:size], non_blocking=True)
+        self._mark(idx)
+        self.last_h2d_bytes = 4 * size
+        self.last_step_used_graph = False
+        tokens, up = dev[:T], dev[T:2 * T]
+        table = dev[off + 3 * B:].view(B, mp)
+        plan = ops.draft_plan(up, dev[off:off + B], dev[off + B:off + 2 * B], table, page_size=P, max_draft=most)
+        plain = GroupContext(block_table=table, out_loc=plan.out_loc, nsplit=None, max_split=1, window=None)
+        ctx = StepContext(T=T, B=B, page_size=P, input_ids=tokens, positions=plan.positions, q_start=plan.q_start, kv_len=plan.kv_len, token_req=plan.token_req,
+                          slots=dev[off + 2 * B:off + 3 * B], groups=[plain] * len(self._plan_group), host_q_lens=list(lens),
+                          host_kv_lens=[c + n for c, n in zip(cached, lens)], host_slots=[e.slot for e in entries], workspace=self.workspace,
+                          drafts=DraftContext(plan.mask, most))
+        ops.raise_if_failed()
+        logits = self.model.forward(ctx, self._caches(ctx), None)
+        expand = lambda given, default: [v for n, v in zip(lens, given if given is not None else [default] * B) for _ in range(n)]      # noqa: E731
+        step0 = expand(steps, 0)
+        following = sampler.sample(logits, expand(temperatures, 0.0), expand(row_keys, 0), [s + d for s, d in zip(step0, (d for part in depths for d in part))])
+        got = ops.draft_accept(tokens, up, following, plan.q_start, max_draft=most, kv_len=plan.kv_len, block_table=table,
+                               caches=[c for pair in self.storage.kv.values() for c in pair])
+        ops.poll_status()
+        out = torch.cat((got.kept[:, None], got.tokens), dim=1).tolist()          # (waits for the step)
+        ops.raise_if_failed(wait=True)
+        return [row[0] for row in out], [row[1:] for row in out]
 
     def _mark(self, idx: int) -> None:
         ev = self._pinned_ev[idx]

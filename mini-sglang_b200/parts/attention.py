@@ -114,7 +114,7 @@ def paged_attend(q: torch.Tensor, out: torch.Tensor, ctx: StepContext, cache: KV
     run on the tcgen05 prefill kernel on pairs of query tiles where it applies and on the mma kernels otherwise.  null_log2
     (a term in every softmax's denominator that has no key), gate (sigmoids on the output), chunk (keys are seen within chunks
     of the sequence only) and diff (query heads are pairs of maps, `out` holds half as many heads; the mma kernels only):
-    `ops.attention`."""
+    `ops.attention`.  A step of drafted tokens (ctx.drafts) goes to `ops.tree_attention`."""
     plain = keep_first == 0 and bias_log2 is None
     if not plain and not use_mma:
         raise ValueError("kept first tokens and a distance bias are taken by the bfloat16 mma kernels only")
@@ -123,6 +123,12 @@ def paged_attend(q: torch.Tensor, out: torch.Tensor, ctx: StepContext, cache: KV
         raise ValueError("chunks and pairs of maps go with neither kept first tokens nor a distance bias")
     if diff is not None and (joined or not use_mma):
         raise ValueError("pairs of maps are taken by the bfloat16 mma kernels only, without a further term or a gate")
+    if ctx.drafts is not None:
+        if not plain or joined or window or chunk or diff is not None:
+            raise ValueError("drafted tokens are taken by attention over all keys only: no window, chunks, bias, further term, gate or pairs of maps")
+        ops.tree_attention(q, out, cache.k, cache.v, q_start=ctx.q_start, kv_len=ctx.kv_len, block_table=cache.group.block_table, mask=ctx.drafts.mask, n_kv=n_kv,
+                           page_size=cache.page_size, scale=scale, max_draft=ctx.drafts.max_draft)
+        return
     extra = dict(joined, chunk=chunk, diff=diff) if plain else dict(keep_first=keep_first, bias_log2=bias_log2, **joined)
     g = cache.group
     G = n_q // n_kv

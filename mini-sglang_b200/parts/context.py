@@ -29,6 +29,13 @@ class GroupContext:
 
 
 @dataclasses.dataclass
+class DraftContext:
+    """A step whose requests bring trees of drafted tokens (ops.draft_plan)."""
+    mask: torch.Tensor                 # [T, words] int32: the drafts of its request that a draft sees
+    max_draft: int                     # most drafts of a request
+
+
+@dataclasses.dataclass
 class StepContext:
     T: int
     B: int
@@ -46,6 +53,7 @@ class StepContext:
     uniform_decode: bool = False       # every request brings exactly one token (fixed launch shapes)
     all_rows_wanted: bool = False      # the wanted rows are all T rows in order (what a decode step asks for)
     workspace: Optional["Workspace"] = None
+    drafts: Optional[DraftContext] = None       # the tokens are drafts: one sees its ancestors among them, not all that lie before it
     # what parts of one forward pass hand to each other within the step (the first layer's values that later layers blend
     # with their own, the cos | sin rows of the step's positions that layers with the same encoding share); empty at the
     # start of every step

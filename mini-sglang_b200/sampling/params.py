@@ -3,18 +3,26 @@ from __future__ import annotations
 import dataclasses
 from typing import Any, Dict, Optional
 
+MAX_LOGPROBS = 32          # alternatives a token (what the kernel keeps)
+
 
 @dataclasses.dataclass
 class SamplingParams:
     """Names, meanings and defaults of mini_sglang/managers/sampling_params.py:4-19.
     temperature 0 is greedy; eos_token_id -1 means "the model's own end tokens"; `seed` (ours)
-    fixes the noise of temperature sampling for the request."""
+    fixes the noise of temperature sampling for the request; `logprobs` (ours): with every token its log probability
+    under the model (before the temperature), the entropy of its distribution and that many most probable tokens."""
 
     temperature: float = 0.0
     max_new_tokens: int = 64
     ignore_eos: bool = False
     eos_token_id: int = -1
     seed: Optional[int] = None
+    logprobs: Optional[int] = None
+
+    def check_logprobs(self) -> None:
+        if self.logprobs is not None and not 0 <= self.logprobs <= MAX_LOGPROBS:
+            raise ValueError(f"logprobs must be between 0 and {MAX_LOGPROBS}")
 
     @classmethod
     def init_from_dict(cls, d: Optional[Dict[str, Any]]) -> "SamplingParams":
@@ -28,4 +36,5 @@ class SamplingParams:
             raise ValueError("temperature must be >= 0")
         if p.max_new_tokens < 1:
             raise ValueError("max_new_tokens must be >= 1")
+        p.check_logprobs()
         return p

@@ -29,3 +29,11 @@ class Sampler:
         host[2] = torch.tensor([s & 0x7FFFFFFF for s in steps], dtype=torch.int32)
         dev = host.to(self.device, non_blocking=True)
         return ops.sample(logits, dev[0].view(torch.float32), dev[1], dev[2], self.seed)
+
+    def logprobs(self, logits: torch.Tensor, ids: torch.Tensor, rows: Sequence[int], top: int) -> ops.TokenLogprobs:
+        """Log probabilities of the tokens just sampled in `rows` of the batch, on the device: of the model's own distributions,
+        before any temperature."""
+        if len(rows) < logits.shape[0]:
+            pick = torch.tensor(list(rows), dtype=torch.int64, pin_memory=True).to(self.device, non_blocking=True)
+            logits, ids = logits.index_select(0, pick), ids.index_select(0, pick)
+        return ops.token_logprobs(logits, ids, min(top, logits.shape[1]))
