@@ -115,7 +115,8 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const TreeParams
     const unsigned smem0 = (smem_base + 512u + 1280u * 4u + 1023u) & ~1023u;
     const unsigned q_s = smem0, k_s = q_s + 2u * C::TILE, v_s = k_s + ST * C::TILE;
     auto bar_s = [&](int x) { return smem_base + 8u * x; };                  // S_X is in TMEM (tensor core commits)
-    auto bar_p = [&](int x) { return smem_base + 16u + 8u * x; };            // P_X is in TMEM, O_X rescaled (8 softmax warps)
+    // P_X's first 32 of every 64 keys are in TMEM and O_X is rescaled, and the others are there as well (8 softmax warps each)
+    auto bar_p = [&](int x, int part) { return smem_base + (part ? 192u : 16u) + 8u * x; };
     auto bar_o = [&](int x) { return smem_base + 32u + 8u * x; };            // P V_X is done (tensor core commits)
     const unsigned bar_q = smem_base + 48u, bar_vt = smem_base + 56u;        // the segment's Q is there (512 threads); a V tile that is looked at has come
     auto bar_kf = [&](int st) { return smem_base + 64u + 8u * st; };         // stage holds a tile of keys (TMA bytes)
@@ -126,7 +127,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const TreeParams
     const int G = p.G;
 
     if (tid == 0) {
-        for (int x = 0; x < 2; ++x) { tc_mbar_init(bar_s(x), 1); tc_mbar_init(bar_p(x), 8); tc_mbar_init(bar_o(x), 1); }
+        for (int x = 0; x < 2; ++x) { tc_mbar_init(bar_s(x), 1); tc_mbar_init(bar_p(x, 0), 8); tc_mbar_init(bar_p(x, 1), 8); tc_mbar_init(bar_o(x), 1); }
         for (int st = 0; st < ST; ++st) { tc_mbar_init(bar_kf(st), 1); tc_mbar_init(bar_kr(st), 1); tc_mbar_init(bar_vf(st), 1); tc_mbar_init(bar_vr(st), 1); }
         tc_mbar_init(bar_q, TT_SOFT); tc_mbar_init(bar_vt, 1);
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
@@ -224,15 +225,22 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const TreeParams
             auto issue_o = [&](int s) {                               // O_X += P_X V
                 const int x = s & 1;
                 const unsigned c = tile_of(s), st = c % ST;
-                ok = wait(bar_p(x), phase_p[x]);
-                phase_p[x] ^= 1u;
-                if (ok && (!dual || x == 0)) ok = wait(bar_vf(st), (c / ST) & 1);
-                if (!ok) return;
-                tc_fence_async_smem(); tc_fence_after();
+                if (!dual || x == 0) ok = wait(bar_vf(st), (c / ST) & 1);
                 const unsigned long long dv_st = dv + st * step;
                 const unsigned t_o = tm + 256u + (unsigned)x * 128u, t_p = tm + (unsigned)x * 128u;
+                // in two parts, as P comes: of both halves of the keys the first two sixteens, then the others
 #pragma unroll
-                for (int kk = 0; kk < 8; ++kk) tt_mma_ta(leader, t_o, t_p + kk * 8u, dv_st + kk * (2048u >> 4), idesc_o, kk > 0 ? 1u : s < 2 ? 0u : 1u);
+                for (int part = 0; part < 2; ++part) {
+                    if (ok) ok = wait(bar_p(x, part), phase_p[x]);
+                    if (!ok) return;
+                    tc_fence_async_smem(); tc_fence_after();
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int kk = (i >> 1) * 4 + part * 2 + (i & 1);
+                        tt_mma_ta(leader, t_o, t_p + kk * 8u, dv_st + kk * (2048u >> 4), idesc_o, part + i > 0 ? 1u : s < 2 ? 0u : 1u);
+                    }
+                }
+                phase_p[x] ^= 1u;
                 tt_commit(leader, bar_o(x));
                 if (!dual || x == 1) tt_commit(leader, bar_vr(st));
             };
@@ -323,11 +331,11 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const TreeParams
                             if (!(seen1 >> e & 1u)) s1[e] = -INFINITY;
                         }
                     }
-                    float c4[4];
+                    float c4[4];                     // (maxima of three: one instruction)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) c4[e] = fmaxf(s0[e], s1[e]);
 #pragma unroll
-                    for (int e = 4; e < 32; ++e) c4[e & 3] = fmaxf(c4[e & 3], fmaxf(s0[e], s1[e]));
+                    for (int e = 4; e < 32; ++e) c4[e & 3] = fmaxf(fmaxf(c4[e & 3], s0[e]), s1[e]);
                     const float mine = fmaxf(fmaxf(c4[0], c4[1]), fmaxf(c4[2], c4[3])) * sc;
                     ex_max[half * 128 + lane_row] = mine;
                     tc_fence_before();               // (the scores have been read, for the partner's P)
@@ -365,7 +373,12 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const TreeParams
                         }
                         tc_st16(ts + 32 * half + cb * 16, pk);
                     };
-                    expo(s0, 0); expo(s1, 1);
+                    expo(s0, 0);
+                    tc_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) tc_mbar_arrive(bar_p(x, 0));
+                    expo(s1, 1);
                     float lo, hi;
                     tt_unpack(tt_add(tt_add(sum2[0], sum2[1]), tt_add(sum2[2], sum2[3])), lo, hi);
                     l_run += lo + hi;
@@ -373,7 +386,10 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const TreeParams
                 }
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) tc_mbar_arrive(bar_p(x));
+                if (lane == 0) {
+                    if (!active) tc_mbar_arrive(bar_p(x, 0));
+                    tc_mbar_arrive(bar_p(x, 1));
+                }
             }
             // ---- the segment's end
             if (n_mine > 0) {
