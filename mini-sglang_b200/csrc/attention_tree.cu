@@ -204,19 +204,9 @@ __device__ __forceinline__ unsigned tree_seen(const unsigned* row, int words, in
 
 __device__ __forceinline__ int tree_page(const TreeParams& p, int key) { return p.page_shift >= 0 ? key >> p.page_shift : key / p.page_size; }
 
-// ---------------------------------------------------------------------------------------
-// Any head size up to 512, any page size, float32 or bfloat16 data, float32 arithmetic: 32 rows a block, tiles of 32 keys.
-//
-// Warp w owns rows 4 w .. 4 w + 3.  Scores: lane = key, four rows a lane, K rows of odd 16-byte pitch, so that a warp's loads of them
-// meet no bank twice; P^T goes to shared memory (four rows a key side by side) and O is four rows x 4 CB columns a lane.  Bound by what
-// shared memory delivers (two loads for sixteen multiply-adds).  A key that a row does not see has the weight -1, which the product
-// leaves out: its value may be anything.
-// ---------------------------------------------------------------------------------------
-constexpr int TS_ROWS = 32, TS_KT = 32, TS_THREADS = 256;
 struct TreeYes { static constexpr bool value = true; };
 struct TreeNo { static constexpr bool value = false; };
-
-template <typename T> struct TsVec;                  // 16 bytes of a row; MOST: of them a thread has for 128 columns
+template <typename T> struct TsVec;                  // 16 bytes of a row; MOST: of them one of eight threads has for 128 columns
 template <> struct TsVec<float> {
     static constexpr int N = 4, MOST = 4;
     static __device__ __forceinline__ void store(float* to, const uint4& v) { *reinterpret_cast<uint4*>(to) = v; }
@@ -228,6 +218,241 @@ template <> struct TsVec<__nv_bfloat16> {
         *reinterpret_cast<uint4*>(to + 4) = make_uint4(v.z << 16, v.z & 0xffff0000u, v.w << 16, v.w & 0xffff0000u);
     }
 };
+
+// ---------------------------------------------------------------------------------------
+// Head sizes up to 128 and some work, any page size, float32 or bfloat16 data, float32 arithmetic: 64 rows a block, tiles of 64 keys, two blocks an SM.
+//
+// Warp w owns rows 16 (w / 2) .. + 15 and, of the scores, half of the keys, of O, half of the columns.  A thread has four rows (every fourth) against four
+// keys (every eighth) and then against eight columns: eight loads of 16 bytes for 64 multiply-adds, three for 32, and no two lanes meet a
+// bank.  The two warps of a row meet over its maximum.  P takes the place of the keys, key by key, a thread's four rows side by side.  Bound by what
+// shared memory delivers, 128 bytes a cycle: 14,300 cycles a tile, its multiply-adds 8,200.  A key that a row does not see has the weight -1, which the
+// product leaves out: its value may be anything.
+// ---------------------------------------------------------------------------------------
+constexpr int TF_ROWS = 64, TF_KT = 64, TF_D = 128, TF_THREADS = 256, TF_PITCH = TF_D + 4, TF_PPITCH = TF_ROWS + 4;
+constexpr size_t TF_SMEM = (size_t)(TF_ROWS + 2 * TF_KT) * TF_PITCH * sizeof(float);
+static_assert(TF_PPITCH <= TF_PITCH, "P lies over the keys");
+
+__device__ __forceinline__ void tf_cp_async16(float* to, const void* from, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(smem_u32(to)), "l"(from), "r"(there ? 16 : 0));
+}
+
+template <typename T>
+__global__ void __launch_bounds__(TF_THREADS, 2) tree_tile_kernel(const TreeParams p) {
+    extern __shared__ __align__(16) float tf_smem[];
+    __shared__ float sh_max[2][TF_ROWS], sh_sum[2][TF_ROWS];
+    __shared__ TreeStart begun;
+    float* Qs = tf_smem;                             // [64][pitch]; columns from d on are zero, in all three
+    float* Ks = Qs + TF_ROWS * TF_PITCH;
+    float* Vs = Ks + TF_KT * TF_PITCH;
+    float* Ps = Ks;                                  // [64 keys][64 rows + 4]
+    const int d = p.d, d4 = (d + 3) >> 2, G = p.G, j = blockIdx.x;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, side = warp & 1, rg = lane >> 3, kg = lane & 7, row_base = (warp >> 1) * 16;
+    pdl_launch_dependents();
+    pdl_wait();
+    pdl_after_wait();
+    TreeWalk<TF_ROWS, TF_KT> walk(p);
+    TreeRecord record = {};
+    if (walk.begin(j, gridDim.x, begun)) {
+        for (int i = tid; i < (TF_ROWS + 2 * TF_KT) * TF_PITCH; i += TF_THREADS) tf_smem[i] = 0.f;
+        TreeSegment g = begun.first;
+        for (bool more = true; more; more = walk.next(g)) {
+            __syncthreads();                         // the segment before has been read
+            const int my_key = tid >> 2, sub = tid & 3;
+            {
+                const int rr = g.row0 + my_key;
+                const T* src = reinterpret_cast<const T*>(p.q) + ((size_t)(g.tok0 + rr / G) * p.n_q + (size_t)g.kvh * G + rr % G) * d;
+                for (int c = sub; c < d; c += 4) Qs[my_key * TF_PITCH + c] = my_key < g.rows ? to_f32<T>(src[c]) : 0.f;
+            }
+            float o[4][8], m_run[4], l_run[4];
+            const unsigned* row_mask[4];
+#pragma unroll
+            for (int a = 0; a < 4; ++a) {
+                m_run[a] = -INFINITY;
+                l_run[a] = 0.f;
+                row_mask[a] = p.mask + (size_t)(g.tok0 + (g.row0 + min(row_base + rg + 4 * a, g.rows - 1)) / G) * p.words;
+#pragma unroll
+                for (int c = 0; c < 8; ++c) o[a][c] = 0.f;
+            }
+            const bool busy = row_base < g.rows;     // whether the warp has rows
+            for (int t = g.t_lo; t < g.t_hi; ++t) {
+                const int key0 = t * TF_KT;
+                __syncthreads();                     // the tile before has been read
+                {
+                    const int key = key0 + my_key;
+                    long long at = -1;               // element offset of the key's row
+                    if (key < g.kv) {
+                        const int pi = tree_page(p, key), id = p.table[(size_t)g.r * p.table_stride + pi];
+                        if (id >= 0 && id < p.pages) at = (((long long)id * p.n_kv + g.kvh) * p.page_size + (key - pi * p.page_size)) * d;
+                    }
+                    const T* k = reinterpret_cast<const T*>(p.k_cache) + max(at, 0ll);
+                    const T* v = reinterpret_cast<const T*>(p.v_cache) + max(at, 0ll);
+                    float* to_k = Ks + my_key * TF_PITCH;
+                    float* to_v = Vs + my_key * TF_PITCH;
+                    constexpr int N = TsVec<T>::N;
+                    // (P lay over the keys: what is no head element has to be zero again)
+                    for (int c = d + sub; c < TF_PITCH; c += 4) to_k[c] = 0.f;
+                    if (p.vectors && sizeof(T) == 4) {
+#pragma unroll 8
+                        for (int c = sub * N; c < d; c += 4 * N) {
+                            tf_cp_async16(to_k + c, k + c, at >= 0);
+                            tf_cp_async16(to_v + c, v + c, at >= 0);
+                        }
+                        asm volatile("cp.async.commit_group;\ncp.async.wait_group 0;\n" ::: "memory");
+                    } else if (p.vectors) {
+                        uint4 raw[2][TF_D / (4 * N)];
+#pragma unroll
+                        for (int i = 0; i < TF_D / (4 * N); ++i) {
+                            const int c = (sub + 4 * i) * N;
+                            const bool there = at >= 0 && c < d;
+                            raw[0][i] = there ? *reinterpret_cast<const uint4*>(k + c) : make_uint4(0u, 0u, 0u, 0u);
+                            raw[1][i] = there ? *reinterpret_cast<const uint4*>(v + c) : make_uint4(0u, 0u, 0u, 0u);
+                        }
+#pragma unroll
+                        for (int i = 0; i < TF_D / (4 * N); ++i) {
+                            const int c = (sub + 4 * i) * N;
+                            if (c >= d) continue;
+                            TsVec<T>::store(to_k + c, raw[0][i]);
+                            TsVec<T>::store(to_v + c, raw[1][i]);
+                        }
+                    } else {
+                        for (int c = sub; c < d; c += 4) {
+                            to_k[c] = at >= 0 ? to_f32<T>(k[c]) : 0.f;
+                            to_v[c] = at >= 0 ? to_f32<T>(v[c]) : 0.f;
+                        }
+                    }
+                }
+                __syncthreads();
+                float s[4][4];
+#pragma unroll
+                for (int a = 0; a < 4; ++a) s[a][0] = s[a][1] = s[a][2] = s[a][3] = 0.f;
+                const bool ends = key0 + TF_KT > g.base;
+                if (busy) {
+                    const float* q0 = Qs + (row_base + rg) * TF_PITCH;
+                    const float* k0 = Ks + (32 * side + kg) * TF_PITCH;
+#pragma unroll 2
+                    for (int c = 0; c < 4 * d4; c += 4) {
+                        float4 q4[4], k4[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            q4[i] = *reinterpret_cast<const float4*>(q0 + 4 * i * TF_PITCH + c);
+                            k4[i] = *reinterpret_cast<const float4*>(k0 + 8 * i * TF_PITCH + c);
+                        }
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)          // (sixteen sums between two terms of one)
+#pragma unroll
+                            for (int a = 0; a < 4; ++a)
+#pragma unroll
+                                for (int b = 0; b < 4; ++b)
+                                    s[a][b] = fmaf(e == 0 ? q4[a].x : e == 1 ? q4[a].y : e == 2 ? q4[a].z : q4[a].w, e == 0 ? k4[b].x : e == 1 ? k4[b].y : e == 2 ? k4[b].z : k4[b].w, s[a][b]);
+                    }
+#pragma unroll
+                    for (int a = 0; a < 4; ++a) {
+                        const unsigned seen = ends ? tree_seen(row_mask[a], p.words, key0 + 32 * side, g.base, g.kv) : ~0u;
+                        float mx = -INFINITY;
+#pragma unroll
+                        for (int b = 0; b < 4; ++b) {
+                            s[a][b] = seen >> (kg + 8 * b) & 1u ? s[a][b] * p.scale_log2 : -INFINITY;
+                            mx = fmaxf(mx, s[a][b]);
+                        }
+#pragma unroll
+                        for (int w = 1; w < 8; w <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
+                        if (kg == 0) sh_max[side][row_base + rg + 4 * a] = mx;
+                    }
+                }
+                __syncthreads();                     // the keys have been read, the maxima are there
+                if (busy) {
+#pragma unroll
+                    for (int a = 0; a < 4; ++a) {
+                        const int row = row_base + rg + 4 * a;
+                        const float mx = fmaxf(m_run[a], fmaxf(sh_max[0][row], sh_max[1][row])), mu = mx == -INFINITY ? 0.f : mx, f = fast_exp2(m_run[a] - mu);
+                        const unsigned seen = ends ? tree_seen(row_mask[a], p.words, key0 + 32 * side, g.base, g.kv) : ~0u;
+                        m_run[a] = mx;
+                        float sum = 0.f;
+#pragma unroll
+                        for (int b = 0; b < 4; ++b) {
+                            const float e = fast_exp2(s[a][b] - mu);
+                            sum += e;
+                            s[a][b] = seen >> (kg + 8 * b) & 1u ? e : -1.f;
+                        }
+                        l_run[a] = fmaf(l_run[a], f, sum);       // this thread's keys alone
+#pragma unroll
+                        for (int c = 0; c < 8; ++c) o[a][c] *= f;
+                    }
+#pragma unroll
+                    for (int b = 0; b < 4; ++b)
+                        *reinterpret_cast<float4*>(Ps + (32 * side + kg + 8 * b) * TF_PPITCH + row_base + 4 * rg) = make_float4(s[0][b], s[1][b], s[2][b], s[3][b]);
+                }
+                __syncthreads();
+                if (busy) {
+                    auto product = [&](auto guarded) {
+#pragma unroll 4
+                        for (int key = 0; key < TF_KT; ++key) {
+                            const float4 w4 = *reinterpret_cast<const float4*>(Ps + key * TF_PPITCH + row_base + 4 * rg);
+                            const float4 va = *reinterpret_cast<const float4*>(Vs + key * TF_PITCH + 64 * side + 4 * kg);
+                            const float4 vb = *reinterpret_cast<const float4*>(Vs + key * TF_PITCH + 64 * side + 4 * kg + 32);
+                            const float w[4] = {w4.x, w4.y, w4.z, w4.w}, v[8] = {va.x, va.y, va.z, va.w, vb.x, vb.y, vb.z, vb.w};
+#pragma unroll
+                            for (int a = 0; a < 4; ++a) {
+                                if (decltype(guarded)::value && w[a] < 0.f) continue;
+#pragma unroll
+                                for (int c = 0; c < 8; ++c) o[a][c] = fmaf(w[a], v[c], o[a][c]);
+                            }
+                        }
+                    };
+                    if (ends) product(TreeYes());
+                    else product(TreeNo());
+                }
+            }
+            // ---- the segment's end
+#pragma unroll
+            for (int a = 0; a < 4; ++a) {
+                float l = l_run[a];
+#pragma unroll
+                for (int w = 1; w < 8; w <<= 1) l += __shfl_xor_sync(0xffffffffu, l, w);
+                if (kg == 0) sh_sum[side][row_base + rg + 4 * a] = l;
+            }
+            __syncthreads();
+            const bool whole = g.t_lo == 0 && g.t_hi == g.tiles;
+            const int slot = 2 * j + (g.t_lo == 0 ? 1 : 0);
+#pragma unroll
+            for (int a = 0; a < 4; ++a) {
+                const int row = row_base + rg + 4 * a;
+                if (row >= g.rows) continue;
+                const float l = sh_sum[0][row] + sh_sum[1][row];
+                if (whole) {
+                    const int rr = g.row0 + row;
+                    const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
+                    T* dst = reinterpret_cast<T*>(p.out) + ((size_t)(g.tok0 + rr / G) * p.n_q + (size_t)g.kvh * G + rr % G) * d;
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) {
+                        const int col = 64 * side + 4 * kg + (c >> 2) * 32 + (c & 3);
+                        if (col < d) dst[col] = from_f32<T>(o[a][c] * inv);
+                    }
+                } else {
+                    float4* dst = reinterpret_cast<float4*>(p.part_o) + (size_t)slot * d4 * TF_ROWS + row;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        if (16 * side + kg + 8 * h < d4) dst[(16 * side + kg + 8 * h) * TF_ROWS] = make_float4(o[a][4 * h], o[a][4 * h + 1], o[a][4 * h + 2], o[a][4 * h + 3]);
+                    if (side == 0 && kg == 0) *reinterpret_cast<float2*>(p.part_ml + ((size_t)slot * TF_ROWS + row) * 2) = make_float2(m_run[a], l);
+                }
+            }
+            if (!whole && g.t_lo == 0) record = TreeRecord{walk.pieces(g, j), g.rows, g.tok0, g.row0, g.kvh, {0, 0, 0}};
+        }
+    }
+    if (tid == 0) p.record[j] = record;
+}
+
+// ---------------------------------------------------------------------------------------
+// Head sizes up to 512, any page size, float32 or bfloat16 data, float32 arithmetic: 32 rows a block, tiles of 32 keys.
+//
+// Warp w owns rows 4 w .. 4 w + 3.  Scores: lane = key, four rows a lane, K rows of odd 16-byte pitch, so that a warp's loads of them
+// meet no bank twice; P^T goes to shared memory (four rows a key side by side) and O is four rows x 4 CB columns a lane.  Bound by what
+// shared memory delivers (five loads of 16 bytes for sixteen multiply-adds of the scores, two of O's), its steps are shorter than those of the kernel above.
+// float32, head size 128, this one / that one, us: groups of four, 1 request of 32 drafts behind 500 keys 33 / 57, 8 of 20 behind 100 41 / 47, 16 of 30 behind 300
+// 152 / 132, 2 of 12 behind 6,000 155 / 124; of two, 4 of 26 behind 1,500 89 / 84, 1 of 8 behind 1,000 23.5 / 38.7; of five, 2 of 64 behind 4,000 477 / 346.
+// So it stands where there are no more than 32 rows or fewer than eight tiles of the other an SM (as far as the host knows: the table's width).
+// ---------------------------------------------------------------------------------------
+constexpr int TS_ROWS = 32, TS_KT = 32, TS_THREADS = 256;
 
 template <typename T, int CB>
 __global__ void __launch_bounds__(TS_THREADS, CB <= 2 ? 2 : 1) tree_simt_kernel(const TreeParams p) {
@@ -468,16 +693,18 @@ static void tree_join(const TreeParams& p, int blocks, int max_rows, cudaStream_
 
 #include "attention_tree_tc.cuh"
 
-static int tree_simt_blocks_per_sm(int d) { return d <= 256 ? 2 : 1; }
+static int tree_blocks_per_sm(int d) { return d <= 256 ? 2 : 1; }         // of the kernels without tensor cores
 static size_t tree_simt_smem(int cb) { return ((size_t)(TS_ROWS + 2 * TS_KT) * (cb * 128 + 4) + 8 * TS_KT * 4) * sizeof(float); }
 
 // Whether the tensor cores take a launch: bfloat16, head sizes 64 and 128, pages that TMA can fetch, a cache whose rows a coordinate can name.
 MSGL_API int msgl_tree_attention_tensor(int d, int page_size, long long cache_rows, int dtype) {
     return dtype == MSGL_BF16 && (d == 64 || d == 128) && page_size >= 8 && (page_size & (page_size - 1)) == 0 && cache_rows < 0x7fffffffLL - 4096 && tc_encoder() != nullptr;
 }
+// The kernels: 32 rows a block, 64 rows a block, tensor cores.
+enum { TREE_SIMT = 0, TREE_TILE = 1, TREE_TC = 2 };
 // Blocks of a launch and rows of an item, for the sizes of the scratch memory: part_o [2 * blocks][ceil(d / 4)][rows][4], part_ml [2 * blocks][rows][2] float32, record [blocks][8] int32.
-MSGL_API int msgl_tree_attention_blocks(int d, int tensor) { return msgl_sm_count() * (tensor ? 1 : tree_simt_blocks_per_sm(d)); }
-MSGL_API int msgl_tree_attention_rows(int tensor) { return tensor ? TT_ROWS : TS_ROWS; }
+MSGL_API int msgl_tree_attention_blocks(int d, int kind) { return msgl_sm_count() * (kind == TREE_TC ? 1 : tree_blocks_per_sm(d)); }
+MSGL_API int msgl_tree_attention_rows(int kind) { return kind == TREE_TC ? TT_ROWS : kind == TREE_TILE ? TF_ROWS : TS_ROWS; }
 
 template <typename T, int CB>
 static int tree_simt_launch(const TreeParams& p, int blocks, int max_rows, cudaStream_t stream) {
@@ -488,6 +715,18 @@ static int tree_simt_launch(const TreeParams& p, int blocks, int max_rows, cudaS
     }
     msgl_launch_pdl(tree_simt_kernel<T, CB>, dim3(blocks), dim3(TS_THREADS), tree_simt_smem(CB), stream, p);
     tree_join<T, TS_ROWS>(p, blocks, max_rows, stream);
+    return msgl_check_launch();
+}
+
+template <typename T>
+static int tree_tile_launch(const TreeParams& p, int blocks, int max_rows, cudaStream_t stream) {
+    static MsglOncePerDevice attr_set;
+    if (attr_set.due()) {
+        if (cudaFuncSetAttribute(tree_tile_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)TF_SMEM) != cudaSuccess) return msgl_check_launch();
+        attr_set.mark();
+    }
+    msgl_launch_pdl(tree_tile_kernel<T>, dim3(blocks), dim3(TF_THREADS), TF_SMEM, stream, p);
+    tree_join<T, TF_ROWS>(p, blocks, max_rows, stream);
     return msgl_check_launch();
 }
 
@@ -507,10 +746,10 @@ static int tree_tc_launch(const TreeParams& p, int* status, int blocks, int max_
     return msgl_check_launch();
 }
 
-// tensor: whether the tensor cores are to take it (status then points at the status word); max_rows: the most rows that a request has under a kv head.
+// kind: the kernel (of the tensor cores, status points at the status word); max_rows: the most rows that a request has under a kv head.
 MSGL_API int msgl_tree_attention(const void* q, void* out, const void* k_cache, const void* v_cache, const int* q_start, const int* kv_len, const int* table,
                                  const void* mask, int B, int T, int n_q, int n_kv, int d, int page_size, int table_stride, int table_width, int words,
-                                 long long pages, float scale, float* part_o, float* part_ml, int* record, int blocks, int max_rows, int tensor, int* status,
+                                 long long pages, float scale, float* part_o, float* part_ml, int* record, int blocks, int max_rows, int kind, int* status,
                                  int dtype, cudaStream_t stream) {
     if (B <= 0 || T <= 0) return MSGL_OK;
     if (n_kv <= 0 || n_q <= 0 || n_q % n_kv || d < 1 || d > 512 || page_size < 1 || table_width < 1 || words < 1 || blocks < 1 || pages < 0 || max_rows < 1) return MSGL_ERR_SIZE;
@@ -527,14 +766,15 @@ MSGL_API int msgl_tree_attention(const void* q, void* out, const void* k_cache, 
     if ((page_size & (page_size - 1)) == 0) { int sh = 0; while ((1 << sh) < page_size) ++sh; p.page_shift = sh; }
     p.scale_log2 = scale * 1.4426950408889634f;
     p.vectors = (((uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)(d * (dtype == MSGL_F32 ? 4 : 2))) & 15) == 0;
-    if (tensor) {
+    if (kind == TREE_TC) {
         if (status == nullptr || pages < 1 || !msgl_tree_attention_tensor(d, page_size, pages * n_kv * page_size, dtype)) return MSGL_ERR_SIZE;
         if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_cache | (uintptr_t)v_cache) & 15) return MSGL_ERR_ALIGN;
         return d == 128 ? tree_tc_launch<128>(p, status, blocks, max_rows, stream) : tree_tc_launch<64>(p, status, blocks, max_rows, stream);
     }
-#define MSGL_TREE(T, CB) tree_simt_launch<T, CB>(p, blocks, max_rows, stream)
-    if (dtype == MSGL_F32) return d <= 128 ? MSGL_TREE(float, 1) : d <= 256 ? MSGL_TREE(float, 2) : MSGL_TREE(float, 4);
-    if (dtype == MSGL_BF16) return d <= 128 ? MSGL_TREE(__nv_bfloat16, 1) : d <= 256 ? MSGL_TREE(__nv_bfloat16, 2) : MSGL_TREE(__nv_bfloat16, 4);
+    if (kind == TREE_TILE && d > TF_D) return MSGL_ERR_SIZE;
+#define MSGL_TREE(T) (kind == TREE_TILE ? tree_tile_launch<T>(p, blocks, max_rows, stream) : d <= 128 ? tree_simt_launch<T, 1>(p, blocks, max_rows, stream) : d <= 256 ? tree_simt_launch<T, 2>(p, blocks, max_rows, stream) : tree_simt_launch<T, 4>(p, blocks, max_rows, stream))
+    if (dtype == MSGL_F32) return MSGL_TREE(float);
+    if (dtype == MSGL_BF16) return MSGL_TREE(__nv_bfloat16);
 #undef MSGL_TREE
     return MSGL_ERR_DTYPE;
 }

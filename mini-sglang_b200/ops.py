@@ -2427,6 +2427,7 @@ def _draft_lib():
         lib.msgl_draft_accept.argtypes = [c_void_p] * 4 + [c_int] * 3 + [c_void_p] * 5 + [c_int] * 3 + [c_ll, c_int, c_int, c_void_p, c_int, c_int, c_void_p]
         lib.msgl_tree_attention.argtypes = [c_void_p] * 8 + [c_int] * 9 + [c_ll, c_float] + [c_void_p] * 3 + [c_int] * 3 + [c_void_p, c_int, c_void_p]
         lib.msgl_tree_attention_tensor.argtypes = [c_int, c_int, c_ll, c_int]
+        lib.msgl_tree_attention_blocks.argtypes = [c_int, c_int]
         lib.msgl_token_logprobs.argtypes = [c_void_p, c_int, c_int, c_ll, c_void_p, c_int] + [c_void_p] * 4 + [c_int] * 3 + [c_void_p]
         _drafts = lib
     return _drafts
@@ -2525,33 +2526,35 @@ def tree_attention(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_
     lib = _draft_lib()
     facts = _tree_facts.get((dev, d, page_size, dt))
     if facts is None:
-        sizes = [(lib.msgl_tree_attention_blocks(d, t), lib.msgl_tree_attention_rows(t)) for t in (0, 1)]
-        facts = (lib.msgl_tree_attention_tensor(d, page_size, 1, _DT[dt]), sizes)
+        facts = (bool(lib.msgl_tree_attention_tensor(d, page_size, 1, _DT[dt])), [(lib.msgl_tree_attention_blocks(d, k), lib.msgl_tree_attention_rows(k)) for k in (0, 1, 2)])
         _tree_facts[(dev, d, page_size, dt)] = facts
     at_q, at_out, at_k, at_v, pages = q.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_shape[0]
-    tensor, status = int(facts[0] and pages > 0 and pages * n_kv * page_size < _TREE_ROWS_MAX and not (at_q | at_out | at_k | at_v) & 15), None
-    if tensor:
-        # the status words lie on the first device that asked for them, and are not made in a stream capture: elsewhere the kernel that has no waits
+    max_rows, kind, status = max_draft * (n_q // n_kv), _TREE_SIMT, None
+    if facts[0] and 0 < pages * n_kv * page_size < _TREE_ROWS_MAX and not (at_q | at_out | at_k | at_v) & 15:
+        # the status words lie on the first device that asked for them, and are not made in a stream capture: elsewhere a kernel that has no waits
         status = _status if _status is not None else _status_words(q.device)
-        tensor = int(status is not None and status.get_device() == dev)
+        if status is not None and status.get_device() == dev:
+            kind = _TREE_TC
     while True:
-        blocks, rows = facts[1][tensor]
-        n_part = 2 * blocks * rows
-        d4 = d + 3 & ~3
+        if kind == _TREE_SIMT and d <= 128 and max_rows > 32 and B * n_kv * -(-max_rows // 64) * -(-width * page_size // 64) >= 8 * sm_count(q.device):
+            kind = _TREE_TILE     # (measured in csrc/attention_tree.cu)
+        blocks, rows = facts[1][kind]
+        n_part, d4 = 2 * blocks * rows, d + 3 & ~3
         part = torch.empty(n_part * (d4 + 2) + 8 * blocks, dtype=torch.float32, device=q.device)
         at = part.data_ptr()
         code = lib.msgl_tree_attention(at_q, at_out, at_k, at_v, q_start.data_ptr(), kv_len.data_ptr(), block_table.data_ptr(), mask.data_ptr(), B, T, n_q, n_kv, d,
                                        page_size, block_table.stride(0), width, words, pages, scale, at, at + 4 * n_part * d4, at + 4 * n_part * (d4 + 2), blocks,
-                                       max_draft * (n_q // n_kv), tensor, status.data_ptr() if tensor else None, _DT[dt], _stream())
-        if code != 2 or not tensor:
+                                       max_rows, kind, status.data_ptr() if kind == _TREE_TC else None, _DT[dt], _stream())
+        if code != 2 or kind != _TREE_TC:
             break
-        tensor = 0                # (no tensor map of this layout)
+        kind = _TREE_SIMT         # (no tensor map of this layout)
     _check(code, "tree_attention")
     global LAUNCHES
     LAUNCHES += 1                # the join of cut items is a kernel of its own
 
 
-_tree_facts = {}                  # (device, head size, page size, type): whether the tensor cores take it, (blocks, rows of an item) without and with them
+_TREE_SIMT, _TREE_TILE, _TREE_TC = 0, 1, 2
+_tree_facts = {}                  # (device, head size, page size, type): whether the tensor cores take it, (blocks, rows of an item) of the three kernels
 _TREE_ROWS_MAX = 0x7fffffff - 4096          # rows of a cache that a TMA coordinate can name
 
 
