@@ -685,8 +685,9 @@ __global__ void __launch_bounds__(TJ_WARPS * 32) tree_join_kernel(const TreePara
             if ((c0 + c) * 4 + e < d) dst[c * 4 + e] = from_f32<T>(x[e] * inv);
     }
 }
-template <typename T, int ROWS>
+template <typename T, int ROWS, int KT>
 static void tree_join(const TreeParams& p, int blocks, int max_rows, cudaStream_t stream) {
+    if ((long long)p.table_width * p.page_size <= KT) return;        // one tile at most: nothing is cut
     const int tasks = ((max_rows < ROWS ? max_rows : ROWS) + 31) / 32 * (((p.d + 3) / 4 + TJ_C - 1) / TJ_C);
     msgl_launch_pdl(tree_join_kernel<T, ROWS>, dim3(blocks, (tasks + TJ_WARPS - 1) / TJ_WARPS), dim3(TJ_WARPS * 32), 0, stream, p);
 }
@@ -714,7 +715,7 @@ static int tree_simt_launch(const TreeParams& p, int blocks, int max_rows, cudaS
         attr_set.mark();
     }
     msgl_launch_pdl(tree_simt_kernel<T, CB>, dim3(blocks), dim3(TS_THREADS), tree_simt_smem(CB), stream, p);
-    tree_join<T, TS_ROWS>(p, blocks, max_rows, stream);
+    tree_join<T, TS_ROWS, TS_KT>(p, blocks, max_rows, stream);
     return msgl_check_launch();
 }
 
@@ -726,7 +727,7 @@ static int tree_tile_launch(const TreeParams& p, int blocks, int max_rows, cudaS
         attr_set.mark();
     }
     msgl_launch_pdl(tree_tile_kernel<T>, dim3(blocks), dim3(TF_THREADS), TF_SMEM, stream, p);
-    tree_join<T, TF_ROWS>(p, blocks, max_rows, stream);
+    tree_join<T, TF_ROWS, TF_KT>(p, blocks, max_rows, stream);
     return msgl_check_launch();
 }
 
@@ -742,7 +743,7 @@ static int tree_tc_launch(const TreeParams& p, int* status, int blocks, int max_
     CUtensorMap kmap, vmap;
     if (!tc_matrix_map(p.k_cache, rows, D, (long long)D * 2, box, &kmap) || !tc_matrix_map(p.v_cache, rows, D, (long long)D * 2, box, &vmap)) return MSGL_ERR_SIZE;
     msgl_launch_pdl(tree_tc_kernel<D>, dim3(blocks), dim3(TT_THREADS), TreeTc<D>::ALLOC, stream, p, status, kmap, vmap, box);
-    tree_join<__nv_bfloat16, TT_ROWS>(p, blocks, max_rows, stream);
+    tree_join<__nv_bfloat16, TT_ROWS, TT_KT>(p, blocks, max_rows, stream);
     return msgl_check_launch();
 }
 

@@ -18,6 +18,7 @@ from __future__ import annotations
 import array
 import ctypes
 import math
+import operator
 import os
 from typing import NamedTuple, Optional, Sequence, Tuple
 
@@ -2549,8 +2550,9 @@ def tree_attention(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_
             break
         kind = _TREE_SIMT         # (no tensor map of this layout)
     _check(code, "tree_attention")
-    global LAUNCHES
-    LAUNCHES += 1                # the join of cut items is a kernel of its own
+    if width * page_size > 128:
+        global LAUNCHES
+        LAUNCHES += 1            # the join of cut items is a kernel of its own (none is cut where all keys are one tile; an estimate for tiles of 32 and 64)
 
 
 _TREE_SIMT, _TREE_TILE, _TREE_TC = 0, 1, 2
@@ -2584,16 +2586,17 @@ def _refuse_tree_attention(q, out, k_cache, v_cache, q_start, kv_len, block_tabl
     raise KernelError(f"{what}: arguments that do not go together")
 
 
+_SHAPE, _DTYPE = operator.attrgetter("shape"), operator.attrgetter("dtype")
+
+
 def _cache_groups(caches: Sequence[torch.Tensor], like: torch.Tensor):
     """Addresses of the caches of draft_accept, those of one shape and element size together, each once (keys and values may be one array)."""
-    c0, dev = caches[0], like.get_device()
-    shape, dtype = c0.shape, c0.dtype
-    if c0.dim() == 4:
-        for c in caches:                     # (a model's layers are alike: looked at with few calls each)
-            if c.shape != shape or c.dtype is not dtype or c.get_device() != dev or not c.is_contiguous():
-                break
-        else:
-            return [(shape, c0.element_size(), list(dict.fromkeys([c.data_ptr() for c in caches])))]
+    c0, dev, n = caches[0], like.get_device(), len(caches)
+    shape = c0.shape
+    # a model's layers are alike: looked at in a few passes over all of them (one by one they cost the host half a microsecond each)
+    if len(shape) == 4 and list(map(_SHAPE, caches)).count(shape) == n and list(map(_DTYPE, caches)).count(c0.dtype) == n and \
+            list(map(torch.Tensor.get_device, caches)).count(dev) == n and all(map(torch.Tensor.is_contiguous, caches)):
+        return [(shape, c0.element_size(), list(dict.fromkeys(map(torch.Tensor.data_ptr, caches))))]
     groups = {}
     for c in caches:
         if c.dim() != 4 or not c.is_contiguous() or c.get_device() != dev or c.shape[2] != shape[2]:
