@@ -115,7 +115,7 @@ __global__ void __launch_bounds__(DR_COPY_THREADS) draft_accept_kernel(const int
     pdl_launch_dependents();
     pdl_wait();
     pdl_after_wait();
-    const int start = min(max(q_start[r], 0), T), n = min(min(max(q_start[r + 1] - start, 0), max_draft), T - start);
+    const int start = min(max(q_start[r], 0), T), brought = min(max(q_start[r + 1] - start, 0), T - start), n = min(brought, max_draft);
     int tok = 0, up = -1;
     child[tid] = DR_MAX;
     if (tid < n) {
@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(DR_COPY_THREADS) draft_accept_kernel(const int
         }
     }
     if (n_caches == 0 || first >= kept) return;
-    const int base = kv_len[r] - n;
+    const int base = kv_len[r] - brought;
     auto place = [&](int i) {
         const int at = base + i, page = at / page_size;
         if (at < 0 || page >= table_width) return make_int2(-1, 0);

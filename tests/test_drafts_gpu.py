@@ -126,6 +126,14 @@ def test_accept_leaves_out_what_is_not_there():
     ops.draft_accept(*args, max_draft=5, kv_len=i32([5]), block_table=i32([[1, 400, -3]]), caches=[cache])
     assert torch.equal(cache, before)
     assert ops.draft_accept(*args, max_draft=2).path.tolist() == [[0, 1]]
+    two = ops.draft_accept(i32([9, 7, 4]), i32([-1, 0, 0]), i32([4, 0, 0]), i32([0, 3]), max_draft=3, kv_len=i32([5]), block_table=i32([[1, 2, 3]]), caches=[cache])
+    assert two.path.tolist() == [[0, 2, -1]]                 # place 4 moves to place 3
+    want = before.clone()
+    want[2, :, 1] = before[3, :, 0]
+    assert torch.equal(cache, want)
+    cache.copy_(before)
+    cut = ops.draft_accept(i32([9, 7, 4, 1]), i32([-1, 0, 0, 0]), i32([4, 0, 0, 0]), i32([0, 4]), max_draft=3, kv_len=i32([6]), block_table=i32([[1, 2, 3]]), caches=[cache])
+    assert cut.path.tolist() == [[0, 2, -1]] and torch.equal(cache, want)          # a draft beyond the bound: the places are what they were
 
 
 def test_plan_and_accept_in_a_graph():
