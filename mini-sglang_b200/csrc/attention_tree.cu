@@ -52,6 +52,7 @@ struct TreeParams {
     int B, T, n_q, n_kv, G, d, page_size, page_shift, table_stride, table_width, words;
     long long pages;
     float scale_log2;             // scale * log2(e)
+    int max_draft;                // most drafts of a request
     int vectors;                  // rows of the caches are whole 16 bytes, on 16-byte boundaries
 };
 
@@ -87,12 +88,14 @@ struct TreeWalk {
     __device__ __forceinline__ TreeWalk(const TreeParams& q) : p(q) {}
     __device__ __forceinline__ void store(TreeWalkState& s) const { s.whole = whole; s.rest = rest; s.x_lo = x_lo; s.x_hi = x_hi; s.start = start; s.blocks = blocks; s.r = r; s.item = item; }
     __device__ __forceinline__ void load(const TreeWalkState& s) { whole = s.whole; rest = s.rest; x_lo = s.x_lo; x_hi = s.x_hi; start = s.start; blocks = s.blocks; r = s.r; item = s.item; }
-    struct Request { int tok0, n, kv, tiles, groups, items; };      // groups: items under a kv head
+    struct Request { int tok0, n, kv, base, tiles, groups, items; };      // groups: items under a kv head
     __device__ __forceinline__ Request request(int i) const {
         Request w;
         w.tok0 = min(max(p.q_start[i], 0), p.T);
-        w.n = min(max(p.q_start[i + 1], w.tok0), p.T) - w.tok0;
+        const int brought = min(max(p.q_start[i + 1], w.tok0), p.T) - w.tok0;
+        w.n = min(brought, p.max_draft);             // (drafts beyond the host's bound have no rows; their keys are the last ones all the same)
         w.kv = (int)min((long long)max(p.kv_len[i], 0), (long long)p.table_width * p.page_size);
+        w.base = w.kv - brought;
         w.tiles = max(1, (w.kv + KT - 1) / KT);
         w.groups = (w.n * p.G + ROWS - 1) / ROWS;
         w.items = p.n_kv * w.groups;
@@ -163,7 +166,7 @@ struct TreeWalk {
                 g.kvh = w.groups == 1 ? item : item / w.groups;
                 g.row0 = (item - g.kvh * w.groups) * ROWS;
                 g.rows = min(ROWS, w.n * p.G - g.row0);
-                g.tok0 = w.tok0; g.n = w.n; g.kv = w.kv; g.base = w.kv - w.n;
+                g.tok0 = w.tok0; g.n = w.n; g.kv = w.kv; g.base = w.base;
                 g.t_lo = lo; g.t_hi = hi; g.tiles = w.tiles;
                 ++item;
                 return true;
@@ -747,13 +750,14 @@ static int tree_tc_launch(const TreeParams& p, int* status, int blocks, int max_
     return msgl_check_launch();
 }
 
-// kind: the kernel (of the tensor cores, status points at the status word); max_rows: the most rows that a request has under a kv head.
+// kind: the kernel (of the tensor cores, status points at the status word); max_draft: the most drafts that a request has.
 MSGL_API int msgl_tree_attention(const void* q, void* out, const void* k_cache, const void* v_cache, const int* q_start, const int* kv_len, const int* table,
                                  const void* mask, int B, int T, int n_q, int n_kv, int d, int page_size, int table_stride, int table_width, int words,
-                                 long long pages, float scale, float* part_o, float* part_ml, int* record, int blocks, int max_rows, int kind, int* status,
+                                 long long pages, float scale, float* part_o, float* part_ml, int* record, int blocks, int max_draft, int kind, int* status,
                                  int dtype, cudaStream_t stream) {
     if (B <= 0 || T <= 0) return MSGL_OK;
-    if (n_kv <= 0 || n_q <= 0 || n_q % n_kv || d < 1 || d > 512 || page_size < 1 || table_width < 1 || words < 1 || blocks < 1 || pages < 0 || max_rows < 1) return MSGL_ERR_SIZE;
+    if (n_kv <= 0 || n_q <= 0 || n_q % n_kv || d < 1 || d > 512 || page_size < 1 || table_width < 1 || words < 1 || blocks < 1 || pages < 0 || max_draft < 1) return MSGL_ERR_SIZE;
+    const int max_rows = max_draft < T ? max_draft * (n_q / n_kv) : T * (n_q / n_kv);            // most rows of a request under a kv head
     if ((long long)table_width * page_size > 0x7fffffffLL - 1024 || (long long)T * (n_q / n_kv) > 0x7fffffffLL / 2) return MSGL_ERR_SIZE;
     // the length of the work, in whole numbers of 32 bits: at most this many tiles and heads of items
     if ((long long)B * n_kv * ((long long)max_rows / TS_ROWS + 1) * ((long long)table_width * page_size / TS_KT + 1 + TREE_HEAD) > 0x7fffffffLL) return MSGL_ERR_SIZE;
@@ -762,7 +766,7 @@ MSGL_API int msgl_tree_attention(const void* q, void* out, const void* k_cache, 
     p.q = q; p.out = out; p.k_cache = k_cache; p.v_cache = v_cache; p.q_start = q_start; p.kv_len = kv_len; p.table = table; p.mask = (const unsigned*)mask;
     p.part_o = part_o; p.part_ml = part_ml; p.record = (TreeRecord*)record;
     p.B = B; p.T = T; p.n_q = n_q; p.n_kv = n_kv; p.G = n_q / n_kv; p.d = d; p.page_size = page_size; p.table_stride = table_stride; p.table_width = table_width; p.words = words;
-    p.pages = pages;
+    p.pages = pages; p.max_draft = max_draft;
     p.page_shift = -1;
     if ((page_size & (page_size - 1)) == 0) { int sh = 0; while ((1 << sh) < page_size) ++sh; p.page_shift = sh; }
     p.scale_log2 = scale * 1.4426950408889634f;

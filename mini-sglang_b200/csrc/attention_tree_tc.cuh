@@ -132,14 +132,14 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const TreeParams
         tc_mbar_init(bar_q, TT_SOFT); tc_mbar_init(bar_vt, 1);
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
-    if (warp == 0) {             // all 512 columns of tensor memory: S_A | S_B | O_A | O_B
+    pdl_launch_dependents();
+    pdl_wait();
+    pdl_after_wait();
+    if (warp == 0) {             // all 512 columns of tensor memory: S_A | S_B | O_A | O_B (behind the wait: a kernel ahead of this one may want some)
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;\n" ::"r"(smem_u32(&tmem_base_s)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
     }
     tc_fence_before();
-    pdl_launch_dependents();
-    pdl_wait();
-    pdl_after_wait();
     TreeWalk<TT_ROWS, TT_KT> walk(p);
     const bool stop = __syncthreads_or(*reinterpret_cast<volatile int*>(status) != 0) != 0;      // an earlier block gave up: do not pile up
     const bool work = walk.begin(j, gridDim.x, begun) && !stop && smem0 + C::SMEM <= smem_base + C::ALLOC;      // (a barrier of the block stands in begin)

@@ -2504,9 +2504,10 @@ def tree_attention(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_
     """Attention of a step whose requests bring drafted tokens: q and out [T, heads, d] float32 or bfloat16, the paged caches as for
     `attention`, q_start, kv_len and mask as `draft_plan` makes them (any other mask will do).  A draft sees all keys of its request before
     the drafts, and of these the ones whose bits are set in its mask row; what it does not see counts for nothing, whatever it holds, and
-    a draft that sees no key gets 0.  No request brings more than max_draft (the host's bound; it sizes the launch).  Rows of out behind the
-    last draft are left as they were.  Head sizes up to 512; bfloat16 heads of 128 on pages that TMA can fetch (a power of two from 8
-    on) go through the tensor cores.  A page number outside the cache reads as zeros."""
+    a draft that sees no key gets 0.  No request brings more than max_draft (the host's bound; it sizes the launch): drafts beyond it, and rows of
+    out behind the last draft, are left as they were.  Head sizes up to 512; bfloat16 heads of 64 and 128 on pages that TMA can fetch (a power of
+    two from 8 on) go through the tensor cores, whose waits are bounded: `check_kernel_status` says whether one ever gave up.  A page number
+    outside the cache reads as zeros."""
     i32, dt, dev = torch.int32, q.dtype, q.get_device()
     k_shape, words = k_cache.shape, mask.shape[-1] if mask.dim() else 0
     # every argument is looked at in one go, and told apart only where something is wrong: small steps wait for the host
@@ -2545,7 +2546,7 @@ def tree_attention(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_
         at = part.data_ptr()
         code = lib.msgl_tree_attention(at_q, at_out, at_k, at_v, q_start.data_ptr(), kv_len.data_ptr(), block_table.data_ptr(), mask.data_ptr(), B, T, n_q, n_kv, d,
                                        page_size, block_table.stride(0), width, words, pages, scale, at, at + 4 * n_part * d4, at + 4 * n_part * (d4 + 2), blocks,
-                                       max_rows, kind, status.data_ptr() if kind == _TREE_TC else None, _DT[dt], _stream())
+                                       max_draft, kind, status.data_ptr() if kind == _TREE_TC else None, _DT[dt], _stream())
         if code != 2 or kind != _TREE_TC:
             break
         kind = _TREE_SIMT         # (no tensor map of this layout)
