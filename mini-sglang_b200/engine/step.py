@@ -634,9 +634,10 @@ class ModelRunner:
 
     # -- drafted tokens ------------------------------------------------------------------------
     def drafts_supported(self) -> bool:
-        """Whether `verify` takes this model: every mixer attends to all keys of a paged cache (no windows, chunks or per-request states)."""
+        """Whether `verify` takes this model: every mixer is one that takes drafts and attends to all keys of a paged cache (no windows, chunks or
+        per-request states) with heads of up to 512."""
         return bool(self.mgr.groups) and not self.mgr.state_ids and all(g.span is None for g in self.mgr.groups) and \
-            all(n.library == "attention" and (n.v_head_dim or n.head_dim) == n.head_dim <= 512 for n in self.mgr.needs.values())
+            all(layer.mixer.takes_drafts for layer in self.model.layers) and all((n.v_head_dim or n.head_dim) == n.head_dim <= 512 for n in self.mgr.needs.values())
 
     @torch.no_grad()
     def verify(self, entries: Sequence[DraftEntry], sampler, temperatures: Optional[Sequence[float]] = None, row_keys: Optional[Sequence[int]] = None,
@@ -653,6 +654,8 @@ class ModelRunner:
         if not entries:
             return []
         V, lens, parents, depths = self.vocab_size, [], [], []
+        if any(given is not None and len(given) != len(entries) for given in (temperatures, row_keys, steps)):
+            raise ValueError("temperatures, row_keys and steps have one value an entry")
         if len({e.slot for e in entries}) != len(entries):
             raise ValueError("a request can bring one tree a step")
         for e in entries:

@@ -27,6 +27,7 @@ class PagedAttention(Mixer):
     """
 
     graph_safe = True
+    takes_drafts = True
 
     def __init__(self, spec, prefix, env, position=None):
         super().__init__(spec, prefix, env)

@@ -67,6 +67,9 @@ class Mixer(Part):
     # everything else (lengths, slots, tables) from the context's device tensors, so that a decode
     # step can be captured once and replayed.  Mixers that loop over requests on the host say False.
     graph_safe = False
+    # True if forward() takes a step of drafted tokens (ctx.drafts): over positions it reads only ctx.positions, over other
+    # tokens only what `paged_attend` reads.
+    takes_drafts = False
 
     def cache_need(self):
         return None

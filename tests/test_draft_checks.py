@@ -115,3 +115,47 @@ def test_tree_attention_refuses():
     refused("mask", f, q, q, c, c, **dict(ok, mask=I(3, 1)))
     refused("mask", f, q, q, c, c, **dict(ok, mask=I(4, 1).long()))
     refused("CUDA device", f, q, q, c, c, **ok)
+
+
+def test_logprobs_of_sampling_params():
+    from mini_sglang_b200 import SamplingParams
+    assert SamplingParams.init_from_dict({}).logprobs is None
+    for n in (0, 1, 32):
+        assert SamplingParams.init_from_dict({"logprobs": n}).logprobs == n
+    for n in (-1, 33):
+        with pytest.raises(ValueError, match="logprobs"):
+            SamplingParams.init_from_dict({"logprobs": n})
+
+
+def test_unreserved_tokens_leave_the_pages_as_they_were():
+    from mini_sglang_b200.cache import CacheManager, PagedKVNeed
+    mgr = CacheManager({0: PagedKVNeed(2, 8)}, page_size=4, num_pages=12, max_reqs=2, max_context_len=64)
+    slot = mgr.open()
+    mgr.reserve(slot, 6)
+    mgr.commit(slot, 6)
+    for n, kept in ((9, 3), (5, 1), (12, 12)):
+        before = mgr.owned_pages(slot)
+        mgr.reserve(slot, n)
+        assert mgr.owned_pages(slot)[:len(before)] == before
+        held = mgr.owned_pages(slot)
+        at = int(mgr.length[slot])
+        mgr.commit(slot, kept)
+        mgr.unreserve(slot)
+        assert int(mgr.length[slot]) == int(mgr.reserved[slot]) == at + kept and mgr.owned_pages(slot) == held
+        assert mgr.pages_needed(slot, 1) in ([0], (0,)) or at + kept == 4 * len(held)
+    mgr.close(slot)
+    mgr.check_idle()
+
+
+def test_scores_reach_the_tokens_they_belong_to():
+    """The scheduler hands every request that asked its own rows, cut to the number it asked for, in step with its tokens."""
+    from mini_sglang_b200.engine.scheduler import Req, Scheduler, _InFlight
+    from mini_sglang_b200.ops import TokenLogprobs
+    from mini_sglang_b200.sampling import SamplingParams
+    reqs = [Req(str(i), [1, 2, 3], SamplingParams(max_new_tokens=8, ignore_eos=True, logprobs=n), []) for i, n in enumerate((2, None, 0))]
+    rows = [0, 2]
+    scores = TokenLogprobs(torch.tensor([-1.0, -3.0]), torch.tensor([0.5, 0.25]), torch.tensor([[-0.5, -1.0], [-0.1, -3.0]]), torch.tensor([[7, 4], [9, 6]]))
+    flight = _InFlight(reqs, torch.tensor([4, 5, 6]), None, None, (rows, scores))
+    flight.dead.add("2")
+    Scheduler._collect(None, flight, None)                   # (of the scheduler itself only what ends a request is used)
+    assert reqs[0].logprobs == [(-1.0, 0.5, [(7, -0.5), (4, -1.0)])] and reqs[1].logprobs == [] and reqs[2].logprobs == []

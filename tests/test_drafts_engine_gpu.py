@@ -186,3 +186,58 @@ def test_logprobs_refused():
             eng.generate(input_ids=[1, 2], sampling_params={"logprobs": bad})
         with pytest.raises(ValueError, match="logprobs"):
             eng.generate(input_ids=[1, 2], sampling_params=SamplingParams(logprobs=bad))
+
+
+def pokatar_runner(layers, tmp, **kw):
+    from mini_sglang_b200.engine.step import ModelRunner
+    from tiny_models import write_model_dir
+    from tiny_pokatar import make_weights, model
+    cfg = model(64, 97, 1e-5, layers)
+    weights = make_weights(cfg, 8)
+    write_model_dir(str(tmp), cfg, weights)
+    return cfg, weights, ModelRunner.from_model_dir(str(tmp), dtype="float32", page_size=4, num_pages=200, max_reqs=4, max_context_len=256, **kw)
+
+
+def test_verify_over_caches_whose_values_lie_in_the_key_rows(tmp_path):
+    """Latent attention keeps one array a cache: its rows move once.  Drafts of the plain model's own tokens beside wrong ones."""
+    import plain_pokatar as pk
+    from mini_sglang_b200.engine import DraftEntry
+    from mini_sglang_b200.engine.step import StepEntry
+    from tiny_pokatar import dense, latent, layer
+    cfg, weights, runner = pokatar_runner([layer(latent(3, 24, 16, 20, 40, base=500.0), dense(56)), layer(latent(2, 64, 32, 64, 96), None)], tmp_path)
+    assert runner.drafts_supported()
+    smp, rng, prompt = sampler(runner), random.Random(2), random_tokens(21, 97, 5)
+    slot = runner.open()
+    want = decode(runner, slot, prompt, 40, smp, 0.0, 0)
+    runner.close(slot)
+    slot = runner.open()
+    got = [int(smp.sample(runner.step([StepEntry(slot, prompt, [20])]), [0.0], [0], [0])[0])]
+    rounds = 0
+    while len(got) < 30:
+        toks, up = guess(rng, want[len(got) - 1:], 12, 97)
+        got.extend(runner.verify([DraftEntry(slot, toks, up)], smp)[0])
+        rounds += 1
+    assert got[:30] == want[:30] and rounds < 20
+    row = runner.step([StepEntry(slot, [got[-1]], [0])]).float().cpu()[0]
+    ref = pk.forward_sequence(cfg, weights, prompt + got, dtype=torch.float64).float()[-1]
+    torch.testing.assert_close(row, ref, rtol=1e-4, atol=5e-5)
+    runner.close(slot)
+
+
+def test_attention_with_a_further_term_is_refused(tmp_path):
+    from mini_sglang_b200.engine import DraftEntry
+    from tiny_pokatar import att, dense, layer
+    _, _, runner = pokatar_runner([layer(att(4, 2, 32, 32), dense(56))], tmp_path)
+    assert not runner.drafts_supported()
+    with pytest.raises(ValueError, match="all keys"):
+        runner.verify([DraftEntry(runner.open(), [1, 2])], sampler(runner))
+
+
+def test_verify_wants_one_value_an_entry():
+    from mini_sglang_b200.engine import DraftEntry
+    runner = make_runner("B", "float32", num_pages=8)
+    slot = runner.open()
+    for kw in ({"temperatures": [0.0, 0.0]}, {"row_keys": []}, {"steps": [1, 2]}):
+        with pytest.raises(ValueError, match="one value an entry"):
+            runner.verify([DraftEntry(slot, [1, 2])], sampler(runner), **kw)
+    assert int(runner.mgr.reserved[slot]) == 0
