@@ -11,7 +11,7 @@
 //
 // Work.  A row is a (draft, head of the group) pair, so all rows of a kv head share its keys.  An item is up to ROWS rows of one request
 // under one kv head; its keys are cut into tiles of KT.  All items are laid end to end, an item as long as its tiles and TREE_HEAD
-// more (what it costs beside them), and cut into one run a block, equal but for TREE_SNAP: every block works out its run from the
+// more (what it costs beside them), and cut into one equal run a block: every block works out its run from the
 // requests' lengths by itself, so the host knows none of them and a captured launch serves any.  A block that has a whole item writes
 // its rows; of one that is cut every block leaves float32 partial sums with their maximum and sum of weights, and a second launch joins
 // them in the order of the keys.
@@ -60,8 +60,7 @@ struct TreeParams {
 // the cut of the work
 // ---------------------------------------------------------------------------------------
 constexpr int TREE_HEAD = 1;      // what an item costs beside its tiles, in tiles
-constexpr int TREE_SNAP = 1;      // a cut this close to an item's edge, or closer, moves onto it
-constexpr int TREE_SHARE = TREE_HEAD + TREE_SNAP + 1;      // a block's run is no shorter: so no piece of an item is empty and none lies in more than its blocks
+constexpr int TREE_SHARE = TREE_HEAD + 1;      // a block's run is no shorter: so no piece of an item is empty and none lies in more than its blocks
 
 struct TreeSegment {              // tiles [t_lo, t_hi) of one item
     int r, kvh, row0, rows;       // row0: first row of the item among the request's n * G under the kv head
@@ -110,9 +109,7 @@ struct TreeWalk {
     __device__ __forceinline__ int cut_at(int k) const { return whole * k + quotient(rest * k, blocks); }      // floor(total k / blocks); (k and rest: some hundreds)
     // the tile that a cut at x falls on, in an item that starts at `s`
     __device__ __forceinline__ int tile_at(int x, int s, int tiles) const {
-        const int t = x - s - TREE_HEAD;
-        if (t < TREE_SNAP) return 0;
-        return tiles - t < TREE_SNAP ? tiles : t;
+        return min(max(x - s - TREE_HEAD, 0), tiles);
     }
     // All threads of the block: the run of block j of nb; false: it has none.  The thread whose request the run starts in finds the first segment for all:
     // every further look at the lengths would be a wait for memory (walking from its start each by itself took the warps 2 us longer).
@@ -619,13 +616,15 @@ __global__ void __launch_bounds__(TS_THREADS, CB <= 2 ? 2 : 1) tree_simt_kernel(
 }
 
 // ---------------------------------------------------------------------------------------
-// The pieces of cut items, joined in the order of the keys.  A warp takes 32 rows, a lane each, and 16 columns of the item whose first piece block j
-// has.  Bound by latency: a record, the pieces' maxima, then their rows, 24 loads of 512 bytes of a warp at a time.
+// The pieces of cut items, joined in the order of the keys.  A warp takes 32 rows, a lane each, and TJ_C fours of columns of the item whose first piece
+// block j has.  Bound by latency: a record, the pieces' maxima, then their rows, TJ_K pieces and so 24 loads of 512 bytes of a warp at a time.
 // ---------------------------------------------------------------------------------------
-constexpr int TJ_WARPS = 4, TJ_C = 4, TJ_K = 6;       // warps of a block, fours of columns of a warp, pieces at a time
+constexpr int TJ_WARPS = 4;
 
-template <typename T, int ROWS>
+
+template <typename T, int ROWS, int TJ_C, int TJ_K>
 __global__ void __launch_bounds__(TJ_WARPS * 32) tree_join_kernel(const TreeParams p) {
+    static_assert(TJ_C % 2 == 0, "16 bytes of bfloat16 are two fours of columns");
     const int lane = threadIdx.x & 31, j = blockIdx.x, d4 = (p.d + 3) >> 2, n_cols = (d4 + TJ_C - 1) / TJ_C, task = blockIdx.y * TJ_WARPS + (threadIdx.x >> 5);
     const int row = task / n_cols * 32 + lane, c0 = task % n_cols * TJ_C;       // of the item; in fours of columns
     pdl_wait();
@@ -688,11 +687,18 @@ __global__ void __launch_bounds__(TJ_WARPS * 32) tree_join_kernel(const TreePara
             if ((c0 + c) * 4 + e < d) dst[c * 4 + e] = from_f32<T>(x[e] * inv);
     }
 }
+// Eight columns a warp and twelve pieces at a time where there are some pieces an item, or few warps anyhow (whole calls in bfloat16, 32 query heads on 8: 8 drafts
+// behind 4,096 keys 16.1 us against 19.9 with sixteen columns and six pieces, 64 drafts 26.5 against 28.0); with two or three pieces of many rows that
+// is more blocks than it helps (8 requests of 32 drafts behind 1,000 keys 28.2 against 26.2).
 template <typename T, int ROWS, int KT>
 static void tree_join(const TreeParams& p, int blocks, int max_rows, cudaStream_t stream) {
     if ((long long)p.table_width * p.page_size <= KT) return;        // one tile at most: nothing is cut
-    const int tasks = ((max_rows < ROWS ? max_rows : ROWS) + 31) / 32 * (((p.d + 3) / 4 + TJ_C - 1) / TJ_C);
-    msgl_launch_pdl(tree_join_kernel<T, ROWS>, dim3(blocks, (tasks + TJ_WARPS - 1) / TJ_WARPS), dim3(TJ_WARPS * 32), 0, stream, p);
+    const long long items = (long long)p.B * p.n_kv * ((max_rows + ROWS - 1) / ROWS);
+    const bool narrow = max_rows <= 32 || 4 * items <= blocks;
+    const int columns = narrow ? 8 : 16, tasks = ((max_rows < ROWS ? max_rows : ROWS) + 31) / 32 * ((p.d + columns - 1) / columns);
+    const dim3 grid(blocks, (tasks + TJ_WARPS - 1) / TJ_WARPS);
+    if (narrow) msgl_launch_pdl(tree_join_kernel<T, ROWS, 2, 12>, grid, dim3(TJ_WARPS * 32), 0, stream, p);
+    else msgl_launch_pdl(tree_join_kernel<T, ROWS, 4, 6>, grid, dim3(TJ_WARPS * 32), 0, stream, p);
 }
 
 #include "attention_tree_tc.cuh"

@@ -132,18 +132,22 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const TreeParams
         tc_mbar_init(bar_q, TT_SOFT); tc_mbar_init(bar_vt, 1);
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
+    if (tid == 32) {
+        asm volatile("prefetch.tensormap [%0];\n" ::"l"(&kmap) : "memory");
+        asm volatile("prefetch.tensormap [%0];\n" ::"l"(&vmap) : "memory");
+    }
     pdl_launch_dependents();
     pdl_wait();
     pdl_after_wait();
-    if (warp == 0) {             // all 512 columns of tensor memory: S_A | S_B | O_A | O_B (behind the wait: a kernel ahead of this one may want some)
+    const int gave_up = *reinterpret_cast<volatile int*>(status);           // (on its way while the work is cut)
+    if (warp == 18) {            // all 512 columns of tensor memory: S_A | S_B | O_A | O_B (behind the wait: a kernel ahead of this one may want some)
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;\n" ::"r"(smem_u32(&tmem_base_s)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
     }
     tc_fence_before();
     TreeWalk<TT_ROWS, TT_KT> walk(p);
-    const bool stop = __syncthreads_or(*reinterpret_cast<volatile int*>(status) != 0) != 0;      // an earlier block gave up: do not pile up
-    const bool work = walk.begin(j, gridDim.x, begun) && !stop && smem0 + C::SMEM <= smem_base + C::ALLOC;      // (a barrier of the block stands in begin)
-    __syncthreads();
+    const bool mine = walk.begin(j, gridDim.x, begun) && smem0 + C::SMEM <= smem_base + C::ALLOC;
+    const bool work = __syncthreads_or(gave_up != 0) == 0 && mine;           // (an earlier block gave up: do not pile up)
     tc_fence_after();
     const unsigned tmem = tmem_base_s;
     int fail = 0;
@@ -481,5 +485,5 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const TreeParams
     const bool failed = __syncthreads_or(fail) != 0;
     tc_fence_after();
     if (failed && tid == 0) atomicExch(status, 1);
-    if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;\n" ::"r"(tmem) : "memory");
+    if (warp == 18) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;\n" ::"r"(tmem) : "memory");
 }
