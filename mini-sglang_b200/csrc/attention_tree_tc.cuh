@@ -5,7 +5,7 @@
 //
 //     S = Q K^T     tcgen05.mma 128 x 128 x 16, operands in shared memory, accumulator in tensor memory
 //     softmax       two threads a row (TMEM lane), 64 scores each in registers; P, rounded to bfloat16 (half a step, 2^-9, of each weight;
-//                   the sum of the weights is taken before), goes back over the columns of S
+//                   the sum of the weights is taken before), goes back over the columns that each thread's scores had
 //     O += P V      tcgen05.mma 128 x D x 16, P from tensor memory, V from shared memory as it lies in the cache
 //
 // The products of a tile keep the tensor core about as busy as its exponentials the special-function units, and one follows the other for
@@ -23,8 +23,7 @@
 // drafts that do not see them; the drafts that do see them get them back at the end.
 //
 // The exponentials' reference m need not be a row's maximum: it moves where a tile's maximum is 2^8 above it, and O is scaled in tensor
-// memory then.  The two threads of a row meet once a tile, over the maximum, when both have their scores in registers (P of the one
-// lies over scores of the other), so they move alike.
+// memory then.  The two threads of a row meet once a tile, over the maximum, so they move alike.
 //
 // Every wait is bounded; a block that gives up sets the status word, waits for its copies, frees its tensor memory and returns.
 //
@@ -111,6 +110,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const TreeParams
     __shared__ bool sh_more[2];
     __shared__ TreeWalkState sh_walk;                 // their walk
     __shared__ TreeStart begun;
+    __shared__ TreeRecord sh_record;                 // (thread 0's; there is no register for it either)
     const unsigned smem_base = smem_u32(tt_smem);
     const unsigned smem0 = (smem_base + 512u + 1280u * 4u + 1023u) & ~1023u;
     const unsigned q_s = smem0, k_s = q_s + 2u * C::TILE, v_s = k_s + ST * C::TILE;
@@ -127,6 +127,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const TreeParams
     const int G = p.G;
 
     if (tid == 0) {
+        sh_record = TreeRecord{};
         for (int x = 0; x < 2; ++x) { tc_mbar_init(bar_s(x), 1); tc_mbar_init(bar_p(x, 0), 8); tc_mbar_init(bar_p(x, 1), 8); tc_mbar_init(bar_o(x), 1); }
         for (int st = 0; st < ST; ++st) { tc_mbar_init(bar_kf(st), 1); tc_mbar_init(bar_kr(st), 1); tc_mbar_init(bar_vf(st), 1); tc_mbar_init(bar_vr(st), 1); }
         tc_mbar_init(bar_q, TT_SOFT); tc_mbar_init(bar_vt, 1);
@@ -151,7 +152,6 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const TreeParams
     tc_fence_after();
     const unsigned tmem = tmem_base_s;
     int fail = 0;
-    TreeRecord record = {};
 
     if (!work) {
         if (tid == 0 && smem0 + C::SMEM > smem_base + C::ALLOC) atomicExch(status, 2);      // allocation not aligned as assumed
@@ -237,11 +237,11 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const TreeParams
                 for (int part = 0; part < 2; ++part) {
                     if (ok) ok = wait(bar_p(x, part), phase_p[x]);
                     if (!ok) return;
-                    tc_fence_async_smem(); tc_fence_after();
+                    tc_fence_after();
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const int kk = (i >> 1) * 4 + part * 2 + (i & 1);
-                        tt_mma_ta(leader, t_o, t_p + kk * 8u, dv_st + kk * (2048u >> 4), idesc_o, part + i > 0 ? 1u : s < 2 ? 0u : 1u);
+                        tt_mma_ta(leader, t_o, t_p + (kk >> 2) * 64u + (kk & 3) * 8u, dv_st + kk * (2048u >> 4), idesc_o, part + i > 0 ? 1u : s < 2 ? 0u : 1u);
                     }
                 }
                 phase_p[x] ^= 1u;
@@ -249,12 +249,13 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const TreeParams
                 if (!dual || x == 1) tt_commit(leader, bar_vr(st));
             };
             ok = wait(bar_q, seg & 1);
+            tc_fence_async_smem();                    // Q came by plain copies (keys and values by TMA; the values that are looked at are fenced where they are written)
             for (int s = 0; s < steps && ok; ++s) {
                 const int x = s & 1;
                 const unsigned c = tile_of(s), st = c % ST;
                 if (!dual || x == 0) ok = wait(bar_kf(st), (c / ST) & 1);
                 if (!ok) break;
-                tc_fence_async_smem(); tc_fence_after();
+                tc_fence_after();
                 const unsigned long long dq_x = dq + (dual && x ? step : 0u), dk_st = dk + st * step;
                 const unsigned t_s = tm + (unsigned)x * 128u;
 #pragma unroll
@@ -307,7 +308,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const TreeParams
             if (tid == 0) {
                 if (cut && g.t_lo == 0) {
                     walk.load(sh_walk);
-                    record = TreeRecord{walk.pieces(g, j), g.rows, g.tok0, g.row0, g.kvh, {0, 0, 0}};
+                    sh_record = TreeRecord{walk.pieces(g, j), g.rows, g.tok0, g.row0, g.kvh, {0, 0, 0}};
                 }
                 find(seg + 1);                       // (the segment before the present one has been left by all)
             }
@@ -315,85 +316,90 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const TreeParams
             const int tiles = g.t_hi - g.t_lo, n_mine = dual ? tiles : (tiles + 1 - x) >> 1;
             const int row = dual ? x * 128 + lane_row : lane_row, rr = g.row0 + row;
             const bool valid = row < g.rows, active = row - lane < g.rows;               // whether the row, and any of the warp's, exists
-            const size_t tok = (size_t)g.tok0 + (valid ? rr / G : 0);
+            const int tok = g.tok0 + (valid ? rr / G : 0);
             float m_run = -INFINITY, l_run = 0.f;    // of the row; of this thread's half of the keys
-            for (int it = 0; it < n_mine; ++it) {    // (a warp that gave up goes on to meet its partner)
+            if (!active)                             // (P of rows that do not exist may be anything)
+                for (int it = 0; it < n_mine; ++it) {
+                    if (!fail && __any_sync(0xffffffffu, !tc_mbar_wait(bar_s(x), phase_s))) fail = 1;
+                    phase_s ^= 1u;
+                    if (lane == 0) { tc_mbar_arrive(bar_p(x, 0)); tc_mbar_arrive(bar_p(x, 1)); }
+                }
+            else for (int it = 0; it < n_mine; ++it) {          // (a warp that gave up goes on to meet its partner)
                 if (!fail && __any_sync(0xffffffffu, !tc_mbar_wait(bar_s(x), phase_s))) fail = 1;
                 phase_s ^= 1u;
                 tc_fence_after();
-                if (active) {                        // (P of rows that do not exist may be anything)
-                    const int key0 = (g.t_lo + (dual ? it : 2 * it + x)) * TT_KT + 64 * half;
-                    float s0[32], s1[32];
-                    tc_ld32(ts + 64 * half, s0); tc_ld32(ts + 64 * half + 32, s1);
-                    tc_wait_ld(s0); tc_wait_ld(s1);
-                    if (key0 + 64 > g.base) {
-                        const unsigned* row_mask = p.mask + tok * p.words;
-                        const unsigned seen0 = tree_seen(row_mask, p.words, key0, g.base, g.kv), seen1 = tree_seen(row_mask, p.words, key0 + 32, g.base, g.kv);
+                const int key0 = (g.t_lo + (dual ? it : 2 * it + x)) * TT_KT + 64 * half;
+                float s0[32], s1[32];
+                tc_ld32(ts + 64 * half, s0); tc_ld32(ts + 64 * half + 32, s1);
+                tc_wait_ld(s0); tc_wait_ld(s1);
+                unsigned seen1 = ~0u;
+                auto hide = [&](float (&sv)[32], unsigned seen) {
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) {
-                            if (!(seen0 >> e & 1u)) s0[e] = -INFINITY;
-                            if (!(seen1 >> e & 1u)) s1[e] = -INFINITY;
-                        }
-                    }
-                    float c4[4];                     // (maxima of three: one instruction)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) c4[e] = fmaxf(s0[e], s1[e]);
-#pragma unroll
-                    for (int e = 4; e < 32; ++e) c4[e & 3] = fmaxf(fmaxf(c4[e & 3], s0[e]), s1[e]);
-                    const float mine = fmaxf(fmaxf(c4[0], c4[1]), fmaxf(c4[2], c4[3])) * sc;
-                    ex_max[half * 128 + lane_row] = mine;
-                    tc_fence_before();               // (the scores have been read, for the partner's P)
-                    asm volatile("bar.sync %0, 64;\n" ::"r"(pair) : "memory");
-                    tc_fence_after();
-                    const float mx = fmaxf(mine, ex_max[(1 - half) * 128 + lane_row]);
-                    const bool move = mx > m_run + 8.f || (m_run == -INFINITY && mx > -INFINITY);
-                    if (__any_sync(0xffffffffu, move)) {
-                        const float a = move ? fast_exp2(m_run - mx) : 1.f;              // 0 for the first
-                        if (move) { m_run = mx; l_run *= a; }
-                        if (it >= 1) {               // (P V of this group's tile before is done: this S was issued after it)
-#pragma unroll 1
-                            for (int cb = half * (D / 32); cb < (half + 1) * (D / 32); ++cb) {
-                                unsigned v0[16];
-                                tc_ld16(to + cb * 16, v0);
-                                tc_wait_ld16(v0);
-#pragma unroll
-                                for (int e = 0; e < 16; ++e) v0[e] = __float_as_uint(__uint_as_float(v0[e]) * a);
-                                tc_st16(to + cb * 16, v0);
-                            }
-                        }
-                    }
-                    const float mu = m_run == -INFINITY ? 0.f : m_run;
-                    const unsigned long long sc2 = tt_pack(sc, sc), nmu2 = tt_pack(-mu, -mu);
-                    unsigned long long sum2[4] = {0ull, 0ull, 0ull, 0ull};               // (0.f, 0.f)
-                    auto expo = [&](const float (&sv)[32], int cb) {
-                        unsigned pk[16];
-#pragma unroll
-                        for (int e = 0; e < 32; e += 2) {
-                            float x0, x1;
-                            tt_unpack(tt_fma(tt_pack(sv[e], sv[e + 1]), sc2, nmu2), x0, x1);
-                            const float e0 = fast_exp2(x0), e1 = fast_exp2(x1);
-                            sum2[(e >> 1) & 3] = tt_add(sum2[(e >> 1) & 3], tt_pack(e0, e1));
-                            pk[e >> 1] = pack_bf16(e0, e1);
-                        }
-                        tc_st16(ts + 32 * half + cb * 16, pk);
-                    };
-                    expo(s0, 0);
-                    tc_wait_st();
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) tc_mbar_arrive(bar_p(x, 0));
-                    expo(s1, 1);
-                    float lo, hi;
-                    tt_unpack(tt_add(tt_add(sum2[0], sum2[1]), tt_add(sum2[2], sum2[3])), lo, hi);
-                    l_run += lo + hi;
-                    tc_wait_st();
+                    for (int e = 0; e < 32; ++e)
+                        if (!(seen >> e & 1u)) sv[e] = -INFINITY;
+                };
+                if (key0 + 64 > g.base) {
+                    const unsigned* row_mask = p.mask + (size_t)tok * p.words;
+                    hide(s0, tree_seen(row_mask, p.words, key0, g.base, g.kv));
+                    seen1 = tree_seen(row_mask, p.words, key0 + 32, g.base, g.kv);
+                    hide(s1, seen1);
                 }
+                float c4[4];                     // (maxima of three: one instruction)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) c4[e] = fmaxf(s0[e], s1[e]);
+#pragma unroll
+                for (int e = 4; e < 32; ++e) c4[e & 3] = fmaxf(fmaxf(c4[e & 3], s0[e]), s1[e]);
+                const float mine = fmaxf(fmaxf(c4[0], c4[1]), fmaxf(c4[2], c4[3])) * sc;
+                ex_max[half * 128 + lane_row] = mine;
+                asm volatile("bar.sync %0, 64;\n" ::"r"(pair) : "memory");
+                const float mx = fmaxf(mine, ex_max[(1 - half) * 128 + lane_row]);
+                const bool move = mx > m_run + 8.f || (m_run == -INFINITY && mx > -INFINITY);
+                if (__any_sync(0xffffffffu, move)) {
+                    const float a = move ? fast_exp2(m_run - mx) : 1.f;              // 0 for the first
+                    if (move) { m_run = mx; l_run *= a; }
+                    if (it >= 1) {               // (P V of this group's tile before is done: this S was issued after it)
+#pragma unroll 1
+                        for (int cb = half * (D / 32); cb < (half + 1) * (D / 32); ++cb) {
+                            unsigned v0[16];
+                            tc_ld16(to + cb * 16, v0);
+                            tc_wait_ld16(v0);
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) v0[e] = __float_as_uint(__uint_as_float(v0[e]) * a);
+                            tc_st16(to + cb * 16, v0);
+                        }
+                    }
+                }
+                const float mu = m_run == -INFINITY ? 0.f : m_run;
+                const unsigned long long sc2 = tt_pack(sc, sc), nmu2 = tt_pack(-mu, -mu);
+                unsigned long long sum2[4] = {0ull, 0ull, 0ull, 0ull};               // (0.f, 0.f)
+                auto expo = [&](const float (&sv)[32], int cb) {
+                    unsigned pk[16];
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2) {
+                        float x0, x1;
+                        tt_unpack(tt_fma(tt_pack(sv[e], sv[e + 1]), sc2, nmu2), x0, x1);
+                        const float e0 = fast_exp2(x0), e1 = fast_exp2(x1);
+                        sum2[(e >> 1) & 3] = tt_add(sum2[(e >> 1) & 3], tt_pack(e0, e1));
+                        pk[e >> 1] = pack_bf16(e0, e1);
+                    }
+                    tc_st16(ts + 64 * half + cb * 16, pk);
+                };
+                expo(s0, 0);
+                tc_ld32(ts + 64 * half + 32, s1);            // (read again: kept, they would push others out of the registers)
+                tc_wait_st();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) {
-                    if (!active) tc_mbar_arrive(bar_p(x, 0));
-                    tc_mbar_arrive(bar_p(x, 1));
-                }
+                if (lane == 0) tc_mbar_arrive(bar_p(x, 0));
+                tc_wait_ld(s1);
+                if (seen1 != ~0u) hide(s1, seen1);
+                expo(s1, 1);
+                tc_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) tc_mbar_arrive(bar_p(x, 1));
+                float lo, hi;
+                tt_unpack(tt_add(tt_add(sum2[0], sum2[1]), tt_add(sum2[2], sum2[3])), lo, hi);
+                l_run += lo + hi;
             }
             // ---- the segment's end
             if (n_mine > 0) {
@@ -423,7 +429,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const TreeParams
             }
             if (active && !fail) {
                 const bool whole = !cut;
-                const unsigned* row_mask = p.mask + tok * p.words;
+                const unsigned* row_mask = p.mask + (size_t)tok * p.words;
                 const float inv = whole ? (l_all > 0.f ? 1.f / l_all : (l_all == l_all ? 0.f : l_all)) : 1.f;
                 const unsigned* bad = bad_words + (seg % TT_BAD) * 8;
                 unsigned any_bad = 0u;
@@ -433,7 +439,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const TreeParams
                 // blocks of 32 columns: two threads a row share them out, or four
                 const int cb0 = dual ? half * (D / 64) : D == 128 ? 2 * x + half : x, cb1 = dual ? cb0 + D / 64 : D == 128 || half == 0 ? cb0 + 1 : cb0;
                 const bool two = !dual && tiles > 1;
-                __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(p.out) + (tok * p.n_q + (size_t)g.kvh * G + (valid ? rr % G : 0)) * D;
+                __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(p.out) + ((size_t)tok * p.n_q + (size_t)g.kvh * G + (valid ? rr % G : 0)) * D;
                 float4* part = reinterpret_cast<float4*>(p.part_o) + (size_t)slot * (D / 4) * TT_ROWS + row;
                 const unsigned t_own = dual ? to : tmem + 256u + lane_sel, t_other = tmem + 384u + lane_sel;
 #pragma unroll 1
@@ -479,7 +485,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const TreeParams
             asm volatile("bar.sync 1, 512;\n" ::: "memory");                 // the exchange and both accumulators are free
         }
     }
-    if (tid == 0) p.record[j] = record;
+    if (tid == 0) p.record[j] = sh_record;
     pdl_late();
     tc_fence_before();
     const bool failed = __syncthreads_or(fail) != 0;
