@@ -14,7 +14,8 @@
 // more (what it costs beside them), and cut into one equal run a block: every block works out its run from the
 // requests' lengths by itself, so the host knows none of them and a captured launch serves any.  A block that has a whole item writes
 // its rows; of one that is cut every block leaves float32 partial sums with their maximum and sum of weights, and a second launch joins
-// them in the order of the keys.
+// them in the order of the keys.  What a small launch takes, at 8 drafts behind 1,000 keys (32 query heads on 8) 13 us: 2.2 until the work is cut, 1.5 for a
+// page's number and its copy's start, 5 for two tiles, 1.5 to the last store, 1 to the join's start and 2 in it.
 #include "common.cuh"
 #include <math.h>
 
@@ -224,9 +225,10 @@ template <> struct TsVec<__nv_bfloat16> {
 //
 // Warp w owns rows 16 (w / 2) .. + 15 and, of the scores, half of the keys, of O, half of the columns.  A thread has four rows (every fourth) against four
 // keys (every eighth) and then against eight columns: eight loads of 16 bytes for 64 multiply-adds, three for 32, and no two lanes meet a
-// bank.  The two warps of a row meet over its maximum.  P takes the place of the keys, key by key, a thread's four rows side by side.  Bound by what
-// shared memory delivers, 128 bytes a cycle: 14,300 cycles a tile, its multiply-adds 8,200.  A key that a row does not see has the weight -1, which the
-// product leaves out: its value may be anything.
+// bank.  The two warps of a row meet over its maximum.  P takes the place of the keys, key by key, a thread's four rows side by side.  A tile takes an SM 18,700
+// cycles (2 requests of 64 drafts behind 4,000 keys, 40 query heads on 8: 344 us, 30 TFLOP/s), of which shared memory's 128 bytes a cycle account for 14,300 and the
+// multiply-adds for 8,200; eight rows a thread, which takes a third off the first, leaves too few warps to hide its latency (342 us).  A key that a row does not see
+// has the weight -1, which the product leaves out: its value may be anything.
 // ---------------------------------------------------------------------------------------
 constexpr int TF_ROWS = 64, TF_KT = 64, TF_D = 128, TF_THREADS = 256, TF_PITCH = TF_D + 4, TF_PPITCH = TF_ROWS + 4;
 constexpr size_t TF_SMEM = (size_t)(TF_ROWS + 2 * TF_KT) * TF_PITCH * sizeof(float);
@@ -448,9 +450,10 @@ __global__ void __launch_bounds__(TF_THREADS, 2) tree_tile_kernel(const TreePara
 // Warp w owns rows 4 w .. 4 w + 3.  Scores: lane = key, four rows a lane, K rows of odd 16-byte pitch, so that a warp's loads of them
 // meet no bank twice; P^T goes to shared memory (four rows a key side by side) and O is four rows x 4 CB columns a lane.  Bound by what
 // shared memory delivers (five loads of 16 bytes for sixteen multiply-adds of the scores, two of O's), its steps are shorter than those of the kernel above.
-// float32, head size 128, this one / that one, us: groups of four, 1 request of 32 drafts behind 500 keys 33 / 57, 8 of 20 behind 100 41 / 47, 16 of 30 behind 300
-// 152 / 132, 2 of 12 behind 6,000 155 / 124; of two, 4 of 26 behind 1,500 89 / 84, 1 of 8 behind 1,000 23.5 / 38.7; of five, 2 of 64 behind 4,000 477 / 346.
-// So it stands where there are no more than 32 rows or fewer than eight tiles of the other an SM (as far as the host knows: the table's width).
+// float32, head size 128, this one / that one, us: groups of four, 1 request of 32 drafts behind 500 keys 26 / 49, 8 of 20 behind 100 40 / 41, 16 of 30 behind 300
+// 151 / 131, 2 of 12 behind 6,000 152 / 117, 4 of 26 behind 1,500 158 / 123; of two, 4 of 26 behind 1,500 86 / 72, 1 of 64 behind 2,000 66 / 56, 8 of 40 behind 500 (80 rows,
+// of 96 and of 128) 95 / 104; of five, 2 of 64 behind 4,000 475 / 344.  So it stands where there are no more than 32 rows, fewer than three tiles of the other an
+// SM, or where these are more than a third of its own tiles (as far as the host knows: the table's width).
 // ---------------------------------------------------------------------------------------
 constexpr int TS_ROWS = 32, TS_KT = 32, TS_THREADS = 256;
 

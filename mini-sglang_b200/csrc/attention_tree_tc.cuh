@@ -25,6 +25,11 @@
 // The exponentials' reference m need not be a row's maximum: it moves where a tile's maximum is 2^8 above it, and O is scaled in tensor
 // memory then.  The two threads of a row meet once a tile, over the maximum, so they move alike.
 //
+// Bound, at 32 query heads on 8 kv heads of 128: up to 128 rows by the stream of keys and values (37 requests behind 8,192 keys: 1 draft 191 us, 6.5 TB/s, 8 drafts 196, 16 drafts 205, 32
+// drafts 218, 5.7 TB/s); beyond by a tile's chain from scores over P to P V (64 drafts 330 to 350 us, some 900 TFLOP/s).  There a tile of 256 rows takes
+// 3,700 to 3,900 cycles, 2,048 of them in the tensor core, 2,048 in the exponentials: scores come 710 cycles after their first product was issued, 950 beside the
+// other group's work (Q and K out of shared memory take all of its 128 bytes a cycle), the softmax takes 2,100, the issuer sees P 300 later.
+//
 // Every wait is bounded; a block that gives up sets the status word, waits for its copies, frees its tensor memory and returns.
 //
 // Warps: 0-7 softmax A, 8-15 softmax B (all also fetch Q), 16 keys, 17 values, 18 issuer.  A softmax warp w works on TMEM lanes 32 (w % 4) .., and

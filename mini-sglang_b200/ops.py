@@ -2538,8 +2538,10 @@ def tree_attention(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_
         if status is not None and status.get_device() == dev:
             kind = _TREE_TC
     while True:
-        if kind == _TREE_SIMT and d <= 128 and max_rows > 32 and B * n_kv * -(-max_rows // 64) * -(-width * page_size // 64) >= 8 * sm_count(q.device):
-            kind = _TREE_TILE     # (measured in csrc/attention_tree.cu)
+        if kind == _TREE_SIMT and d <= 128 and max_rows > 32:          # (measured in csrc/attention_tree.cu)
+            large, small = -(-max_rows // 64) * -(-width * page_size // 64), -(-max_rows // 32) * -(-width * page_size // 32)
+            if B * n_kv * large >= 3 * sm_count(q.device) and 3 * large <= small:
+                kind = _TREE_TILE
         blocks, rows = facts[1][kind]
         n_part, d4 = 2 * blocks * rows, d + 3 & ~3
         part = torch.empty(n_part * (d4 + 2) + 8 * blocks, dtype=torch.float32, device=q.device)
