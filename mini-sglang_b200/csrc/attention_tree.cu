@@ -14,8 +14,8 @@
 // more (what it costs beside them), and cut into one equal run a block: every block works out its run from the
 // requests' lengths by itself, so the host knows none of them and a captured launch serves any.  A block that has a whole item writes
 // its rows; of one that is cut every block leaves float32 partial sums with their maximum and sum of weights, and a second launch joins
-// them in the order of the keys.  What a small launch takes, at 8 drafts behind 1,000 keys (32 query heads on 8) 13 us: 2.2 until the work is cut, 1.5 for a
-// page's number and its copy's start, 5 for two tiles, 1.5 to the last store, 1 to the join's start and 2 in it.
+// them in the order of the keys.  What a small launch takes, at 8 drafts behind 1,000 keys (32 query heads on 8) 12.5 us: 1.8 until the work is cut, 1.5 for a
+// page's number and its copy's start, 2.5 for a tile, 1.8 to the last store, 1 to the join's start and 2 in it.
 #include "common.cuh"
 #include <math.h>
 
@@ -119,7 +119,8 @@ struct TreeWalk {
         const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n_warps = blockDim.x >> 5;
         const int per = (p.B + blockDim.x - 1) / blockDim.x, i0 = min(p.B, tid * per), i1 = min(p.B, i0 + per);
         int mine = 0;
-        for (int i = i0; i < i1; ++i) { const Request w = request(i); mine += w.items * (w.tiles + TREE_HEAD); }
+        Request w = {};                              // the thread's last request: where each has one, it is not looked at again
+        for (int i = i0; i < i1; ++i) { w = request(i); mine += w.items * (w.tiles + TREE_HEAD); }
         int upto = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) { const int v = __shfl_up_sync(0xffffffffu, upto, o); if (lane >= o) upto += v; }
@@ -127,7 +128,8 @@ struct TreeWalk {
         if (tid == 0) to.work = 0;
         __syncthreads();
         int before = upto - mine, total = 0;
-        for (int w = 0; w < n_warps; ++w) { if (w < warp) before += sums[w]; total += sums[w]; }
+        const int warps = per == 1 ? (p.B + 31) >> 5 : n_warps;          // that have any
+        for (int k = 0; k < warps; ++k) { if (k < warp) before += sums[k]; total += sums[k]; }
         blocks = max(1, min(nb, total / TREE_SHARE));
         if (total == 0 || j >= blocks) return false;
         whole = total / blocks;
@@ -136,19 +138,30 @@ struct TreeWalk {
         x_hi = cut_at(j + 1);
         if (x_lo >= before && x_lo < before + mine) {
             start = before;
-            for (r = i0; r < i1; ++r) {
-                const Request w = request(r);
-                const int len = w.items * (w.tiles + TREE_HEAD);
-                if (x_lo < start + len) { item = (x_lo - start) / (w.tiles + TREE_HEAD); break; }
-                start += len;
-            }
-            TreeSegment g;
-            if (next(g)) { to.first = g; to.work = 1; }
+            r = i0;
+            if (per > 1)
+                for (;; ++r) {
+                    w = request(r);
+                    const int len = w.items * (w.tiles + TREE_HEAD);
+                    if (x_lo < start + len || r + 1 >= i1) break;
+                    start += len;
+                }
+            item = (x_lo - start) / (w.tiles + TREE_HEAD);
+            // (a run is long enough to hold a tile of the item that it starts in)
+            const int s = start + item * (w.tiles + TREE_HEAD), e = s + w.tiles + TREE_HEAD;
+            to.first = segment(w, x_lo > s ? tile_at(x_lo, s, w.tiles) : 0, x_hi < e ? tile_at(x_hi, s, w.tiles) : w.tiles);
+            ++item;
+            to.work = 1;
             store(to.walk);
         }
         __syncthreads();
         load(to.walk);
         return to.work != 0;
+    }
+    // tiles [lo, hi) of item `item` of request r, which is w
+    __device__ __forceinline__ TreeSegment segment(const Request& w, int lo, int hi) const {
+        const int kvh = w.groups == 1 ? item : item / w.groups, row0 = (item - kvh * w.groups) * ROWS;
+        return TreeSegment{r, kvh, row0, min(ROWS, w.n * p.G - row0), w.tok0, w.n, w.kv, w.base, lo, hi, w.tiles};
     }
     // the next segment of the run; false: it is done
     __device__ __forceinline__ bool next(TreeSegment& g) {
@@ -160,12 +173,7 @@ struct TreeWalk {
                 if (s >= x_hi) return false;
                 const int lo = x_lo > s ? tile_at(x_lo, s, w.tiles) : 0, hi = x_hi < s + len ? tile_at(x_hi, s, w.tiles) : w.tiles;
                 if (lo >= hi) continue;
-                g.r = r;
-                g.kvh = w.groups == 1 ? item : item / w.groups;
-                g.row0 = (item - g.kvh * w.groups) * ROWS;
-                g.rows = min(ROWS, w.n * p.G - g.row0);
-                g.tok0 = w.tok0; g.n = w.n; g.kv = w.kv; g.base = w.base;
-                g.t_lo = lo; g.t_hi = hi; g.tiles = w.tiles;
+                g = segment(w, lo, hi);
                 ++item;
                 return true;
             }
