@@ -17,10 +17,10 @@
 // A row is read by a cluster of C blocks, whose first merges the others' sums and keys out of their shared memory: no scratch memory,
 // no counters, one launch.
 //
-// Many rows are bound by their bytes, or by the instructions of a value where these are few bytes: 2,048 rows of 151,936 in float32 take 185 us without top tokens (6.7 TB/s), 198 with
-// five, 206 with twenty, in bfloat16 155 with five (4.0 TB/s; some ten instructions a value).  Values go in pairs through the packed float32
+// Many rows are bound by their bytes, or by the instructions of a value where these are few bytes: 2,048 rows of 151,936 in float32 take 184 us without top tokens (6.8 TB/s), 198 with
+// five, 205 with twenty, in bfloat16 153 with five (4.1 TB/s; some ten instructions a value).  Values go in pairs through the packed float32
 // instructions, and the next stretch is asked for before the present one is worked on.  Few rows are bound by latency: one row with twenty takes
-// 11 us, of which the launch, eight blocks' share of the row, two merges and the cluster's two barriers follow on one another.
+// 10.8 us (4.5 without): the launch, the first bound (1.2), eight blocks' share of the row, two merges and the cluster's two barriers follow on one another.
 //
 // A logit of -inf adds nothing.  A row with a NaN, with +inf or with nothing but -inf has NaN in all its probabilities, as the
 // formula has; its top tokens are those of the highest numbers (a NaN is none).  A token outside the vocabulary gets NaN.
@@ -83,19 +83,18 @@ struct LpSums {
         s *= f;
         m = to;
     }
-    __device__ __forceinline__ void join(LpSums o) {
-        const float to = fmaxf(m, o.m);
-        if (to == -INFINITY) { s += o.s; t += o.t; return; }       // (nothing, or NaN)
-        move(to);
-        o.move(to);
-        s += o.s;
-        t += o.t;
-    }
 };
+// the sums of a warp's lanes, to all of them: the maximum first, so that every lane moves once
 __device__ __forceinline__ LpSums lp_warp_join(LpSums a) {
+    float to = a.m;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
-        a.join(LpSums{__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o), __shfl_xor_sync(0xffffffffu, a.t, o)});
+    for (int o = 16; o > 0; o >>= 1) to = fmaxf(to, __shfl_xor_sync(0xffffffffu, to, o));
+    a.move(to);                                      // (all -inf: to is -inf as a.m is, and nothing changes)
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        a.s += __shfl_xor_sync(0xffffffffu, a.s, o);
+        a.t += __shfl_xor_sync(0xffffffffu, a.t, o);
+    }
     return a;
 }
 
