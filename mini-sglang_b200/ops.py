@@ -2490,7 +2490,7 @@ def draft_plan(parents: torch.Tensor, draft_lens: torch.Tensor, cached: torch.Te
         buf = torch.zeros(1 + T * (3 + words), dtype=torch.int32, device=parents.device)
     else:
         buf = torch.empty(2 * B + 1 + T * (3 + words), dtype=torch.int32, device=parents.device)
-    q_start, kv_len, positions, token_req, out_loc, mask = buf.split((B + 1, B, T, T, T, T * words))
+    q_start, kv_len, positions, token_req, out_loc, mask = buf.split_with_sizes((B + 1, B, T, T, T, T * words))
     at = buf.data_ptr()
     rows = at + 4 * (2 * B + 1)
     code = _draft_lib().msgl_draft_plan(parents.data_ptr(), T, draft_lens.data_ptr(), cached.data_ptr(), B, block_table.data_ptr(), block_table.stride(0), width,
@@ -2640,7 +2640,7 @@ def draft_accept(tokens: torch.Tensor, parents: torch.Tensor, following: torch.T
         groups = _cache_groups(caches, tokens)
     _same_device("draft_accept", tokens, parents, following, q_start, kv_len, block_table)
     buf = torch.empty(B * (1 + 2 * max_draft), dtype=torch.int32, device=tokens.device)
-    kept, path, after = buf.split((B, B * max_draft, B * max_draft))
+    kept, path, after = buf.split_with_sizes((B, B * max_draft, B * max_draft))
     launches = [(shape, item, ptrs[i:i + _ACCEPT_CACHES]) for shape, item, ptrs in groups for i in range(0, len(ptrs), _ACCEPT_CACHES)]
     out = (kept.data_ptr(), path.data_ptr(), after.data_ptr())
     for shape, item, ptrs in launches or [((0, 1, 1, 1), 2, [])]:
@@ -2677,7 +2677,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
         raise KernelError(f"token_logprobs: top {top} is outside [0, {min(MAX_TOP, V)}]")
     _same_device("token_logprobs", logits, tokens)
     buf = torch.empty(N * (2 + top), dtype=torch.float32, device=logits.device)
-    lp, entropy, best = buf.split((N, N, N * top))
+    lp, entropy, best = buf.split_with_sizes((N, N, N * top))
     ids = torch.empty((N, top), dtype=torch.int32, device=logits.device)
     if N == 0:
         return TokenLogprobs(lp, entropy, best.view(N, top), ids)
