@@ -166,6 +166,37 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const TreeParams
         const CUtensorMap* map = is_k ? &kmap : &vmap;
         const int n_box = TT_KT / tma_box;
         unsigned vt_phase = 0, count = 0, seg = 0;
+        // Values that are looked at: clears the rows behind the last key and what is no number, once the tile has come.  Put off until the next tile's pages are known.
+        int due = -1, due_key0 = 0, due_base = 0, due_kv = 0;                        // the stage of such a tile
+        unsigned due_seg = 0;
+        auto look = [&]() {
+            const int st = due;
+            due = -1;
+            if (__any_sync(0xffffffffu, !tc_mbar_wait(bar_vt, vt_phase))) return false;
+            vt_phase ^= 1u;
+            const unsigned dst_tile = v_s + (unsigned)st * C::TILE;
+            auto chunk_at = [&](int row, int c) { return dst_tile + tt_off(row, c); };
+            const int end = min(max(due_kv - due_key0, 0), TT_KT);           // rows that hold keys
+            for (int i = lane; i < (TT_KT - end) * H * 8; i += 32)
+                asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};\n" ::"r"(chunk_at(end + i / (H * 8), i % (H * 8))), "r"(0u) : "memory");
+            const int first = min(max(due_base - due_key0, 0), end);         // the drafts among them
+            for (int i = lane; i < (end - first) * H * 8; i += 32) {
+                const int row = first + i / (H * 8);
+                const unsigned a = chunk_at(row, i % (H * 8));
+                uint4 v;
+                asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+                const unsigned bx = tt_nonfinite(v.x), by = tt_nonfinite(v.y), bz = tt_nonfinite(v.z), bw = tt_nonfinite(v.w);
+                if ((bx | by | bz | bw) != 0u) {
+                    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};\n" ::"r"(a), "r"(v.x & ~bx), "r"(v.y & ~by), "r"(v.z & ~bz), "r"(v.w & ~bw) : "memory");
+                    const int draft = due_key0 + row - due_base;
+                    if (draft >= 0 && draft < 256) atomicOr(&bad_words[(due_seg % TT_BAD) * 8 + (draft >> 5)], 1u << (draft & 31));
+                }
+            }
+            tc_fence_async_smem();
+            __syncwarp();
+            if (lane == 0) tc_mbar_arrive(bar_vf(st));
+            return true;
+        };
         TreeSegment g = begun.first;
         for (bool more = true; !fail && more; more = walk.next(g), ++seg) {
             const int* bt = p.table + (size_t)g.r * p.table_stride;
@@ -180,6 +211,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const TreeParams
                 }
                 const unsigned n_act = __popc(__ballot_sync(0xffffffffu, y != -1));
                 const bool looked_at = !is_k && key0 + TT_KT > g.base;
+                if (due >= 0 && !look()) { fail = 1; break; }
                 if (count >= ST && __any_sync(0xffffffffu, !tc_mbar_wait(is_k ? bar_kr(st) : bar_vr(st), (count / ST - 1) & 1))) { fail = 1; break; }
                 const unsigned bar = looked_at ? bar_vt : (is_k ? bar_kf(st) : bar_vf(st)), dst_tile = (is_k ? k_s : v_s) + (unsigned)st * C::TILE;
                 if (lane == 0) tc_mbar_expect_tx(bar, n_act * H * (unsigned)tma_box * 128u);
@@ -189,31 +221,10 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const TreeParams
 #pragma unroll
                     for (int h = 0; h < H; ++h) tc_tma_load(dst + h * TT_HALF, map, 64 * h, y, bar);
                 }
-                if (!looked_at) continue;
-                if (__any_sync(0xffffffffu, !tc_mbar_wait(bar_vt, vt_phase))) { fail = 1; ++count; break; }
-                vt_phase ^= 1u;
-                auto chunk_at = [&](int row, int c) { return dst_tile + tt_off(row, c); };
-                const int end = min(max(g.kv - key0, 0), TT_KT);             // rows that hold keys
-                for (int i = lane; i < (TT_KT - end) * H * 8; i += 32)
-                    asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};\n" ::"r"(chunk_at(end + i / (H * 8), i % (H * 8))), "r"(0u) : "memory");
-                const int first = min(max(g.base - key0, 0), end);           // the drafts among them
-                for (int i = lane; i < (end - first) * H * 8; i += 32) {
-                    const int row = first + i / (H * 8);
-                    const unsigned a = chunk_at(row, i % (H * 8));
-                    uint4 v;
-                    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
-                    const unsigned bx = tt_nonfinite(v.x), by = tt_nonfinite(v.y), bz = tt_nonfinite(v.z), bw = tt_nonfinite(v.w);
-                    if ((bx | by | bz | bw) != 0u) {
-                        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};\n" ::"r"(a), "r"(v.x & ~bx), "r"(v.y & ~by), "r"(v.z & ~bz), "r"(v.w & ~bw) : "memory");
-                        const int draft = key0 + row - g.base;
-                        if (draft >= 0 && draft < 256) atomicOr(&bad_words[(seg % TT_BAD) * 8 + (draft >> 5)], 1u << (draft & 31));
-                    }
-                }
-                tc_fence_async_smem();
-                __syncwarp();
-                if (lane == 0) tc_mbar_arrive(bar_vf(st));
+                if (looked_at) { due = st; due_key0 = key0; due_base = g.base; due_kv = g.kv; due_seg = seg; }
             }
         }
+        if (!fail && due >= 0 && !look()) fail = 1;
         // nobody leaves with copies under way (values that are looked at have been waited for above)
         for (unsigned c = count > ST ? count - ST : 0; c < count; ++c) tc_mbar_wait(is_k ? bar_kf(c % ST) : bar_vf(c % ST), (c / ST) & 1);
     } else if (warp == 18) {
@@ -310,7 +321,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const TreeParams
             const TreeSegment& g = sh_seg[seg & 1];
             const bool dual = g.rows > 128;
             const bool cut = g.t_lo != 0 || g.t_hi != g.tiles;
-            if (tid == 0) {
+            if (tid == TT_SOFT - 32) {               // (of the last warp: with few rows it has nothing else to do, and the first has all)
                 if (cut && g.t_lo == 0) {
                     walk.load(sh_walk);
                     sh_record = TreeRecord{walk.pieces(g, j), g.rows, g.tok0, g.row0, g.kvh, {0, 0, 0}};
