@@ -112,7 +112,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const TreeParams
     unsigned* bad_words = reinterpret_cast<unsigned*>(tt_smem + 256);                     // [TT_BAD][8]
     float* exchange = reinterpret_cast<float*>(tt_smem + 512);                            // [2 groups][2 halves][128] maxima, the same of sums, [2][128] references
     __shared__ TreeSegment sh_seg[2];                // the softmax groups' segment and the one after it
-    __shared__ bool sh_more[2];
+    __shared__ int sh_more[2];                        // 0: there is none; the rows of Q to write for it
     __shared__ TreeWalkState sh_walk;                 // their walk
     __shared__ TreeStart begun;
     __shared__ TreeRecord sh_record;                 // (thread 0's; there is no register for it either)
@@ -296,28 +296,32 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const TreeParams
         const int pair = 2 + x * 4 + (warp & 3);     // the barrier of the two warps of these rows
         unsigned phase_s = 0, phase_o = 0, seg = 0;
         const float sc = p.scale_log2;
+        // before: of the segment ahead (of none: 256)
+        auto rows_to_write = [](int rows, int before) { return max(rows, rows <= 128 ? min(before, 128) : before > 128 ? before : 256); };
         auto find = [&](unsigned s) {                // (one thread)
             walk.load(sh_walk);
             TreeSegment w;
             const bool more = walk.next(w);
+            sh_more[s & 1] = more ? rows_to_write(w.rows, sh_seg[(s - 1) & 1].rows) : 0;
             if (more) sh_seg[s & 1] = w;
-            sh_more[s & 1] = more;
             walk.store(sh_walk);
         };
-        auto load_q = [&](const TreeSegment& w) {    // 16-byte chunks over all softmax threads; rows without a query are zero
+        // 16-byte chunks over all softmax threads.  Rows without a query are zero, which spares the tensor cores' power; only those are written that held one for the
+        // segment before (all of them each time took a segment 0.8 us).  (An item's rows are below 2^24: divided by way of the reciprocal.)
+        auto load_q = [&](const TreeSegment& w, int upto) {
             const __nv_bfloat16* qg = reinterpret_cast<const __nv_bfloat16*>(p.q);
-            for (int i = tid; i < (w.rows > 128 ? 256 : 128) * H * 8; i += TT_SOFT) {
-                const int row = i / (H * 8), c = i % (H * 8), rr = w.row0 + row;
+            for (int i = tid; i < upto * H * 8; i += TT_SOFT) {
+                const int row = i / (H * 8), c = i % (H * 8), rr = w.row0 + row, draft = walk.quotient(rr, G);
                 const bool valid = row < w.rows;
-                const __nv_bfloat16* src = valid ? qg + ((size_t)(w.tok0 + rr / G) * p.n_q + (size_t)w.kvh * G + rr % G) * D + c * 8 : qg;
-                tt_cp_async16(q_s + (unsigned)(row >> 7) * C::TILE + tt_off(row & 127, c), src, valid);
+                tt_cp_async16(q_s + (unsigned)(row >> 7) * C::TILE + tt_off(row & 127, c),
+                              valid ? qg + ((size_t)(w.tok0 + draft) * p.n_q + (size_t)w.kvh * G + (rr - draft * G)) * D + c * 8 : qg, valid);
             }
             tc_cp_async_arrive(bar_q);
         };
-        load_q(begun.first);
-        if (tid == 0) { sh_seg[0] = begun.first; sh_more[0] = true; sh_walk = begun.walk; }
+        load_q(begun.first, rows_to_write(begun.first.rows, TT_ROWS));
+        if (tid == 0) { sh_seg[0] = begun.first; sh_more[0] = 1; sh_walk = begun.walk; }
         asm volatile("bar.sync 1, 512;\n" ::: "memory");
-        for (; *reinterpret_cast<volatile bool*>(&sh_more[seg & 1]); ++seg) {
+        for (; *reinterpret_cast<volatile int*>(&sh_more[seg & 1]) != 0; ++seg) {
             const TreeSegment& g = sh_seg[seg & 1];
             const bool dual = g.rows > 128;
             const bool cut = g.t_lo != 0 || g.t_hi != g.tiles;
@@ -332,7 +336,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const TreeParams
             const int tiles = g.t_hi - g.t_lo, n_mine = dual ? tiles : (tiles + 1 - x) >> 1;
             const int row = dual ? x * 128 + lane_row : lane_row, rr = g.row0 + row;
             const bool valid = row < g.rows, active = row - lane < g.rows;               // whether the row, and any of the warp's, exists
-            const int tok = g.tok0 + (valid ? rr / G : 0);
+            const int tok = g.tok0 + (valid ? walk.quotient(rr, G) : 0);
             float m_run = -INFINITY, l_run = 0.f;    // of the row; of this thread's half of the keys
             if (!active)                             // (P of rows that do not exist may be anything)
                 for (int it = 0; it < n_mine; ++it) {
@@ -431,7 +435,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const TreeParams
             tc_fence_after();
             // both groups have seen the last of this segment's scores, so Q is free: the next segment's comes while this one's rows are written, and its first
             // scores are made meanwhile
-            if (*reinterpret_cast<volatile bool*>(&sh_more[(seg + 1) & 1])) load_q(sh_seg[(seg + 1) & 1]);
+            if (const int upto = *reinterpret_cast<volatile int*>(&sh_more[(seg + 1) & 1])) load_q(sh_seg[(seg + 1) & 1], upto);
             float fa = 1.f, fb = 0.f, m_all = m_run, l_all;                              // factors of O_A and O_B (dual: of the group's own alone)
             if (dual) {
                 l_all = ex_sum[x * 256 + lane_row] + ex_sum[x * 256 + 128 + lane_row];
@@ -455,7 +459,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_tc_kernel(const TreeParams
                 // blocks of 32 columns: two threads a row share them out, or four
                 const int cb0 = dual ? half * (D / 64) : D == 128 ? 2 * x + half : x, cb1 = dual ? cb0 + D / 64 : D == 128 || half == 0 ? cb0 + 1 : cb0;
                 const bool two = !dual && tiles > 1;
-                __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(p.out) + ((size_t)tok * p.n_q + (size_t)g.kvh * G + (valid ? rr % G : 0)) * D;
+                __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(p.out) + ((size_t)tok * p.n_q + (size_t)g.kvh * G + (valid ? rr - (tok - g.tok0) * G : 0)) * D;
                 float4* part = reinterpret_cast<float4*>(p.part_o) + (size_t)slot * (D / 4) * TT_ROWS + row;
                 const unsigned t_own = dual ? to : tmem + 256u + lane_sel, t_other = tmem + 384u + lane_sel;
 #pragma unroll 1
