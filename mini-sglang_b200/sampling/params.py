@@ -1,6 +1,7 @@
 from __future__ import annotations
 
 import dataclasses
+import operator
 from typing import Any, Dict, Optional
 
 MAX_LOGPROBS = 32          # alternatives a token (what the kernel keeps)
@@ -21,8 +22,16 @@ class SamplingParams:
     logprobs: Optional[int] = None
 
     def check_logprobs(self) -> None:
-        if self.logprobs is not None and not 0 <= self.logprobs <= MAX_LOGPROBS:
-            raise ValueError(f"logprobs must be between 0 and {MAX_LOGPROBS}")
+        """Anything but a whole number in range is refused (inside a step it would stop every other request of the batch as well)."""
+        if self.logprobs is None:
+            return
+        try:
+            n = -1 if isinstance(self.logprobs, bool) else operator.index(self.logprobs)
+        except TypeError:
+            n = -1
+        if not 0 <= n <= MAX_LOGPROBS:
+            raise ValueError(f"logprobs must be a whole number between 0 and {MAX_LOGPROBS}; got {self.logprobs!r}")
+        self.logprobs = n
 
     @classmethod
     def init_from_dict(cls, d: Optional[Dict[str, Any]]) -> "SamplingParams":
