@@ -2673,8 +2673,13 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
         raise KernelError(f"token_logprobs: logits are float32 or bfloat16 [rows, vocabulary] with adjacent columns; got {logits.dtype} {tuple(logits.shape)}")
     N, V = logits.shape
     _index("token_logprobs", "tokens", tokens, N)
-    if type(top) is not int or not 0 <= top <= min(MAX_TOP, V) or V < 1:
-        raise KernelError(f"token_logprobs: top {top!r} is no whole number in [0, {min(MAX_TOP, V)}]")
+    if type(top) is not int:
+        try:
+            top = -1 if isinstance(top, bool) else operator.index(top)          # (numpy's whole numbers are taken)
+        except TypeError:
+            raise KernelError(f"token_logprobs: top {top!r} is no whole number") from None
+    if not 0 <= top <= min(MAX_TOP, V) or V < 1:
+        raise KernelError(f"token_logprobs: top {top} is outside [0, {min(MAX_TOP, V)}]")
     _same_device("token_logprobs", logits, tokens)
     buf = torch.empty(N * (2 + top), dtype=torch.float32, device=logits.device)
     lp, entropy, best = buf.split_with_sizes((N, N, N * top))

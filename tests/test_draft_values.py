@@ -23,3 +23,8 @@ def test_whole_numbers_are_taken(n):
 def test_top_is_a_whole_number(top):
     with pytest.raises(ops.KernelError, match="top"):
         ops.token_logprobs(torch.zeros(3, 50), torch.zeros(3, dtype=torch.int32), top)
+
+
+def test_whole_numbers_of_numpy_are_taken_as_top():
+    with pytest.raises(ops.KernelError, match="CUDA device"):          # (nothing but the device is wrong)
+        ops.token_logprobs(torch.zeros(3, 50), torch.zeros(3, dtype=torch.int32), np.int64(3))
