@@ -62,6 +62,17 @@ class DraftEntry:
     parents: Optional[Sequence[int]] = None
 
 
+def join_equal_drafts(tokens: Sequence[int], parents: Sequence[int]) -> List[int]:
+    """Parents of the same drafts where no two that are followed have both parent and token in common: what follows the second of two such siblings
+    is put behind the first, whose key and value are the same, and the second is left without children.  Then a walk along the first fitting child
+    takes the longest path that the tokens allow."""
+    first, seen, out = [], {}, []          # first: of every draft the one that stands for it
+    for i, (token, p) in enumerate(zip(tokens, parents)):
+        out.append(first[p] if p >= 0 else p)
+        first.append(seen.setdefault((out[i], int(token)), i))
+    return out
+
+
 def _align4(n: int) -> int:
     return (n + 3) & ~3
 
@@ -667,6 +678,7 @@ class ModelRunner:
                 raise ValueError(f"slot {e.slot}: the first draft has parent -1, every other an earlier draft")
             if min(e.tokens) < 0 or max(e.tokens) >= V:
                 raise ValueError(f"token id outside [0, {V}) in the drafts of slot {e.slot}")
+            up = join_equal_drafts(e.tokens, up)
             depth = [0] * n
             for i in range(1, n):
                 depth[i] = depth[up[i]] + 1

@@ -1,0 +1,71 @@
+"""The host's part of ModelRunner.verify, without a GPU: what it hands to the step, what it keeps, what it leaves of the reservations."""
+import random
+
+import plain_drafts as P
+import pytest
+
+from mini_sglang_b200.cache import CacheManager, OutOfPages, PagedKVNeed
+from mini_sglang_b200.engine import DraftEntry
+from mini_sglang_b200.engine.step import ModelRunner
+
+
+def make_runner(model, vocab=9, num_pages=64, max_context_len=128, page_size=4, max_reqs=4):
+    """A runner without a device: a step keeps the path of first children as `draft_accept` does; `model` gives the token after a sequence of tokens."""
+    r = ModelRunner.__new__(ModelRunner)
+    r.mgr = CacheManager({0: PagedKVNeed(2, 8)}, page_size=page_size, num_pages=num_pages, max_reqs=max_reqs, max_context_len=max_context_len)
+    r.vocab_size, r.page_size, r.max_context_len, r.calls = vocab, page_size, max_context_len, 0
+    r.drafts_supported = lambda: True
+
+    def step(entries, lens, parents, depths, *_):
+        r.calls += 1
+        kept, tokens = [], []
+        for e, up, depth in zip(entries, parents, depths):
+            anc = [sorted(a) for a in P.ancestors(up)]
+            assert depth == [len(a) - 1 for a in anc]
+            after = [model([e.tokens[a] for a in path]) for path in anc]
+            path = P.accepted(up, list(e.tokens), after)
+            kept.append(len(path))
+            tokens.append([after[i] for i in path] + [-1] * (len(up) - len(path)))
+        return kept, tokens
+
+    r._verify = step
+    return r
+
+
+def longest(up, tokens, model):
+    """The model's tokens along the longest path that it agrees with, by trying every draft."""
+    best = []
+    for anc in (sorted(a) for a in P.ancestors(up)):
+        said = [model([tokens[a] for a in anc[:k + 1]]) for k in range(len(anc))]
+        if anc[0] == 0 and all(tokens[b] == s for b, s in zip(anc[1:], said)) and len(said) > len(best):
+            best = said
+    return best
+
+
+def test_siblings_of_one_token():
+    """The longer path hangs below the second of two siblings that hold the same token."""
+    follow = {1: 2, 2: 3, 3: 4}
+    runner = make_runner(lambda seq: follow[seq[-1]])
+    slot = runner.mgr.open()
+    assert runner.verify([DraftEntry(slot, [1, 2, 2, 3], [-1, 0, 0, 2])], None) == [[2, 3, 4]]
+    assert int(runner.mgr.length[slot]) == 3
+
+
+def test_the_path_kept_is_the_longest():
+    rng = random.Random(4)
+    gained = 0
+    for _ in range(300):
+        n, vocab = rng.randint(1, 24), rng.choice((2, 3, 5))
+        up = [-1] + [rng.randrange(max(0, i - rng.choice((2, 9))), i) for i in range(1, n)]
+        tokens = [rng.randrange(vocab) for _ in range(n)]
+        table = {}
+
+        def model(seq):
+            return table.setdefault(tuple(seq), rng.randrange(vocab))
+
+        runner = make_runner(model, vocab)
+        slot = runner.mgr.open()
+        got = runner.verify([DraftEntry(slot, tokens, up)], None)[0]
+        assert got == longest(up, tokens, model)
+        gained += len(got) > len(P.accepted(up, tokens, [model([tokens[a] for a in sorted(anc)]) for anc in P.ancestors(up)]))
+    assert gained > 10                                   # trees where the first child alone would have lost tokens
