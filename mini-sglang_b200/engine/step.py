@@ -658,7 +658,10 @@ class ModelRunner:
 
         `sampler` (a Sampler) draws the model's token after every draft as it would after the same tokens fed one by one: with the entry's
         temperature (default 0), its key and, for a draft of depth d, step + d (default 0).  So the tokens are those of plain decoding, drawn
-        with the same noise.  The path's keys and values are in the cache afterwards, in order; the rest is forgotten."""
+        with the same noise.  The path's keys and values are in the cache afterwards, in order; the rest is forgotten.
+
+        Every draft has a place in the cache during the step: a tree whose drafts and cached tokens together are beyond the context limit is refused
+        (ValueError, naming the slot, before anything is taken for any entry), so callers bring smaller trees near the limit."""
         if not self.drafts_supported():
             raise ValueError("drafted tokens need a model whose layers attend to all keys of a paged cache")
         entries = list(entries)
@@ -678,6 +681,10 @@ class ModelRunner:
                 raise ValueError(f"slot {e.slot}: the first draft has parent -1, every other an earlier draft")
             if min(e.tokens) < 0 or max(e.tokens) >= V:
                 raise ValueError(f"token id outside [0, {V}) in the drafts of slot {e.slot}")
+            if not 0 < e.slot <= self.mgr.max_reqs or not self.mgr.is_open(e.slot):
+                raise ValueError(f"slot {e.slot} is not open")
+            if self.mgr.length[e.slot] + n > self.max_context_len:
+                raise ValueError(f"slot {e.slot}: {self.mgr.length[e.slot]} tokens in the cache and a tree of {n} are more than the context limit of {self.max_context_len}")
             up = join_equal_drafts(e.tokens, up)
             depth = [0] * n
             for i in range(1, n):

@@ -4,7 +4,7 @@ import random
 import plain_drafts as P
 import pytest
 
-from mini_sglang_b200.cache import CacheManager, OutOfPages, PagedKVNeed
+from mini_sglang_b200.cache import CacheManager, PagedKVNeed
 from mini_sglang_b200.engine import DraftEntry
 from mini_sglang_b200.engine.step import ModelRunner
 
@@ -69,3 +69,30 @@ def test_the_path_kept_is_the_longest():
         assert got == longest(up, tokens, model)
         gained += len(got) > len(P.accepted(up, tokens, [model([tokens[a] for a in sorted(anc)]) for anc in P.ancestors(up)]))
     assert gained > 10                                   # trees where the first child alone would have lost tokens
+
+
+def test_a_tree_beyond_the_context_is_refused_before_anything_is_taken():
+    """The slot is named, and the entries ahead of it have taken no pages."""
+    runner = make_runner(lambda seq: 1, max_context_len=20)
+    a, b = runner.mgr.open(), runner.mgr.open()
+    runner.mgr.reserve(b, 15)
+    runner.mgr.commit(b, 15)
+    free = runner.mgr.available_pages()
+    with pytest.raises(ValueError, match=f"slot {b}: .*15.* 6 .*20"):
+        runner.verify([DraftEntry(a, [1] * 9), DraftEntry(b, [1] * 6)], None)
+    assert runner.mgr.available_pages() == free and runner.mgr.owned_pages(a) == [] and runner.calls == 0
+    assert runner.verify([DraftEntry(a, [1] * 9), DraftEntry(b, [1] * 5)], None) == [[1] * 9, [1] * 5]
+    assert int(runner.mgr.length[b]) == 20
+
+
+@pytest.mark.parametrize("slot", [0, -1, 2, 99])
+def test_slots_that_are_not_open_are_refused(slot):
+    runner = make_runner(lambda seq: 1)
+    a = runner.mgr.open()
+    while runner.mgr.free_slots:
+        runner.mgr.open()
+    runner.mgr.close(2)
+    free = runner.mgr.available_pages()
+    with pytest.raises(ValueError, match=f"slot {slot} is not open"):
+        runner.verify([DraftEntry(a, [1, 2]), DraftEntry(slot, [1, 2])], None)
+    assert runner.mgr.available_pages() == free and int(runner.mgr.reserved[a]) == 0
