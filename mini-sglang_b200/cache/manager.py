@@ -20,7 +20,7 @@ every block table and in every state array) from `open` to `close`.
     mgr.slot_mapping(g, slot, s, n)   token slots (page * P + offset) of positions s..s+n-1
     mgr.commit(slot, n)               the n tokens are in the cache; pages a window has passed
                                       are given back
-    mgr.unreserve(slot)               what was reserved beyond the committed tokens is reserved no more
+    mgr.unreserve(slot, held)         what was reserved beyond `held` tokens (default 0) and the committed ones is reserved no more
     mgr.close(slot)                   everything the request holds is given back
 
 Pages are given back when a request ends or a window or chunk has passed them, and are handed out again
@@ -246,9 +246,9 @@ class CacheManager:
                 g.first_live[slot] = dead
                 g.dirty.add(slot)
 
-    def unreserve(self, slot: int) -> None:
-        """Take back what was reserved and not committed: the pages stay the request's and are the next to be filled."""
-        self.reserved[slot] = self.length[slot]
+    def unreserve(self, slot: int, held: int = 0) -> None:
+        """Take back what was reserved beyond `held` tokens and not committed: the pages stay the request's and are the next to be filled."""
+        self.reserved[slot] = max(int(self.length[slot]), min(held, int(self.reserved[slot])))
 
     def owned_pages(self, slot: int, group: int = 0) -> List[int]:
         g = self.groups[group]

@@ -692,20 +692,20 @@ class ModelRunner:
             lens.append(n)
             parents.append(up)
             depths.append(depth)
-        short = [max(0, n - g.pool.available) for n, g in zip(map(sum, zip(*(self.mgr.pages_needed(e.slot, n) for e, n in zip(entries, lens)))), self.mgr.groups)]
+        held = [int(self.mgr.reserved[e.slot]) for e in entries]          # (the caller's reservations, which stay)
+        more = [max(0, int(self.mgr.length[e.slot]) + n - h) for e, n, h in zip(entries, lens, held)]
+        short = [max(0, n - g.pool.available) for n, g in zip(map(sum, zip(*(self.mgr.pages_needed(e.slot, n) for e, n in zip(entries, more)))), self.mgr.groups)]
         if any(short):
             raise OutOfPages(f"the step needs {short} more pages than are free (per group)")
-        reserved: List[int] = []
         try:
-            for e, n in zip(entries, lens):
+            for e, n in zip(entries, more):
                 self.mgr.reserve(e.slot, n)
-                reserved.append(e.slot)
             kept, tokens = self._verify(entries, lens, parents, depths, sampler, temperatures, row_keys, steps)
             for e, k in zip(entries, kept):
                 self.mgr.commit(e.slot, k)
         finally:
-            for slot in reserved:
-                self.mgr.unreserve(slot)
+            for e, h in zip(entries, held):
+                self.mgr.unreserve(e.slot, h)
         return [row[:k] for row, k in zip(tokens, kept)]
 
     def _verify(self, entries, lens, parents, depths, sampler, temperatures, row_keys, steps):

@@ -4,7 +4,7 @@ import random
 import plain_drafts as P
 import pytest
 
-from mini_sglang_b200.cache import CacheManager, PagedKVNeed
+from mini_sglang_b200.cache import CacheManager, OutOfPages, PagedKVNeed
 from mini_sglang_b200.engine import DraftEntry
 from mini_sglang_b200.engine.step import ModelRunner
 
@@ -96,3 +96,38 @@ def test_slots_that_are_not_open_are_refused(slot):
     with pytest.raises(ValueError, match=f"slot {slot} is not open"):
         runner.verify([DraftEntry(a, [1, 2]), DraftEntry(slot, [1, 2])], None)
     assert runner.mgr.available_pages() == free and int(runner.mgr.reserved[a]) == 0
+
+
+@pytest.mark.parametrize("fails", [False, True])
+def test_what_a_caller_has_reserved_stays_reserved(fails):
+    runner = make_runner(lambda seq: 1)
+    slot = runner.mgr.open()
+    runner.mgr.reserve(slot, 30)
+    runner.mgr.commit(slot, 10)
+
+    def broken(*_):
+        raise RuntimeError("a step that fails")
+
+    if fails:
+        runner._verify = broken
+        with pytest.raises(RuntimeError, match="fails"):
+            runner.verify([DraftEntry(slot, [1, 1, 1])], None)
+    else:
+        assert runner.verify([DraftEntry(slot, [1, 1, 1])], None) == [[1, 1, 1]]
+    assert int(runner.mgr.length[slot]) == (10 if fails else 13) and int(runner.mgr.reserved[slot]) == 30
+    with pytest.raises(OutOfPages):
+        runner.verify([DraftEntry(slot, [1] * 90), DraftEntry(runner.mgr.open(), [1] * 128), DraftEntry(runner.mgr.open(), [1] * 128)], None)
+    assert int(runner.mgr.reserved[slot]) == 30
+    runner._verify = make_runner(lambda seq: 1)._verify
+    assert len(runner.verify([DraftEntry(slot, [1] * 25)], None)[0]) == 25
+    assert int(runner.mgr.reserved[slot]) == max(30, int(runner.mgr.length[slot]))
+
+
+def test_drafts_lie_within_what_is_reserved_already():
+    """Places that a caller reserved for the next tokens are the ones that the drafts take: no further pages, and nothing beyond the context limit."""
+    runner = make_runner(lambda seq: 1, num_pages=5, max_context_len=20)
+    slot = runner.mgr.open()
+    runner.mgr.reserve(slot, 20)
+    runner.mgr.commit(slot, 8)
+    assert runner.verify([DraftEntry(slot, [1] * 12)], None) == [[1] * 12]
+    assert int(runner.mgr.length[slot]) == int(runner.mgr.reserved[slot]) == 20
