@@ -53,6 +53,9 @@ class StepEntry:
     want: Sequence[int] = ()          # places among `tokens` whose logits are wanted
 
 
+VERIFY_LOGITS_BYTES = 1 << 30         # of all drafts' logits, what `verify` makes at a time (256 requests of 64 drafts over 151,936 tokens would be 10 GB)
+
+
 @dataclasses.dataclass
 class DraftEntry:
     """A tree of drafted tokens of one request.  tokens[0] is its newest token, which is not in the cache yet; parents[i] is the index of
@@ -740,10 +743,14 @@ class ModelRunner:
                           host_kv_lens=[c + n for c, n in zip(cached, lens)], host_slots=[e.slot for e in entries], workspace=self.workspace,
                           drafts=DraftContext(plan.mask, most))
         ops.raise_if_failed()
-        logits = self.model.forward(ctx, self._caches(ctx), None)
+        h = self.model.forward(ctx, self._caches(ctx), None, with_head=False)
         expand = lambda given, default: [v for n, v in zip(lens, given if given is not None else [default] * B) for _ in range(n)]      # noqa: E731
         step0 = expand(steps, 0)
-        following = sampler.sample(logits, expand(temperatures, 0.0), expand(row_keys, 0), [s + d for s, d in zip(step0, (d for part in depths for d in part))])
+        fields = expand(temperatures, 0.0), expand(row_keys, 0), [s + d for s, d in zip(step0, (d for part in depths for d in part))]
+        portions = -(-T // max(1, VERIFY_LOGITS_BYTES // (4 * self.vocab_size)))
+        rows = -(-T // portions)
+        following = [sampler.sample(self.model.head.forward(h[a:a + rows]), *(f[a:a + rows] for f in fields)) for a in range(0, T, rows)]
+        following = following[0] if len(following) == 1 else torch.cat(following)
         got = ops.draft_accept(tokens, up, following, plan.q_start, max_draft=most, kv_len=plan.kv_len, block_table=table,
                                caches=[c for pair in self.storage.kv.values() for c in pair])
         ops.poll_status()

@@ -72,22 +72,23 @@ class DecoderModel:
         return needs
 
     # -- compute -----------------------------------------------------------------------
-    def forward(self, ctx: StepContext, caches: Dict[int, object], want_rows: Optional[torch.Tensor]) -> torch.Tensor:
-        """-> float32 logits [len(want_rows), vocab] (all T rows if want_rows is None)."""
-        if self.fused_decode is not None and self.fused_decode.takes(ctx):
+    def forward(self, ctx: StepContext, caches: Dict[int, object], want_rows: Optional[torch.Tensor], with_head: bool = True) -> torch.Tensor:
+        """-> float32 logits [len(want_rows), vocab] (all T rows if want_rows is None); without the head its input, which `head.forward` takes
+        in portions where the logits of all rows at once would be too many."""
+        if with_head and self.fused_decode is not None and self.fused_decode.takes(ctx):
             return self.fused_decode.forward(ctx, caches)       # the whole step in one persistent kernel
         ctx.shared.clear()          # what the parts of one pass hand to each other starts empty (a context may be run again)
         if NVTX_RANGES:
-            return self._forward_marked(ctx, caches, want_rows)
+            return self._forward_marked(ctx, caches, want_rows, with_head)
         residual = self.embedding.forward(ctx.input_ids, ctx)
         delta = None
         for run in self.schedule:
             cache = caches.get(run.cache) if run.cache is not None else None
             delta, residual = self.layers[run.layer].forward(delta, residual, ctx, cache, run.writes_cache)
         h = self.final_norm.forward(x=delta, residual=residual, rows=want_rows)
-        return self.head.forward(h)
+        return self.head.forward(h) if with_head else h
 
-    def _forward_marked(self, ctx, caches, want_rows):
+    def _forward_marked(self, ctx, caches, want_rows, with_head=True):
         """The same with an NVTX range around the embedding, every run of a layer and the head, for profilers
         that show them on the timeline."""
         nvtx = torch.cuda.nvtx
@@ -102,7 +103,7 @@ class DecoderModel:
             nvtx.range_pop()
         nvtx.range_push("final norm + head")
         h = self.final_norm.forward(x=delta, residual=residual, rows=want_rows)
-        out = self.head.forward(h)
+        out = self.head.forward(h) if with_head else h
         nvtx.range_pop()
         return out
 
