@@ -2452,6 +2452,8 @@ def _index(what: str, name: str, t: torch.Tensor, numel: Optional[int] = None) -
 def _table(what: str, t: torch.Tensor, B: int) -> None:
     if t.dtype != torch.int32 or t.dim() != 2 or t.shape[0] != B or t.shape[1] < 1 or t.stride(1) != 1:
         raise KernelError(f"{what}: block_table is int32 [requests, pages] with adjacent columns; got {t.dtype} {tuple(t.shape)}")
+    if t.stride(0) >> 31 and B > 1:          # (the kernels take it as 32 bits)
+        raise KernelError(f"{what}: the rows of block_table are less than 2^31 elements apart; got {t.stride(0)}")
 
 
 def _draft_limit(what: str, max_draft: int) -> None:
@@ -2515,6 +2517,7 @@ def tree_attention(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_
             and k_cache.dtype is dt and v_cache.dtype is dt and k_shape == v_cache.shape and k_shape[1:] == (n_kv, page_size, q.shape[2]) and k_cache.is_contiguous()
             and v_cache.is_contiguous() and n_kv >= 1 and q.shape[1] % n_kv == 0 and 1 <= q.shape[2] <= 512 and 0.0 < scale < math.inf
             and block_table.dtype is i32 and block_table.dim() == 2 and block_table.shape[1] >= 1 and block_table.stride(1) == 1
+            and (block_table.stride(0) >> 31 == 0 or block_table.shape[0] == 1)
             and q_start.dtype is i32 and q_start.numel() == block_table.shape[0] + 1 and q_start.is_contiguous()
             and kv_len.dtype is i32 and kv_len.numel() == block_table.shape[0] and kv_len.is_contiguous()
             and 1 <= max_draft <= MAX_DRAFTS and max_draft <= 32 * words and mask.dtype is i32 and mask.dim() == 2 and mask.shape[0] == q.shape[0] and mask.is_contiguous()

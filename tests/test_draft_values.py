@@ -28,3 +28,17 @@ def test_top_is_a_whole_number(top):
 def test_whole_numbers_of_numpy_are_taken_as_top():
     with pytest.raises(ops.KernelError, match="CUDA device"):          # (nothing but the device is wrong)
         ops.token_logprobs(torch.zeros(3, 50), torch.zeros(3, dtype=torch.int32), np.int64(3))
+
+
+def test_tables_whose_rows_lie_beyond_32_bits_are_refused():
+    """The kernels take the distance of a table's rows as 32 bits: a longer one would be cut and other rows read."""
+    I = lambda *s: torch.zeros(s, dtype=torch.int32)      # noqa: E731, E741
+    far = torch.empty_strided((2, 3), (2 ** 31, 1), dtype=torch.int32, device="meta")
+    with pytest.raises(ops.KernelError, match="block_table"):
+        ops.draft_plan(I(4), I(2), I(2), far, page_size=16, max_draft=4)
+    cache = torch.zeros(5, 2, 16, 16)
+    with pytest.raises(ops.KernelError, match="block_table"):
+        ops.draft_accept(I(4), I(4), I(4), I(3), max_draft=4, kv_len=I(2), block_table=far, caches=[cache])
+    q = torch.zeros(4, 8, 16)
+    with pytest.raises(ops.KernelError, match="block_table"):
+        ops.tree_attention(q, q, cache, cache, q_start=I(3), kv_len=I(2), block_table=far, mask=I(4, 1), n_kv=2, page_size=16, scale=1.0, max_draft=4)
