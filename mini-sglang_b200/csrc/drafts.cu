@@ -189,7 +189,7 @@ MSGL_API int msgl_draft_accept(const int* tokens, const int* parents, const int*
     const int unit = bits % 16 == 0 ? 16 : bits % 4 == 0 ? 4 : 2;
     if (bits % 2) return MSGL_ERR_ALIGN;
     const int units = row_bytes / unit;
-    if ((long long)n_caches * n_kv * units > 0x7fffffffLL) return MSGL_ERR_SIZE;
+    if ((long long)n_caches * n_kv * units + (long long)blocks_y * DR_COPY_THREADS > 0x7fffffffLL) return MSGL_ERR_SIZE;      // (a thread's counter steps once past the last column)
 #define MSGL_ACCEPT(U)                                                                                                                                          \
     msgl_launch_pdl(draft_accept_kernel<U>, dim3(B, blocks_y), dim3(DR_COPY_THREADS), 0, stream, tokens, parents, following, q_start, T, max_draft, kept, path,   \
                     token, kv_len, table, table_stride, table_width, page_size, pages, n_kv, units, n_caches, c)

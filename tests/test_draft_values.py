@@ -42,3 +42,17 @@ def test_tables_whose_rows_lie_beyond_32_bits_are_refused():
     q = torch.zeros(4, 8, 16)
     with pytest.raises(ops.KernelError, match="block_table"):
         ops.tree_attention(q, q, cache, cache, q_start=I(3), kv_len=I(2), block_table=far, mask=I(4, 1), n_kv=2, page_size=16, scale=1.0, max_draft=4)
+
+
+def test_accept_takes_no_more_columns_than_its_counter_has_room_for():
+    """A block's threads step over the columns of all caches with a 32-bit counter: sizes where it would pass its end are refused before a launch."""
+    import ctypes
+    lib = ops._draft_lib()
+    there = torch.zeros(64, dtype=torch.uint8)
+
+    def call(n_caches, row_bytes):
+        addresses = (ctypes.c_void_p * n_caches)(*[there.data_ptr() // 16 * 16 + 2] * n_caches)          # (2 bytes a column)
+        return lib.msgl_draft_accept(None, None, None, None, 0 if n_caches == 1 else 1, 0, 4, None, None, None, there.data_ptr(), there.data_ptr(), 1, 1, 16, 1, 1, row_bytes,
+                                     addresses, n_caches, 1, None)
+    assert call(1, 64) == 0                              # (no request: nothing to do)
+    assert call(2, 2 ** 31 - 256) == 2                   # (2^31 - 256 columns, and a block steps by 256)
