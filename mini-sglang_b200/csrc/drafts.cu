@@ -66,7 +66,9 @@ __global__ void __launch_bounds__(DR_MAX) draft_plan_kernel(const int* __restric
         }
         positions[t] = base + depth;
         token_req[t] = r;
-        out_loc[t] = page < table_width ? table[(size_t)r * table_stride + page] * page_size + (place - page * page_size) : 0;
+        const int id = page < table_width ? table[(size_t)r * table_stride + page] : -1;
+        const long long slot = (long long)id * page_size + (place - page * page_size);
+        out_loc[t] = id >= 0 && slot <= 0x7fffffffLL ? (int)slot : 0;          // (a negative slot would be written to in front of the caches)
     }
     if (r == B - 1) {                                // rows behind the last draft: position 0 on the page for padding, nothing seen
         for (int t = start + n + tid; t < T; t += n_threads) {

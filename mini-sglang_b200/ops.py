@@ -2477,7 +2477,8 @@ def draft_plan(parents: torch.Tensor, draft_lens: torch.Tensor, cached: torch.Te
     request after request in `parents` [T], behind cached[r] tokens whose pages stand in block_table [B, pages].  A draft's parent is the
     index within the request of an earlier draft; anything else stands for none.  Draft i lies in the cache at place cached + i.
     Lengths are taken within [0, max_draft] and drafts past the end of `parents` are cut; rows of `parents` behind the last draft become
-    padding: position 0 and slot 0 (the page for padding) with an empty mask.  A place beyond the block table gets slot 0 too."""
+    padding: position 0 and slot 0 (the page for padding) with an empty mask.  A place beyond the block table gets slot 0 too, and
+    so does one whose page number is negative or gives a slot beyond 32 bits."""
     T, B, width = parents.numel(), draft_lens.numel(), block_table.shape[-1] if block_table.dim() else 0
     _index("draft_plan", "parents", parents)
     _index("draft_plan", "draft_lens", draft_lens)
