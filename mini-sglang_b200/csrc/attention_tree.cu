@@ -461,7 +461,10 @@ __global__ void __launch_bounds__(TF_THREADS, 2) tree_tile_kernel(const TreePara
 // float32, head size 128, this one / that one, us: groups of four, 1 request of 32 drafts behind 500 keys 26 / 49, 8 of 20 behind 100 40 / 41, 16 of 30 behind 300
 // 151 / 131, 2 of 12 behind 6,000 152 / 117, 4 of 26 behind 1,500 158 / 123; of two, 4 of 26 behind 1,500 86 / 72, 1 of 64 behind 2,000 66 / 56, 8 of 40 behind 500 (80 rows,
 // of 96 and of 128) 95 / 104; of five, 2 of 64 behind 4,000 475 / 344.  So it stands where there are no more than 32 rows, fewer than three tiles of the other an
-// SM, or where these are more than a third of its own tiles (as far as the host knows: the table's width).
+// SM, or where these are more than a third of its own tiles (as far as the host knows: the table's width; a table of some thousand keys a request whose
+// requests are short goes to that one all the same: 4 of 26 behind 200 26 / 49, groups of four, 2 of 12 behind 600 31 / 47, 8 of 20 behind 100 40 / 40, 16 of 30 behind 100, groups of two, 49 / 56).
+// bfloat16 heads other than the tensor cores' (4 requests behind 4,000 keys, 16 heads on 4; us, 8 / 32 drafts): heads of 96 52 / 116, of 192 88 / 289, of 256 106 / 349 (keys and values alone
+// 4, 8 and 10); rows of 320 that are key and value of 16 heads at once, 1 request 56 / 143, 16 requests 538 / 2,071 (6): multiply-adds at 0.2 to 0.37 of their rate, and keys read again for every 32 rows.
 // ---------------------------------------------------------------------------------------
 constexpr int TS_ROWS = 32, TS_KT = 32, TS_THREADS = 256;
 

@@ -4,7 +4,7 @@
 // against tiles of 128 keys.
 //
 //     S = Q K^T     tcgen05.mma 128 x 128 x 16, operands in shared memory, accumulator in tensor memory
-//     softmax       two threads a row (TMEM lane), 64 scores each in registers; P, rounded to bfloat16 (half a step, 2^-9, of each weight;
+//     softmax       two threads a row (TMEM lane), 64 scores each in registers; P, rounded to bfloat16 (by up to half a step, 2^-8 of each weight;
 //                   the sum of the weights is taken before), goes back over the columns that each thread's scores had
 //     O += P V      tcgen05.mma 128 x D x 16, P from tensor memory, V from shared memory as it lies in the cache
 //
