@@ -2623,7 +2623,7 @@ class DraftPath(NamedTuple):
 def draft_accept(tokens: torch.Tensor, parents: torch.Tensor, following: torch.Tensor, q_start: torch.Tensor, *, max_draft: int,
                  kv_len: Optional[torch.Tensor] = None, block_table: Optional[torch.Tensor] = None, caches: Sequence[torch.Tensor] = ()) -> DraftPath:
     """The path of drafts that the model agrees with, for every request (all int32): from draft 0, the newest accepted token, to its child
-    whose token is following[its parent] (the first of them), and so on.  tokens, parents and following [T] as in `draft_plan`; `following`
+    whose token is following[its parent] (the first of them: what follows a later sibling of the same token is not looked at), and so on.  tokens, parents and following [T] as in `draft_plan`; `following`
     is the model's token after every draft, of `sample` say.  The keys and values of the path move to the places behind the cached
     tokens in all `caches` ([pages, kv heads, page size, row size] of one page size, each handed over once), so that the request
     holds kv_len - (its drafts) + kept tokens afterwards; no two requests may share the pages that their drafts lie in."""
