@@ -140,6 +140,7 @@ GATED_MIXER_SOURCES = ["mixers_gated.cu"]
 DELTA_MIXER_SOURCES = ["mixers_delta.cu"]
 STREAM_MIXER_SOURCES = ["mixers_streams.cu"]
 DRAFT_SOURCES = ["drafts.cu", "logprobs.cu", "attention_tree.cu"]
+KV4_SOURCES = ["kv4.cu"]
 MMA_HEAD_DIMS = tuple(range(16, 257, 16))   # head sizes the tensor-core attention kernel is built for
 
 
@@ -181,6 +182,11 @@ def drafts_library() -> ctypes.CDLL:
     return load_library("drafts", DRAFT_SOURCES)
 
 
+def kv4_library() -> ctypes.CDLL:
+    """The kernels of a key/value cache in 4 bits (csrc/kv4.cu); built at their first use."""
+    return load_library("kv4", KV4_SOURCES)
+
+
 def attention_library(head_dim: int) -> ctypes.CDLL:
     """Attention kernels with the tensor-core variant instantiated for `head_dim` when it is one
     of MMA_HEAD_DIMS; other head sizes get the library of head size 128, whose float32-arithmetic
@@ -212,7 +218,8 @@ def build_all(head_dims: Sequence[int] = (16, 32, 48, 64, 128)) -> List[str]:
     """Compile every library ahead of time (used by the repository's build check)."""
     paths = [compile_library("common", COMMON_SOURCES), compile_library("mixers", MIXER_SOURCES),
              compile_library("mixers_gated", GATED_MIXER_SOURCES), compile_library("mixers_delta", DELTA_MIXER_SOURCES),
-             compile_library("mixers_streams", STREAM_MIXER_SOURCES), compile_library("drafts", DRAFT_SOURCES)]
+             compile_library("mixers_streams", STREAM_MIXER_SOURCES), compile_library("drafts", DRAFT_SOURCES),
+             compile_library("kv4", KV4_SOURCES)]
     for hd in head_dims:
         paths.append(compile_library(f"attention_d{hd}", ATTENTION_SOURCES, {"MSGL_HEAD_DIM": hd}))
     paths.append(compile_library("attention_noalloc_d128", ["attention_noalloc.cu"], {"MSGL_HEAD_DIM": 128}))

@@ -1,0 +1,628 @@
+// A paged key/value cache held in 4 bits: appending to it, reading pages back, attention over it.
+//
+// A row is one token's key or value under one kv head: d codes c in 0..15, two to a byte (the even element in the low half), and two
+// bfloat16 numbers, a step and a base; an element stands for base + c * step, summed in float32 (the product of a 4-bit and an 8-bit
+// number is exact).  Arrays: k, v [pages][kv heads][page][d / 2] bytes, steps [pages][kv heads][page][4] = k step, k base, v step, v base.
+// 68 bytes a row of 128 where bfloat16 takes 256.
+//
+// A row x becomes: base = bf16(min x), step = bf16((max x - base) / 15), c = rint((x - base) / step) within 0..15.  Codes are made against
+// the step and base as they are kept, so their rounding costs no more than the code's own half step.  The base is the least element (not a
+// midpoint), since that is exact for bfloat16 rows.  A row without width (step below 2^-100) has step 0; one with an infinite element or a NaN, or
+// wider than bfloat16 reaches, stands for NaN throughout, so that it shows in every result that it enters.
+//
+//   kv4_append_vec_kernel / kv4_append_kernel   norm, rotation, codes, q            (bound by bytes)
+//   kv4_restore_kernel                          rows back to bfloat16 or float32    (bound by bytes)
+//   kv4_attn_any_kernel                         attention, any head size and type   (float32 arithmetic)
+//   kv4_attn_runs_kernel (kv4_runs.cuh)         attention on mma, bfloat16, head sizes 64 and 128
+#include "common.cuh"
+#include <float.h>
+#include <math_constants.h>
+
+constexpr int KV4_MAX_D = 512;
+
+__device__ __forceinline__ float bf16_of(unsigned short b) { return __uint_as_float((unsigned)b << 16); }
+
+// min and max that keep a NaN
+__device__ __forceinline__ float min_nan(float a, float b) { float r; asm("min.NaN.f32 %0, %1, %2;\n" : "=f"(r) : "f"(a), "f"(b)); return r; }
+__device__ __forceinline__ float max_nan(float a, float b) { float r; asm("max.NaN.f32 %0, %1, %2;\n" : "=f"(r) : "f"(a), "f"(b)); return r; }
+
+struct Kv4Scale {
+    float base, step;
+    unsigned bits;                  // step in the low half, base in the high one, as they are kept
+    __device__ __forceinline__ Kv4Scale(float lo, float hi) {
+        __nv_bfloat16 b = __float2bfloat16_rn(lo), s = __float2bfloat16_rn(__fmul_rn(__fsub_rn(hi, __bfloat162float(b)), 1.f / 15.f));
+        base = __bfloat162float(b);
+        step = __bfloat162float(s);
+        if (!(fabsf(base) <= FLT_MAX) || !(fabsf(step) <= FLT_MAX)) { base = CUDART_NAN_F; step = 0.f; }
+        else if (!(step >= 0x1p-100f)) step = 0.f;
+        bits = (unsigned)__bfloat16_as_ushort(__float2bfloat16_rn(step)) | ((unsigned)__bfloat16_as_ushort(__float2bfloat16_rn(base)) << 16);
+    }
+    // the division is correctly rounded: an element half way between two codes takes the even one whoever computes it
+    __device__ __forceinline__ unsigned code(float x) const {
+        if (!(step > 0.f)) return 0u;
+        return (unsigned)fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x, base), step)), 0.f), 15.f);
+    }
+};
+
+// x * inv * w and the rotation in separately rounded operations, so that the codes are those of the written formula whichever kernel makes them
+__device__ __forceinline__ float rot_sub(float a, float c, float b, float s) { return __fsub_rn(__fmul_rn(a, c), __fmul_rn(b, s)); }
+__device__ __forceinline__ float rot_add(float a, float s, float b, float c) { return __fadd_rn(__fmul_rn(a, s), __fmul_rn(b, c)); }
+// The squares are summed in 64 bits: a code next to a border must not hang on the order of a sum (the same token gives the same row in a step of any make-up).
+__device__ __forceinline__ float inv_rms(double ss, int d, float eps) { return __fdiv_rn(1.f, __fsqrt_rn(__fadd_rn((float)(ss / (double)d), eps))); }
+template <typename T> __device__ __forceinline__ double square(float x) { return sizeof(T) == 2 ? (double)(x * x) : (double)x * (double)x; }      // (a bfloat16's square is exact in float32)
+
+struct Kv4Append {
+    const void* qkv; long long stride;                    // [T] rows of (n_q + 2 n_kv) d elements
+    const int* positions; const int* out_loc;
+    const void* qw; const void* kw; int w_f32; float eps;
+    const float* table; int rot, max_pos, interleaved;
+    void* q_out;
+    unsigned char* k; unsigned char* v; unsigned* steps;  // steps: two words a row, keys' and values'
+    long long slots;                                      // of the cache: page numbers beyond are left out
+    int page_size, n_q, n_kv, d, T;
+    __device__ __forceinline__ long long row_of(int t, int kvh) const {      // -1: nowhere
+        const int slot = out_loc[t];
+        if (slot < 0 || slot >= slots) return -1;
+        const int page = slot / page_size;
+        return ((long long)page * n_kv + kvh) * page_size + (slot - page * page_size);
+    }
+};
+
+// Any head size in steps of 8, partial and pairwise rotations: a warp a head of a token.
+template <typename T>
+__global__ void kv4_append_kernel(const Kv4Append p) {
+    extern __shared__ float kv4_sh[];
+    const int lane = threadIdx.x & 31, n_heads = p.n_q + 2 * p.n_kv, d = p.d;
+    const long long unit = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+    float* hv = kv4_sh + (size_t)(threadIdx.x >> 5) * d;
+    pdl_wait();
+    pdl_small();
+    if (unit >= (long long)p.T * n_heads) return;
+    const int t = (int)(unit / n_heads), head = (int)(unit - (long long)t * n_heads);
+    const bool is_q = head < p.n_q, is_k = !is_q && head < p.n_q + p.n_kv;
+    const T* src = reinterpret_cast<const T*>(p.qkv) + (size_t)t * p.stride + (size_t)head * d;
+    const void* nw = is_q ? p.qw : (is_k ? p.kw : nullptr);
+    double ss = 0.0;
+    for (int i = lane; i < d; i += 32) {
+        const float x = to_f32<T>(src[i]);
+        hv[i] = x;
+        ss += square<T>(x);
+    }
+    if (nw != nullptr) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        const float inv = inv_rms(ss, d, p.eps);
+        for (int i = lane; i < d; i += 32) hv[i] = __fmul_rn(__fmul_rn(hv[i], inv), load_weight(nw, i, p.w_f32));
+    }
+    __syncwarp();
+    const int rot = (is_q || is_k) && p.table != nullptr ? p.rot : 0, half = rot >> 1;
+    int pos = rot ? p.positions[t] : 0;
+    pos = pos < 0 ? 0 : (pos >= p.max_pos ? p.max_pos - 1 : pos);
+    const float* cs = p.table + (size_t)pos * rot;
+    auto turned = [&](int i) -> float {
+        if (i >= rot) return hv[i];
+        if (p.interleaved) {
+            const int a = i >> 1;
+            return (i & 1) ? rot_add(hv[i - 1], cs[half + a], hv[i], cs[a]) : rot_sub(hv[i], cs[a], hv[i + 1], cs[half + a]);
+        }
+        return i < half ? rot_sub(hv[i], cs[i], hv[i + half], cs[half + i]) : rot_add(hv[i - half], cs[i], hv[i], cs[i - half]);
+    };
+    if (is_q) {
+        T* dst = reinterpret_cast<T*>(p.q_out) + ((size_t)t * p.n_q + head) * d;
+        for (int i = lane; i < d; i += 32) dst[i] = from_f32<T>(turned(i));
+        return;
+    }
+    // eight neighbouring elements a lane: a word of codes
+    float x[KV4_MAX_D / 256][8], lo = CUDART_INF_F, hi = -CUDART_INF_F;
+#pragma unroll
+    for (int j = 0; j < KV4_MAX_D / 256; ++j) {
+        const int w = lane + 32 * j;
+        if (8 * w >= d) continue;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            x[j][e] = turned(8 * w + e);
+            lo = min_nan(lo, x[j][e]);
+            hi = max_nan(hi, x[j][e]);
+        }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+        hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    }
+    const Kv4Scale sc(lo, hi);
+    const long long row = p.row_of(t, is_k ? head - p.n_q : head - p.n_q - p.n_kv);
+    if (row < 0) return;
+    unsigned* dst = reinterpret_cast<unsigned*>((is_k ? p.k : p.v) + row * (d >> 1));
+#pragma unroll
+    for (int j = 0; j < KV4_MAX_D / 256; ++j) {
+        const int w = lane + 32 * j;
+        if (8 * w >= d) continue;
+        unsigned word = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) word |= sc.code(x[j][e]) << (4 * e);
+        dst[w] = word;
+    }
+    if (lane == 0) p.steps[2 * row + (is_k ? 0 : 1)] = sc.bits;
+}
+
+// Head sizes 32, 64, 128, 256 whose rotation (if any) covers the whole head in halves: L = d / 16 lanes own one head of a token, a lane eight
+// elements of the lower half and the eight that they are rotated with, so that every copy is 16 bytes, every word of codes one lane's, and only the sum
+// and the extremes take shuffles.
+constexpr int KV4_APPEND_THREADS = 256;
+template <typename T, int L>
+__global__ void __launch_bounds__(KV4_APPEND_THREADS) kv4_append_vec_kernel(const Kv4Append p) {
+    constexpr int d = 16 * L, half = 8 * L, V = 16 / sizeof(T), N = 8 / V;          // elements of a 16-byte piece, pieces of eight elements
+    const int l = threadIdx.x & (L - 1), n_heads = p.n_q + 2 * p.n_kv;
+    const long long unit = (long long)blockIdx.x * (KV4_APPEND_THREADS / L) + threadIdx.x / L;
+    const bool active = unit < (long long)p.T * n_heads;
+    const int t = active ? (int)(unit / n_heads) : 0, head = active ? (int)(unit - (long long)t * n_heads) : 0;
+    const bool is_q = head < p.n_q, is_k = !is_q && head < p.n_q + p.n_kv, turns = (is_q || is_k) && p.table != nullptr;
+    const void* nw = is_q ? p.qw : (is_k ? p.kw : nullptr);
+    pdl_wait();
+    pdl_small();
+    float x[16];
+    const T* src = reinterpret_cast<const T*>(p.qkv) + (size_t)t * p.stride + (size_t)head * d + 8 * l;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const uint4 raw = *reinterpret_cast<const uint4*>(src + h * half + i * V);
+            const T* e = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+            for (int j = 0; j < V; ++j) x[8 * h + i * V + j] = to_f32<T>(e[j]);
+        }
+    if (nw != nullptr) {
+        double ss = 0.0;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) ss += square<T>(x[j]);
+        const unsigned group = (unsigned)(((1ull << L) - 1) << (threadIdx.x & 31 & ~(L - 1)));
+#pragma unroll
+        for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(group, ss, o);
+        const float inv = inv_rms(ss, d, p.eps);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) x[j] = __fmul_rn(__fmul_rn(x[j], inv), load_weight(nw, (j < 8 ? 0 : half - 8) + 8 * l + j, p.w_f32));
+    }
+    if (turns) {
+        int pos = p.positions[t];
+        pos = pos < 0 ? 0 : (pos >= p.max_pos ? p.max_pos - 1 : pos);
+        const float4* cs = reinterpret_cast<const float4*>(p.table + (size_t)pos * d + 8 * l);
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            const float4 c4 = cs[q], s4 = cs[half / 4 + q];
+            const float c[4] = {c4.x, c4.y, c4.z, c4.w}, s[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int j = 4 * q + e;
+                const float a = x[j], b = x[8 + j];
+                x[j] = rot_sub(a, c[e], b, s[e]);
+                x[8 + j] = rot_add(a, s[e], b, c[e]);
+            }
+        }
+    }
+    if (is_q) {
+        if (!active) return;
+        T* dst = reinterpret_cast<T*>(p.q_out) + ((size_t)t * p.n_q + head) * d + 8 * l;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                uint4 raw;
+                T* e = reinterpret_cast<T*>(&raw);
+#pragma unroll
+                for (int j = 0; j < V; ++j) e[j] = from_f32<T>(x[8 * h + i * V + j]);
+                *reinterpret_cast<uint4*>(dst + h * half + i * V) = raw;
+            }
+        return;
+    }
+    float lo = x[0], hi = x[0];
+#pragma unroll
+    for (int j = 1; j < 16; ++j) { lo = min_nan(lo, x[j]); hi = max_nan(hi, x[j]); }
+    const unsigned group = (unsigned)(((1ull << L) - 1) << (threadIdx.x & 31 & ~(L - 1)));
+#pragma unroll
+    for (int o = L / 2; o > 0; o >>= 1) {
+        lo = min_nan(lo, __shfl_xor_sync(group, lo, o));
+        hi = max_nan(hi, __shfl_xor_sync(group, hi, o));
+    }
+    const Kv4Scale sc(lo, hi);
+    const long long row = active ? p.row_of(t, is_k ? head - p.n_q : head - p.n_q - p.n_kv) : -1;
+    if (row < 0) return;
+    unsigned* dst = reinterpret_cast<unsigned*>((is_k ? p.k : p.v) + row * (d / 2)) + l;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        unsigned word = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) word |= sc.code(x[8 * h + e]) << (4 * e);
+        dst[h * L] = word;
+    }
+    if (l == 0) p.steps[2 * row + (is_k ? 0 : 1)] = sc.bits;
+}
+
+MSGL_API int msgl_kv4_append(const void* qkv, long long stride, const int* positions, const int* out_loc, const void* qw, const void* kw, int w_f32, float eps,
+                             const float* table, int rot, int max_pos, int interleaved, void* q_out, void* k, void* v, void* steps, long long slots, int page_size,
+                             int n_q, int n_kv, int d, int T, int dtype, cudaStream_t stream) {
+    if (T <= 0) return MSGL_OK;
+    if (d < 8 || d > KV4_MAX_D || d % 8 || n_q < 0 || n_kv < 1 || page_size < 1 || rot > d || (rot & 1)) return MSGL_ERR_SIZE;
+    if (dtype != MSGL_F32 && dtype != MSGL_BF16) return MSGL_ERR_DTYPE;
+    if (((uintptr_t)k | (uintptr_t)v | (uintptr_t)steps) & 15) return MSGL_ERR_ALIGN;
+    Kv4Append p = {qkv, stride, positions, out_loc, qw, kw, w_f32, eps, table, rot, max_pos, interleaved, q_out, (unsigned char*)k, (unsigned char*)v, (unsigned*)steps,
+                   slots, page_size, n_q, n_kv, d, T};
+    const long long units = (long long)T * (n_q + 2 * n_kv);
+    const int item = dtype == MSGL_F32 ? 4 : 2;
+    const bool whole = table == nullptr || (rot == d && !interleaved && ((uintptr_t)table & 15) == 0);
+    if (whole && (d == 32 || d == 64 || d == 128 || d == 256) && ((uintptr_t)qkv & 15) == 0 && ((uintptr_t)q_out & 15) == 0 && (stride * item) % 16 == 0) {
+        const int L = d / 16;
+        const long long blocks = (units + KV4_APPEND_THREADS / L - 1) / (KV4_APPEND_THREADS / L);
+        if (blocks > 0x7fffffffLL) return MSGL_ERR_SIZE;
+#define KV4_VEC(TT, LL) msgl_launch_pdl(kv4_append_vec_kernel<TT, LL>, dim3((unsigned)blocks), dim3(KV4_APPEND_THREADS), 0, stream, p)
+#define KV4_VEC_L(TT) do { if (L == 2) KV4_VEC(TT, 2); else if (L == 4) KV4_VEC(TT, 4); else if (L == 8) KV4_VEC(TT, 8); else KV4_VEC(TT, 16); } while (0)
+        if (dtype == MSGL_F32) KV4_VEC_L(float); else KV4_VEC_L(__nv_bfloat16);
+#undef KV4_VEC_L
+#undef KV4_VEC
+        return msgl_check_launch();
+    }
+    constexpr int WARPS = 4;
+    const long long blocks = (units + WARPS - 1) / WARPS;
+    if (blocks > 0x7fffffffLL) return MSGL_ERR_SIZE;
+    const size_t smem = (size_t)WARPS * d * 4;
+    if (dtype == MSGL_F32) msgl_launch_pdl(kv4_append_kernel<float>, dim3((unsigned)blocks), dim3(WARPS * 32), smem, stream, p);
+    else msgl_launch_pdl(kv4_append_kernel<__nv_bfloat16>, dim3((unsigned)blocks), dim3(WARPS * 32), smem, stream, p);
+    return msgl_check_launch();
+}
+
+// ---------------------------------------------------------------------------------------------------------------------------------------------
+// Rows back to bfloat16 or float32.
+//
+// Two uses.  By pages: pages[i] of the cache becomes page i of the results, [n][kv heads][page][d].  By requests: the keys that the requests with
+// at least min_q tokens see are packed into pages of KV4_RESTORED keys, request after request, and `table` names those pages as a block table does
+// (the tensor-core prefill kernel then fetches whole tiles of keys; a key's place in its page is that of its position).  Keys behind a request's
+// last one are zeros.  bfloat16 results are rounded once, as a bfloat16 cache would hold them.
+constexpr int KV4_RESTORED = 128;
+
+struct Kv4Restore {
+    const unsigned char* k; const unsigned char* v; const uint2* steps;
+    void* k_out; void* v_out;
+    const int* pages_in;             // by pages: [n]
+    const int* q_start; const int* kv_len; const int* block_table; int* table;      // by requests: [B + 1], [B], [B, bt_width], [B, t_width]
+    long long bt_stride;
+    int B, bt_width, t_width, window, min_q, n_kv, page_size, pages, d, n;        // n: pages of results
+};
+
+// what a request needs restored: its pages of KV4_RESTORED keys from the first one that its first token sees on
+__device__ __forceinline__ void kv4_span(const Kv4Restore& p, int r, int& first, int& n) {
+    const int tokens = p.q_start[r + 1] - p.q_start[r], kv = min(p.kv_len[r], p.bt_width * p.page_size);
+    first = n = 0;
+    if (tokens < p.min_q || kv <= 0) return;
+    first = (p.window > 0 ? max(p.kv_len[r] - tokens - p.window + 1, 0) : 0) / KV4_RESTORED;
+    n = max(min((kv + KV4_RESTORED - 1) / KV4_RESTORED, p.t_width) - first, 0);
+}
+
+template <bool WIDE>
+__device__ __forceinline__ void kv4_put(void* out, long long at, unsigned word, float step, float base) {
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = fmaf((float)((word >> (4 * e)) & 15u), step, base);
+    if (WIDE) {
+        float4* o = reinterpret_cast<float4*>(reinterpret_cast<float*>(out) + at);
+        o[0] = make_float4(x[0], x[1], x[2], x[3]);
+        o[1] = make_float4(x[4], x[5], x[6], x[7]);
+    } else {
+        uint4 o;
+        __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&o);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) h[e] = __floats2bfloat162_rn(x[2 * e], x[2 * e + 1]);
+        *reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(out) + at) = o;
+    }
+}
+
+// a block: a page of results under one kv head; by requests one more along x, which writes the table
+template <bool WIDE>
+__global__ void __launch_bounds__(256) kv4_restore_kernel(const Kv4Restore p) {
+    __shared__ int sh[2];
+    const int kvh = blockIdx.y, words = p.d >> 3;
+    pdl_wait();
+    pdl_small();
+    if ((int)blockIdx.x == p.n) {
+        if (kvh > 0) return;
+        int before = 0;
+        for (int r = 0; r < p.B; ++r) {                   // whatever the lengths say, every entry names a page of the results
+            int first, n;
+            kv4_span(p, r, first, n);
+            for (int i = threadIdx.x; i < p.t_width; i += 256) p.table[(long long)r * p.t_width + i] = min(max(before + i - first, 0), p.n - 1);
+            before += n;
+        }
+        return;
+    }
+    const int* pages = p.pages_in;
+    int from = 0, rows = p.page_size, per = p.page_size, width = 0x7fffffff;      // by pages: one page, all of its rows
+    long long to = (long long)blockIdx.x;
+    if (pages != nullptr) {
+        pages += blockIdx.x;
+    } else {
+        // the request that result page blockIdx.x is of: a warp looks through the requests, 32 at a time
+        if (threadIdx.x < 32) {
+            int before = 0, r = -1, page = 0;
+            for (int r0 = 0; r0 < p.B; r0 += 32) {
+                int first = 0, n = 0;
+                if (r0 + (int)threadIdx.x < p.B) kv4_span(p, r0 + threadIdx.x, first, n);
+                int sum = n;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int u = __shfl_up_sync(0xffffffffu, sum, o);
+                    if ((int)threadIdx.x >= o) sum += u;
+                }
+                const int at = (int)blockIdx.x - before - (sum - n);
+                const unsigned hit = __ballot_sync(0xffffffffu, at >= 0 && at < n);
+                if (hit) {
+                    const int src = __ffs(hit) - 1;
+                    page = __shfl_sync(0xffffffffu, first + at, src);
+                    r = r0 + src;
+                    break;
+                }
+                before += __shfl_sync(0xffffffffu, sum, 31);
+            }
+            if (threadIdx.x == 0) { sh[0] = r; sh[1] = page; }
+        }
+        __syncthreads();
+        const int r = sh[0];
+        if (r < 0) return;
+        pages = p.block_table + r * p.bt_stride;
+        width = p.bt_width;
+        from = sh[1] * KV4_RESTORED;
+        rows = min(p.kv_len[r] - from, KV4_RESTORED);
+        per = KV4_RESTORED;
+    }
+    to = (to * p.n_kv + kvh) * per * p.d;
+    for (int i = threadIdx.x; i < per * words; i += 256) {
+        const int row = i / words, w = i - row * words, key = from + row, at = key / p.page_size;
+        const int page = row < rows && at < width ? pages[at] : -1;
+        unsigned kw = 0, vw = 0;
+        uint2 st = make_uint2(0u, 0u);
+        if (page >= 0 && page < p.pages) {
+            const long long src = ((long long)page * p.n_kv + kvh) * p.page_size + (key - at * p.page_size);
+            kw = reinterpret_cast<const unsigned*>(p.k)[src * words + w];
+            vw = reinterpret_cast<const unsigned*>(p.v)[src * words + w];
+            st = p.steps[src];
+        }
+        kv4_put<WIDE>(p.k_out, to + 8ll * i, kw, bf16_of(st.x & 0xffffu), bf16_of(st.x >> 16));
+        kv4_put<WIDE>(p.v_out, to + 8ll * i, vw, bf16_of(st.y & 0xffffu), bf16_of(st.y >> 16));
+    }
+}
+
+MSGL_API int msgl_kv4_restored_page(void) { return KV4_RESTORED; }
+
+// n: pages of results.  pages_in null: by requests.
+MSGL_API int msgl_kv4_restore(const void* k, const void* v, const void* steps, void* k_out, void* v_out, const int* pages_in, int n, const int* q_start, const int* kv_len,
+                              const int* block_table, long long bt_stride, int bt_width, int* table, int t_width, int B, int window, int min_q, int n_kv, int page_size,
+                              int pages, int d, int dtype, cudaStream_t stream) {
+    if (n <= 0) return MSGL_OK;
+    if (d < 8 || d > KV4_MAX_D || d % 8 || n_kv < 1 || n_kv > 65535 || page_size < 1 || pages < 1) return MSGL_ERR_SIZE;
+    if (dtype != MSGL_F32 && dtype != MSGL_BF16) return MSGL_ERR_DTYPE;
+    if (((uintptr_t)k | (uintptr_t)v | (uintptr_t)steps | (uintptr_t)k_out | (uintptr_t)v_out) & 15) return MSGL_ERR_ALIGN;
+    if (pages_in == nullptr && (q_start == nullptr || kv_len == nullptr || block_table == nullptr || table == nullptr || B < 1 || t_width < 1)) return MSGL_ERR_SIZE;
+    Kv4Restore p = {(const unsigned char*)k, (const unsigned char*)v, (const uint2*)steps, k_out, v_out, pages_in, q_start, kv_len, block_table, table, bt_stride, B, bt_width,
+                    t_width, window, min_q, n_kv, page_size, pages, d, n};
+    const int blocks = pages_in == nullptr ? n + 1 : n;
+    if (dtype == MSGL_F32) msgl_launch_pdl(kv4_restore_kernel<true>, dim3(blocks, n_kv), dim3(256), 0, stream, p);
+    else msgl_launch_pdl(kv4_restore_kernel<false>, dim3(blocks, n_kv), dim3(256), 0, stream, p);
+    return msgl_check_launch();
+}
+
+// ---------------------------------------------------------------------------------------------------------------------------------------------
+// Attention of requests with few tokens, any head size in steps of 8 and either type, float32 arithmetic throughout.
+//
+// A block: up to 8 rows (token, query head) of one kv head and one of `splits` equal parts of the request's keys; four warps take units of 32 keys in
+// turn.  A lane owns a key for the scores (its row's words one after the other, the queries broadcast from shared memory) and words of eight
+// elements for the values (where a row has 16 words or fewer, lanes stand on several keys side by side).  The warps' results meet in shared memory;
+// with several splits they are left as partial results for kv4_join_kernel.
+constexpr int KV4_ANY_WARPS = 4, KV4_ANY_ROWS = 8;
+
+struct Kv4Attn {
+    const void* q; void* out;
+    const unsigned char* k; const unsigned char* v; const uint2* steps;
+    const int* q_start; const int* kv_len; const int* block_table;
+    float* part;                     // splits > 1: [splits][T * n_q][d + 2]
+    long long bt_stride, part_rows;
+    int B, T, n_q, n_kv, d, page_size, pages, bt_width, window, max_q, splits, tiles_q;      // tiles_q: blocks a request and kv head
+    float scale;
+};
+
+template <typename T, int WPL>       // WPL: words of a value row a lane
+__global__ void __launch_bounds__(KV4_ANY_WARPS * 32) kv4_attn_any_kernel(const Kv4Attn p) {
+    extern __shared__ float any_sh[];
+    constexpr int R = KV4_ANY_ROWS, NW = KV4_ANY_WARPS;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, d = p.d, words = d >> 3, G = p.n_q / p.n_kv;
+    float* qs = any_sh;                                  // [R][d]
+    float* ps = qs + R * d;                              // [NW][R][32]
+    float* os = ps + NW * R * 32;                        // [NW][R][d]
+    float* ms = os + NW * R * d;                         // [NW][R][2]
+    pdl_wait();
+    pdl_small();
+    const int tile = blockIdx.x % p.tiles_q, rest = blockIdx.x / p.tiles_q, kvh = rest % p.n_kv, req = rest / p.n_kv;
+    const int tok0 = p.q_start != nullptr ? p.q_start[req] : req, n_tok = p.q_start != nullptr ? p.q_start[req + 1] - tok0 : 1;
+    const int row0 = tile * R, n_rows = min(R, n_tok * G - row0);
+    if (n_tok < 1 || n_tok > p.max_q || n_rows <= 0 || tok0 < 0 || tok0 + n_tok > p.T) return;
+    const int kv = min(p.kv_len[req], p.bt_width * p.page_size), pos0 = p.kv_len[req] - n_tok;
+    auto row_at = [&](int r) -> long long { return (long long)(tok0 + (row0 + r) / G) * p.n_q + kvh * G + (row0 + r) % G; };
+    for (int i = tid; i < R * d; i += NW * 32) qs[i] = i / d < n_rows ? to_f32<T>(reinterpret_cast<const T*>(p.q)[row_at(i / d) * d + i % d]) : 0.f;
+    __syncthreads();
+    // this block's keys
+    const int k_first = p.window > 0 ? max(pos0 + row0 / G - p.window + 1, 0) : 0;
+    const int u0 = k_first >> 5, u1 = max((min(kv, pos0 + (row0 + n_rows - 1) / G + 1) + 31) >> 5, u0);
+    const int a = u0 + (int)((long long)(u1 - u0) * blockIdx.y / p.splits), b = u0 + (int)((long long)(u1 - u0) * (blockIdx.y + 1) / p.splits);
+    const float sc = p.scale * 1.4426950408889634f;
+    int wp = 1;                                          // lanes that stand on one value row
+    while (wp < words && wp < 32) wp <<= 1;
+    const int sub = lane / wp, subs = 32 / wp, my = lane - sub * wp;
+    float m[R], l[R], acc[R][8 * WPL];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        m[r] = -INFINITY; l[r] = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8 * WPL; ++e) acc[r][e] = 0.f;
+    }
+    float* pw = ps + warp * R * 32;
+    for (int u = a + warp; u < b; u += NW) {
+        const int key = 32 * u + lane;
+        long long src = -1;
+        if (key < kv) {
+            const int at = key / p.page_size, page = p.block_table[req * p.bt_stride + at];
+            if (page >= 0 && page < p.pages) src = ((long long)page * p.n_kv + kvh) * p.page_size + (key - at * p.page_size);
+        }
+        const uint2 st = src >= 0 ? p.steps[src] : make_uint2(0u, 0u);
+        const float ks = bf16_of(st.x & 0xffffu), kb = bf16_of(st.x >> 16);
+        float s[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) s[r] = 0.f;
+        for (int w = 0; w < words; ++w) {
+            const unsigned word = src >= 0 ? reinterpret_cast<const unsigned*>(p.k)[src * words + w] : 0u;
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = fmaf((float)((word >> (4 * e)) & 15u), ks, kb);
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const float4 q0 = *reinterpret_cast<const float4*>(qs + r * d + 8 * w), q1 = *reinterpret_cast<const float4*>(qs + r * d + 8 * w + 4);
+                s[r] = fmaf(q0.x, x[0], fmaf(q0.y, x[1], fmaf(q0.z, x[2], fmaf(q0.w, x[3], s[r]))));
+                s[r] = fmaf(q1.x, x[4], fmaf(q1.y, x[5], fmaf(q1.z, x[6], fmaf(q1.w, x[7], s[r]))));
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int pos = pos0 + (row0 + r) / G;
+            const bool seen = r < n_rows && key < kv && key <= pos && (p.window <= 0 || key > pos - p.window);
+            const float v = seen ? s[r] * sc : -INFINITY;
+            const float mn = fmaxf(m[r], warp_max(v)), mu = mn == -INFINITY ? 0.f : mn;
+            const float e = seen ? exp2f(v - mu) : 0.f, f = exp2f(m[r] - mu);
+            m[r] = mn;
+            l[r] = fmaf(l[r], f, e);
+            pw[r * 32 + lane] = e;
+#pragma unroll
+            for (int c = 0; c < 8 * WPL; ++c) acc[r][c] *= f;
+        }
+        __syncwarp();
+        for (int j = sub; j < 32; j += subs) {
+            const long long vs = __shfl_sync(0xffffffffu, src, j);
+            const unsigned sy = __shfl_sync(0xffffffffu, st.y, j);
+            if (vs < 0) continue;
+            const float step = bf16_of(sy & 0xffffu), base = bf16_of(sy >> 16);
+#pragma unroll
+            for (int w2 = 0; w2 < WPL; ++w2) {
+                const int w = my + 32 * w2;
+                if (w >= words) continue;
+                const unsigned word = reinterpret_cast<const unsigned*>(p.v)[vs * words + w];
+                float x[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = fmaf((float)((word >> (4 * e)) & 15u), step, base);
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    const float pr = pw[r * 32 + j];
+                    if (pr == 0.f) continue;             // a key that the row does not see counts for nothing, whatever it holds
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) acc[r][8 * w2 + e] = fmaf(pr, x[e], acc[r][8 * w2 + e]);
+                }
+            }
+        }
+        __syncwarp();
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        l[r] = warp_sum(l[r]);
+        for (int o = wp; o < 32; o <<= 1)
+#pragma unroll
+            for (int c = 0; c < 8 * WPL; ++c) acc[r][c] += __shfl_xor_sync(0xffffffffu, acc[r][c], o);
+        if (sub == 0)
+#pragma unroll
+            for (int w2 = 0; w2 < WPL; ++w2)
+                if (my + 32 * w2 < words)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) os[(warp * R + r) * d + 8 * (my + 32 * w2) + e] = acc[r][8 * w2 + e];
+        if (lane == 0) { ms[(warp * R + r) * 2] = m[r]; ms[(warp * R + r) * 2 + 1] = l[r]; }
+    }
+    __syncthreads();
+    for (int i = tid; i < n_rows * d; i += NW * 32) {
+        const int r = i / d, c = i - r * d;
+        float M = -INFINITY, L = 0.f, o = 0.f;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) M = fmaxf(M, ms[(w * R + r) * 2]);
+        const float mu = M == -INFINITY ? 0.f : M;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+            const float f = exp2f(ms[(w * R + r) * 2] - mu);
+            L = fmaf(f, ms[(w * R + r) * 2 + 1], L);
+            o = fmaf(f, os[(w * R + r) * d + c], o);
+        }
+        if (p.splits == 1) {
+            reinterpret_cast<T*>(p.out)[row_at(r) * d + c] = from_f32<T>(L != 0.f ? o / L : 0.f);
+        } else {
+            float* part = p.part + (blockIdx.y * p.part_rows + row_at(r)) * (d + 2);
+            part[c] = o;
+            if (c == 0) { part[d] = M; part[d + 1] = L; }
+        }
+    }
+}
+
+// the rows of the requests taken, from their partial results; a warp a row
+template <typename T>
+__global__ void __launch_bounds__(128) kv4_join_kernel(const Kv4Attn p) {
+    pdl_wait();
+    pdl_small();
+    const int lane = threadIdx.x & 31, G = p.n_q / p.n_kv, R = KV4_ANY_ROWS, d = p.d;
+    const int tile = blockIdx.x % p.tiles_q, rest = blockIdx.x / p.tiles_q, kvh = rest % p.n_kv, req = rest / p.n_kv;
+    const int tok0 = p.q_start != nullptr ? p.q_start[req] : req, n_tok = p.q_start != nullptr ? p.q_start[req + 1] - tok0 : 1;
+    if (n_tok < 1 || n_tok > p.max_q || tok0 < 0 || tok0 + n_tok > p.T) return;
+    for (int r = tile * R + (threadIdx.x >> 5); r < min(n_tok * G, (tile + 1) * R); r += 4) {
+        const long long row = (long long)(tok0 + r / G) * p.n_q + kvh * G + r % G;
+        float M = -INFINITY, L = 0.f;
+        for (int s = 0; s < p.splits; ++s) M = fmaxf(M, p.part[(s * p.part_rows + row) * (d + 2) + d]);
+        const float mu = M == -INFINITY ? 0.f : M;
+        for (int s = 0; s < p.splits; ++s) {
+            const float* part = p.part + (s * p.part_rows + row) * (d + 2);
+            L = fmaf(exp2f(part[d] - mu), part[d + 1], L);
+        }
+        for (int c = lane; c < d; c += 32) {
+            float o = 0.f;
+            for (int s = 0; s < p.splits; ++s) {
+                const float* part = p.part + (s * p.part_rows + row) * (d + 2);
+                o = fmaf(exp2f(part[d] - mu), part[c], o);
+            }
+            reinterpret_cast<T*>(p.out)[row * d + c] = from_f32<T>(L != 0.f ? o / L : 0.f);
+        }
+    }
+}
+
+// q_start null: request r has token r.  Requests with 1 .. max_q tokens are taken, the others' rows left alone.
+MSGL_API int msgl_kv4_attention_any(const void* q, void* out, const void* k, const void* v, const void* steps, const int* q_start, const int* kv_len, const int* block_table,
+                                    long long bt_stride, int bt_width, float* part, int splits, int B, int T, int n_q, int n_kv, int d, int page_size, int pages,
+                                    int window, int max_q, float scale, int dtype, cudaStream_t stream) {
+    if (B <= 0 || T <= 0) return MSGL_OK;
+    if (d < 8 || d > KV4_MAX_D || d % 8 || n_kv < 1 || n_q < 1 || n_q % n_kv || page_size < 1 || pages < 1 || bt_width < 1 || max_q < 1 || splits < 1 || splits > 65535 ||
+        (long long)bt_width * page_size > 0x7fffffffLL - 64)
+        return MSGL_ERR_SIZE;
+    if (dtype != MSGL_F32 && dtype != MSGL_BF16) return MSGL_ERR_DTYPE;
+    if (((uintptr_t)k | (uintptr_t)v | (uintptr_t)steps) & 15) return MSGL_ERR_ALIGN;
+    const int G = n_q / n_kv, tiles_q = (int)(((long long)max_q * G + KV4_ANY_ROWS - 1) / KV4_ANY_ROWS);
+    const long long grid = (long long)B * n_kv * tiles_q;
+    if (grid > 0x7fffffffLL || (splits > 1 && part == nullptr)) return MSGL_ERR_SIZE;
+    Kv4Attn p = {q, out, (const unsigned char*)k, (const unsigned char*)v, (const uint2*)steps, q_start, kv_len, block_table, part, bt_stride, (long long)T * n_q,
+                 B, T, n_q, n_kv, d, page_size, pages, bt_width, window, max_q, splits, tiles_q, scale};
+    const size_t smem = ((size_t)KV4_ANY_ROWS * d * (1 + KV4_ANY_WARPS) + KV4_ANY_WARPS * KV4_ANY_ROWS * 34) * 4;
+    static MsglOncePerDevice attr_set;
+    if (attr_set.due()) {
+        const int most = (int)(((size_t)KV4_ANY_ROWS * KV4_MAX_D * (1 + KV4_ANY_WARPS) + KV4_ANY_WARPS * KV4_ANY_ROWS * 34) * 4);
+        if (cudaFuncSetAttribute(kv4_attn_any_kernel<float, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, most) != cudaSuccess ||
+            cudaFuncSetAttribute(kv4_attn_any_kernel<float, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, most) != cudaSuccess ||
+            cudaFuncSetAttribute(kv4_attn_any_kernel<__nv_bfloat16, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, most) != cudaSuccess ||
+            cudaFuncSetAttribute(kv4_attn_any_kernel<__nv_bfloat16, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, most) != cudaSuccess)
+            return msgl_check_launch();
+        attr_set.mark();
+    }
+    const dim3 g((unsigned)grid, splits), b(KV4_ANY_WARPS * 32);
+    const bool two = d > 256;
+    if (dtype == MSGL_F32) msgl_launch_pdl(two ? kv4_attn_any_kernel<float, 2> : kv4_attn_any_kernel<float, 1>, g, b, smem, stream, p);
+    else msgl_launch_pdl(two ? kv4_attn_any_kernel<__nv_bfloat16, 2> : kv4_attn_any_kernel<__nv_bfloat16, 1>, g, b, smem, stream, p);
+    int rc = msgl_check_launch();
+    if (rc != MSGL_OK || splits == 1) return rc;
+    if (dtype == MSGL_F32) msgl_launch_pdl(kv4_join_kernel<float>, dim3((unsigned)grid), dim3(128), 0, stream, p);
+    else msgl_launch_pdl(kv4_join_kernel<__nv_bfloat16>, dim3((unsigned)grid), dim3(128), 0, stream, p);
+    return msgl_check_launch();
+}

@@ -2700,6 +2700,218 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
 
 
 # ---------------------------------------------------------------------------------------
+# a key/value cache held in 4 bits (csrc/kv4.cu)
+# ---------------------------------------------------------------------------------------
+KV4_MAX_HEAD_DIM = 512
+KV4_DIRECT_ROWS = 32              # (token, query head) rows of a request under a kv head up to which the codes are read directly; longer runs restore the keys first
+KV4_RESTORE_BYTES = 1 << 30       # of restored keys and values, what a step makes at a time
+_kv4 = None
+
+
+def _kv4_lib():
+    global _kv4
+    if _kv4 is None:
+        lib = _build.kv4_library()
+        lib.msgl_kv4_append.argtypes = [c_void_p, c_ll] + [c_void_p] * 4 + [c_int, c_float, c_void_p, c_int, c_int, c_int] + [c_void_p] * 4 + [c_ll] + [c_int] * 6 + [c_void_p]
+        lib.msgl_kv4_restore.argtypes = [c_void_p] * 6 + [c_int] + [c_void_p] * 3 + [c_ll, c_int, c_void_p] + [c_int] * 9 + [c_void_p]
+        lib.msgl_kv4_attention_any.argtypes = [c_void_p] * 8 + [c_ll, c_int, c_void_p] + [c_int] * 10 + [c_float, c_int, c_void_p]
+        _kv4 = lib
+    return _kv4
+
+
+class KV4Cache(NamedTuple):
+    """A paged cache of keys and values in 4 bits.  A row (one token under one kv head) is head_dim codes of 4 bits, the even element in the low half of a byte,
+    and two bfloat16 numbers: an element stands for base + code * step."""
+    k: torch.Tensor               # [pages, kv heads, page size, head_dim / 2] uint8
+    v: torch.Tensor               # the same
+    steps: torch.Tensor           # [pages, kv heads, page size, 4] bfloat16: k step, k base, v step, v base
+
+
+def kv4_cache(pages: int, n_kv: int, page_size: int, head_dim: int, device="cuda") -> KV4Cache:
+    """An empty cache (every row stands for zeros)."""
+    if head_dim % 8 or not 8 <= head_dim <= KV4_MAX_HEAD_DIM:
+        raise KernelError(f"a cache in 4 bits: head sizes up to {KV4_MAX_HEAD_DIM} in steps of 8; got {head_dim}")
+    rows = (pages, n_kv, page_size)
+    return KV4Cache(torch.zeros((*rows, head_dim // 2), dtype=torch.uint8, device=device), torch.zeros((*rows, head_dim // 2), dtype=torch.uint8, device=device),
+                    torch.zeros((*rows, 4), dtype=torch.bfloat16, device=device))
+
+
+def kv4_row_bytes(head_dim: int) -> int:
+    """Bytes of a key and a value of one token under one kv head."""
+    return head_dim + 8
+
+
+def _kv4_sizes(what: str, cache: KV4Cache) -> Tuple[int, int, int, int]:
+    """(pages, kv heads, page size, head size) of a cache that is laid out as it has to be."""
+    k, v, steps = cache
+    if not (k.dtype is v.dtype is torch.uint8 and steps.dtype is torch.bfloat16 and k.dim() == 4 and v.shape == k.shape and steps.shape == k.shape[:3] + (4,)
+            and k.is_contiguous() and v.is_contiguous() and steps.is_contiguous()):
+        raise KernelError(f"{what}: a cache in 4 bits is contiguous uint8 keys and values [pages, kv heads, page size, head size / 2] and bfloat16 steps [.., 4]; got "
+                          f"{k.dtype} {tuple(k.shape)}, {v.dtype} {tuple(v.shape)}, {steps.dtype} {tuple(steps.shape)}")
+    pages, n_kv, page_size, half = k.shape
+    if not (pages >= 1 and n_kv >= 1 and page_size >= 1 and half >= 4 and half % 4 == 0 and half <= KV4_MAX_HEAD_DIM // 2):
+        raise KernelError(f"{what}: a cache of at least one page, head sizes up to {KV4_MAX_HEAD_DIM} in steps of 8; got {tuple(k.shape)}")
+    if pages * page_size > 0x7fffffff:
+        raise KernelError(f"{what}: {pages} pages of {page_size} tokens: slots are 32 bits")
+    return pages, n_kv, page_size, 2 * half
+
+
+def qknorm_rope_kv4write(qkv: torch.Tensor, positions: torch.Tensor, n_q: int, n_kv: int, d: int, *, q_weight: Optional[torch.Tensor], k_weight: Optional[torch.Tensor],
+                         eps: float, rope_table: Optional[torch.Tensor], out_loc: torch.Tensor, cache: KV4Cache, q_out: Optional[torch.Tensor] = None,
+                         interleaved: bool = False) -> torch.Tensor:
+    """`qknorm_rope_kvwrite` for a cache in 4 bits: qkv [T, (n_q + 2 n_kv) d] float32 or bfloat16 (rows any distance apart), per-head RMSNorm of q and k (if weights
+    are given), rotation from `rope_table` [max_pos, rot] float32 = cos | sin (if given), the rotated k and v put into 4 bits at token slots `out_loc` (int32; a
+    slot outside the cache is left out), q returned as [T, n_q, d] in qkv's type.  Keys are coded from their float32 values, before any rounding to
+    qkv's type.  Two tokens with one slot leave one of the two rows or parts of both.  A row with a NaN or an infinity, or wider than bfloat16 reaches, stands for NaN."""
+    what = "qknorm_rope_kv4write"
+    pages, heads, page_size, size = _kv4_sizes(what, cache)
+    if qkv.dim() != 2 or qkv.dtype not in _DT or qkv.shape[1] != (n_q + 2 * n_kv) * d or qkv.stride(1) != 1 or n_q < 1:
+        raise KernelError(f"{what}: qkv is float32 or bfloat16 [tokens, {(n_q + 2 * n_kv) * d}] with adjacent columns; got {qkv.dtype} {tuple(qkv.shape)}")
+    if (heads, size) != (n_kv, d):
+        raise KernelError(f"{what}: {n_kv} kv heads of size {d} and a cache with {heads} of size {size}")
+    T = qkv.shape[0]
+    _index(what, "positions", positions, T)
+    _index(what, "out_loc", out_loc, T)
+    if (q_weight is None) != (k_weight is None):
+        raise KernelError(f"{what}: q and k have norm weights, or neither")
+    if q_weight is not None and not (q_weight.dtype == k_weight.dtype and q_weight.dtype in _DT and q_weight.numel() == k_weight.numel() == d
+                                     and q_weight.is_contiguous() and k_weight.is_contiguous()):
+        raise KernelError(f"{what}: norm weights are {d} float32 or bfloat16 elements each, of one type")
+    rot = max_pos = 0
+    if rope_table is not None:
+        if rope_table.dtype != torch.float32 or rope_table.dim() != 2 or not rope_table.is_contiguous() or rope_table.shape[0] < 1 or not 2 <= rope_table.shape[1] <= d \
+                or rope_table.shape[1] % 2:
+            raise KernelError(f"{what}: rope_table is contiguous float32 [positions, rotated elements], an even number of them up to {d}; got {rope_table.dtype} {tuple(rope_table.shape)}")
+        max_pos, rot = rope_table.shape
+    if q_out is None:
+        q_out = torch.empty((T, n_q, d), dtype=qkv.dtype, device=qkv.device)
+    elif q_out.dtype != qkv.dtype or tuple(q_out.shape) != (T, n_q, d) or not q_out.is_contiguous():
+        raise KernelError(f"{what}: q_out is contiguous [{T}, {n_q}, {d}] of qkv's type; got {q_out.dtype} {tuple(q_out.shape)}")
+    _same_device(what, qkv, positions, out_loc, *cache, q_weight, k_weight, rope_table, q_out)
+    if T == 0:
+        return q_out
+    code = _kv4_lib().msgl_kv4_append(qkv.data_ptr(), qkv.stride(0), positions.data_ptr(), out_loc.data_ptr(), _ptr(q_weight), _ptr(k_weight),
+                                      int(q_weight is not None and q_weight.dtype == torch.float32), float(eps), _ptr(rope_table), rot, max_pos, int(bool(interleaved)),
+                                      q_out.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), cache.steps.data_ptr(), pages * page_size, page_size, n_q, n_kv, d, T,
+                                      _DT[qkv.dtype], _stream())
+    _check(code, f"{what} (head size {d})")
+    return q_out
+
+
+def kv4_restore(cache: KV4Cache, pages: torch.Tensor, dtype: torch.dtype) -> Tuple[torch.Tensor, torch.Tensor]:
+    """What the pages of a cache in 4 bits stand for: keys and values [len(pages), kv heads, page size, head size] as float32 or bfloat16 (rounded once).  pages:
+    int32; a number outside the cache reads as zeros."""
+    what = "kv4_restore"
+    n_pages, n_kv, page_size, d = _kv4_sizes(what, cache)
+    if dtype not in _DT:
+        raise KernelError(f"{what}: results are float32 or bfloat16; got {dtype}")
+    _index(what, "pages", pages)
+    _same_device(what, *cache, pages)
+    n = pages.numel()
+    out = torch.empty((2, n, n_kv, page_size, d), dtype=dtype, device=pages.device)
+    if n:
+        code = _kv4_lib().msgl_kv4_restore(cache.k.data_ptr(), cache.v.data_ptr(), cache.steps.data_ptr(), out[0].data_ptr(), out[1].data_ptr(), pages.data_ptr(), n, None, None,
+                                           None, 0, 0, None, 0, 0, 0, 0, n_kv, page_size, n_pages, d, _DT[dtype], _stream())
+        _check(code, what)
+    return out[0], out[1]
+
+
+def kv4_attention(q: torch.Tensor, out: torch.Tensor, cache: KV4Cache, *, kv_len: torch.Tensor, block_table: torch.Tensor, scale: float, window: int = 0,
+                  q_start: Optional[torch.Tensor] = None, q_lens: Optional[Sequence[int]] = None, kv_lens: Optional[Sequence[int]] = None, workspace=None) -> None:
+    """Causal attention of a step's tokens over a paged cache in 4 bits: q and out [T, heads, head size] float32 or bfloat16, kv_len int32 [B] the tokens of every request in
+    the cache with this step's, block_table int32 [B, pages].  Without q_lens every request brings one token, request r token r (the form that a graph
+    captures); with it, the host's number of tokens of every request, which lie at q_start[r] .. q_start[r + 1] (int32 [B + 1]), and kv_lens, the host's copy of kv_len.
+    A token at position p sees the keys 0 .. p, with a window the last `window` of them; one that sees none gets 0.  Rows of out behind the last request
+    stay as they are, and so do all rows of a request without tokens.  A page number outside the cache reads as zeros.
+
+    Requests with few tokens read the codes themselves; for longer runs the keys and values that they see are first put back into q's type, once a call, in scratch
+    memory of up to KV4_RESTORE_BYTES (more only where one request needs it).  workspace: where scratch memory is kept between calls (`parts.Workspace`); calls that share one run one after the other."""
+    what = "kv4_attention"
+    pages, n_kv, page_size, d = _kv4_sizes(what, cache)
+    if q.dim() != 3 or q.dtype not in _DT or out.dtype != q.dtype or out.shape != q.shape or not q.is_contiguous() or not out.is_contiguous():
+        raise KernelError(f"{what}: q and out are contiguous [tokens, heads, head size], both float32 or both bfloat16; got {q.dtype} {tuple(q.shape)}, {out.dtype} {tuple(out.shape)}")
+    T, n_q, size = q.shape
+    if size != d or n_q < 1 or n_q % n_kv:
+        raise KernelError(f"{what}: {n_q} query heads of size {size} over a cache of {n_kv} kv heads of size {d}: whole groups of one size")
+    if not 0.0 < scale < math.inf:
+        raise KernelError(f"{what}: scale {scale} is not above 0")
+    if not 0 <= window <= 0x3fffffff:
+        raise KernelError(f"{what}: window {window}: 0 (all keys) or a number of keys")
+    B = block_table.shape[0] if block_table.dim() == 2 else -1
+    _table(what, block_table, B)
+    _index(what, "kv_len", kv_len, B)
+    if block_table.shape[1] * page_size > 0x3fffffff:
+        raise KernelError(f"{what}: a block table of {block_table.shape[1]} pages of {page_size} tokens: up to 2^30 tokens a request")
+    if q_lens is None:
+        if T != B:
+            raise KernelError(f"{what}: {T} tokens of {B} requests: without q_lens every request brings one")
+    else:
+        if kv_lens is None or q_start is None or len(q_lens) != B or len(kv_lens) != B:
+            raise KernelError(f"{what}: q_lens come with kv_lens, one of both a request ({B}), and q_start")
+        _index(what, "q_start", q_start, B + 1)
+        if B and (min(q_lens) < 0 or sum(q_lens) > T):
+            raise KernelError(f"{what}: {sum(q_lens)} tokens of all requests, and q has {T}")
+        if any(kv < n or kv > block_table.shape[1] * page_size for n, kv in zip(q_lens, kv_lens)):
+            raise KernelError(f"{what}: a request has as many tokens in the cache as it brings, and its block table holds them")
+    _same_device(what, q, out, *cache, kv_len, block_table, q_start)
+    if T == 0 or B == 0:
+        return
+    G = n_q // n_kv
+    direct = max(1, KV4_DIRECT_ROWS // G)          # most tokens of a request that reads the codes directly
+    few = 1 if q_lens is None else max((n for n in q_lens if n <= direct), default=0)
+    if few:
+        longest = block_table.shape[1] * page_size if q_lens is None else max(kv for n, kv in zip(q_lens, kv_lens) if 0 < n <= direct)
+        _kv4_few(q, out, cache, kv_len, block_table, scale, window, q_start if q_lens is not None else None, few, longest)
+    if q_lens is not None and max(q_lens) > direct:
+        _kv4_portions(q, out, cache, kv_len, block_table, scale, window, q_start, q_lens, kv_lens, direct + 1, workspace)
+
+
+def _kv4_few(q, out, cache, kv_len, block_table, scale, window, q_start, max_q, longest) -> None:
+    """The requests with 1 to max_q tokens, from the codes; `longest` bounds their keys."""
+    (T, n_q, d), (pages, n_kv, page_size, _), (B, width) = q.shape, cache.k.shape, block_table.shape
+    tiles = B * n_kv * -(-max_q * (n_q // n_kv) // 8)
+    splits = max(1, min(4 * sm_count(q.device) // tiles, (min(longest, window + 8) if window else longest) // 128, 64))
+    part = torch.empty(splits * T * n_q * (d + 2), dtype=torch.float32, device=q.device) if splits > 1 else None
+    code = _kv4_lib().msgl_kv4_attention_any(q.data_ptr(), out.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), cache.steps.data_ptr(), _ptr(q_start), kv_len.data_ptr(),
+                                             block_table.data_ptr(), block_table.stride(0), width, _ptr(part), splits, B, T, n_q, n_kv, d, page_size, pages, window, max_q,
+                                             scale, _DT[q.dtype], _stream())
+    _check(code, "kv4_attention")
+
+
+def _kv4_portions(q, out, cache, kv_len, block_table, scale, window, q_start, q_lens, kv_lens, min_q, workspace) -> None:
+    """The requests with at least min_q tokens: what they see is restored into pages of its own, which the prefill kernels then read."""
+    (T, n_q, d), (pages, n_kv, page_size, _), width = q.shape, cache.k.shape, block_table.shape[1]
+    lib, G, big = _kv4_lib(), n_q // n_kv, 1 << 30
+    per = int(lib.msgl_kv4_restored_page())
+    need = [0 if n < min_q else -(-kv // per) - (max(kv - n - window + 1, 0) // per if window else 0) for n, kv in zip(q_lens, kv_lens)]
+    page_numel = n_kv * per * d
+    most = max(1, KV4_RESTORE_BYTES // (2 * page_numel * q.element_size()))
+    a = 0
+    while a < len(need):
+        b, n = a, 0
+        while b < len(need) and (n == 0 or n + need[b] <= most):
+            n += need[b]
+            b += 1
+        if n:
+            t_width = max(-(-kv // per) for kv in kv_lens[a:b])
+            sizes = (("kv4_keys", n * page_numel, q.dtype), ("kv4_values", n * page_numel, q.dtype), ("kv4_table", (b - a) * t_width, torch.int32))
+            k, v, table = (torch.empty(m, dtype=t, device=q.device) if workspace is None else workspace.get(name, m, t) for name, m, t in sizes)
+            lens, kvs, starts, kv_part = q_lens[a:b], kv_lens[a:b], q_start[a:b + 1], kv_len[a:b]
+            code = lib.msgl_kv4_restore(cache.k.data_ptr(), cache.v.data_ptr(), cache.steps.data_ptr(), k.data_ptr(), v.data_ptr(), None, n, starts.data_ptr(),
+                                        kv_part.data_ptr(), block_table[a:b].data_ptr(), block_table.stride(0), width, table.data_ptr(), t_width, b - a, window, min_q, n_kv,
+                                        page_size, pages, d, _DT[q.dtype], _stream())
+            _check(code, "kv4_attention (keys restored)")
+            k, v, table = k.view(n, n_kv, per, d), v.view(n, n_kv, per, d), table.view(b - a, t_width)
+            common = dict(q_start=starts, kv_len=kv_part, block_table=table, n_kv=n_kv, page_size=per, window=window, scale=scale, qlen_min=min_q, qlen_max=big)
+            if not (tc_supported(d, q.dtype, G) and attention_tc(q, out, k, v, q_lens=lens, kv_lens=kvs, workspace=workspace, **common)):
+                variant = VARIANT_MMA_ROWS if mma_supported(d, q.dtype) else VARIANT_SIMT
+                qt = attention_tile_tokens(variant, G, d)
+                attention(q, out, k, v, nsplit=None, part_o=None, part_ml=None, max_split=1, uniform_decode=False, variant=variant,
+                          grid_x=sum(-(-m // qt) for m in lens if m >= min_q), **common)
+        a = b
+
+
+# ---------------------------------------------------------------------------------------
 # the whole decode step in one persistent kernel (csrc/decode_step.cu)
 # ---------------------------------------------------------------------------------------
 # Off unless MSGL_FUSED_DECODE=1: measured on B200 at Qwen3-8B's sizes the one-kernel step takes 4.2 / 5.4 ms at batch 1 / 8
