@@ -626,3 +626,5 @@ MSGL_API int msgl_kv4_attention_any(const void* q, void* out, const void* k, con
     else msgl_launch_pdl(kv4_join_kernel<__nv_bfloat16>, dim3((unsigned)grid), dim3(128), 0, stream, p);
     return msgl_check_launch();
 }
+
+#include "kv4_runs.cuh"

@@ -2704,6 +2704,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
 # ---------------------------------------------------------------------------------------
 KV4_MAX_HEAD_DIM = 512
 KV4_DIRECT_ROWS = 32              # (token, query head) rows of a request under a kv head up to which the codes are read directly; longer runs restore the keys first
+_KV4_REQUESTS = 256               # requests of one launch that deals the keys out
 KV4_RESTORE_BYTES = 1 << 30       # of restored keys and values, what a step makes at a time
 _kv4 = None
 
@@ -2714,6 +2715,7 @@ def _kv4_lib():
         lib = _build.kv4_library()
         lib.msgl_kv4_append.argtypes = [c_void_p, c_ll] + [c_void_p] * 4 + [c_int, c_float, c_void_p, c_int, c_int, c_int] + [c_void_p] * 4 + [c_ll] + [c_int] * 6 + [c_void_p]
         lib.msgl_kv4_restore.argtypes = [c_void_p] * 6 + [c_int] + [c_void_p] * 3 + [c_ll, c_int, c_void_p] + [c_int] * 9 + [c_void_p]
+        lib.msgl_kv4_attention_runs.argtypes = [c_void_p] * 8 + [c_ll, c_int] + [c_void_p] * 3 + [c_int] * 10 + [c_float, c_void_p]
         lib.msgl_kv4_attention_any.argtypes = [c_void_p] * 8 + [c_ll, c_int, c_void_p] + [c_int] * 10 + [c_float, c_int, c_void_p]
         _kv4 = lib
     return _kv4
@@ -2861,20 +2863,38 @@ def kv4_attention(q: torch.Tensor, out: torch.Tensor, cache: KV4Cache, *, kv_len
     few = 1 if q_lens is None else max((n for n in q_lens if n <= direct), default=0)
     if few:
         longest = block_table.shape[1] * page_size if q_lens is None else max(kv for n, kv in zip(q_lens, kv_lens) if 0 < n <= direct)
-        _kv4_few(q, out, cache, kv_len, block_table, scale, window, q_start if q_lens is not None else None, few, longest)
+        _kv4_few(q, out, cache, kv_len, block_table, scale, window, q_start if q_lens is not None else None, few, longest, workspace)
     if q_lens is not None and max(q_lens) > direct:
         _kv4_portions(q, out, cache, kv_len, block_table, scale, window, q_start, q_lens, kv_lens, direct + 1, workspace)
 
 
-def _kv4_few(q, out, cache, kv_len, block_table, scale, window, q_start, max_q, longest) -> None:
+def _kv4_few(q, out, cache, kv_len, block_table, scale, window, q_start, max_q, longest, workspace) -> None:
     """The requests with 1 to max_q tokens, from the codes; `longest` bounds their keys."""
     (T, n_q, d), (pages, n_kv, page_size, _), (B, width) = q.shape, cache.k.shape, block_table.shape
-    tiles = B * n_kv * -(-max_q * (n_q // n_kv) // 8)
+    lib, G = _kv4_lib(), n_q // n_kv
+    at_k, at_v, at_steps, at_q, at_out = cache.k.data_ptr(), cache.v.data_ptr(), cache.steps.data_ptr(), q.data_ptr(), out.data_ptr()
+    tiles = -(-max_q * G // 8)
+    if q.dtype == torch.bfloat16 and d in (64, 128) and pages * n_kv * page_size < 0xffffffff and not (at_q | at_out | at_k | at_v | at_steps) & 15 \
+            and min(B, _KV4_REQUESTS) * n_kv * tiles * (width * page_size // 32 + 5) < 1 << 31:
+        blocks = sm_count(q.device)
+        words = (min(_KV4_REQUESTS * max_q, T) * G // 8 + _KV4_REQUESTS) * n_kv          # segments of a launch at most
+        count = workspace.counters("kv4_count", words) if workspace is not None else None
+        if count is None:
+            count = torch.zeros(words, dtype=torch.int32, device=q.device)
+        n = 2 * 8 * blocks
+        part = workspace.whole("kv4_part", n * (d + 2), torch.float32) if workspace is not None else torch.empty(n * (d + 2), dtype=torch.float32, device=q.device)
+        for a in range(0, B, _KV4_REQUESTS):
+            b, row = min(B, a + _KV4_REQUESTS), 0 if q_start is not None else a          # (without q_start token r is request r's)
+            code = lib.msgl_kv4_attention_runs(at_q + row * n_q * d * 2, at_out + row * n_q * d * 2, at_k, at_v, at_steps, None if q_start is None else q_start.data_ptr() + 4 * a,
+                                               kv_len.data_ptr() + 4 * a, block_table.data_ptr() + 4 * a * block_table.stride(0), block_table.stride(0), width, part.data_ptr(),
+                                               part.data_ptr() + 4 * n * d, count.data_ptr(), blocks, b - a, T - row, n_q, n_kv, d, page_size, pages, window, max_q, scale, _stream())
+            _check(code, "kv4_attention")
+        return
+    tiles *= B * n_kv
     splits = max(1, min(4 * sm_count(q.device) // tiles, (min(longest, window + 8) if window else longest) // 128, 64))
     part = torch.empty(splits * T * n_q * (d + 2), dtype=torch.float32, device=q.device) if splits > 1 else None
-    code = _kv4_lib().msgl_kv4_attention_any(q.data_ptr(), out.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), cache.steps.data_ptr(), _ptr(q_start), kv_len.data_ptr(),
-                                             block_table.data_ptr(), block_table.stride(0), width, _ptr(part), splits, B, T, n_q, n_kv, d, page_size, pages, window, max_q,
-                                             scale, _DT[q.dtype], _stream())
+    code = lib.msgl_kv4_attention_any(at_q, at_out, at_k, at_v, at_steps, _ptr(q_start), kv_len.data_ptr(), block_table.data_ptr(), block_table.stride(0), width, _ptr(part),
+                                      splits, B, T, n_q, n_kv, d, page_size, pages, window, max_q, scale, _DT[q.dtype], _stream())
     _check(code, "kv4_attention")
 
 
