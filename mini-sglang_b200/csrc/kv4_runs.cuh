@@ -1,31 +1,35 @@
 // Attention over a cache in 4 bits on the tensor cores: bfloat16, head sizes 64 and 128, requests that bring few tokens.
 //
 // A segment is up to 8 rows (token, query head) of one request under one kv head, and its keys in units of 32.  The units of all segments are dealt out
-// over one block an SM: every block works out from the requests' lengths alone which are its own.
-//   * few keys: a segment of u units has max(1, u / PIECE) equal pieces, a block a piece (or a block a whole segment, where that is nearly even);
-//   * many short segments: a warp takes whole segments;
-//   * otherwise the units of all segments, each with HEAD units ahead for what a segment costs beside its keys, are laid end to end and cut into runs of
-//     equal length; a cut within SNAP units of a segment's edge moves onto the edge.
-// Pieces of a segment lie in consecutive blocks.  A segment within one block is written out by it; of the others every block leaves its partial result
-// in scratch memory, and the one that raises the segment's counter to its number of pieces merges them in the order of the keys and clears the counter.
+// over the warps of one block an SM; every warp works out from the requests' lengths alone which are its own, and goes through them by itself.
+//   * few keys: a segment of u units has max(1, u / PIECE) equal pieces, a block a piece (or a block a whole segment, where that is nearly even), and a piece's
+//     units are dealt out over the block's warps;
+//   * otherwise the units of all segments, each with HEAD units ahead for what a segment costs beside its keys, are laid end to end and cut into as many runs of
+//     equal length as there are warps; a cut within SNAP units of a segment's edge moves onto the edge.
+// A segment within one warp's run is written out by it.  Of the others a warp leaves its part (it has at most two: one that its run starts with, and its last) in
+// shared memory; behind the only barrier after the cut, parts of one segment are added in the order of the keys.  Where other blocks hold parts too, the
+// sum goes to scratch memory, and the block that raises the segment's counter to the number of blocks adds them up and clears the counter.
 //
-// Mathematics.  A code c enters the products as u = 1 + c / 16, which is exact in bfloat16 with the code in the top four bits of the fraction: a shift and
-// a masked "or" make two elements of a word at once.  With a key's step and base,
-//     q k = 16 step (sum q u - sum q) + base sum q                 (the accumulator starts at -sum q, and the rest is one multiplication and one addition a score)
-//     o   = sum_j p_j (base_j + step_j c_j) = sum_j w_j u_j + sum_j (p_j base_j - w_j),   w_j = bf16(16 p_j step_j)
-// where the rounded w_j stands in both sums, so that the offset of u cancels whatever w_j was rounded to; its rounding counts by the code alone.
+// Mathematics.  A code c enters the products as a float16 number without a shift of its exponent: four bits at the bottom of the fraction are the subnormal
+// c 2^-24, four bits above them 16 c 2^-24, both exact, so one "and" makes two elements of a word and every second pair takes no shift.  What the places differ by
+// is put right in Q (elements that meet 16 c are divided by 16) and in rows of O at the end.  With a key's step and base and q^ = q 2^e (e a row's
+// own: |q^| < 2^15, exact unless it is 2^-29 of the row's largest element),
+//     q k = step 2^(24 - e) sum q^ (c 2^-24) + base sum q
+//     o   = sum_j p_j (base_j + step_j c_j) = 2^24 / F sum_j w_j (c_j 2^-24) + sum_j p_j base_j,   w_j = float16(p_j step_j F)
+// F is a power of two of the warp's own that keeps step F <= 64 (p is at most 2^8, see KR_LAZY): where a unit brings a larger step, F and the sums are scaled down.
+// w keeps 11 bits; below 2^-28 of the largest step it loses them one by one.
 // Scores, p, sums and outputs are float32.  S^T = K Q^T with keys on the M dimension, the head's elements permuted so that a lane reads 16 bytes
 // of a row; P goes through movmatrix; V^T fragments come by ldmatrix.trans on 16-bit columns, four codes of two neighbouring keys a register.  The
 // exponentials' reference moves only where a score lies KR_LAZY above it.
 #pragma once
+#include <type_traits>
 
 constexpr float KR_LAZY = 8.f;
 constexpr int KR_KEYS = 32;          // keys of a unit
 constexpr int KR_MAX_B = 256;        // requests of a launch, a thread each
-constexpr int KR_PIECE = 8;          // units of a piece at least, where segments are cut by themselves
-constexpr int KR_SNAP = 3;           // a cut this close to a segment's edge moves onto it
-constexpr int KR_HEAD = 3;           // what a segment costs beside its units, in units
-constexpr int KR_WARP_UNITS = 8;     // longest segment where a warp takes whole segments
+constexpr int KR_PIECE = 12;         // units of a block's piece at least, where segments are cut by themselves
+constexpr int KR_SNAP = 1;           // a cut this close to a segment's edge moves onto it
+constexpr int KR_HEAD = 2;           // what a segment costs beside its units, in units
 
 struct Kv4Runs {
     const __nv_bfloat16* q; __nv_bfloat16* out;
@@ -40,11 +44,16 @@ struct Kv4Runs {
 };
 
 __device__ __forceinline__ unsigned kr_smem(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ void kr_cp16(unsigned s, const void* g, bool there) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(s), "l"(g), "r"(there ? 16 : 0));
+// copies of 16 and 8 bytes, or of that many zeros (bytes = 0); offsets are compile-time numbers, so that they cost no additions
+template <int S, int G> __device__ __forceinline__ void kr_cp16(unsigned s, const void* g, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0 + %3], [%1 + %4], 16, %2;\n" ::"r"(s), "l"(g), "r"(bytes), "n"(S), "n"(G));
 }
-__device__ __forceinline__ void kr_cp8(unsigned s, const void* g, bool there) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;\n" ::"r"(s), "l"(g), "r"(there ? 8 : 0));
+__device__ __forceinline__ void kr_cp8(unsigned s, const void* g, int bytes) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;\n" ::"r"(s), "l"(g), "r"(bytes));
+}
+// f(0), f(1), ... with the number as a constant
+template <int N, int I = 0, typename F> __device__ __forceinline__ void kr_each(F f) {
+    if constexpr (I < N) { f(std::integral_constant<int, I>{}); kr_each<N, I + 1>(f); }
 }
 __device__ __forceinline__ void kr_commit() { asm volatile("cp.async.commit_group;\n"); }
 template <int N> __device__ __forceinline__ void kr_wait() { asm volatile("cp.async.wait_group %0;\n" ::"n"(N)); }
@@ -56,480 +65,629 @@ __device__ __forceinline__ unsigned kr_pack(float lo, float hi) {
 }
 __device__ __forceinline__ unsigned kr_trans(unsigned v) {
     unsigned r;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(r) : "r"(v));
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(r) : "r"(v));
     return r;
 }
 __device__ __forceinline__ void kr_mma(float (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// codes I of both halves of a word as 1 + c / 16 in bfloat16
-template <int I> __device__ __forceinline__ unsigned kr_unit(unsigned w) {
-    const unsigned s = I == 0 ? w << 3 : w >> (4 * I - 3);
-    return (s & 0x00780078u) | 0x3f803f80u;
+// shared memory at an address and a compile-time offset
+template <int O> __device__ __forceinline__ void kr_lds4(unsigned a, unsigned& x, unsigned& y, unsigned& z, unsigned& w) {
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4 + %5];\n" : "=r"(x), "=r"(y), "=r"(z), "=r"(w) : "r"(a), "n"(O));
 }
-
-template <int D, int NW, int ST>
-constexpr size_t kr_smem_bytes() {
-    return (size_t)NW * ST * (KR_KEYS * (D + 8)) + (size_t)NW * 8 * (D + 4) * 4 + (size_t)NW * 8 * 2 * 4 + (8 * KR_MAX_B + 4) * 4;
+template <int O> __device__ __forceinline__ void kr_lds2(unsigned a, unsigned& x, unsigned& y) {
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2 + %3];\n" : "=r"(x), "=r"(y) : "r"(a), "n"(O));
 }
+template <int O> __device__ __forceinline__ void kr_ldsm_t(unsigned a, unsigned (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4 + %5];\n" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a), "n"(O));
+}
+// two floats to float16
+__device__ __forceinline__ unsigned kr_half2(float lo, float hi) {
+    unsigned r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;\n" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+// two rows of A (words wl, wh) times Q: elements 0 4, 1 5 (16 times their codes), 2 6, 3 7 (likewise) of the words
+constexpr unsigned KR_LOW = 0x000f000fu, KR_HIGH = 0x00f000f0u;
 
 struct KrCursor {
     int r, s, kvh, tile, c0, u;      // request, its segment, kv head and tile of rows; first unit of the segment among all, units
+    int key0, keys;                  // (unit among all) * KR_KEYS + key0 is the unit's first key; keys of the request
 };
 
 template <int D, int NW, int ST>
+constexpr size_t kr_smem_bytes() {
+    return (size_t)NW * ST * (KR_KEYS * (D + 8)) + (size_t)NW * 8 * (D + 4) * 4 + (size_t)NW * 2 * (16 + 1) * 4 + (8 * KR_MAX_B + 4) * 4;
+}
+
+template <int D, int NW, int ST, bool WHOLE>
 __global__ void __launch_bounds__(NW * 32, 1) kv4_attn_runs_kernel(const Kv4Runs p) {
     extern __shared__ __align__(128) unsigned char kr_sh[];
-    constexpr int ROW = D / 2, KV_BYTES = KR_KEYS * ROW, STAGE = 2 * KV_BYTES + KR_KEYS * 8, OLD = D + 4, THREADS = NW * 32;
+    constexpr int ROW = D / 2, KV_BYTES = KR_KEYS * ROW, STAGE = 2 * KV_BYTES + KR_KEYS * 8, OLD = D + 4;
     constexpr int CH = ROW / 16;                          // 16-byte chunks of a row
     constexpr int SW = CH == 4 ? 1 : 2;                   // chunk c of row r lies at c ^ (r >> SW & CH - 1): eight rows' chunks c are eight different 16-byte columns
     constexpr int QW = D / 32;                            // words of codes of a key row a lane
     static_assert(D == 64 || D == 128, "lanes read 8 or 16 bytes of a key row");
-    float* Om = reinterpret_cast<float*>(kr_sh + (size_t)NW * ST * STAGE);      // [NW][8][OLD]
-    float* Mm = Om + NW * 8 * OLD;                        // [NW][8]
-    float* Lm = Mm + NW * 8;                              // [NW][8]
-    int* pre_u = reinterpret_cast<int*>(Lm + NW * 8);     // [B + 1] units of all segments of the requests before
+    static_assert(ST * STAGE >= 8 * OLD * 4, "a warp's last result lies where its ring was");
+    float* firsts = reinterpret_cast<float*>(kr_sh + (size_t)NW * ST * STAGE);      // [NW][8][OLD] results that a run starts with
+    float* slot_ml = firsts + NW * 8 * OLD;               // [NW][2][8][2] maxima and sums of a warp's first and last result
+    int* slot_seg = reinterpret_cast<int*>(slot_ml + NW * 32);      // [NW][2] their segments, -1: none
+    int* pre_u = slot_seg + NW * 2;                       // [B + 1] units of all segments of the requests before
     int* pre_s = pre_u + KR_MAX_B + 1;                    // [B + 1] segments of the requests before
-    int* units = pre_s + KR_MAX_B + 1;                    // per request: units of a segment, first unit, keys, first token, tokens, last position + 1
+    int* units = pre_s + KR_MAX_B + 1;                    // per request: units of a segment, first unit, keys, first token, tokens, keys with those beyond the table
     int* first = units + KR_MAX_B;
     int* keys = first + KR_MAX_B;
     int* token = keys + KR_MAX_B;
     int* tokens = token + KR_MAX_B;
     int* ends = tokens + KR_MAX_B;
-    __shared__ int4 sh_sum[NW];
-    __shared__ int2 sh_run;
-    __shared__ int4 sh_seg;                               // request, its segment, (by_piece) pieces of the segment, this block's
-    __shared__ int sh_last;
+    __shared__ int sh_all[4];                             // units and segments of all requests; whether segments are cut by themselves; (by_piece) blocks of this block's segment
+    __shared__ int sh_mine;                               // by_piece: this block's number among them
+    __shared__ int sh_x[NW + 1], sh_r[NW], sh_s[NW];      // the warps' runs: where they start among all units, the request, its segment
+    __shared__ int sh_last[2];
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-    const int G = p.n_q / p.n_kv, NB = (int)gridDim.x, j = (int)blockIdx.x;
+    const int G = p.n_q / p.n_kv, NB = (int)gridDim.x, j = (int)blockIdx.x, W = NB * NW;      // W: warps of the launch
     pdl_wait();
 
-    // ---- the requests, their units, segments and pieces, and the sums over those before; a request a thread
-    int my_u = 0, my_segs = 0, my_pc = 0;
-    if (tid < p.B) {
-        const int t0 = p.q_start != nullptr ? p.q_start[tid] : tid, n = p.q_start != nullptr ? p.q_start[tid + 1] - t0 : 1, len = p.kv_len[tid];
-        const int kv = max(min(len, p.bt_width * p.page_size), 0), f = (p.window > 0 ? max(len - n - p.window + 1, 0) : 0) / KR_KEYS;
-        if (n >= 1 && n <= p.max_q && t0 >= 0 && t0 + n <= p.T) {
-            my_u = max((kv + KR_KEYS - 1) / KR_KEYS - f, 1);
-            my_segs = p.n_kv * ((n * G + 7) >> 3);
-            my_pc = max(1, my_u / KR_PIECE);
-        }
-        units[tid] = my_u; first[tid] = f; keys[tid] = kv; token[tid] = t0; tokens[tid] = n; ends[tid] = len;
-    }
-    int at_u = my_u * my_segs, at_s = my_segs, at_p = my_pc * my_segs;
+    // ---- one warp finds the block's runs: neighbouring requests a lane, their units, segments and pieces and the sums over those before
+    if (warp == 0) {
+        constexpr int RL = KR_MAX_B / 32;
+        const int per = (p.B + 31) >> 5, r0 = lane * per;
+        int t0[RL], n[RL], len[RL], u[RL], segs[RL];
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int a = __shfl_up_sync(0xffffffffu, at_u, o), b = __shfl_up_sync(0xffffffffu, at_s, o), c = __shfl_up_sync(0xffffffffu, at_p, o);
-        if (lane >= o) { at_u += a; at_s += b; at_p += c; }
-    }
-    const int most = __reduce_max_sync(0xffffffffu, my_u);
-    if (lane == 31) sh_sum[warp] = make_int4(at_u, at_s, at_p, most);
-    __syncthreads();
-    int U = 0, S = 0, pieces_all = 0, longest = 0;
-    at_u -= my_u * my_segs; at_s -= my_segs; at_p -= my_pc * my_segs;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) {
-        const int4 x = sh_sum[w];
-        if (w < warp) { at_u += x.x; at_s += x.y; at_p += x.z; }
-        U += x.x; S += x.y; pieces_all += x.z;
-        longest = max(longest, x.w);
-    }
-    if (tid < p.B) { pre_u[tid] = at_u; pre_s[tid] = at_s; }
-    if (tid == 0) { pre_u[p.B] = U; pre_s[p.B] = S; sh_run = make_int2(0, 0); }
-    if (S == 0) return;
-    if (pieces_all > NB && S <= NB && 3ll * longest * NB <= 4ll * U) {        // a block a segment is nearly even, and nothing is left to merge
-        pieces_all = S;
-        at_p = at_s;
-        my_pc = my_segs > 0 ? 1 : 0;
-    }
-    const bool by_piece = pieces_all <= NB;
-    const bool by_warp = !by_piece && longest <= KR_WARP_UNITS && (8ll * longest + 6) * NB < 11ll * S;
-
-    // ---- this block's run of units [lo, hi) of the segments laid end to end, and the segment it starts in
-    const long long V = U + (long long)KR_HEAD * S;
-    __syncthreads();
-    if (by_piece) {
-        const int in_r = j - at_p;
-        if (in_r >= 0 && in_r < my_pc * my_segs) {
-            const int s = in_r / my_pc, piece = in_r - s * my_pc, c0 = at_u + s * my_u;
-            sh_seg = make_int4(tid, s, my_pc, piece);
-            sh_run = make_int2(c0 + (int)((long long)my_u * piece / my_pc), c0 + (int)((long long)my_u * (piece + 1) / my_pc));
-        }
-    } else if (!by_warp) {
-        // the thread whose request holds the raw cut floor(V i / NB) finds the cut: a segment's edge or a unit within it
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const int i = j + e;
-            if (i == NB && tid == 0) sh_run.y = U;
-            const long long in_r = V * i / NB - (at_u + (long long)KR_HEAD * at_s);
-            if (in_r >= 0 && in_r < (long long)(my_u + KR_HEAD) * my_segs) {
-                const int s = (int)in_r / (my_u + KR_HEAD), off = (int)in_r - s * (my_u + KR_HEAD) - KR_HEAD;
-                const int unit = off <= KR_SNAP ? 0 : my_u - off <= KR_SNAP ? my_u : off, x = at_u + s * my_u + unit;
-                if (e == 1) { sh_run.y = x; continue; }
-                sh_run.x = x;
-                sh_seg = make_int4(tid, unit == my_u ? s + 1 : s, 1, 0);      // a cut at the end: the run starts with the segment behind
+        for (int k = 0; k < RL; ++k) {
+            const int r = r0 + k;
+            t0[k] = 0; n[k] = 0; len[k] = 0;
+            if (k < per && r < p.B) {
+                t0[k] = p.q_start != nullptr ? p.q_start[r] : r;
+                n[k] = p.q_start != nullptr ? p.q_start[r + 1] - t0[k] : 1;
+                len[k] = p.kv_len[r];
             }
         }
+        int at_u = 0, at_s = 0, at_p = 0, longest = 0;
+#pragma unroll
+        for (int k = 0; k < RL; ++k) {
+            const int r = r0 + k;
+            u[k] = segs[k] = 0;
+            if (k >= per || r >= p.B) continue;
+            const int kv = max(min(len[k], p.bt_width * p.page_size), 0), f = (p.window > 0 ? max(len[k] - n[k] - p.window + 1, 0) : 0) / KR_KEYS;
+            if (n[k] >= 1 && n[k] <= p.max_q && t0[k] >= 0 && t0[k] + n[k] <= p.T) {
+                u[k] = max((kv + KR_KEYS - 1) / KR_KEYS - f, 1);
+                segs[k] = p.n_kv * ((n[k] * G + 7) >> 3);
+                longest = max(longest, u[k]);
+            }
+            units[r] = u[k]; first[r] = f; keys[r] = kv; token[r] = t0[k]; tokens[r] = n[k]; ends[r] = len[k];
+            at_u += u[k] * segs[k];
+            at_s += segs[k];
+            at_p += max(segs[k] > 0 ? 1 : 0, u[k] / KR_PIECE) * segs[k];
+        }
+        int U = at_u, S = at_s, P = at_p;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, U, o), y = __shfl_up_sync(0xffffffffu, S, o), z = __shfl_up_sync(0xffffffffu, P, o);
+            if (lane >= o) { U += x; S += y; P += z; }
+        }
+        at_u = U - at_u; at_s = S - at_s; at_p = P - at_p;
+        U = __shfl_sync(0xffffffffu, U, 31); S = __shfl_sync(0xffffffffu, S, 31); P = __shfl_sync(0xffffffffu, P, 31);
+        longest = __reduce_max_sync(0xffffffffu, longest);
+        const bool whole = P > NB && S <= NB && 3ll * longest * NB <= 4ll * U;      // a block a segment is nearly even, and nothing is left to merge
+        const bool by_piece = whole || P <= NB;
+        if (whole) at_p = at_s;
+        if (lane <= NW) sh_x[lane] = 0;
+        if (lane == 0) { sh_all[0] = U; sh_all[1] = S; sh_all[2] = by_piece; sh_all[3] = 1; pre_u[p.B] = U; pre_s[p.B] = S; }
+        __syncwarp();
+#pragma unroll
+        for (int k = 0; k < RL; ++k) {
+            const int r = r0 + k;
+            if (k >= per || r >= p.B) continue;
+            pre_u[r] = at_u; pre_s[r] = at_s;
+            const int pc = whole ? 1 : max(1, u[k] / KR_PIECE), in_r = j - at_p;
+            if (by_piece && in_r >= 0 && in_r < pc * segs[k]) {      // the block's piece, dealt out over its warps
+                const int s = in_r / pc, piece = in_r - s * pc, c0 = at_u + s * u[k];
+                const int a = (int)((long long)u[k] * piece / pc), b = (int)((long long)u[k] * (piece + 1) / pc);
+                sh_all[3] = pc;
+                sh_mine = piece;
+                for (int w = 0; w < NW; ++w) { sh_x[w] = c0 + a + (b - a) * w / NW; sh_r[w] = r; sh_s[w] = s; }
+                sh_x[NW] = c0 + b;
+            }
+            at_u += u[k] * segs[k]; at_s += segs[k]; at_p += pc * segs[k];
+        }
+        __syncwarp();
+        if (!by_piece && lane <= NW) {
+            // cut i = floor(V i / W) falls into a request (the last whose V-sum before it is no larger), there into a segment, there onto an edge or a unit; a cut a lane
+            const int V = U + KR_HEAD * S, V_per = V / W, i = j * NW + lane;
+            if (i >= W) {
+                sh_x[lane] = U;
+            } else {
+                const int raw = i * V_per + (int)((unsigned)i * (unsigned)(V - V_per * W) / (unsigned)W);
+                int a = 0, b = p.B;
+                while (b - a > 1) {
+                    const int m = (a + b) >> 1;
+                    if (pre_u[m] + KR_HEAD * pre_s[m] <= raw) a = m; else b = m;
+                }
+                const int un = units[a], in_r = raw - pre_u[a] - KR_HEAD * pre_s[a];      // (requests without segments lie ahead of one with the same sum)
+                int s = in_r / (un + KR_HEAD);
+                const int off = in_r - s * (un + KR_HEAD) - KR_HEAD, unit = off <= KR_SNAP ? 0 : un - off <= KR_SNAP ? un : off;
+                sh_x[lane] = pre_u[a] + s * un + unit;
+                if (lane < NW) { sh_r[lane] = a; sh_s[lane] = unit == un ? s + 1 : s; }      // a cut at the end: the run starts with the segment behind
+            }
+        }
+    } else if (warp == NW - 1 && lane < 2 * NW) {
+        slot_seg[lane] = -1;
     }
+    static_assert(NW >= 2 && NW < 32, "a warp for the cut, a lane a cut");
     __syncthreads();
+
+    // ---- this warp's run of units [lo, hi) of the segments laid end to end, and the segment it starts in
+    const bool by_piece = sh_all[2];
+    if (sh_x[0] >= sh_x[NW]) return;                      // (the whole block)
     auto settle = [&](KrCursor& c) {                      // from a request's end to the next segment; there is one
         while (c.s >= pre_s[c.r + 1] - pre_s[c.r]) { ++c.r; c.s = 0; }
         c.u = units[c.r];
         const int tiles = (tokens[c.r] * G + 7) >> 3;
-        c.kvh = c.s / tiles;
-        c.tile = c.s - c.kvh * tiles;
+        c.kvh = c.s;
+        c.tile = 0;
+        if (tiles > 1) { c.kvh = c.s / tiles; c.tile = c.s - c.kvh * tiles; }
         c.c0 = pre_u[c.r] + c.s * c.u;
+        c.key0 = (first[c.r] - c.c0) * KR_KEYS;
+        c.keys = keys[c.r];
     };
-    int lo, hi, seg_pieces = 1, piece = 0;
+    const int lo = sh_x[warp], hi = sh_x[warp + 1];
     KrCursor seg;
-    if (by_warp) {                                        // segments [s0, s1) in order are this warp's
-        const int idx = warp * NB + j, W = NB * NW, s0 = (int)((long long)S * idx / W), s1 = (int)((long long)S * (idx + 1) / W);
-        if (s0 >= s1) return;                             // (no barrier of the block lies behind)
-        auto find = [&](int s, KrCursor& c) {             // the request of segment s
-            int a = 0, b = p.B;                           // pre_s[a] <= s < pre_s[b]
-            while (b - a > 1) {
-                const int m = (a + b) >> 1;
-                if (pre_s[m] <= s) a = m; else b = m;
-            }
-            c.r = a;
-            c.s = s - pre_s[a];
-            settle(c);
-        };
-        find(s1 - 1, seg);
-        hi = seg.c0 + seg.u;
-        find(s0, seg);
-        lo = seg.c0;
-    } else {
-        lo = sh_run.x; hi = sh_run.y;
-        if (lo >= hi) return;
-        seg_pieces = sh_seg.z; piece = sh_seg.w;
-        seg.r = sh_seg.x; seg.s = sh_seg.y;
-        settle(seg);
-    }
-    // the warp's units: x0, x0 + step, ... below hi
-    const int step = by_warp ? 1 : NW, x0 = by_warp ? lo : lo + warp, n_my = hi > x0 ? (hi - x0 + step - 1) / step : 0;
+    seg.r = sh_r[warp]; seg.s = sh_s[warp];
+    const int n_my = max(hi - lo, 0);
     const unsigned ring = kr_smem(kr_sh) + (unsigned)warp * ST * STAGE;
+    if (n_my > 0) {
+        settle(seg);
 
-    // ---- the warp's loader: a lane knows the row of key `lane` of the unit that is asked for next, its page looked up a unit before
-    KrCursor ld = seg;
-    auto row_of = [&](int i) -> unsigned {
-        if (i >= n_my) return 0xffffffffu;
-        const int x = x0 + i * step;
-        while (x >= ld.c0 + ld.u) { ++ld.s; settle(ld); }
-        const int key = (x - ld.c0 + first[ld.r]) * KR_KEYS + lane;
-        if (key >= keys[ld.r]) return 0xffffffffu;
-        const int at = p.page_shift >= 0 ? key >> p.page_shift : key / p.page_size;
-        const int page = p.block_table[ld.r * p.bt_stride + at];
-        return page >= 0 && page < p.pages ? ((unsigned)page * p.n_kv + ld.kvh) * p.page_size + (key - at * p.page_size) : 0xffffffffu;
-    };
-    auto load = [&](int i, unsigned row) {
-        const unsigned st = ring + (unsigned)(i % ST) * STAGE;
+        // ---- the warp's loader.  WHOLE: a page holds whole runs of 16 keys, and all lanes know where the unit's two runs lie (rows behind the request's last key are
+        // copied as they are, and hidden); else a lane knows the row of key `lane`.  The pages are looked up a unit before they are asked for.
+        KrCursor ld = seg;
+        struct Place { int page0, page1, add0, add1; };      // row: page * n_kv * page_size + add
+        const int page_rows = p.n_kv * p.page_size;
+        auto look_up = [&](int key, int& page, int& add) {
+            page = -1;
+            add = 0;
+            if (key >= ld.keys) return;
+            const int at = p.page_shift >= 0 ? key >> p.page_shift : key / p.page_size;
+            add = ld.kvh * p.page_size + (key - at * p.page_size);
+            page = p.block_table[ld.r * p.bt_stride + at];
+        };
+        auto place_of = [&](int x) -> Place {
+            Place w = {-1, -1, 0, 0};
+            if (x >= hi) return w;
+            while (x >= ld.c0 + ld.u) { ++ld.s; settle(ld); }
+            const int key = x * KR_KEYS + ld.key0;
+            look_up(WHOLE ? key : key + lane, w.page0, w.add0);
+            if (WHOLE) look_up(key + 16, w.page1, w.add1);
+            return w;
+        };
+        constexpr int PER = 32 / CH;                      // rows that a copy of the warp takes: CH copies a unit
+        const int l_row = lane / CH, l_ch = lane % CH;
+        const unsigned l_dst = ring + l_row * ROW + ((l_ch ^ ((l_row >> SW) & (CH - 1))) << 4);
+        static_assert(PER % (CH << SW) == 0, "one place for all copies");
+        auto load = [&](unsigned st, const Place& w) {    // st: the stage's offset in the ring
+            if (WHOLE) {
+                const int b0 = (unsigned)w.page0 < (unsigned)p.pages ? 16 : 0, b1 = (unsigned)w.page1 < (unsigned)p.pages ? 16 : 0;
+                const unsigned r0 = b0 ? (unsigned)w.page0 * page_rows + w.add0 : 0u, r1 = b1 ? (unsigned)w.page1 * page_rows + w.add1 : 0u;
+                const size_t o0 = (size_t)r0 * ROW + lane * 16, o1 = (size_t)r1 * ROW + lane * 16;
+                const unsigned char *k0 = p.k + o0, *v0 = p.v + o0, *k1 = p.k + o1, *v1 = p.v + o1;
+                kr_each<CH>([&](auto m) {
+                    constexpr int R = m.value * PER, H = R / 16, S = R * ROW, O = (R - 16 * H) * ROW;
+                    kr_cp16<S, O>(l_dst + st, H ? k1 : k0, H ? b1 : b0);
+                    kr_cp16<S + KV_BYTES, O>(l_dst + st, H ? v1 : v0, H ? b1 : b0);
+                });
+                const bool up = lane & 16;
+                kr_cp8(ring + st + 2 * KV_BYTES + lane * 8, p.steps + (up ? r1 : r0) + (lane & 15), up ? b1 >> 1 : b0 >> 1);
+            } else {
+                const unsigned row = (unsigned)w.page0 < (unsigned)p.pages ? (unsigned)w.page0 * page_rows + w.add0 : 0xffffffffu;
+                kr_each<CH>([&](auto m) {
+                    constexpr int S = m.value * PER * ROW;
+                    const unsigned src = __shfl_sync(0xffffffffu, row, m.value * PER + l_row);
+                    const size_t off = src != 0xffffffffu ? (size_t)src * ROW + l_ch * 16 : 0;
+                    kr_cp16<S, 0>(l_dst + st, p.k + off, src != 0xffffffffu ? 16 : 0);
+                    kr_cp16<S + KV_BYTES, 0>(l_dst + st, p.v + off, src != 0xffffffffu ? 16 : 0);
+                });
+                kr_cp8(ring + st + 2 * KV_BYTES + lane * 8, p.steps + (row != 0xffffffffu ? row : 0u), row != 0xffffffffu ? 8 : 0);
+            }
+        };
+        // Q as B operand: lane (g, t) holds row g's elements e, e + 4 of each of its words of eight, e = 0..3
+        const float sc = p.scale * 1.4426950408889634f;
+        unsigned qf[QW][4];
+        float q_base[2], q_step[2];                       // of rows 2 t and 2 t + 1: what a key's base and its step times the accumulated sum count in a score (log2 units)
+        int c_end[2], c_from[2];                          // of these rows: the last key seen + 1, the first
+        int all_end = 0, all_from = 0;                    // keys below all_end and from all_from on are seen by every row
+        uint4 x_q[QW];                                    // the queries as they come
+        auto fetch_q = [&](const KrCursor& c) {
+            const int row = c.tile * 8 + g;
+            const bool there = row < tokens[c.r] * G;
+            const int tok = row / G;
+            const __nv_bfloat16* src = p.q + ((size_t)(token[c.r] + (there ? tok : 0)) * p.n_q + (size_t)c.kvh * G + (there ? row - tok * G : 0)) * D + t * (D / 4);
 #pragma unroll
-        for (int m = 0; m < CH; ++m) {                    // 32 rows of CH chunks: CH a lane
-            const int r = m * (32 / CH) + lane / CH, c = lane % CH;
-            const unsigned src = __shfl_sync(0xffffffffu, row, r), dst = st + r * ROW + ((c ^ ((r >> SW) & (CH - 1))) << 4);
-            const bool there = src != 0xffffffffu;
-            const size_t off = there ? (size_t)src * ROW + c * 16 : 0;
-            kr_cp16(dst, p.k + off, there);
-            kr_cp16(dst + KV_BYTES, p.v + off, there);
-        }
-        const bool there = row != 0xffffffffu;
-        kr_cp8(st + 2 * KV_BYTES + lane * 8, p.steps + (there ? row : 0u), there);
-    };
+            for (int w = 0; w < QW; ++w) x_q[w] = there ? *reinterpret_cast<const uint4*>(src + 8 * w) : make_uint4(0u, 0u, 0u, 0u);
+        };
+        auto take_q = [&](const KrCursor& c) {
+            const int n = tokens[c.r] * G;
+            float sum = 0.f, top = 0.f;
 #pragma unroll
-    for (int i = 0; i < ST - 1; ++i) {
-        const unsigned row = row_of(i);
-        if (i < n_my) load(i, row);
-        kr_commit();
-    }
-    unsigned next = row_of(ST - 1);
-
-    // Q as B operand: lane (g, t) holds row g's elements e, e + 4 of each of its words of eight, e = 0..3
-    unsigned qf[QW][4];
-    float qsum[2];                                        // of rows 2 t and 2 t + 1
-    int c_end[2], c_from[2];                              // of these rows: the last key seen + 1, the first
-    int all_end = 0, all_from = 0;                        // keys below all_end and from all_from on are seen by every row
-    auto load_q = [&](const KrCursor& c) {
-        const int n = tokens[c.r] * G, row = c.tile * 8 + g;
-        const bool there = row < n;
-        const int tok = row / G;
-        const __nv_bfloat16* src = p.q + ((size_t)(token[c.r] + (there ? tok : 0)) * p.n_q + (size_t)c.kvh * G + (there ? row - tok * G : 0)) * D + t * (D / 4);
+            for (int w = 0; w < QW; ++w) {
+                const unsigned y[4] = {x_q[w].x, x_q[w].y, x_q[w].z, x_q[w].w};
 #pragma unroll
-        for (int w = 0; w < QW; ++w) {
-            const uint4 x = there ? *reinterpret_cast<const uint4*>(src + 8 * w) : make_uint4(0u, 0u, 0u, 0u);      // elements 01 23 45 67
-            qf[w][0] = __byte_perm(x.x, x.z, 0x5410);
-            qf[w][1] = __byte_perm(x.x, x.z, 0x7632);
-            qf[w][2] = __byte_perm(x.y, x.w, 0x5410);
-            qf[w][3] = __byte_perm(x.y, x.w, 0x7632);
-        }
-        float one[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int w = 0; w < QW; ++w) {
-            kr_mma(one, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u, qf[w][0], qf[w][1]);
-            kr_mma(one, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u, qf[w][2], qf[w][3]);
-        }
-        qsum[0] = one[0]; qsum[1] = one[1];
-        const int p0 = ends[c.r] - tokens[c.r], kv = keys[c.r];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const int pos = p0 + min(c.tile * 8 + 2 * t + e, n - 1) / G;
-            c_end[e] = min(pos + 1, kv);
-            c_from[e] = p.window > 0 ? pos - p.window + 1 : 0;
-        }
-        all_end = min(p0 + c.tile * 8 / G + 1, kv);
-        all_from = p.window > 0 ? p0 + min(c.tile * 8 + 7, n - 1) / G - p.window + 1 : 0;
-    };
-    load_q(seg);
-    const float sc = p.scale * 1.4426950408889634f;
-    int i = 0;
-    bool first_segment = true;
-    for (int begin = lo; begin < hi;) {
-        const int end = min(hi, seg.c0 + seg.u);
-        float o[D / 16][4];
-#pragma unroll
-        for (int mt = 0; mt < D / 16; ++mt) o[mt][0] = o[mt][1] = o[mt][2] = o[mt][3] = 0.f;
-        float m_c[2] = {-INFINITY, -INFINITY}, l_c[2] = {0.f, 0.f}, z_c[2] = {0.f, 0.f};
-
-        for (; i < n_my; ++i) {
-            const int x = x0 + i * step;
-            if (x >= end) break;
-            kr_wait<ST - 2>();
-            __syncwarp();                     // unit i has come for all lanes, and all have left the stage that is filled next
-            if (i + ST - 1 < n_my) load(i + ST - 1, next);
-            kr_commit();
-            next = row_of(i + ST);
-            const unsigned st = ring + (unsigned)(i % ST) * STAGE;
-            const int key0 = (x - seg.c0 + first[seg.r]) * KR_KEYS;
-            // ---- S^T = K Q^T, 16 keys a time
-            float v[2][4];
-            uint2 row_st[2][2];
-#pragma unroll
-            for (int m = 0; m < 2; ++m) {
-                const int r = 16 * m + g;
-                unsigned kl[QW], kh[QW];
-                if constexpr (D == 128) {
-                    const unsigned a = st + r * ROW + ((t ^ ((r >> SW) & 3)) << 4);      // (row r + 8 has the same permutation)
-                    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(kl[0]), "=r"(kl[1]), "=r"(kl[QW - 2]), "=r"(kl[QW - 1]) : "r"(a));
-                    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(kh[0]), "=r"(kh[1]), "=r"(kh[QW - 2]), "=r"(kh[QW - 1]) : "r"(a + 8 * ROW));
-                } else {
-                    const unsigned a = st + r * ROW + (((t >> 1) ^ ((r >> SW) & 1)) << 4) + (t & 1) * 8;
-                    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];\n" : "=r"(kl[0]), "=r"(kl[1]) : "r"(a));
-                    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];\n" : "=r"(kh[0]), "=r"(kh[1]) : "r"(a + 8 * ROW));
-                }
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-                    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];\n" : "=r"(row_st[m][h].x), "=r"(row_st[m][h].y) : "r"(st + 2 * KV_BYTES + (r + 8 * h) * 8));
-                float s[4] = {-qsum[0], -qsum[1], -qsum[0], -qsum[1]}, s2[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int w = 0; w < QW; ++w) {
-                    kr_mma(s, kr_unit<0>(kl[w]), kr_unit<0>(kh[w]), kr_unit<1>(kl[w]), kr_unit<1>(kh[w]), qf[w][0], qf[w][1]);
-                    kr_mma(s2, kr_unit<2>(kl[w]), kr_unit<2>(kh[w]), kr_unit<3>(kl[w]), kr_unit<3>(kh[w]), qf[w][2], qf[w][3]);
-                }
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const float a = bf16_of(row_st[m][h].x & 0xffffu) * (16.f * sc), b = bf16_of(row_st[m][h].x >> 16) * sc;
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) v[m][2 * h + e] = fmaf(a, s[2 * h + e] + s2[2 * h + e], b * qsum[e]);
+                for (int e = 0; e < 4; ++e) {
+                    const float a = __uint_as_float(y[e] << 16), b = __uint_as_float(y[e] & 0xffff0000u);
+                    sum += a + b;
+                    top = fmaxf(top, fmaxf(fabsf(a), fabsf(b)));
                 }
             }
-            const bool edge = key0 + KR_KEYS > all_end || key0 < all_from;
-            unsigned hidden = 0;                          // bit 4 m + e: value e of part m is a key that its row does not see
-            if (edge) {
+#pragma unroll
+            for (int d = 1; d < 4; d <<= 1) {
+                sum += __shfl_xor_sync(0xffffffffu, sum, d);
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+            }
+            const int e2 = min(max(14 - ((int)(__float_as_uint(top) >> 23) - 127), -100), 100);      // top 2^e2 lies in [2^14, 2^15)
+            const float up = __uint_as_float((unsigned)(127 + e2) << 23), up16 = up * 0.0625f, down = __uint_as_float((unsigned)(127 - e2) << 23) * 16777216.f;
+#pragma unroll
+            for (int w = 0; w < QW; ++w) {                // elements 01 23 45 67
+                const unsigned y[4] = {x_q[w].x, x_q[w].y, x_q[w].z, x_q[w].w};
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    qf[w][2 * e] = kr_half2(__uint_as_float(y[e] << 16) * up, __uint_as_float(y[e + 2] << 16) * up);
+                    qf[w][2 * e + 1] = kr_half2(__uint_as_float(y[e] & 0xffff0000u) * up16, __uint_as_float(y[e + 2] & 0xffff0000u) * up16);
+                }
+            }
+            const int p0 = ends[c.r] - tokens[c.r], kv = keys[c.r];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                q_base[e] = __shfl_sync(0xffffffffu, sum, (2 * t + e) * 4) * sc;
+                q_step[e] = __shfl_sync(0xffffffffu, down, (2 * t + e) * 4) * sc;
+                const int pos = p0 + min(c.tile * 8 + 2 * t + e, n - 1) / G;
+                c_end[e] = min(pos + 1, kv);
+                c_from[e] = p.window > 0 ? pos - p.window + 1 : 0;
+            }
+            all_end = min(p0 + c.tile * 8 / G + 1, kv);
+            all_from = p.window > 0 ? p0 + min(c.tile * 8 + 7, n - 1) / G - p.window + 1 : 0;
+        };
+        fetch_q(seg);
+        Place next;
+        {
+            Place w[ST - 1];
+#pragma unroll
+            for (int i = 0; i < ST - 1; ++i) w[i] = place_of(lo + i);
+            next = place_of(lo + ST - 1);
+#pragma unroll
+            for (int i = 0; i < ST - 1; ++i) {
+                if (i < n_my) load(i * STAGE, w[i]);
+                kr_commit();
+            }
+        }
+        take_q(seg);
+        // where this lane reads in a stage: its key rows, its rows' steps, its matrix rows of the values (of two chunk pairs)
+        const unsigned at_k = ring + (D == 128 ? g * ROW + ((t ^ ((g >> SW) & 3)) << 4) : g * ROW + (((t >> 1) ^ ((g >> SW) & 1)) << 4) + (t & 1) * 8);
+        const unsigned at_s = ring + 2 * KV_BYTES + g * 8;
+        const unsigned at_v = ring + KV_BYTES + (lane & 15) * ROW + (((lane >> 4) ^ (((lane & 15) >> SW) & (CH - 1))) << 4);
+        unsigned st = 0, st_load = (ST - 1) * STAGE;      // offsets of the stage that is worked on and of the one that is filled
+        for (int x = lo; x < hi;) {
+            const int begin = x, end = min(hi, seg.c0 + seg.u);
+            float o[D / 16][4];
+#pragma unroll
+            for (int mt = 0; mt < D / 16; ++mt) o[mt][0] = o[mt][1] = o[mt][2] = o[mt][3] = 0.f;
+            float m_c[2] = {-INFINITY, -INFINITY}, mu_c[2] = {0.f, 0.f}, l_c[2] = {0.f, 0.f}, z_c[2] = {0.f, 0.f};      // mu_c: the exponentials' reference (m_c, or 0 before a key)
+            float F = 0.f;                                // 0: no step seen yet
+
+            for (; x < end; ++x) {
+                kr_wait<ST - 2>();
+                __syncwarp();                             // the unit has come for all lanes, and all have left the stage that is filled next
+                if (x + ST - 1 < hi) load(st_load, next);
+                kr_commit();
+                next = place_of(x + ST);
+                const int key0 = x * KR_KEYS + seg.key0;
+                // ---- S^T = K Q^T, 16 keys a time; v: scores less their reference, log2 units
+                float v[2][4], s[2][2][4];
+                uint2 row_st[2][2];
+                unsigned kl[2][QW], kh[2][QW];
+                kr_each<2>([&](auto mm) {
+                    constexpr int m = mm.value;
+                    if constexpr (D == 128) {
+                        kr_lds4<16 * m * ROW>(at_k + st, kl[m][0], kl[m][1], kl[m][QW - 2], kl[m][QW - 1]);
+                        kr_lds4<(16 * m + 8) * ROW>(at_k + st, kh[m][0], kh[m][1], kh[m][QW - 2], kh[m][QW - 1]);
+                    } else {
+                        kr_lds2<16 * m * ROW>(at_k + st, kl[m][0], kl[m][1]);
+                        kr_lds2<(16 * m + 8) * ROW>(at_k + st, kh[m][0], kh[m][1]);
+                    }
+                });
+                kr_each<2>([&](auto mm) {
+                    constexpr int m = mm.value;
+                    kr_lds2<128 * m>(at_s + st, row_st[m][0].x, row_st[m][0].y);
+                    kr_lds2<128 * m + 64>(at_s + st, row_st[m][1].x, row_st[m][1].y);
+                });
 #pragma unroll
                 for (int m = 0; m < 2; ++m)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int key = key0 + 16 * m + g + ((e & 2) ? 8 : 0);
-                        if (key >= c_end[e & 1] || key < c_from[e & 1]) { v[m][e] = -INFINITY; hidden |= 1u << (4 * m + e); }
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) s[m][h][e] = 0.f;
+#pragma unroll
+                for (int w = 0; w < QW; ++w)              // four chains side by side
+#pragma unroll
+                    for (int m = 0; m < 2; ++m) {
+                        const unsigned l = kl[m][w], u = kh[m][w], l8 = l >> 8, u8 = u >> 8;
+                        kr_mma(s[m][0], l & KR_LOW, u & KR_LOW, l & KR_HIGH, u & KR_HIGH, qf[w][0], qf[w][1]);
+                        kr_mma(s[m][1], l8 & KR_LOW, u8 & KR_LOW, l8 & KR_HIGH, u8 & KR_HIGH, qf[w][2], qf[w][3]);
                     }
-            }
-            bool behind = false;
 #pragma unroll
-            for (int m = 0; m < 2; ++m)
+                for (int m = 0; m < 2; ++m)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) behind = behind || v[m][e] > m_c[e & 1] + KR_LAZY;
-            if (__any_sync(0xffffffffu, behind)) {
-                float alpha[2];
+                    for (int h = 0; h < 2; ++h) {
+                        const float a = __uint_as_float(row_st[m][h].x << 16), b = __uint_as_float(row_st[m][h].x & 0xffff0000u);
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    float mx = fmaxf(fmaxf(v[0][e], v[0][e + 2]), fmaxf(v[1][e], v[1][e + 2]));
-                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-                    const float mn = fmaxf(m_c[e], mx), mu = mn == -INFINITY ? 0.f : mn;
-                    alpha[e] = kr_exp2(m_c[e] - mu);
-                    m_c[e] = mn;
-                    l_c[e] *= alpha[e];
-                    z_c[e] *= alpha[e];
+                        for (int e = 0; e < 2; ++e) v[m][2 * h + e] = fmaf(a * q_step[e], s[m][0][2 * h + e] + s[m][1][2 * h + e], fmaf(b, q_base[e], -mu_c[e]));
+                    }
+                const bool edge = key0 + KR_KEYS > all_end || key0 < all_from;
+                unsigned hidden = 0;                      // bit 4 m + e: value e of part m is a key that its row does not see
+                if (edge) {
+#pragma unroll
+                    for (int m = 0; m < 2; ++m)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int key = key0 + 16 * m + g + ((e & 2) ? 8 : 0);
+                            if (key >= c_end[e & 1] || key < c_from[e & 1]) { v[m][e] = -INFINITY; hidden |= 1u << (4 * m + e); }
+                            if (key >= seg.keys) row_st[m][e >> 1].y = 0u;      // (whatever lies behind the request's last key)
+                        }
                 }
+                const float most_step = fmaxf(fmaxf(__uint_as_float(row_st[0][0].y << 16), __uint_as_float(row_st[0][1].y << 16)),
+                                              fmaxf(__uint_as_float(row_st[1][0].y << 16), __uint_as_float(row_st[1][1].y << 16)));
+                // how far the largest score lies above its reference (a first key lies above any)
+                float above[2];
 #pragma unroll
-                for (int mt = 0; mt < D / 16; ++mt) {
-                    o[mt][0] *= alpha[0]; o[mt][1] *= alpha[1];
-                    o[mt][2] *= alpha[0]; o[mt][3] *= alpha[1];
-                }
-            }
-            // ---- weights of the codes, and what the bases add
-            unsigned pb[2][2];
-#pragma unroll
-            for (int m = 0; m < 2; ++m)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const float step16 = 16.f * bf16_of(row_st[m][h].y & 0xffffu), base = bf16_of(row_st[m][h].y >> 16);
-                    float pr[2];
+                for (int e = 0; e < 2; ++e) above[e] = fmaxf(fmaxf(v[0][e], v[0][e + 2]), fmaxf(v[1][e], v[1][e + 2]));
+                if (__any_sync(0xffffffffu, above[0] > (m_c[0] == -INFINITY ? -INFINITY : KR_LAZY) || above[1] > (m_c[1] == -INFINITY ? -INFINITY : KR_LAZY) ||
+                                                most_step * F > 64.f || F == 0.f)) {
+                    float alpha[2], down = 1.f;
+                    if (F == 0.f || __any_sync(0xffffffffu, most_step * F > 64.f)) {      // the largest step of the unit, to the power of two above it
+                        const unsigned bits = __reduce_max_sync(0xffffffffu, __float_as_uint(most_step));
+                        const float lim = fminf(fmaxf(__uint_as_float((bits + 0x007fffffu) & 0x7f800000u), 0x1p-100f), 0x1p127f), f = 64.f / lim;
+                        down = F == 0.f ? 1.f : f / F;
+                        F = f;
+                    }
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        const float mu = m_c[e] == -INFINITY ? 0.f : m_c[e];
-                        pr[e] = kr_exp2(v[m][2 * h + e] - mu);
-                        l_c[e] += pr[e];
+                        float mx = above[e];
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                        const float mn = fmaxf(m_c[e], mx + mu_c[e]), mu = mn == -INFINITY ? 0.f : mn;
+                        alpha[e] = kr_exp2(m_c[e] - mu);
+#pragma unroll
+                        for (int m = 0; m < 2; ++m) { v[m][e] -= mu - mu_c[e]; v[m][e + 2] -= mu - mu_c[e]; }
+                        m_c[e] = mn;
+                        mu_c[e] = mu;
+                        l_c[e] *= alpha[e];
+                        z_c[e] *= alpha[e];
+                        alpha[e] *= down;
                     }
-                    const unsigned w = kr_pack(pr[0] * step16, pr[1] * step16);
-                    const float w0 = __uint_as_float(w << 16), w1 = __uint_as_float(w & 0xffff0000u);
-                    if (edge) {                           // a key that a row does not see counts for nothing, whatever it holds
-                        z_c[0] += ((hidden >> (4 * m + 2 * h)) & 1u ? 0.f : pr[0] * base) - w0;
-                        z_c[1] += ((hidden >> (4 * m + 2 * h + 1)) & 1u ? 0.f : pr[1] * base) - w1;
-                    } else {
-                        z_c[0] += fmaf(pr[0], base, -w0);
-                        z_c[1] += fmaf(pr[1], base, -w1);
-                    }
-                    pb[m][h] = kr_trans(w);
-                }
-            // ---- O^T += U^T W^T
 #pragma unroll
-            for (int m = 0; m < 2; ++m) {
-                const int r = 16 * m + (lane & 15);       // matrices: keys 0-7 and 8-15 of two neighbouring chunks
-#pragma unroll
-                for (int c2 = 0; c2 < CH / 2; ++c2) {
-                    unsigned a[4];
-                    const unsigned va = st + KV_BYTES + r * ROW + (((2 * c2 + (lane >> 4)) ^ ((r >> SW) & (CH - 1))) << 4);
-                    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];\n" : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3]) : "r"(va));
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {         // 32 elements: lane g has codes 4 g .. 4 g + 3 of keys 2 t, 2 t + 1
-                        const unsigned lo8 = a[2 * h], hi8 = a[2 * h + 1];
-                        kr_mma(o[4 * c2 + 2 * h], kr_unit<0>(lo8), kr_unit<1>(lo8), kr_unit<0>(hi8), kr_unit<1>(hi8), pb[m][0], pb[m][1]);
-                        kr_mma(o[4 * c2 + 2 * h + 1], kr_unit<2>(lo8), kr_unit<3>(lo8), kr_unit<2>(hi8), kr_unit<3>(hi8), pb[m][0], pb[m][1]);
+                    for (int mt = 0; mt < D / 16; ++mt) {
+                        o[mt][0] *= alpha[0]; o[mt][1] *= alpha[1];
+                        o[mt][2] *= alpha[0]; o[mt][3] *= alpha[1];
                     }
                 }
+                // ---- weights of the codes, and what the bases add
+                unsigned pb[2][2];
+#pragma unroll
+                for (int m = 0; m < 2; ++m)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const float st_f = __uint_as_float(row_st[m][h].y << 16) * F, base = __uint_as_float(row_st[m][h].y & 0xffff0000u);
+                        const float p0 = kr_exp2(v[m][2 * h]), p1 = kr_exp2(v[m][2 * h + 1]);
+                        l_c[0] += p0;
+                        l_c[1] += p1;
+                        unsigned w = kr_half2(p0 * st_f, p1 * st_f);
+                        if (edge) {                       // a key that a row does not see counts for nothing, whatever it holds
+                            const bool h0 = hidden >> (4 * m + 2 * h) & 1u, h1 = hidden >> (4 * m + 2 * h + 1) & 1u;
+                            if (!h0) z_c[0] = fmaf(p0, base, z_c[0]);
+                            if (!h1) z_c[1] = fmaf(p1, base, z_c[1]);
+                            w &= (h0 ? 0u : 0xffffu) | (h1 ? 0u : 0xffff0000u);
+                        } else {
+                            z_c[0] = fmaf(p0, base, z_c[0]);
+                            z_c[1] = fmaf(p1, base, z_c[1]);
+                        }
+                        pb[m][h] = kr_trans(w);
+                    }
+                // ---- O^T += C^T W^T; matrices: keys 0-7 and 8-15 of two neighbouring chunks.  Lane g gets codes 4 g .. 4 g + 3 of keys 2 t, 2 t + 1 of a chunk
+                kr_each<2>([&](auto mm) {
+                    constexpr int m = mm.value;
+                    kr_each<CH / 2>([&](auto cc) {
+                        constexpr int c2 = cc.value;
+                        unsigned a[4];
+                        kr_ldsm_t<16 * m * ROW>((at_v ^ (32 * c2)) + st, a);
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const unsigned a_lo = a[2 * h], a_hi = a[2 * h + 1], b_lo = a_lo >> 8, b_hi = a_hi >> 8;
+                            kr_mma(o[4 * c2 + 2 * h], a_lo & KR_LOW, a_lo & KR_HIGH, a_hi & KR_LOW, a_hi & KR_HIGH, pb[m][0], pb[m][1]);
+                            kr_mma(o[4 * c2 + 2 * h + 1], b_lo & KR_LOW, b_lo & KR_HIGH, b_hi & KR_LOW, b_hi & KR_HIGH, pb[m][0], pb[m][1]);
+                        }
+                    });
+                });
+                st = st == (ST - 1) * STAGE ? 0 : st + STAGE;
+                st_load = st_load == (ST - 1) * STAGE ? 0 : st_load + STAGE;
             }
-        }
-        // ---- the warps' results through shared memory, added in warp order
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-#pragma unroll
-            for (int d = 4; d < 32; d <<= 1) {
-                l_c[e] += __shfl_xor_sync(0xffffffffu, l_c[e], d);
-                z_c[e] += __shfl_xor_sync(0xffffffffu, z_c[e], d);
-            }
-        const KrCursor now = seg;
-        if (end >= hi) pdl_late();
-        else { ++seg.s; settle(seg); load_q(seg); }       // the next segment's
-        if (by_warp) __syncwarp();
-        else if (!first_segment) __syncthreads();         // the segment before has been read
-        first_segment = false;
-#pragma unroll
-        for (int mt = 0; mt < D / 16; ++mt)               // columns of o[2 x + y]: elements 32 (x / 1) ... : chunk mt / 2, elements 4 g + 2 (mt & 1) and the next
+            // ---- the segment's result, or this warp's part of it
+            const KrCursor now = seg;
+            if (end < hi) { ++seg.s; settle(seg); fetch_q(seg); }
+            const float of = F > 0.f ? 16777216.f / F : 0.f, of16 = of * 0.0625f;
 #pragma unroll
             for (int e = 0; e < 2; ++e)
-                *reinterpret_cast<float2*>(Om + (warp * 8 + 2 * t + e) * OLD + (mt >> 1) * 32 + 4 * g + 2 * (mt & 1)) = make_float2(o[mt][e] + z_c[e], o[mt][e + 2] + z_c[e]);
-        if (g == 0) {
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                Mm[warp * 8 + 2 * t + e] = m_c[e];
-                Lm[warp * 8 + 2 * t + e] = l_c[e];
+                for (int d = 4; d < 32; d <<= 1) {
+                    l_c[e] += __shfl_xor_sync(0xffffffffu, l_c[e], d);
+                    z_c[e] += __shfl_xor_sync(0xffffffffu, z_c[e], d);
+                }
+            if (begin == now.c0 && end == now.c0 + now.u) {      // all of it: rows 2 t and 2 t + 1, elements 4 g .. 4 g + 3 of every chunk
+                const int n = tokens[now.r] * G;
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int row = now.tile * 8 + 2 * t + e;
+                    if (row >= n) continue;
+                    const int tok = row / G;
+                    __nv_bfloat16* dst = p.out + ((size_t)(token[now.r] + tok) * p.n_q + (size_t)now.kvh * G + (row - tok * G)) * D + 4 * g;
+                    const float inv = l_c[e] != 0.f ? 1.f / l_c[e] : 0.f, a = of * inv, b = of16 * inv, z = z_c[e] * inv;
+#pragma unroll
+                    for (int c = 0; c < CH; ++c)
+                        *reinterpret_cast<uint2*>(dst + 32 * c) = make_uint2(kr_pack(fmaf(o[2 * c][e], a, z), fmaf(o[2 * c][e + 2], b, z)),
+                                                                             kr_pack(fmaf(o[2 * c + 1][e], a, z), fmaf(o[2 * c + 1][e + 2], b, z)));
+                }
+            } else {
+                const int slot = end == hi ? 1 : 0;
+                if (slot) { kr_wait<0>(); __syncwarp(); }      // the ring has been read
+                float* to = slot ? reinterpret_cast<float*>(kr_sh + (size_t)warp * ST * STAGE) : firsts + warp * 8 * OLD;
+#pragma unroll
+                for (int mt = 0; mt < D / 16; ++mt)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                        *reinterpret_cast<float2*>(to + (2 * t + e) * OLD + (mt >> 1) * 32 + 4 * g + 2 * (mt & 1)) = make_float2(fmaf(o[mt][e], of, z_c[e]), fmaf(o[mt][e + 2], of16, z_c[e]));
+                if (g == 0)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) *reinterpret_cast<float2*>(slot_ml + ((2 * warp + slot) * 8 + 2 * t + e) * 2) = make_float2(m_c[e], l_c[e]);
+                if (lane == 0) slot_seg[2 * warp + slot] = pre_s[now.r] + now.s;
+            }
+            if (end < hi) take_q(seg);
+        }
+        kr_wait<0>();
+    }
+    pdl_late();
+    __syncthreads();
+
+    // ---- the block's parts of segments, in the order of their keys: neighbours of one segment are a group, added in that order.  A lane knows a slot, and
+    // the lane of a group's first slot its segment
+    static_assert(2 * NW <= 32, "a lane a slot");
+    const int of_slot = lane < 2 * NW ? slot_seg[lane] : -1;
+    const unsigned there = __ballot_sync(0xffffffffu, of_slot >= 0);
+    if (there == 0) return;                               // (all warps see the same)
+    const unsigned under = there & ((1u << lane) - 1u);
+    const int before = __shfl_sync(0xffffffffu, of_slot, 31 - __clz(under | 1u));
+    const bool leads = of_slot >= 0 && (under == 0 || before != of_slot);
+    const unsigned starts = __ballot_sync(0xffffffffu, leads);
+    int pieces = 0, mine = 0, n_rows = 0, row0 = 0, at_token = 0, at_head = 0;      // blocks that hold parts of the segment, this one among them; its rows
+    if (leads) {
+        int a = 0, b = p.B;                               // the segment's request
+        while (b - a > 1) {
+            const int m = (a + b) >> 1;
+            if (pre_s[m] <= of_slot) a = m; else b = m;
+        }
+        const int s = of_slot - pre_s[a], tiles = (tokens[a] * G + 7) >> 3, kvh = s / tiles;
+        row0 = (s - kvh * tiles) * 8;
+        n_rows = min(8, tokens[a] * G - row0);
+        at_token = token[a];
+        at_head = kvh * G;
+        pieces = sh_all[3];
+        mine = sh_mine;
+        if (!by_piece) {                                  // the cuts inside are those of c + SNAP < floor(V i / W) < c + u - SNAP; part k lies in warp first_cut - 1 + k
+            const long long at = pre_u[a] + (long long)s * units[a] + (long long)KR_HEAD * (of_slot + 1);
+            const int V = sh_all[0] + KR_HEAD * sh_all[1];
+            const int first_cut = (int)(((at + KR_SNAP + 1) * W + V - 1) / V), last_cut = (int)(((at + units[a] - KR_SNAP) * W + V - 1) / V) - 1;
+            const int b0 = (first_cut - 1) / NW;
+            pieces = last_cut / NW - b0 + 1;
+            mine = j - b0;
+        }
+    }
+    constexpr int COLS = D / 4;                           // pieces of four elements a row
+    int sum_rows = n_rows;                                // rows of the groups before
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, sum_rows, o);
+        if (lane >= o) sum_rows += x;
+    }
+    const int all_rows = __shfl_sync(0xffffffffu, sum_rows, 31);
+    sum_rows -= n_rows;
+    auto out_row = [&](int lead, int row) -> __nv_bfloat16* {
+        const int r = __shfl_sync(0xffffffffu, row0, lead) + row, tok = r / G;
+        return p.out + ((size_t)(__shfl_sync(0xffffffffu, at_token, lead) + tok) * p.n_q + (__shfl_sync(0xffffffffu, at_head, lead) + r - tok * G)) * D + 4 * lane;
+    };
+    for (int task = warp; task < all_rows; task += NW) {  // a row a warp
+        const int lead = 31 - __clz(__ballot_sync(0xffffffffu, leads && sum_rows <= task)), row = task - __shfl_sync(0xffffffffu, sum_rows, lead);
+        const unsigned above = starts & ~((2u << lead) - 1u), group = there & ~((1u << lead) - 1u) & (above ? (above & (0u - above)) - 1u : 0xffffffffu);
+        const bool in = group >> lane & 1u;
+        const float2 ml = in ? *reinterpret_cast<const float2*>(slot_ml + (lane * 8 + row) * 2) : make_float2(-INFINITY, 0.f);
+        const float M = warp_max(ml.x), Mu = M == -INFINITY ? 0.f : M, f = in ? kr_exp2(ml.x - Mu) : 0.f, L = warp_sum(f * ml.y);
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (unsigned rest = group; rest; rest &= rest - 1) {
+            const int k = __ffs(rest) - 1;
+            const float w = __shfl_sync(0xffffffffu, f, k);
+            const float* from = (k & 1 ? reinterpret_cast<const float*>(kr_sh + (size_t)(k >> 1) * ST * STAGE) : firsts + (k >> 1) * 8 * OLD) + row * OLD;
+            if (lane < COLS) {
+                const float4 x = *reinterpret_cast<const float4*>(from + 4 * lane);
+                acc.x = fmaf(w, x.x, acc.x); acc.y = fmaf(w, x.y, acc.y);
+                acc.z = fmaf(w, x.z, acc.z); acc.w = fmaf(w, x.w, acc.w);
             }
         }
-        const int row0 = now.tile * 8, n_rows = min(8, tokens[now.r] * G - row0);
-        auto out_row = [&](int c) -> __nv_bfloat16* {
-            const int tok = (row0 + c) / G;
-            return p.out + ((size_t)(token[now.r] + tok) * p.n_q + (size_t)now.kvh * G + (row0 + c - tok * G)) * D;
-        };
-        auto put4 = [&](int c, int col, float4 x, float L) {
+        __nv_bfloat16* dst = out_row(lead, row);
+        const bool alone = __shfl_sync(0xffffffffu, pieces, lead) == 1;
+        const int out_slot = 2 * j + (__shfl_sync(0xffffffffu, mine, lead) == 0 ? 1 : 0);
+        if (lane >= COLS) continue;
+        if (alone) {
             const float inv = L != 0.f ? 1.f / L : 0.f;
-            *reinterpret_cast<uint2*>(out_row(c) + col) = make_uint2(kr_pack(x.x * inv, x.y * inv), kr_pack(x.z * inv, x.w * inv));
-        };
-        constexpr int COLS = D / 4;                       // pieces of four elements a row
-        if (by_warp) {
-            __syncwarp();
-            for (int idx = lane; idx < n_rows * COLS; idx += 32) {
-                const int c = idx / COLS, col = idx % COLS * 4;
-                put4(c, col, *reinterpret_cast<const float4*>(Om + (warp * 8 + c) * OLD + col), Lm[warp * 8 + c]);
-            }
+            *reinterpret_cast<uint2*>(dst) = make_uint2(kr_pack(acc.x * inv, acc.y * inv), kr_pack(acc.z * inv, acc.w * inv));
         } else {
-            int pieces = seg_pieces, mine = piece;        // pieces of this segment, this block's among them
-            if (!by_piece) {
-                pieces = 1; mine = 0;
-                if (begin > now.c0 || end < now.c0 + now.u) {      // the cuts inside are those of c + SNAP < floor(V i / NB) < c + u - SNAP; piece k in block first_cut - 1 + k
-                    const long long c = now.c0 + (long long)KR_HEAD * (pre_s[now.r] + now.s + 1);
-                    const int first_cut = (int)(((c + KR_SNAP + 1) * NB + V - 1) / V), last_cut = (int)(((c + now.u - KR_SNAP) * NB + V - 1) / V) - 1;
-                    pieces = last_cut - first_cut + 2;
-                    mine = j - (first_cut - 1);
-                }
-            }
-            __syncthreads();
-            const int slot = 2 * j + (mine == 0 ? 1 : 0);      // a run has at most one segment's first piece (its end) and one's later one (its start)
-            for (int idx = tid; idx < n_rows * COLS; idx += THREADS) {
-                const int c = idx / COLS, col = idx % COLS * 4;
-                float M = -INFINITY;
-#pragma unroll
-                for (int w = 0; w < NW; ++w) M = fmaxf(M, Mm[w * 8 + c]);
-                const float Mu = M == -INFINITY ? 0.f : M;
-                float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-                float L = 0.f;
-#pragma unroll
-                for (int w = 0; w < NW; ++w) {
-                    const float f = kr_exp2(Mm[w * 8 + c] - Mu);
-                    const float4 ov = *reinterpret_cast<const float4*>(Om + (w * 8 + c) * OLD + col);
-                    acc.x = fmaf(f, ov.x, acc.x); acc.y = fmaf(f, ov.y, acc.y);
-                    acc.z = fmaf(f, ov.z, acc.z); acc.w = fmaf(f, ov.w, acc.w);
-                    L += f * Lm[w * 8 + c];
-                }
-                if (pieces == 1) {
-                    put4(c, col, acc, L);
-                } else {
-                    *reinterpret_cast<float4*>(p.part_o + ((size_t)slot * 8 + c) * D + col) = acc;
-                    if (col == 0) *reinterpret_cast<float2*>(p.part_ml + ((size_t)slot * 8 + c) * 2) = make_float2(M, L);
-                }
-            }
-            if (pieces > 1) {
-                __syncthreads();
-                int* count = p.count + pre_s[now.r] + now.s;
-                if (tid == 0) {                           // the fence behind the barrier covers what the block's other threads wrote
-                    __threadfence();
-                    sh_last = atomicAdd(count, 1) == pieces - 1;
-                    __threadfence();
-                }
-                __syncthreads();
-                if (sh_last) {                            // all pieces are there: merged in the order of the keys
-                    const int b0 = j - mine;              // the block of piece 0
-                    if (tid == 0) *count = 0;
-                    for (int idx = tid; idx < n_rows * COLS; idx += THREADS) {
-                        const int c = idx / COLS, col = idx % COLS * 4;
-                        auto row_at = [&](int k) -> size_t { return (size_t)(2 * (b0 + k) + (k == 0 ? 1 : 0)) * 8 + c; };
-                        float M = -INFINITY, L = 0.f;
-                        for (int k = 0; k < pieces; ++k) M = fmaxf(M, __ldcg(p.part_ml + row_at(k) * 2));
-                        const float Mu = M == -INFINITY ? 0.f : M;
-                        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-                        for (int k = 0; k < pieces; ++k) {
-                            const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml + row_at(k) * 2));
-                            const float4 ov = __ldcg(reinterpret_cast<const float4*>(p.part_o + row_at(k) * D + col));
-                            const float f = kr_exp2(ml.x - Mu);
-                            L = fmaf(f, ml.y, L);
-                            acc.x = fmaf(f, ov.x, acc.x); acc.y = fmaf(f, ov.y, acc.y);
-                            acc.z = fmaf(f, ov.z, acc.z); acc.w = fmaf(f, ov.w, acc.w);
-                        }
-                        put4(c, col, acc, L);
+            *reinterpret_cast<float4*>(p.part_o + ((size_t)out_slot * 8 + row) * D + 4 * lane) = acc;
+            if (lane == 0) *reinterpret_cast<float2*>(p.part_ml + ((size_t)out_slot * 8 + row) * 2) = make_float2(M, L);
+        }
+    }
+    // segments that other blocks hold parts of as well: one from before, one that goes on
+    const unsigned open = __ballot_sync(0xffffffffu, pieces > 1);
+    if (open == 0) return;
+    __syncthreads();
+    if (warp == 0) {                                      // the fence behind the barrier covers what the block's other threads wrote
+        if (pieces > 1) {
+            __threadfence();
+            sh_last[open & ((1u << lane) - 1u) ? 1 : 0] = atomicAdd(p.count + of_slot, 1) == pieces - 1;
+            __threadfence();
+        }
+    }
+    __syncthreads();
+#pragma unroll 1
+    for (int q = 0; q < __popc(open); ++q) {
+        if (!sh_last[q]) continue;                        // the last block of a segment: all parts are there, and are merged in the order of the keys
+        const int lead = q == 0 ? __ffs(open) - 1 : 31 - __clz(open);
+        const int n = __shfl_sync(0xffffffffu, pieces, lead), b0 = j - __shfl_sync(0xffffffffu, mine, lead), rows = __shfl_sync(0xffffffffu, n_rows, lead);      // b0: the block of part 0
+        if (tid == lead) p.count[of_slot] = 0;
+        for (int row = warp; row < rows; row += NW) {
+            auto at = [&](int k) -> size_t { return (size_t)(2 * (b0 + k) + (k == 0 ? 1 : 0)) * 8 + row; };
+            float2 ml = lane < n ? __ldcg(reinterpret_cast<const float2*>(p.part_ml + at(lane) * 2)) : make_float2(-INFINITY, 0.f);
+            float M = ml.x;
+            for (int k = lane + 32; k < n; k += 32) M = fmaxf(M, __ldcg(p.part_ml + at(k) * 2));
+            M = warp_max(M);
+            const float Mu = M == -INFINITY ? 0.f : M;
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+            float L = 0.f;
+            for (int k0 = 0; k0 < n; k0 += 32) {
+                if (k0 > 0) ml = k0 + lane < n ? __ldcg(reinterpret_cast<const float2*>(p.part_ml + at(k0 + lane) * 2)) : make_float2(-INFINITY, 0.f);
+                const float w = kr_exp2(ml.x - Mu);
+                L = fmaf(w, ml.y, L);
+                const int m = min(n - k0, 32);
+#pragma unroll 8
+                for (int k = 0; k < m; ++k) {
+                    const float f = __shfl_sync(0xffffffffu, w, k);
+                    if (lane < COLS) {
+                        const float4 x = __ldcg(reinterpret_cast<const float4*>(p.part_o + at(k0 + k) * D + 4 * lane));
+                        acc.x = fmaf(f, x.x, acc.x); acc.y = fmaf(f, x.y, acc.y);
+                        acc.z = fmaf(f, x.z, acc.z); acc.w = fmaf(f, x.w, acc.w);
                     }
                 }
             }
+            L = warp_sum(L);
+            __nv_bfloat16* dst = out_row(lead, row);
+            const float inv = L != 0.f ? 1.f / L : 0.f;
+            if (lane < COLS) *reinterpret_cast<uint2*>(dst) = make_uint2(kr_pack(acc.x * inv, acc.y * inv), kr_pack(acc.z * inv, acc.w * inv));
         }
-        begin = end;
     }
-    kr_wait<0>();
 }
 
-constexpr int KR_NW = 8, KR_ST = 4;
+#ifndef KR_WARPS
+#define KR_WARPS 12
+#define KR_STAGES 3
+#endif
+constexpr int KR_NW = KR_WARPS, KR_ST = KR_STAGES;
 
 // Requests with 1 .. max_q tokens; q_start null: request r has token r.  count: a word for every 8 rows of a request under a kv head, zero before and after.
 MSGL_API int msgl_kv4_attention_runs(const void* q, void* out, const void* k, const void* v, const void* steps, const int* q_start, const int* kv_len, const int* block_table,
@@ -543,16 +701,20 @@ MSGL_API int msgl_kv4_attention_runs(const void* q, void* out, const void* k, co
     if (most * (((long long)bt_width * page_size + KR_KEYS - 1) / KR_KEYS + KR_HEAD + 1) >= (1LL << 31)) return MSGL_ERR_SIZE;
     if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)k | (uintptr_t)v | (uintptr_t)steps | (uintptr_t)part_o | (uintptr_t)part_ml) & 15) return MSGL_ERR_ALIGN;
     static MsglOncePerDevice attr_set;
+#define KR_EACH(DO) DO(64, true) DO(64, false) DO(128, true) DO(128, false)
     if (attr_set.due()) {
-        if (cudaFuncSetAttribute(kv4_attn_runs_kernel<64, KR_NW, KR_ST>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kr_smem_bytes<64, KR_NW, KR_ST>()) != cudaSuccess ||
-            cudaFuncSetAttribute(kv4_attn_runs_kernel<128, KR_NW, KR_ST>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kr_smem_bytes<128, KR_NW, KR_ST>()) != cudaSuccess)
-            return msgl_check_launch();
+#define KR_SET(DD, WW) if (cudaFuncSetAttribute(kv4_attn_runs_kernel<DD, KR_NW, KR_ST, WW>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kr_smem_bytes<DD, KR_NW, KR_ST>()) != cudaSuccess) return msgl_check_launch();
+        KR_EACH(KR_SET)
+#undef KR_SET
         attr_set.mark();
     }
     Kv4Runs p = {(const __nv_bfloat16*)q, (__nv_bfloat16*)out, (const unsigned char*)k, (const unsigned char*)v, (const uint2*)steps, q_start, kv_len, block_table, part_o,
                  part_ml, count, bt_stride, B, T, n_q, n_kv, page_size, -1, pages, bt_width, window, max_q, scale};
     if ((page_size & (page_size - 1)) == 0) { p.page_shift = 0; while ((1 << p.page_shift) < page_size) ++p.page_shift; }
-    if (d == 64) msgl_launch_pdl(kv4_attn_runs_kernel<64, KR_NW, KR_ST>, dim3(blocks), dim3(KR_NW * 32), kr_smem_bytes<64, KR_NW, KR_ST>(), stream, p);
-    else msgl_launch_pdl(kv4_attn_runs_kernel<128, KR_NW, KR_ST>, dim3(blocks), dim3(KR_NW * 32), kr_smem_bytes<128, KR_NW, KR_ST>(), stream, p);
+    const bool whole = page_size % 16 == 0;
+#define KR_GO(DD, WW) if (d == DD && whole == WW) msgl_launch_pdl(kv4_attn_runs_kernel<DD, KR_NW, KR_ST, WW>, dim3(blocks), dim3(KR_NW * 32), kr_smem_bytes<DD, KR_NW, KR_ST>(), stream, p);
+    KR_EACH(KR_GO)
+#undef KR_GO
+#undef KR_EACH
     return msgl_check_launch();
 }
