@@ -238,9 +238,22 @@ __global__ void __launch_bounds__(KV4_APPEND_THREADS) kv4_append_vec_kernel(cons
     if (l == 0) p.steps[2 * row + (is_k ? 0 : 1)] = sc.bits;
 }
 
-MSGL_API int msgl_kv4_append(const void* qkv, long long stride, const int* positions, const int* out_loc, const void* qw, const void* kw, int w_f32, float eps,
-                             const float* table, int rot, int max_pos, int interleaved, void* q_out, void* k, void* v, void* steps, long long slots, int page_size,
-                             int n_q, int n_kv, int d, int T, int dtype, cudaStream_t stream) {
+// The entry points take their arguments in one piece, 8 bytes each in the order of these structs.
+struct Kv4AppendArgs {
+    long long qkv, stride, positions, out_loc, qw, kw, w_f32, table, rot, max_pos, interleaved, q_out, k, v, steps, slots, page_size, n_q, n_kv, d, T, dtype, stream;
+    double eps;
+};
+
+MSGL_API int msgl_kv4_append(const Kv4AppendArgs* x) {
+    const long long stride = x->stride, slots = x->slots;
+    const void *qkv = (const void*)x->qkv, *qw = (const void*)x->qw, *kw = (const void*)x->kw, *k = (const void*)x->k, *v = (const void*)x->v, *steps = (const void*)x->steps;
+    const int *positions = (const int*)x->positions, *out_loc = (const int*)x->out_loc;
+    const float* table = (const float*)x->table;
+    void* q_out = (void*)x->q_out;
+    const int w_f32 = (int)x->w_f32, rot = (int)x->rot, max_pos = (int)x->max_pos, interleaved = (int)x->interleaved, page_size = (int)x->page_size, n_q = (int)x->n_q, n_kv = (int)x->n_kv,
+              d = (int)x->d, T = (int)x->T, dtype = (int)x->dtype;
+    const float eps = (float)x->eps;
+    cudaStream_t stream = (cudaStream_t)x->stream;
     if (T <= 0) return MSGL_OK;
     if (d < 8 || d > KV4_MAX_D || d % 8 || n_q < 0 || n_kv < 1 || page_size < 1 || rot > d || (rot & 1)) return MSGL_ERR_SIZE;
     if (dtype != MSGL_F32 && dtype != MSGL_BF16) return MSGL_ERR_DTYPE;
@@ -392,9 +405,19 @@ __global__ void __launch_bounds__(256) kv4_restore_kernel(const Kv4Restore p) {
 MSGL_API int msgl_kv4_restored_page(void) { return KV4_RESTORED; }
 
 // n: pages of results.  pages_in null: by requests.
-MSGL_API int msgl_kv4_restore(const void* k, const void* v, const void* steps, void* k_out, void* v_out, const int* pages_in, int n, const int* q_start, const int* kv_len,
-                              const int* block_table, long long bt_stride, int bt_width, int* table, int t_width, int B, int window, int min_q, int n_kv, int page_size,
-                              int pages, int d, int dtype, cudaStream_t stream) {
+struct Kv4RestoreArgs {
+    long long k, v, steps, k_out, v_out, pages_in, n, q_start, kv_len, block_table, bt_stride, bt_width, table, t_width, B, window, min_q, n_kv, page_size, pages, d, dtype, stream;
+};
+
+MSGL_API int msgl_kv4_restore(const Kv4RestoreArgs* x) {
+    const void *k = (const void*)x->k, *v = (const void*)x->v, *steps = (const void*)x->steps;
+    void *k_out = (void*)x->k_out, *v_out = (void*)x->v_out;
+    const int *pages_in = (const int*)x->pages_in, *q_start = (const int*)x->q_start, *kv_len = (const int*)x->kv_len, *block_table = (const int*)x->block_table;
+    int* table = (int*)x->table;
+    const long long bt_stride = x->bt_stride;
+    const int n = (int)x->n, bt_width = (int)x->bt_width, t_width = (int)x->t_width, B = (int)x->B, window = (int)x->window, min_q = (int)x->min_q, n_kv = (int)x->n_kv,
+              page_size = (int)x->page_size, pages = (int)x->pages, d = (int)x->d, dtype = (int)x->dtype;
+    cudaStream_t stream = (cudaStream_t)x->stream;
     if (n <= 0) return MSGL_OK;
     if (d < 8 || d > KV4_MAX_D || d % 8 || n_kv < 1 || n_kv > 65535 || page_size < 1 || pages < 1) return MSGL_ERR_SIZE;
     if (dtype != MSGL_F32 && dtype != MSGL_BF16) return MSGL_ERR_DTYPE;
@@ -591,9 +614,21 @@ __global__ void __launch_bounds__(128) kv4_join_kernel(const Kv4Attn p) {
 }
 
 // q_start null: request r has token r.  Requests with 1 .. max_q tokens are taken, the others' rows left alone.
-MSGL_API int msgl_kv4_attention_any(const void* q, void* out, const void* k, const void* v, const void* steps, const int* q_start, const int* kv_len, const int* block_table,
-                                    long long bt_stride, int bt_width, float* part, int splits, int B, int T, int n_q, int n_kv, int d, int page_size, int pages,
-                                    int window, int max_q, float scale, int dtype, cudaStream_t stream) {
+struct Kv4AnyArgs {
+    long long q, out, k, v, steps, q_start, kv_len, block_table, bt_stride, bt_width, part, splits, B, T, n_q, n_kv, d, page_size, pages, window, max_q, dtype, stream;
+    double scale;
+};
+
+MSGL_API int msgl_kv4_attention_any(const Kv4AnyArgs* x) {
+    const void *q = (const void*)x->q, *k = (const void*)x->k, *v = (const void*)x->v, *steps = (const void*)x->steps;
+    void* out = (void*)x->out;
+    const int *q_start = (const int*)x->q_start, *kv_len = (const int*)x->kv_len, *block_table = (const int*)x->block_table;
+    float* part = (float*)x->part;
+    const long long bt_stride = x->bt_stride;
+    const int bt_width = (int)x->bt_width, splits = (int)x->splits, B = (int)x->B, T = (int)x->T, n_q = (int)x->n_q, n_kv = (int)x->n_kv, d = (int)x->d, page_size = (int)x->page_size,
+              pages = (int)x->pages, window = (int)x->window, max_q = (int)x->max_q, dtype = (int)x->dtype;
+    const float scale = (float)x->scale;
+    cudaStream_t stream = (cudaStream_t)x->stream;
     if (B <= 0 || T <= 0) return MSGL_OK;
     if (d < 8 || d > KV4_MAX_D || d % 8 || n_kv < 1 || n_q < 1 || n_q % n_kv || page_size < 1 || pages < 1 || bt_width < 1 || max_q < 1 || splits < 1 || splits > 65535 ||
         (long long)bt_width * page_size > 0x7fffffffLL - 64)

@@ -12,7 +12,8 @@
 //
 // Mathematics.  A code c enters the products as a float16 number without a shift of its exponent: four bits at the bottom of the fraction are the subnormal
 // c 2^-24, four bits above them 16 c 2^-24, both exact, so one "and" makes two elements of a word and every second pair takes no shift.  What the places differ by
-// is put right in Q (elements that meet 16 c are divided by 16) and in rows of O at the end.  With a key's step and base and q^ = q 2^e (e a row's
+// is put right in Q (elements that meet 16 c are divided by 16) and in rows of O at the end.  Of the values a byte goes in whole, as c + 16 c' 2^-24, beside its upper
+// code alone, and the sums are told apart at the end: the upper bytes then take no masks (four operations eight codes instead of five).  With a key's step and base and q^ = q 2^e (e a row's
 // own: |q^| < 2^15, exact unless it is 2^-29 of the row's largest element),
 //     q k = step 2^(24 - e) sum q^ (c 2^-24) + base sum q
 //     o   = sum_j p_j (base_j + step_j c_j) = 2^24 / F sum_j w_j (c_j 2^-24) + sum_j p_j base_j,   w_j = float16(p_j step_j F)
@@ -82,6 +83,11 @@ template <int O> __device__ __forceinline__ void kr_lds2(unsigned a, unsigned& x
 template <int O> __device__ __forceinline__ void kr_ldsm_t(unsigned a, unsigned (&r)[4]) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4 + %5];\n" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a), "n"(O));
 }
+// with an accumulator of zeros
+__device__ __forceinline__ void kr_mma0(float (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
 // two floats to float16
 __device__ __forceinline__ unsigned kr_half2(float lo, float hi) {
     unsigned r;
@@ -89,7 +95,7 @@ __device__ __forceinline__ unsigned kr_half2(float lo, float hi) {
     return r;
 }
 // two rows of A (words wl, wh) times Q: elements 0 4, 1 5 (16 times their codes), 2 6, 3 7 (likewise) of the words
-constexpr unsigned KR_LOW = 0x000f000fu, KR_HIGH = 0x00f000f0u;
+constexpr unsigned KR_LOW = 0x000f000fu, KR_HIGH = 0x00f000f0u, KR_BYTE = 0x00ff00ffu;
 
 struct KrCursor {
     int r, s, kvh, tile, c0, u;      // request, its segment, kv head and tile of rows; first unit of the segment among all, units
@@ -123,85 +129,74 @@ __global__ void __launch_bounds__(NW * 32, 1) kv4_attn_runs_kernel(const Kv4Runs
     int* ends = tokens + KR_MAX_B;
     __shared__ int sh_all[4];                             // units and segments of all requests; whether segments are cut by themselves; (by_piece) blocks of this block's segment
     __shared__ int sh_mine;                               // by_piece: this block's number among them
-    __shared__ int sh_x[NW + 1], sh_r[NW], sh_s[NW];      // the warps' runs: where they start among all units, the request, its segment
+    __shared__ int sh_x[NW + 1], sh_r[NW + 1], sh_s[NW + 1];      // the warps' runs: where they start among all units, the request, its segment
     __shared__ int sh_last[2];
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const int G = p.n_q / p.n_kv, NB = (int)gridDim.x, j = (int)blockIdx.x, W = NB * NW;      // W: warps of the launch
     pdl_wait();
 
-    // ---- one warp finds the block's runs: neighbouring requests a lane, their units, segments and pieces and the sums over those before
+    // ---- the requests, a thread each; then one warp sums up their units, segments and pieces, neighbouring requests a lane, and cuts.  (Short code: it runs once, from a
+    // cold instruction cache.)
+    static_assert(NW * 32 >= KR_MAX_B || NW * 64 >= KR_MAX_B, "one or two requests a thread");
+#pragma unroll 1
+    for (int r = tid; r < p.B; r += NW * 32) {
+        const int t0 = p.q_start != nullptr ? p.q_start[r] : r, n = p.q_start != nullptr ? p.q_start[r + 1] - t0 : 1, len = p.kv_len[r];
+        const int kv = max(min(len, p.bt_width * p.page_size), 0), f = (p.window > 0 ? max(len - n - p.window + 1, 0) : 0) / KR_KEYS;
+        const bool taken = n >= 1 && n <= p.max_q && t0 >= 0 && t0 + n <= p.T;
+        units[r] = taken ? max((kv + KR_KEYS - 1) / KR_KEYS - f, 1) : 0;
+        pre_s[r] = taken ? p.n_kv * ((n * G + 7) >> 3) : 0;      // (its own segments, until they are summed up)
+        first[r] = f; keys[r] = kv; token[r] = t0; tokens[r] = n; ends[r] = len;
+    }
+    if (lane < 2) slot_seg[2 * warp + lane] = -1;
+    if (tid <= NW) sh_x[tid] = 0;
+    __syncthreads();
     if (warp == 0) {
-        constexpr int RL = KR_MAX_B / 32;
-        const int per = (p.B + 31) >> 5, r0 = lane * per;
-        int t0[RL], n[RL], len[RL], u[RL], segs[RL];
-#pragma unroll
-        for (int k = 0; k < RL; ++k) {
-            const int r = r0 + k;
-            t0[k] = 0; n[k] = 0; len[k] = 0;
-            if (k < per && r < p.B) {
-                t0[k] = p.q_start != nullptr ? p.q_start[r] : r;
-                n[k] = p.q_start != nullptr ? p.q_start[r + 1] - t0[k] : 1;
-                len[k] = p.kv_len[r];
-            }
+        const int per = (p.B + 31) >> 5, r0 = lane * per, r1 = min(r0 + per, p.B);
+        int U = 0, S = 0, P = 0, longest = 0;
+#pragma unroll 1
+        for (int r = r0; r < r1; ++r) {
+            const int u = units[r], segs = pre_s[r];
+            U += u * segs;
+            S += segs;
+            P += max(1, u / KR_PIECE) * segs;
+            longest = max(longest, u);
         }
-        int at_u = 0, at_s = 0, at_p = 0, longest = 0;
-#pragma unroll
-        for (int k = 0; k < RL; ++k) {
-            const int r = r0 + k;
-            u[k] = segs[k] = 0;
-            if (k >= per || r >= p.B) continue;
-            const int kv = max(min(len[k], p.bt_width * p.page_size), 0), f = (p.window > 0 ? max(len[k] - n[k] - p.window + 1, 0) : 0) / KR_KEYS;
-            if (n[k] >= 1 && n[k] <= p.max_q && t0[k] >= 0 && t0[k] + n[k] <= p.T) {
-                u[k] = max((kv + KR_KEYS - 1) / KR_KEYS - f, 1);
-                segs[k] = p.n_kv * ((n[k] * G + 7) >> 3);
-                longest = max(longest, u[k]);
-            }
-            units[r] = u[k]; first[r] = f; keys[r] = kv; token[r] = t0[k]; tokens[r] = n[k]; ends[r] = len[k];
-            at_u += u[k] * segs[k];
-            at_s += segs[k];
-            at_p += max(segs[k] > 0 ? 1 : 0, u[k] / KR_PIECE) * segs[k];
-        }
-        int U = at_u, S = at_s, P = at_p;
+        int at_u = -U, at_s = -S, at_p = -P;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int x = __shfl_up_sync(0xffffffffu, U, o), y = __shfl_up_sync(0xffffffffu, S, o), z = __shfl_up_sync(0xffffffffu, P, o);
             if (lane >= o) { U += x; S += y; P += z; }
         }
-        at_u = U - at_u; at_s = S - at_s; at_p = P - at_p;
+        at_u += U; at_s += S; at_p += P;
         U = __shfl_sync(0xffffffffu, U, 31); S = __shfl_sync(0xffffffffu, S, 31); P = __shfl_sync(0xffffffffu, P, 31);
         longest = __reduce_max_sync(0xffffffffu, longest);
         const bool whole = P > NB && S <= NB && 3ll * longest * NB <= 4ll * U;      // a block a segment is nearly even, and nothing is left to merge
         const bool by_piece = whole || P <= NB;
         if (whole) at_p = at_s;
-        if (lane <= NW) sh_x[lane] = 0;
         if (lane == 0) { sh_all[0] = U; sh_all[1] = S; sh_all[2] = by_piece; sh_all[3] = 1; pre_u[p.B] = U; pre_s[p.B] = S; }
-        __syncwarp();
-#pragma unroll
-        for (int k = 0; k < RL; ++k) {
-            const int r = r0 + k;
-            if (k >= per || r >= p.B) continue;
+#pragma unroll 1
+        for (int r = r0; r < r1; ++r) {
+            const int u = units[r], segs = pre_s[r], pc = whole ? 1 : max(1, u / KR_PIECE), in_r = j - at_p;
             pre_u[r] = at_u; pre_s[r] = at_s;
-            const int pc = whole ? 1 : max(1, u[k] / KR_PIECE), in_r = j - at_p;
-            if (by_piece && in_r >= 0 && in_r < pc * segs[k]) {      // the block's piece, dealt out over its warps
-                const int s = in_r / pc, piece = in_r - s * pc, c0 = at_u + s * u[k];
-                const int a = (int)((long long)u[k] * piece / pc), b = (int)((long long)u[k] * (piece + 1) / pc);
+            if (by_piece && in_r >= 0 && in_r < pc * segs) {      // the block's piece, dealt out over its warps
+                const int s = in_r / pc, piece = in_r - s * pc, a = (int)((long long)u * piece / pc), n = (int)((long long)u * (piece + 1) / pc) - a;
                 sh_all[3] = pc;
                 sh_mine = piece;
-                for (int w = 0; w < NW; ++w) { sh_x[w] = c0 + a + (b - a) * w / NW; sh_r[w] = r; sh_s[w] = s; }
-                sh_x[NW] = c0 + b;
+#pragma unroll 1
+                for (int w = 0; w <= NW; ++w) { sh_x[w] = at_u + s * u + a + n * w / NW; sh_r[w] = r; sh_s[w] = s; }
             }
-            at_u += u[k] * segs[k]; at_s += segs[k]; at_p += pc * segs[k];
+            at_u += u * segs; at_s += segs; at_p += pc * segs;
         }
         __syncwarp();
         if (!by_piece && lane <= NW) {
             // cut i = floor(V i / W) falls into a request (the last whose V-sum before it is no larger), there into a segment, there onto an edge or a unit; a cut a lane
             const int V = U + KR_HEAD * S, V_per = V / W, i = j * NW + lane;
-            if (i >= W) {
-                sh_x[lane] = U;
-            } else {
+            int x = U;
+            if (i < W) {
                 const int raw = i * V_per + (int)((unsigned)i * (unsigned)(V - V_per * W) / (unsigned)W);
                 int a = 0, b = p.B;
+#pragma unroll 1
                 while (b - a > 1) {
                     const int m = (a + b) >> 1;
                     if (pre_u[m] + KR_HEAD * pre_s[m] <= raw) a = m; else b = m;
@@ -209,14 +204,14 @@ __global__ void __launch_bounds__(NW * 32, 1) kv4_attn_runs_kernel(const Kv4Runs
                 const int un = units[a], in_r = raw - pre_u[a] - KR_HEAD * pre_s[a];      // (requests without segments lie ahead of one with the same sum)
                 int s = in_r / (un + KR_HEAD);
                 const int off = in_r - s * (un + KR_HEAD) - KR_HEAD, unit = off <= KR_SNAP ? 0 : un - off <= KR_SNAP ? un : off;
-                sh_x[lane] = pre_u[a] + s * un + unit;
-                if (lane < NW) { sh_r[lane] = a; sh_s[lane] = unit == un ? s + 1 : s; }      // a cut at the end: the run starts with the segment behind
+                x = pre_u[a] + s * un + unit;
+                sh_r[lane] = a;
+                sh_s[lane] = unit == un ? s + 1 : s;      // a cut at the end: the run starts with the segment behind
             }
+            sh_x[lane] = x;
         }
-    } else if (warp == NW - 1 && lane < 2 * NW) {
-        slot_seg[lane] = -1;
     }
-    static_assert(NW >= 2 && NW < 32, "a warp for the cut, a lane a cut");
+    static_assert(2 * NW <= 32, "a lane a cut, and later a part");
     __syncthreads();
 
     // ---- this warp's run of units [lo, hi) of the segments laid end to end, and the segment it starts in
@@ -373,6 +368,7 @@ __global__ void __launch_bounds__(NW * 32, 1) kv4_attn_runs_kernel(const Kv4Runs
 #pragma unroll
             for (int mt = 0; mt < D / 16; ++mt) o[mt][0] = o[mt][1] = o[mt][2] = o[mt][3] = 0.f;
             float m_c[2] = {-INFINITY, -INFINITY}, mu_c[2] = {0.f, 0.f}, l_c[2] = {0.f, 0.f}, z_c[2] = {0.f, 0.f};      // mu_c: the exponentials' reference (m_c, or 0 before a key)
+            float lim_c[2] = {-INFINITY, -INFINITY};      // how far above it a score may lie (a first key lies above any)
             float F = 0.f;                                // 0: no step seen yet
 
             for (; x < end; ++x) {
@@ -402,18 +398,17 @@ __global__ void __launch_bounds__(NW * 32, 1) kv4_attn_runs_kernel(const Kv4Runs
                     kr_lds2<128 * m + 64>(at_s + st, row_st[m][1].x, row_st[m][1].y);
                 });
 #pragma unroll
-                for (int m = 0; m < 2; ++m)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) s[m][h][e] = 0.f;
-#pragma unroll
                 for (int w = 0; w < QW; ++w)              // four chains side by side
 #pragma unroll
                     for (int m = 0; m < 2; ++m) {
                         const unsigned l = kl[m][w], u = kh[m][w], l8 = l >> 8, u8 = u >> 8;
-                        kr_mma(s[m][0], l & KR_LOW, u & KR_LOW, l & KR_HIGH, u & KR_HIGH, qf[w][0], qf[w][1]);
-                        kr_mma(s[m][1], l8 & KR_LOW, u8 & KR_LOW, l8 & KR_HIGH, u8 & KR_HIGH, qf[w][2], qf[w][3]);
+                        if (w == 0) {
+                            kr_mma0(s[m][0], l & KR_LOW, u & KR_LOW, l & KR_HIGH, u & KR_HIGH, qf[w][0], qf[w][1]);
+                            kr_mma0(s[m][1], l8 & KR_LOW, u8 & KR_LOW, l8 & KR_HIGH, u8 & KR_HIGH, qf[w][2], qf[w][3]);
+                        } else {
+                            kr_mma(s[m][0], l & KR_LOW, u & KR_LOW, l & KR_HIGH, u & KR_HIGH, qf[w][0], qf[w][1]);
+                            kr_mma(s[m][1], l8 & KR_LOW, u8 & KR_LOW, l8 & KR_HIGH, u8 & KR_HIGH, qf[w][2], qf[w][3]);
+                        }
                     }
 #pragma unroll
                 for (int m = 0; m < 2; ++m)
@@ -435,21 +430,25 @@ __global__ void __launch_bounds__(NW * 32, 1) kv4_attn_runs_kernel(const Kv4Runs
                             if (key >= seg.keys) row_st[m][e >> 1].y = 0u;      // (whatever lies behind the request's last key)
                         }
                 }
-                const float most_step = fmaxf(fmaxf(__uint_as_float(row_st[0][0].y << 16), __uint_as_float(row_st[0][1].y << 16)),
-                                              fmaxf(__uint_as_float(row_st[1][0].y << 16), __uint_as_float(row_st[1][1].y << 16)));
-                // how far the largest score lies above its reference (a first key lies above any)
-                float above[2];
+                float st_f[2][2];                         // values' steps times F
 #pragma unroll
-                for (int e = 0; e < 2; ++e) above[e] = fmaxf(fmaxf(v[0][e], v[0][e + 2]), fmaxf(v[1][e], v[1][e + 2]));
-                if (__any_sync(0xffffffffu, above[0] > (m_c[0] == -INFINITY ? -INFINITY : KR_LAZY) || above[1] > (m_c[1] == -INFINITY ? -INFINITY : KR_LAZY) ||
-                                                most_step * F > 64.f || F == 0.f)) {
-                    float alpha[2], down = 1.f;
-                    if (F == 0.f || __any_sync(0xffffffffu, most_step * F > 64.f)) {      // the largest step of the unit, to the power of two above it
-                        const unsigned bits = __reduce_max_sync(0xffffffffu, __float_as_uint(most_step));
-                        const float lim = fminf(fmaxf(__uint_as_float((bits + 0x007fffffu) & 0x7f800000u), 0x1p-100f), 0x1p127f), f = 64.f / lim;
-                        down = F == 0.f ? 1.f : f / F;
-                        F = f;
-                    }
+                for (int m = 0; m < 2; ++m)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) st_f[m][h] = __uint_as_float(row_st[m][h].y << 16) * F;
+                // how far the largest score lies above its reference, and the largest step
+                const float above[2] = {fmaxf(fmaxf(v[0][0], v[0][2]), fmaxf(v[1][0], v[1][2])), fmaxf(fmaxf(v[0][1], v[0][3]), fmaxf(v[1][1], v[1][3]))};
+                const float most_step = fmaxf(fmaxf(st_f[0][0], st_f[0][1]), fmaxf(st_f[1][0], st_f[1][1]));
+                if (__any_sync(0xffffffffu, above[0] > lim_c[0] || above[1] > lim_c[1] || most_step > 64.f)) {
+                    float alpha[2];
+                    // the largest step of the unit, to the power of two above it
+                    float step = 0.f;
+#pragma unroll
+                    for (int m = 0; m < 2; ++m)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) step = fmaxf(step, __uint_as_float(row_st[m][h].y << 16));
+                    const unsigned bits = __reduce_max_sync(0xffffffffu, __float_as_uint(step));
+                    const float f = 64.f / fminf(fmaxf(__uint_as_float((bits + 0x007fffffu) & 0x7f800000u), 0x1p-100f), 0x1p127f), down = F == 0.f || f >= F ? 1.f : f / F;
+                    if (F == 0.f || f < F) F = f;
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
                         float mx = above[e];
@@ -465,7 +464,12 @@ __global__ void __launch_bounds__(NW * 32, 1) kv4_attn_runs_kernel(const Kv4Runs
                         l_c[e] *= alpha[e];
                         z_c[e] *= alpha[e];
                         alpha[e] *= down;
+                        lim_c[e] = mn == -INFINITY ? -INFINITY : KR_LAZY;
                     }
+#pragma unroll
+                    for (int m = 0; m < 2; ++m)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) st_f[m][h] = __uint_as_float(row_st[m][h].y << 16) * F;
 #pragma unroll
                     for (int mt = 0; mt < D / 16; ++mt) {
                         o[mt][0] *= alpha[0]; o[mt][1] *= alpha[1];
@@ -478,11 +482,11 @@ __global__ void __launch_bounds__(NW * 32, 1) kv4_attn_runs_kernel(const Kv4Runs
                 for (int m = 0; m < 2; ++m)
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        const float st_f = __uint_as_float(row_st[m][h].y << 16) * F, base = __uint_as_float(row_st[m][h].y & 0xffff0000u);
+                        const float base = __uint_as_float(row_st[m][h].y & 0xffff0000u);
                         const float p0 = kr_exp2(v[m][2 * h]), p1 = kr_exp2(v[m][2 * h + 1]);
                         l_c[0] += p0;
                         l_c[1] += p1;
-                        unsigned w = kr_half2(p0 * st_f, p1 * st_f);
+                        unsigned w = kr_half2(p0 * st_f[m][h], p1 * st_f[m][h]);
                         if (edge) {                       // a key that a row does not see counts for nothing, whatever it holds
                             const bool h0 = hidden >> (4 * m + 2 * h) & 1u, h1 = hidden >> (4 * m + 2 * h + 1) & 1u;
                             if (!h0) z_c[0] = fmaf(p0, base, z_c[0]);
@@ -503,9 +507,9 @@ __global__ void __launch_bounds__(NW * 32, 1) kv4_attn_runs_kernel(const Kv4Runs
                         kr_ldsm_t<16 * m * ROW>((at_v ^ (32 * c2)) + st, a);
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            const unsigned a_lo = a[2 * h], a_hi = a[2 * h + 1], b_lo = a_lo >> 8, b_hi = a_hi >> 8;
-                            kr_mma(o[4 * c2 + 2 * h], a_lo & KR_LOW, a_lo & KR_HIGH, a_hi & KR_LOW, a_hi & KR_HIGH, pb[m][0], pb[m][1]);
-                            kr_mma(o[4 * c2 + 2 * h + 1], b_lo & KR_LOW, b_lo & KR_HIGH, b_hi & KR_LOW, b_hi & KR_HIGH, pb[m][0], pb[m][1]);
+                            const unsigned a_lo = a[2 * h], a_hi = a[2 * h + 1], b_lo = __byte_perm(a_lo, 0u, 0x4341), b_hi = __byte_perm(a_hi, 0u, 0x4341);
+                            kr_mma(o[4 * c2 + 2 * h], a_lo & KR_BYTE, a_lo & KR_HIGH, a_hi & KR_BYTE, a_hi & KR_HIGH, pb[m][0], pb[m][1]);
+                            kr_mma(o[4 * c2 + 2 * h + 1], b_lo, b_lo & KR_HIGH, b_hi, b_hi & KR_HIGH, pb[m][0], pb[m][1]);
                         }
                     });
                 });
@@ -514,8 +518,9 @@ __global__ void __launch_bounds__(NW * 32, 1) kv4_attn_runs_kernel(const Kv4Runs
             }
             // ---- the segment's result, or this warp's part of it
             const KrCursor now = seg;
-            if (end < hi) { ++seg.s; settle(seg); fetch_q(seg); }
             const float of = F > 0.f ? 16777216.f / F : 0.f, of16 = of * 0.0625f;
+#pragma unroll
+            for (int mt = 0; mt < D / 16; ++mt) { o[mt][0] -= o[mt][2]; o[mt][1] -= o[mt][3]; }      // (even elements come with 16 times the odd one behind them)
 #pragma unroll
             for (int e = 0; e < 2; ++e)
 #pragma unroll
@@ -551,7 +556,7 @@ __global__ void __launch_bounds__(NW * 32, 1) kv4_attn_runs_kernel(const Kv4Runs
                     for (int e = 0; e < 2; ++e) *reinterpret_cast<float2*>(slot_ml + ((2 * warp + slot) * 8 + 2 * t + e) * 2) = make_float2(m_c[e], l_c[e]);
                 if (lane == 0) slot_seg[2 * warp + slot] = pre_s[now.r] + now.s;
             }
-            if (end < hi) take_q(seg);
+            if (end < hi) { ++seg.s; settle(seg); fetch_q(seg); take_q(seg); }
         }
         kr_wait<0>();
     }
@@ -560,7 +565,6 @@ __global__ void __launch_bounds__(NW * 32, 1) kv4_attn_runs_kernel(const Kv4Runs
 
     // ---- the block's parts of segments, in the order of their keys: neighbours of one segment are a group, added in that order.  A lane knows a slot, and
     // the lane of a group's first slot its segment
-    static_assert(2 * NW <= 32, "a lane a slot");
     const int of_slot = lane < 2 * NW ? slot_seg[lane] : -1;
     const unsigned there = __ballot_sync(0xffffffffu, of_slot >= 0);
     if (there == 0) return;                               // (all warps see the same)
@@ -665,7 +669,7 @@ __global__ void __launch_bounds__(NW * 32, 1) kv4_attn_runs_kernel(const Kv4Runs
                 const float w = kr_exp2(ml.x - Mu);
                 L = fmaf(w, ml.y, L);
                 const int m = min(n - k0, 32);
-#pragma unroll 8
+#pragma unroll 4
                 for (int k = 0; k < m; ++k) {
                     const float f = __shfl_sync(0xffffffffu, w, k);
                     if (lane < COLS) {
@@ -684,15 +688,28 @@ __global__ void __launch_bounds__(NW * 32, 1) kv4_attn_runs_kernel(const Kv4Runs
 }
 
 #ifndef KR_WARPS
-#define KR_WARPS 12
-#define KR_STAGES 3
+#define KR_WARPS 16
+#define KR_STAGES 2
 #endif
 constexpr int KR_NW = KR_WARPS, KR_ST = KR_STAGES;
 
 // Requests with 1 .. max_q tokens; q_start null: request r has token r.  count: a word for every 8 rows of a request under a kv head, zero before and after.
-MSGL_API int msgl_kv4_attention_runs(const void* q, void* out, const void* k, const void* v, const void* steps, const int* q_start, const int* kv_len, const int* block_table,
-                                     long long bt_stride, int bt_width, float* part_o, float* part_ml, int* count, int blocks, int B, int T, int n_q, int n_kv, int d,
-                                     int page_size, int pages, int window, int max_q, float scale, cudaStream_t stream) {
+struct Kv4RunsArgs {
+    long long q, out, k, v, steps, q_start, kv_len, block_table, bt_stride, bt_width, part_o, part_ml, count, blocks, B, T, n_q, n_kv, d, page_size, pages, window, max_q, stream;
+    double scale;
+};
+
+MSGL_API int msgl_kv4_attention_runs(const Kv4RunsArgs* x) {
+    const void *q = (const void*)x->q, *k = (const void*)x->k, *v = (const void*)x->v, *steps = (const void*)x->steps;
+    void* out = (void*)x->out;
+    const int *q_start = (const int*)x->q_start, *kv_len = (const int*)x->kv_len, *block_table = (const int*)x->block_table;
+    float *part_o = (float*)x->part_o, *part_ml = (float*)x->part_ml;
+    int* count = (int*)x->count;
+    const long long bt_stride = x->bt_stride;
+    const int bt_width = (int)x->bt_width, blocks = (int)x->blocks, B = (int)x->B, T = (int)x->T, n_q = (int)x->n_q, n_kv = (int)x->n_kv, d = (int)x->d, page_size = (int)x->page_size,
+              pages = (int)x->pages, window = (int)x->window, max_q = (int)x->max_q;
+    const float scale = (float)x->scale;
+    cudaStream_t stream = (cudaStream_t)x->stream;
     if (B <= 0 || T <= 0) return MSGL_OK;
     if ((d != 64 && d != 128) || B > KR_MAX_B || n_kv < 1 || n_q < 1 || n_q % n_kv || page_size < 1 || pages < 1 || bt_width < 1 || max_q < 1 || blocks < 1 || blocks > 4096 ||
         (long long)bt_width * page_size > 0x3fffffffLL || (long long)pages * n_kv * page_size >= 0xffffffffLL || part_o == nullptr || part_ml == nullptr || count == nullptr)

@@ -20,6 +20,7 @@ import ctypes
 import math
 import operator
 import os
+import struct
 from typing import NamedTuple, Optional, Sequence, Tuple
 
 import torch
@@ -2707,18 +2708,20 @@ KV4_DIRECT_ROWS = 32              # (token, query head) rows of a request under 
 _KV4_REQUESTS = 256               # requests of one launch that deals the keys out
 KV4_RESTORE_BYTES = 1 << 30       # of restored keys and values, what a step makes at a time
 _kv4 = None
+_sms = {}                        # SMs of the devices, by number
 
 
 def _kv4_lib():
     global _kv4
     if _kv4 is None:
         lib = _build.kv4_library()
-        lib.msgl_kv4_append.argtypes = [c_void_p, c_ll] + [c_void_p] * 4 + [c_int, c_float, c_void_p, c_int, c_int, c_int] + [c_void_p] * 4 + [c_ll] + [c_int] * 6 + [c_void_p]
-        lib.msgl_kv4_restore.argtypes = [c_void_p] * 6 + [c_int] + [c_void_p] * 3 + [c_ll, c_int, c_void_p] + [c_int] * 9 + [c_void_p]
-        lib.msgl_kv4_attention_runs.argtypes = [c_void_p] * 8 + [c_ll, c_int] + [c_void_p] * 3 + [c_int] * 10 + [c_float, c_void_p]
-        lib.msgl_kv4_attention_any.argtypes = [c_void_p] * 8 + [c_ll, c_int, c_void_p] + [c_int] * 10 + [c_float, c_int, c_void_p]
+        lib.msgl_kv4_append.argtypes = lib.msgl_kv4_restore.argtypes = lib.msgl_kv4_attention_any.argtypes = lib.msgl_kv4_attention_runs.argtypes = [ctypes.c_char_p]
         _kv4 = lib
     return _kv4
+
+
+# The entry points take their arguments packed in one piece, 8 bytes each (ctypes takes 3 us to convert 25 of them one by one, which small steps wait for).
+_KV4_APPEND, _KV4_RESTORE, _KV4_ANY, _KV4_RUNS = (struct.Struct(f).pack for f in ("23qd", "23q", "23qd", "24qd"))
 
 
 class KV4Cache(NamedTuple):
@@ -2765,6 +2768,46 @@ def qknorm_rope_kv4write(qkv: torch.Tensor, positions: torch.Tensor, n_q: int, n
     are given), rotation from `rope_table` [max_pos, rot] float32 = cos | sin (if given), the rotated k and v put into 4 bits at token slots `out_loc` (int32; a
     slot outside the cache is left out), q returned as [T, n_q, d] in qkv's type.  Keys are coded from their float32 values, before any rounding to
     qkv's type.  Two tokens with one slot leave one of the two rows or parts of both.  A row with a NaN or an infinity, or wider than bfloat16 reaches, stands for NaN."""
+    (k, v, steps), dt, dev = cache, qkv.dtype, qkv.get_device()
+    shape, rot, max_pos = k.shape, 0, 0
+    # every argument is looked at in one go, and told apart only where something is wrong: small steps wait for the host
+    ok = (len(shape) == 4 and shape[1] == n_kv >= 1 and 2 * shape[3] == d and d % 8 == 0 and 8 <= d <= KV4_MAX_HEAD_DIM and n_q >= 1 and shape[0] >= 1 and shape[2] >= 1
+          and k.dtype is v.dtype is torch.uint8 and v.shape == shape and steps.dtype is torch.bfloat16 and steps.shape == (*shape[:3], 4)
+          and k.is_contiguous() and v.is_contiguous() and steps.is_contiguous() and shape[0] * shape[2] <= 0x7fffffff
+          and dt in _DT and qkv.dim() == 2 and qkv.shape[1] == (n_q + 2 * n_kv) * d and qkv.stride(1) == 1
+          and positions.dtype is torch.int32 and positions.numel() == qkv.shape[0] and positions.is_contiguous()
+          and out_loc.dtype is torch.int32 and out_loc.numel() == qkv.shape[0] and out_loc.is_contiguous()
+          and (q_weight is None) == (k_weight is None) and k.get_device() == v.get_device() == steps.get_device() == positions.get_device() == out_loc.get_device() == dev >= 0
+          and dev == torch._C._cuda_getDevice())
+    if ok and q_weight is not None:
+        ok = (q_weight.dtype is k_weight.dtype and q_weight.dtype in _DT and q_weight.numel() == k_weight.numel() == d and q_weight.is_contiguous() and k_weight.is_contiguous()
+              and q_weight.get_device() == k_weight.get_device() == dev)
+    if ok and rope_table is not None:
+        ok = rope_table.dtype is torch.float32 and rope_table.dim() == 2 and rope_table.is_contiguous() and rope_table.get_device() == dev
+        if ok:
+            max_pos, rot = rope_table.shape
+            ok = max_pos >= 1 and 2 <= rot <= d and rot % 2 == 0
+    if ok and q_out is not None:
+        ok = q_out.dtype is dt and q_out.shape == (qkv.shape[0], n_q, d) and q_out.is_contiguous() and q_out.get_device() == dev
+    if not ok:
+        _refuse_kv4write(qkv, positions, n_q, n_kv, d, q_weight, k_weight, rope_table, out_loc, cache, q_out)
+    T = qkv.shape[0]
+    if q_out is None:
+        q_out = qkv.new_empty((T, n_q, d))
+    if T == 0:
+        return q_out
+    code = _kv4_lib().msgl_kv4_append(_KV4_APPEND(
+        qkv.data_ptr(), qkv.stride(0), positions.data_ptr(), out_loc.data_ptr(), 0 if q_weight is None else q_weight.data_ptr(), 0 if k_weight is None else k_weight.data_ptr(),
+        q_weight is not None and q_weight.dtype is torch.float32, 0 if rope_table is None else rope_table.data_ptr(), rot, max_pos, bool(interleaved), q_out.data_ptr(),
+        k.data_ptr(), v.data_ptr(), steps.data_ptr(), shape[0] * shape[2], shape[2], n_q, n_kv, d, T, _DT[dt], _stream(), eps))
+    if code:
+        _check(code, f"qknorm_rope_kv4write (head size {d})")
+    _count_launch()
+    return q_out
+
+
+def _refuse_kv4write(qkv, positions, n_q, n_kv, d, q_weight, k_weight, rope_table, out_loc, cache, q_out) -> None:
+    """What is wrong with the arguments of qknorm_rope_kv4write."""
     what = "qknorm_rope_kv4write"
     pages, heads, page_size, size = _kv4_sizes(what, cache)
     if qkv.dim() != 2 or qkv.dtype not in _DT or qkv.shape[1] != (n_q + 2 * n_kv) * d or qkv.stride(1) != 1 or n_q < 1:
@@ -2779,43 +2822,46 @@ def qknorm_rope_kv4write(qkv: torch.Tensor, positions: torch.Tensor, n_q: int, n
     if q_weight is not None and not (q_weight.dtype == k_weight.dtype and q_weight.dtype in _DT and q_weight.numel() == k_weight.numel() == d
                                      and q_weight.is_contiguous() and k_weight.is_contiguous()):
         raise KernelError(f"{what}: norm weights are {d} float32 or bfloat16 elements each, of one type")
-    rot = max_pos = 0
-    if rope_table is not None:
-        if rope_table.dtype != torch.float32 or rope_table.dim() != 2 or not rope_table.is_contiguous() or rope_table.shape[0] < 1 or not 2 <= rope_table.shape[1] <= d \
-                or rope_table.shape[1] % 2:
-            raise KernelError(f"{what}: rope_table is contiguous float32 [positions, rotated elements], an even number of them up to {d}; got {rope_table.dtype} {tuple(rope_table.shape)}")
-        max_pos, rot = rope_table.shape
-    if q_out is None:
-        q_out = torch.empty((T, n_q, d), dtype=qkv.dtype, device=qkv.device)
-    elif q_out.dtype != qkv.dtype or tuple(q_out.shape) != (T, n_q, d) or not q_out.is_contiguous():
+    if rope_table is not None and (rope_table.dtype != torch.float32 or rope_table.dim() != 2 or not rope_table.is_contiguous() or rope_table.shape[0] < 1
+                                   or not 2 <= rope_table.shape[1] <= d or rope_table.shape[1] % 2):
+        raise KernelError(f"{what}: rope_table is contiguous float32 [positions, rotated elements], an even number of them up to {d}; got {rope_table.dtype} {tuple(rope_table.shape)}")
+    if q_out is not None and (q_out.dtype != qkv.dtype or tuple(q_out.shape) != (T, n_q, d) or not q_out.is_contiguous()):
         raise KernelError(f"{what}: q_out is contiguous [{T}, {n_q}, {d}] of qkv's type; got {q_out.dtype} {tuple(q_out.shape)}")
     _same_device(what, qkv, positions, out_loc, *cache, q_weight, k_weight, rope_table, q_out)
-    if T == 0:
-        return q_out
-    code = _kv4_lib().msgl_kv4_append(qkv.data_ptr(), qkv.stride(0), positions.data_ptr(), out_loc.data_ptr(), _ptr(q_weight), _ptr(k_weight),
-                                      int(q_weight is not None and q_weight.dtype == torch.float32), float(eps), _ptr(rope_table), rot, max_pos, int(bool(interleaved)),
-                                      q_out.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), cache.steps.data_ptr(), pages * page_size, page_size, n_q, n_kv, d, T,
-                                      _DT[qkv.dtype], _stream())
-    _check(code, f"{what} (head size {d})")
-    return q_out
+    raise KernelError(f"{what}: arguments that do not go together")
+
+
+def _count_launch() -> None:
+    global LAUNCHES
+    LAUNCHES += 1
 
 
 def kv4_restore(cache: KV4Cache, pages: torch.Tensor, dtype: torch.dtype) -> Tuple[torch.Tensor, torch.Tensor]:
     """What the pages of a cache in 4 bits stand for: keys and values [len(pages), kv heads, page size, head size] as float32 or bfloat16 (rounded once).  pages:
     int32; a number outside the cache reads as zeros."""
-    what = "kv4_restore"
-    n_pages, n_kv, page_size, d = _kv4_sizes(what, cache)
-    if dtype not in _DT:
-        raise KernelError(f"{what}: results are float32 or bfloat16; got {dtype}")
-    _index(what, "pages", pages)
-    _same_device(what, *cache, pages)
-    n = pages.numel()
-    out = torch.empty((2, n, n_kv, page_size, d), dtype=dtype, device=pages.device)
+    (k, v, steps), dev = cache, pages.get_device()
+    shape = k.shape
+    if not (len(shape) == 4 and shape[0] >= 1 and shape[1] >= 1 and shape[2] >= 1 and shape[3] % 4 == 0 and 4 <= shape[3] <= KV4_MAX_HEAD_DIM // 2
+            and k.dtype is v.dtype is torch.uint8 and v.shape == shape and steps.dtype is torch.bfloat16 and steps.shape == (*shape[:3], 4)
+            and k.is_contiguous() and v.is_contiguous() and steps.is_contiguous() and shape[0] * shape[2] <= 0x7fffffff
+            and dtype in _DT and pages.dtype is torch.int32 and pages.is_contiguous()
+            and k.get_device() == v.get_device() == steps.get_device() == dev >= 0 and dev == torch._C._cuda_getDevice()):
+        what = "kv4_restore"
+        _kv4_sizes(what, cache)
+        if dtype not in _DT:
+            raise KernelError(f"{what}: results are float32 or bfloat16; got {dtype}")
+        _index(what, "pages", pages)
+        _same_device(what, *cache, pages)
+        raise KernelError(f"{what}: arguments that do not go together")
+    n, d = pages.numel(), 2 * shape[3]
+    keys, values = pages.new_empty((2, n, shape[1], shape[2], d), dtype=dtype).unbind(0)
     if n:
-        code = _kv4_lib().msgl_kv4_restore(cache.k.data_ptr(), cache.v.data_ptr(), cache.steps.data_ptr(), out[0].data_ptr(), out[1].data_ptr(), pages.data_ptr(), n, None, None,
-                                           None, 0, 0, None, 0, 0, 0, 0, n_kv, page_size, n_pages, d, _DT[dtype], _stream())
-        _check(code, what)
-    return out[0], out[1]
+        code = _kv4_lib().msgl_kv4_restore(_KV4_RESTORE(k.data_ptr(), v.data_ptr(), steps.data_ptr(), keys.data_ptr(), values.data_ptr(), pages.data_ptr(), n, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0,
+                                                        shape[1], shape[2], shape[0], d, _DT[dtype], _stream()))
+        if code:
+            _check(code, "kv4_restore")
+        _count_launch()
+    return keys, values
 
 
 def kv4_attention(q: torch.Tensor, out: torch.Tensor, cache: KV4Cache, *, kv_len: torch.Tensor, block_table: torch.Tensor, scale: float, window: int = 0,
@@ -2828,6 +2874,46 @@ def kv4_attention(q: torch.Tensor, out: torch.Tensor, cache: KV4Cache, *, kv_len
 
     Requests with few tokens read the codes themselves; for longer runs the keys and values that they see are first put back into q's type, once a call, in scratch
     memory of up to KV4_RESTORE_BYTES (more only where one request needs it).  workspace: where scratch memory is kept between calls (`parts.Workspace`); calls that share one run one after the other."""
+    (k, v, steps), dt, dev = cache, q.dtype, q.get_device()
+    shape, i32 = k.shape, torch.int32
+    # every argument is looked at in one go, and told apart only where something is wrong: small steps wait for the host
+    ok = (len(shape) == 4 and shape[0] >= 1 and shape[1] >= 1 and shape[2] >= 1 and shape[3] % 4 == 0 and 4 <= shape[3] <= KV4_MAX_HEAD_DIM // 2
+          and k.dtype is v.dtype is torch.uint8 and v.shape == shape and steps.dtype is torch.bfloat16 and steps.shape == (*shape[:3], 4)
+          and k.is_contiguous() and v.is_contiguous() and steps.is_contiguous() and shape[0] * shape[2] <= 0x7fffffff
+          and q.dim() == 3 and dt in _DT and out.dtype is dt and out.shape == q.shape and q.is_contiguous() and out.is_contiguous()
+          and q.shape[2] == 2 * shape[3] and q.shape[1] >= 1 and q.shape[1] % shape[1] == 0 and 0.0 < scale < math.inf and 0 <= window <= 0x3fffffff
+          and block_table.dtype is i32 and block_table.dim() == 2 and block_table.shape[1] >= 1 and block_table.stride(1) == 1
+          and (block_table.stride(0) >> 31 == 0 or block_table.shape[0] == 1) and block_table.shape[1] * shape[2] <= 0x3fffffff
+          and kv_len.dtype is i32 and kv_len.numel() == block_table.shape[0] and kv_len.is_contiguous()
+          and k.get_device() == v.get_device() == steps.get_device() == out.get_device() == kv_len.get_device() == block_table.get_device() == dev >= 0
+          and dev == torch._C._cuda_getDevice())
+    B, few, most = block_table.shape[0] if ok else 0, 1, 0
+    direct = max(1, KV4_DIRECT_ROWS * shape[1] // q.shape[1]) if ok else 1          # most tokens of a request that reads the codes directly
+    if ok and q_lens is None:
+        ok = q.shape[0] == B
+    elif ok:
+        ok = (kv_lens is not None and q_start is not None and len(q_lens) == len(kv_lens) == B and q_start.dtype is i32 and q_start.numel() == B + 1
+              and q_start.is_contiguous() and q_start.get_device() == dev)
+        if ok and B:
+            few, most, places = 0, max(q_lens), block_table.shape[1] * shape[2]
+            ok = min(q_lens) >= 0 and sum(q_lens) <= q.shape[0] and max(kv_lens) <= places and all(map(operator.le, q_lens, kv_lens))
+            if most <= direct:
+                few = most
+            elif ok:
+                few = max((n for n in q_lens if n <= direct), default=0)
+    if not ok:
+        _refuse_kv4_attention(q, out, cache, kv_len, block_table, scale, window, q_start, q_lens, kv_lens)
+    if q.shape[0] == 0 or B == 0:
+        return
+    if few:
+        _kv4_few(q, out, cache, kv_len, block_table, scale, window, q_start if q_lens is not None else None, few,
+                 None if q_lens is None else max(kv for n, kv in zip(q_lens, kv_lens) if 0 < n <= direct), workspace)
+    if most > direct:
+        _kv4_portions(q, out, cache, kv_len, block_table, scale, window, q_start, q_lens, kv_lens, direct + 1, workspace)
+
+
+def _refuse_kv4_attention(q, out, cache, kv_len, block_table, scale, window, q_start, q_lens, kv_lens) -> None:
+    """What is wrong with the arguments of kv4_attention."""
     what = "kv4_attention"
     pages, n_kv, page_size, d = _kv4_sizes(what, cache)
     if q.dim() != 3 or q.dtype not in _DT or out.dtype != q.dtype or out.shape != q.shape or not q.is_contiguous() or not out.is_contiguous():
@@ -2855,47 +2941,46 @@ def kv4_attention(q: torch.Tensor, out: torch.Tensor, cache: KV4Cache, *, kv_len
             raise KernelError(f"{what}: {sum(q_lens)} tokens of all requests, and q has {T}")
         if any(kv < n or kv > block_table.shape[1] * page_size for n, kv in zip(q_lens, kv_lens)):
             raise KernelError(f"{what}: a request has as many tokens in the cache as it brings, and its block table holds them")
-    _same_device(what, q, out, *cache, kv_len, block_table, q_start)
-    if T == 0 or B == 0:
-        return
-    G = n_q // n_kv
-    direct = max(1, KV4_DIRECT_ROWS // G)          # most tokens of a request that reads the codes directly
-    few = 1 if q_lens is None else max((n for n in q_lens if n <= direct), default=0)
-    if few:
-        longest = block_table.shape[1] * page_size if q_lens is None else max(kv for n, kv in zip(q_lens, kv_lens) if 0 < n <= direct)
-        _kv4_few(q, out, cache, kv_len, block_table, scale, window, q_start if q_lens is not None else None, few, longest, workspace)
-    if q_lens is not None and max(q_lens) > direct:
-        _kv4_portions(q, out, cache, kv_len, block_table, scale, window, q_start, q_lens, kv_lens, direct + 1, workspace)
+    _same_device(what, q, out, *cache, kv_len, block_table, q_start if q_lens is not None else None)
+    raise KernelError(f"{what}: arguments that do not go together")
 
 
 def _kv4_few(q, out, cache, kv_len, block_table, scale, window, q_start, max_q, longest, workspace) -> None:
-    """The requests with 1 to max_q tokens, from the codes; `longest` bounds their keys."""
+    """The requests with 1 to max_q tokens, from the codes; `longest` bounds their keys (None: the block table does)."""
     (T, n_q, d), (pages, n_kv, page_size, _), (B, width) = q.shape, cache.k.shape, block_table.shape
-    lib, G = _kv4_lib(), n_q // n_kv
-    at_k, at_v, at_steps, at_q, at_out = cache.k.data_ptr(), cache.v.data_ptr(), cache.steps.data_ptr(), q.data_ptr(), out.data_ptr()
+    lib, G, dev = _kv4_lib(), n_q // n_kv, q.get_device()
+    sms = _sms.get(dev) or _sms.setdefault(dev, sm_count(q.device))
+    at_k, at_v, at_steps, at_q, at_out, at_kv, at_table, row = (cache.k.data_ptr(), cache.v.data_ptr(), cache.steps.data_ptr(), q.data_ptr(), out.data_ptr(), kv_len.data_ptr(),
+                                                                block_table.data_ptr(), block_table.stride(0))
+    at_start = 0 if q_start is None else q_start.data_ptr()
     tiles = -(-max_q * G // 8)
-    if q.dtype == torch.bfloat16 and d in (64, 128) and pages * n_kv * page_size < 0xffffffff and not (at_q | at_out | at_k | at_v | at_steps) & 15 \
+    if q.dtype is torch.bfloat16 and (d == 128 or d == 64) and pages * n_kv * page_size < 0xffffffff and not (at_q | at_out | at_k | at_v | at_steps) & 15 \
             and min(B, _KV4_REQUESTS) * n_kv * tiles * (width * page_size // 32 + 5) < 1 << 31:
-        blocks = sm_count(q.device)
-        words = (min(_KV4_REQUESTS * max_q, T) * G // 8 + _KV4_REQUESTS) * n_kv          # segments of a launch at most
-        count = workspace.counters("kv4_count", words) if workspace is not None else None
-        if count is None:
-            count = torch.zeros(words, dtype=torch.int32, device=q.device)
-        n = 2 * 8 * blocks
-        part = workspace.whole("kv4_part", n * (d + 2), torch.float32) if workspace is not None else torch.empty(n * (d + 2), dtype=torch.float32, device=q.device)
+        # partial results of two segments a block, and behind them counters, one a segment and zero between launches, in one buffer that is laid out alike for both head sizes
+        n_part = 2 * 8 * sms
+        words = n_part * 130 + _KV4_REQUESTS * tiles * n_kv
+        scratch = workspace.counters("kv4_few", words) if workspace is not None else None
+        if scratch is None:          # (inside a stream capture the zeros are written by every replay)
+            scratch = torch.zeros(words, dtype=torch.int32, device=q.device)
+        at = scratch.data_ptr()
         for a in range(0, B, _KV4_REQUESTS):
-            b, row = min(B, a + _KV4_REQUESTS), 0 if q_start is not None else a          # (without q_start token r is request r's)
-            code = lib.msgl_kv4_attention_runs(at_q + row * n_q * d * 2, at_out + row * n_q * d * 2, at_k, at_v, at_steps, None if q_start is None else q_start.data_ptr() + 4 * a,
-                                               kv_len.data_ptr() + 4 * a, block_table.data_ptr() + 4 * a * block_table.stride(0), block_table.stride(0), width, part.data_ptr(),
-                                               part.data_ptr() + 4 * n * d, count.data_ptr(), blocks, b - a, T - row, n_q, n_kv, d, page_size, pages, window, max_q, scale, _stream())
-            _check(code, "kv4_attention")
+            first = 0 if q_start is not None else a          # (without q_start token r is request r's)
+            code = lib.msgl_kv4_attention_runs(_KV4_RUNS(
+                at_q + first * n_q * d * 2, at_out + first * n_q * d * 2, at_k, at_v, at_steps, at_start + 4 * a if at_start else 0, at_kv + 4 * a, at_table + 4 * a * row, row, width,
+                at, at + 4 * n_part * 128, at + 4 * n_part * 130, sms, min(B - a, _KV4_REQUESTS), T - first, n_q, n_kv, d, page_size, pages, window, max_q, _stream(), scale))
+            if code:
+                _check(code, "kv4_attention")
+            _count_launch()
         return
     tiles *= B * n_kv
-    splits = max(1, min(4 * sm_count(q.device) // tiles, (min(longest, window + 8) if window else longest) // 128, 64))
+    keys = width * page_size if longest is None else longest
+    splits = max(1, min(4 * sms // tiles, (min(keys, window + 8) if window else keys) // 128, 64))
     part = torch.empty(splits * T * n_q * (d + 2), dtype=torch.float32, device=q.device) if splits > 1 else None
-    code = lib.msgl_kv4_attention_any(at_q, at_out, at_k, at_v, at_steps, _ptr(q_start), kv_len.data_ptr(), block_table.data_ptr(), block_table.stride(0), width, _ptr(part),
-                                      splits, B, T, n_q, n_kv, d, page_size, pages, window, max_q, scale, _DT[q.dtype], _stream())
+    code = lib.msgl_kv4_attention_any(_KV4_ANY(at_q, at_out, at_k, at_v, at_steps, at_start, at_kv, at_table, row, width, 0 if part is None else part.data_ptr(), splits, B, T, n_q, n_kv, d,
+                                               page_size, pages, window, max_q, _DT[q.dtype], _stream(), scale))
     _check(code, "kv4_attention")
+    if splits > 1:
+        _count_launch()
 
 
 def _kv4_portions(q, out, cache, kv_len, block_table, scale, window, q_start, q_lens, kv_lens, min_q, workspace) -> None:
@@ -2917,9 +3002,9 @@ def _kv4_portions(q, out, cache, kv_len, block_table, scale, window, q_start, q_
             sizes = (("kv4_keys", n * page_numel, q.dtype), ("kv4_values", n * page_numel, q.dtype), ("kv4_table", (b - a) * t_width, torch.int32))
             k, v, table = (torch.empty(m, dtype=t, device=q.device) if workspace is None else workspace.get(name, m, t) for name, m, t in sizes)
             lens, kvs, starts, kv_part = q_lens[a:b], kv_lens[a:b], q_start[a:b + 1], kv_len[a:b]
-            code = lib.msgl_kv4_restore(cache.k.data_ptr(), cache.v.data_ptr(), cache.steps.data_ptr(), k.data_ptr(), v.data_ptr(), None, n, starts.data_ptr(),
-                                        kv_part.data_ptr(), block_table[a:b].data_ptr(), block_table.stride(0), width, table.data_ptr(), t_width, b - a, window, min_q, n_kv,
-                                        page_size, pages, d, _DT[q.dtype], _stream())
+            code = lib.msgl_kv4_restore(_KV4_RESTORE(cache.k.data_ptr(), cache.v.data_ptr(), cache.steps.data_ptr(), k.data_ptr(), v.data_ptr(), 0, n, starts.data_ptr(),
+                                                     kv_part.data_ptr(), block_table[a:b].data_ptr(), block_table.stride(0), width, table.data_ptr(), t_width, b - a, window, min_q,
+                                                     n_kv, page_size, pages, d, _DT[q.dtype], _stream()))
             _check(code, "kv4_attention (keys restored)")
             k, v, table = k.view(n, n_kv, per, d), v.view(n, n_kv, per, d), table.view(b - a, t_width)
             common = dict(q_start=starts, kv_len=kv_part, block_table=table, n_kv=n_kv, page_size=per, window=window, scale=scale, qlen_min=min_q, qlen_max=big)
