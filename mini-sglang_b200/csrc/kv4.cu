@@ -25,9 +25,20 @@ __device__ __forceinline__ float bf16_of(unsigned short b) { return __uint_as_fl
 // min and max that keep a NaN
 __device__ __forceinline__ float min_nan(float a, float b) { float r; asm("min.NaN.f32 %0, %1, %2;\n" : "=f"(r) : "f"(a), "f"(b)); return r; }
 __device__ __forceinline__ float max_nan(float a, float b) { float r; asm("max.NaN.f32 %0, %1, %2;\n" : "=f"(r) : "f"(a), "f"(b)); return r; }
+__device__ __forceinline__ float min_nan(float a, float b, float c) { float r; asm("min.NaN.f32 %0, %1, %2, %3;\n" : "=f"(r) : "f"(a), "f"(b), "f"(c)); return r; }
+__device__ __forceinline__ float max_nan(float a, float b, float c) { float r; asm("max.NaN.f32 %0, %1, %2, %3;\n" : "=f"(r) : "f"(a), "f"(b), "f"(c)); return r; }
+
+// pairs of floats in the packed instructions of sm_100 (a product and a sum of it may become one operation, so what has to be rounded apart is not written with these)
+typedef unsigned long long F2;
+__device__ __forceinline__ F2 f2(float a, float b) { F2 r; asm("mov.b64 %0, {%1, %2};\n" : "=l"(r) : "f"(a), "f"(b)); return r; }
+__device__ __forceinline__ F2 f2(float a) { return f2(a, a); }
+__device__ __forceinline__ void f2_get(F2 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;\n" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ F2 f2_mul(F2 a, F2 b) { F2 r; asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b)); return r; }
+__device__ __forceinline__ F2 f2_add(F2 a, F2 b) { F2 r; asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b)); return r; }
+__device__ __forceinline__ F2 f2_fma(F2 a, F2 b, F2 c) { F2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
 
 struct Kv4Scale {
-    float base, step;
+    float base, step, inv;
     unsigned bits;                  // step in the low half, base in the high one, as they are kept
     __device__ __forceinline__ Kv4Scale(float lo, float hi) {
         __nv_bfloat16 b = __float2bfloat16_rn(lo), s = __float2bfloat16_rn(__fmul_rn(__fsub_rn(hi, __bfloat162float(b)), 1.f / 15.f));
@@ -35,12 +46,27 @@ struct Kv4Scale {
         step = __bfloat162float(s);
         if (!(fabsf(base) <= FLT_MAX) || !(fabsf(step) <= FLT_MAX)) { base = CUDART_NAN_F; step = 0.f; }
         else if (!(step >= 0x1p-100f)) step = 0.f;
+        inv = step > 0.f ? __fdiv_rn(1.f, step) : 0.f;
         bits = (unsigned)__bfloat16_as_ushort(__float2bfloat16_rn(step)) | ((unsigned)__bfloat16_as_ushort(__float2bfloat16_rn(base)) << 16);
     }
-    // the division is correctly rounded: an element half way between two codes takes the even one whoever computes it
-    __device__ __forceinline__ unsigned code(float x) const {
+    // The codes of eight elements as one word.  A code is the whole number next to the quotient (x - base) / step, an even one where that lies half way between two, so the
+    // quotient has to be right to its last bit there: c = rint(y) of y = (x - base) inv leaves the exact remainder r = (x - base) - c step, and c + r inv is the quotient rounded
+    // once (but for one in 2^24 of those next to a half, either of whose codes is as near).  Adding 1.5 2^23 rounds to whole numbers and leaves them in the low bits.
+    __device__ __forceinline__ unsigned codes(const F2 (&x)[4]) const {
+        const F2 whole = f2(12582912.f), minus = f2(-12582912.f), nb = f2(-base), ns = f2(-step), iv = f2(inv);
+        unsigned word = 0;
         if (!(step > 0.f)) return 0u;
-        return (unsigned)fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x, base), step)), 0.f), 15.f);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const F2 d = f2_add(x[i], nb), c = f2_add(f2_add(f2_mul(d, iv), whole), minus), q = f2_fma(f2_fma(c, ns, d), iv, c);
+            float a, b;
+            f2_get(q, a, b);
+            a = fminf(fmaxf(a, 0.f), 15.f);
+            b = fminf(fmaxf(b, 0.f), 15.f);
+            f2_get(f2_add(f2(a, b), whole), a, b);
+            word += ((__float_as_uint(a) - 0x4b400000u) << (8 * i)) + ((__float_as_uint(b) - 0x4b400000u) << (8 * i + 4));
+        }
+        return word;
     }
 };
 
@@ -60,8 +86,7 @@ struct Kv4Append {
     unsigned char* k; unsigned char* v; unsigned* steps;  // steps: two words a row, keys' and values'
     long long slots;                                      // of the cache: page numbers beyond are left out
     int page_size, n_q, n_kv, d, T;
-    __device__ __forceinline__ long long row_of(int t, int kvh) const {      // -1: nowhere
-        const int slot = out_loc[t];
+    __device__ __forceinline__ long long row_of_slot(int slot, int kvh) const {      // -1: nowhere
         if (slot < 0 || slot >= slots) return -1;
         const int page = slot / page_size;
         return ((long long)page * n_kv + kvh) * page_size + (slot - page * page_size);
@@ -131,110 +156,157 @@ __global__ void kv4_append_kernel(const Kv4Append p) {
         hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
     }
     const Kv4Scale sc(lo, hi);
-    const long long row = p.row_of(t, is_k ? head - p.n_q : head - p.n_q - p.n_kv);
+    const long long row = p.row_of_slot(p.out_loc[t], is_k ? head - p.n_q : head - p.n_q - p.n_kv);
     if (row < 0) return;
     unsigned* dst = reinterpret_cast<unsigned*>((is_k ? p.k : p.v) + row * (d >> 1));
 #pragma unroll
     for (int j = 0; j < KV4_MAX_D / 256; ++j) {
         const int w = lane + 32 * j;
         if (8 * w >= d) continue;
-        unsigned word = 0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) word |= sc.code(x[j][e]) << (4 * e);
-        dst[w] = word;
+        const F2 y[4] = {f2(x[j][0], x[j][1]), f2(x[j][2], x[j][3]), f2(x[j][4], x[j][5]), f2(x[j][6], x[j][7])};
+        dst[w] = sc.codes(y);
     }
     if (lane == 0) p.steps[2 * row + (is_k ? 0 : 1)] = sc.bits;
 }
 
 // Head sizes 32, 64, 128, 256 whose rotation (if any) covers the whole head in halves: L = d / 16 lanes own one head of a token, a lane eight
 // elements of the lower half and the eight that they are rotated with, so that every copy is 16 bytes, every word of codes one lane's, and only the sum
-// and the extremes take shuffles.
-constexpr int KV4_APPEND_THREADS = 256;
+// and the extremes take shuffles.  All that a lane reads is asked for before it works on any of it.
+constexpr int KV4_APPEND_THREADS = 128;
+__device__ __forceinline__ void kv4_weights(const void* w, int at, int f32, F2 (&out)[4]) {      // eight of them, 16 bytes a load
+    if (f32) {
+        const ulonglong2* p = reinterpret_cast<const ulonglong2*>(reinterpret_cast<const float*>(w) + at);
+        const ulonglong2 a = p[0], b = p[1];
+        out[0] = a.x; out[1] = a.y; out[2] = b.x; out[3] = b.y;
+    } else {
+        const uint4 a = *reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(w) + at);
+        const unsigned y[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) out[i] = f2(__uint_as_float(y[i] << 16), __uint_as_float(y[i] & 0xffff0000u));
+    }
+}
+
 template <typename T, int L>
-__global__ void __launch_bounds__(KV4_APPEND_THREADS) kv4_append_vec_kernel(const Kv4Append p) {
+__global__ void __launch_bounds__(KV4_APPEND_THREADS, 9) kv4_append_vec_kernel(const Kv4Append p) {
     constexpr int d = 16 * L, half = 8 * L, V = 16 / sizeof(T), N = 8 / V;          // elements of a 16-byte piece, pieces of eight elements
     const int l = threadIdx.x & (L - 1), n_heads = p.n_q + 2 * p.n_kv;
-    const long long unit = (long long)blockIdx.x * (KV4_APPEND_THREADS / L) + threadIdx.x / L;
-    const bool active = unit < (long long)p.T * n_heads;
-    const int t = active ? (int)(unit / n_heads) : 0, head = active ? (int)(unit - (long long)t * n_heads) : 0;
+    const unsigned unit = blockIdx.x * (KV4_APPEND_THREADS / L) + threadIdx.x / L;
+    const int token = (int)(unit / (unsigned)n_heads), head = (int)(unit - (unsigned)token * n_heads), t = min(token, p.T - 1);      // past the end: the last token again, not stored
     const bool is_q = head < p.n_q, is_k = !is_q && head < p.n_q + p.n_kv, turns = (is_q || is_k) && p.table != nullptr;
     const void* nw = is_q ? p.qw : (is_k ? p.kw : nullptr);
     pdl_wait();
     pdl_small();
-    float x[16];
+    int pos = turns ? p.positions[t] : 0;
+    const int slot = is_q ? 0 : p.out_loc[t];
+    uint4 raw[2][N];
     const T* src = reinterpret_cast<const T*>(p.qkv) + (size_t)t * p.stride + (size_t)head * d + 8 * l;
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const uint4 raw = *reinterpret_cast<const uint4*>(src + h * half + i * V);
-            const T* e = reinterpret_cast<const T*>(&raw);
+        for (int k = 0; k < N; ++k) raw[h][k] = *reinterpret_cast<const uint4*>(src + h * half + k * V);
+    F2 ang[8];                                            // cosines and sines of the lower half's elements
+    if (turns) {
+        pos = pos < 0 ? 0 : (pos >= p.max_pos ? p.max_pos - 1 : pos);
+        const ulonglong2* cs = reinterpret_cast<const ulonglong2*>(p.table + (size_t)pos * d + 8 * l);
 #pragma unroll
-            for (int j = 0; j < V; ++j) x[8 * h + i * V + j] = to_f32<T>(e[j]);
+        for (int k = 0; k < 4; ++k) {
+            const ulonglong2 a = cs[(k & 1) + (k >> 1) * (half / 4)];
+            ang[2 * k] = a.x;
+            ang[2 * k + 1] = a.y;
         }
+    }
+    F2 x[8];                                              // the lower half's elements and the upper half's
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        if constexpr (sizeof(T) == 4) {
+            const F2* e = reinterpret_cast<const F2*>(&raw[h][0]);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) x[4 * h + k] = e[k];
+        } else {
+            const unsigned y[4] = {raw[h][0].x, raw[h][0].y, raw[h][0].z, raw[h][0].w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) x[4 * h + k] = f2(__uint_as_float(y[k] << 16), __uint_as_float(y[k] & 0xffff0000u));
+        }
+    }
+    const unsigned group = (unsigned)(((1ull << L) - 1) << (threadIdx.x & 31 & ~(L - 1)));
     if (nw != nullptr) {
         double ss = 0.0;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) ss += square<T>(x[j]);
-        const unsigned group = (unsigned)(((1ull << L) - 1) << (threadIdx.x & 31 & ~(L - 1)));
+        for (int k = 0; k < 8; ++k) {
+            float a, b;
+            f2_get(sizeof(T) == 2 ? f2_mul(x[k], x[k]) : x[k], a, b);      // (a bfloat16's square is exact in float32)
+            ss += sizeof(T) == 2 ? (double)a : (double)a * (double)a;
+            ss += sizeof(T) == 2 ? (double)b : (double)b * (double)b;
+        }
 #pragma unroll
         for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(group, ss, o);
-        const float inv = inv_rms(ss, d, p.eps);
+        const F2 inv = f2(inv_rms(ss, d, p.eps));
 #pragma unroll
-        for (int j = 0; j < 16; ++j) x[j] = __fmul_rn(__fmul_rn(x[j], inv), load_weight(nw, (j < 8 ? 0 : half - 8) + 8 * l + j, p.w_f32));
+        for (int h = 0; h < 2; ++h) {
+            F2 w[4];
+            kv4_weights(nw, h * half + 8 * l, p.w_f32, w);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) x[4 * h + k] = f2_mul(f2_mul(x[4 * h + k], inv), w[k]);
+        }
     }
     if (turns) {
-        int pos = p.positions[t];
-        pos = pos < 0 ? 0 : (pos >= p.max_pos ? p.max_pos - 1 : pos);
-        const float4* cs = reinterpret_cast<const float4*>(p.table + (size_t)pos * d + 8 * l);
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-            const float4 c4 = cs[q], s4 = cs[half / 4 + q];
-            const float c[4] = {c4.x, c4.y, c4.z, c4.w}, s[4] = {s4.x, s4.y, s4.z, s4.w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int j = 4 * q + e;
-                const float a = x[j], b = x[8 + j];
-                x[j] = rot_sub(a, c[e], b, s[e]);
-                x[8 + j] = rot_add(a, s[e], b, c[e]);
-            }
+        for (int k = 0; k < 4; ++k) {
+            float a[2], b[2], c[2], s[2];                 // (one by one: packed products and sums are contracted)
+            f2_get(x[k], a[0], a[1]);
+            f2_get(x[4 + k], b[0], b[1]);
+            f2_get(ang[k], c[0], c[1]);
+            f2_get(ang[4 + k], s[0], s[1]);
+            x[k] = f2(rot_sub(a[0], c[0], b[0], s[0]), rot_sub(a[1], c[1], b[1], s[1]));
+            x[4 + k] = f2(rot_add(a[0], s[0], b[0], c[0]), rot_add(a[1], s[1], b[1], c[1]));
         }
     }
     if (is_q) {
-        if (!active) return;
-        T* dst = reinterpret_cast<T*>(p.q_out) + ((size_t)t * p.n_q + head) * d + 8 * l;
+        if (token >= p.T) return;
+        T* dst = reinterpret_cast<T*>(p.q_out) + ((size_t)token * p.n_q + head) * d + 8 * l;
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-                uint4 raw;
-                T* e = reinterpret_cast<T*>(&raw);
+            for (int k = 0; k < N; ++k) {
+                uint4 out;
+                T* e = reinterpret_cast<T*>(&out);
 #pragma unroll
-                for (int j = 0; j < V; ++j) e[j] = from_f32<T>(x[8 * h + i * V + j]);
-                *reinterpret_cast<uint4*>(dst + h * half + i * V) = raw;
+                for (int j = 0; j < V / 2; ++j) {
+                    float a, b;
+                    f2_get(x[4 * h + k * (V / 2) + j], a, b);
+                    e[2 * j] = from_f32<T>(a);
+                    e[2 * j + 1] = from_f32<T>(b);
+                }
+                *reinterpret_cast<uint4*>(dst + h * half + k * V) = out;
             }
         return;
     }
-    float lo = x[0], hi = x[0];
+    float lo, hi;
+    f2_get(x[0], lo, hi);
+    {
+        const float a = lo, b = hi;
+        lo = min_nan(a, b);
+        hi = max_nan(a, b);
+    }
 #pragma unroll
-    for (int j = 1; j < 16; ++j) { lo = min_nan(lo, x[j]); hi = max_nan(hi, x[j]); }
-    const unsigned group = (unsigned)(((1ull << L) - 1) << (threadIdx.x & 31 & ~(L - 1)));
+    for (int k = 1; k < 8; ++k) {
+        float a, b;
+        f2_get(x[k], a, b);
+        lo = min_nan(lo, a, b);
+        hi = max_nan(hi, a, b);
+    }
 #pragma unroll
     for (int o = L / 2; o > 0; o >>= 1) {
         lo = min_nan(lo, __shfl_xor_sync(group, lo, o));
         hi = max_nan(hi, __shfl_xor_sync(group, hi, o));
     }
     const Kv4Scale sc(lo, hi);
-    const long long row = active ? p.row_of(t, is_k ? head - p.n_q : head - p.n_q - p.n_kv) : -1;
+    const long long row = token < p.T ? p.row_of_slot(slot, is_k ? head - p.n_q : head - p.n_q - p.n_kv) : -1;
     if (row < 0) return;
     unsigned* dst = reinterpret_cast<unsigned*>((is_k ? p.k : p.v) + row * (d / 2)) + l;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        unsigned word = 0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) word |= sc.code(x[8 * h + e]) << (4 * e);
-        dst[h * L] = word;
-    }
+    const F2 x0[4] = {x[0], x[1], x[2], x[3]}, x1[4] = {x[4], x[5], x[6], x[7]};
+    dst[0] = sc.codes(x0);
+    dst[L] = sc.codes(x1);
     if (l == 0) p.steps[2 * row + (is_k ? 0 : 1)] = sc.bits;
 }
 
@@ -263,10 +335,10 @@ MSGL_API int msgl_kv4_append(const Kv4AppendArgs* x) {
     const long long units = (long long)T * (n_q + 2 * n_kv);
     const int item = dtype == MSGL_F32 ? 4 : 2;
     const bool whole = table == nullptr || (rot == d && !interleaved && ((uintptr_t)table & 15) == 0);
-    if (whole && (d == 32 || d == 64 || d == 128 || d == 256) && ((uintptr_t)qkv & 15) == 0 && ((uintptr_t)q_out & 15) == 0 && (stride * item) % 16 == 0) {
-        const int L = d / 16;
-        const long long blocks = (units + KV4_APPEND_THREADS / L - 1) / (KV4_APPEND_THREADS / L);
-        if (blocks > 0x7fffffffLL) return MSGL_ERR_SIZE;
+    if (whole && (d == 32 || d == 64 || d == 128 || d == 256) && (((uintptr_t)qkv | (uintptr_t)q_out | (uintptr_t)qw | (uintptr_t)kw) & 15) == 0 && (stride * item) % 16 == 0) {
+        const int L = d / 16, per = KV4_APPEND_THREADS / L;
+        const long long blocks = (units + per - 1) / per;
+        if (units > 0x7fffffffLL) return MSGL_ERR_SIZE;
 #define KV4_VEC(TT, LL) msgl_launch_pdl(kv4_append_vec_kernel<TT, LL>, dim3((unsigned)blocks), dim3(KV4_APPEND_THREADS), 0, stream, p)
 #define KV4_VEC_L(TT) do { if (L == 2) KV4_VEC(TT, 2); else if (L == 4) KV4_VEC(TT, 4); else if (L == 8) KV4_VEC(TT, 8); else KV4_VEC(TT, 16); } while (0)
         if (dtype == MSGL_F32) KV4_VEC_L(float); else KV4_VEC_L(__nv_bfloat16);
