@@ -42,6 +42,7 @@ class EngineArgs:
     chunk_size: int = 8192                   # longest portion of one prompt in one step
     max_context_len: Optional[int] = None    # default: the model's max_position_embeddings
     disable_overlap: bool = False            # read every step's tokens before the next step is launched
+    kv_cache_dtype: str = "auto"             # "auto": keys and values in `dtype`; "int4": in 4 bits (68 bytes a key of 128 instead of 256)
     profile_dir: str = "traces"              # where --profile saves its per-step records
     init_new_token_ratio: float = dataclasses.field(default_factory=lambda: _env("SGLANG_INIT_NEW_TOKEN_RATIO", 0.7))
     min_new_token_ratio_factor: float = dataclasses.field(default_factory=lambda: _env("SGLANG_MIN_NEW_TOKEN_RATIO_FACTOR", 0.14))
@@ -60,6 +61,8 @@ class EngineArgs:
             raise ValueError("this engine runs on a CUDA device only")
         if self.dtype not in ("bfloat16", "float32", "bf16", "fp32"):
             raise ValueError("dtype must be bfloat16 or float32")
+        if self.kv_cache_dtype not in ("auto", "int4"):
+            raise ValueError("kv_cache_dtype must be auto or int4")
         if self.schedule_policy not in ("fcfs", "lof", "random", "lpm", "dfs-weight"):
             raise ValueError(f"unknown schedule policy {self.schedule_policy!r}")
         if self.disable_radix_cache and self.schedule_policy not in ("fcfs", "lof", "random"):
@@ -97,6 +100,8 @@ class EngineArgs:
         parser.add_argument("--dummy_load", action="store_true",
                             help="Random weights for the configuration in --model instead of its checkpoint.")
         parser.add_argument("--dtype", type=str, default=d.dtype, choices=["bfloat16", "float32"])
+        parser.add_argument("--kv_cache_dtype", type=str, default=d.kv_cache_dtype, choices=["auto", "int4"],
+                            help="How keys and values are kept: auto as the activations, int4 in 4 bits with a step and a base for every token and kv head (models whose layers all are plain paged attention).")
         parser.add_argument("--num_pages", type=int, default=None, help="Cache size in pages (default: from memory).")
         parser.add_argument("--chunk_size", type=int, default=d.chunk_size, help="Longest prompt portion per step.")
         parser.add_argument("--max_context_len", type=int, default=None)

@@ -4,7 +4,7 @@
         [--prompt "text"] [--prompt_file FILE] [--max_new_tokens 64] [--temperature 0] [--ignore_eos]
         [engine options: --page_size --max_num_reqs --schedule_policy --gpu_memory_utilization
          --random_seed --disable_radix_cache --disable_cuda_graph --max_capture_bs
-         --schedule-conservativeness --max_prefill_tokens --dummy_load --dtype --num_pages ...]
+         --schedule-conservativeness --max_prefill_tokens --dummy_load --dtype --kv_cache_dtype --num_pages ...]
 
 Engine options have the names of the reference's launcher (`python -m mini_sglang.launch_server`,
 mini_sglang/managers/server_args.py:62-183); the reference starts an HTTP server, this prints one

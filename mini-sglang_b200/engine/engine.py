@@ -58,7 +58,7 @@ class Engine:
                                   max_reqs=args.max_num_reqs, max_context_len=max_ctx,
                                   max_step_tokens=args.max_prefill_tokens,
                                   gpu_memory_utilization=args.gpu_memory_utilization,
-                                  use_cuda_graph=not args.disable_cuda_graph, max_capture_bs=args.max_capture_bs)
+                                  use_cuda_graph=not args.disable_cuda_graph, max_capture_bs=args.max_capture_bs, kv_cache_dtype=args.kv_cache_dtype)
         self.sampler = Sampler(args.random_seed, self.runner.device)
         self.scheduler = Scheduler(
             self.runner, self.sampler, max_num_reqs=args.max_num_reqs, max_step_tokens=args.max_prefill_tokens,

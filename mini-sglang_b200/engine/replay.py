@@ -1,6 +1,6 @@
 """Trace replay: feed given token ids through the model step by step and write logits.
 
-    trace_run --model DIR --dtype bfloat16|float32 --out DIR --max-tokens N [--page-size P]
+    trace_run --model DIR --dtype bfloat16|float32 --out DIR --max-tokens N [--page-size P] [--kv-cache-dtype auto|int4]
 
 Reads one JSON object per line from standard input:
 
@@ -35,6 +35,7 @@ def main(argv=None) -> int:
     ap.add_argument("--page-size", type=int, default=16, help="tokens per cache page; must divide 64")
     ap.add_argument("--max-requests", type=int, default=4, help="request slots (live requests at a time)")
     ap.add_argument("--no-cuda-graph", action="store_true")
+    ap.add_argument("--kv-cache-dtype", default="auto", choices=["auto", "int4"], help="keys and values as the activations, or in 4 bits")
     args = ap.parse_args(argv)
     if args.page_size < 1 or 64 % args.page_size:
         ap.error("--page-size must divide 64")
@@ -47,7 +48,7 @@ def main(argv=None) -> int:
     num_pages = max(-(-args.max_tokens // 64) * 64 // args.page_size, 1)
     runner = ModelRunner.from_model_dir(args.model, dtype=args.dtype, page_size=args.page_size, num_pages=num_pages,
                                         max_reqs=args.max_requests, max_context_len=num_pages * args.page_size,
-                                        use_cuda_graph=not args.no_cuda_graph)
+                                        use_cuda_graph=not args.no_cuda_graph, kv_cache_dtype=args.kv_cache_dtype)
     slots = {}
     for line in sys.stdin:
         line = line.strip()

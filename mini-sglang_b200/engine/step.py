@@ -28,10 +28,11 @@ import torch
 from .. import ops
 from ..cache import CacheManager, OutOfPages, PagedKVNeed, StateNeed, keys_seen
 from ..config import ModelSpec, load_config
-from ..parts import BuildEnv, DecoderModel, DraftContext, GroupContext, KVCacheView, StateCacheView, StepContext, Workspace
+from ..parts import BuildEnv, DecoderModel, DraftContext, GroupContext, KV4CacheView, KVCacheView, StateCacheView, StepContext, Workspace
 from ..weights import CheckpointSource, RandomSource
 
 DTYPES = {"bfloat16": torch.bfloat16, "bf16": torch.bfloat16, "float32": torch.float32, "fp32": torch.float32}
+KV_CACHE_DTYPES = ("auto", "int4")          # keys and values as the activations, or in 4 bits (csrc/kv4.cu)
 MAX_KV_SPLIT = 32                 # more than MANY_SPLITS pieces only where they stay long (below)
 MANY_SPLITS, MANY_SPLITS_MIN_KEYS = 16, 512      # one request of 32k keys: 16 pieces 4.54, 32 pieces 4.29 ms a step; of 4k keys: 3.37 / 3.44
 MIN_KEYS_PER_SPLIT = 128          # 64 / 128 / 256 / 512 measured at 1 to 8 requests of 1k to 4k keys: 128 best or level (batch 1, 4,096 keys: 3.46 against 3.54 ms with 256)
@@ -111,15 +112,19 @@ class _Layout:
 
 class CacheStorage:
     """Device arrays behind the cache manager: per cache id K and V [pages + 1, kv heads, page,
-    head size] in the activation dtype, or a state array [max requests + 1, ...]."""
+    head size] in the activation dtype, or (kv4) the same rows in 4 bits (ops.KV4Cache), or a state array [max requests + 1, ...]."""
 
-    def __init__(self, mgr: CacheManager, dtype: torch.dtype, device):
+    def __init__(self, mgr: CacheManager, dtype: torch.dtype, device, kv4: bool = False):
         self.kv: Dict[int, Tuple[torch.Tensor, torch.Tensor]] = {}
+        self.kv4: Dict[int, ops.KV4Cache] = {}
         self.state: Dict[int, torch.Tensor] = {}
         for cid, need in mgr.needs.items():
             if isinstance(need, PagedKVNeed):
                 g = mgr.groups[mgr.group_of_cache[cid]]
                 shape = (g.pool.num_pages + 1, need.n_kv_heads, mgr.page_size, need.head_dim)
+                if kv4:
+                    self.kv4[cid] = ops.kv4_cache(*shape, device=device)
+                    continue
                 k = torch.zeros(shape, dtype=dtype, device=device)
                 v_shape = shape[:3] + (need.v_head_dim or need.head_dim,)
                 self.kv[cid] = (k, k if need.shared_kv else torch.zeros(v_shape, dtype=dtype, device=device))
@@ -137,10 +142,13 @@ class CacheStorage:
 
     def bytes(self) -> int:
         n = sum(k.numel() * k.element_size() + (0 if v is k else v.numel() * v.element_size()) for k, v in self.kv.values())
+        n += sum(t.numel() * t.element_size() for cache in self.kv4.values() for t in cache)
         return n + sum(t.numel() * t.element_size() for t in self.state.values())
 
 
-def kv_bytes_per_page(needs: Dict[int, object], page_size: int, dtype: torch.dtype) -> int:
+def kv_bytes_per_page(needs: Dict[int, object], page_size: int, dtype: torch.dtype, kv4: bool = False) -> int:
+    if kv4:
+        return sum(page_size * n.n_kv_heads * ops.kv4_row_bytes(n.head_dim) for n in needs.values() if isinstance(n, PagedKVNeed))
     item = torch.empty((), dtype=dtype).element_size()
     return sum(page_size * n.n_kv_heads * (n.head_dim + (0 if n.shared_kv else (n.v_head_dim or n.head_dim))) * item
                for n in needs.values() if isinstance(n, PagedKVNeed))
@@ -296,7 +304,7 @@ class ModelRunner:
     def __init__(self, spec: ModelSpec, source_factory, *, dtype: str = "bfloat16", page_size: int = 16,
                  num_pages: Optional[int] = None, max_reqs: int = 64, max_context_len: Optional[int] = None,
                  max_step_tokens: int = 8192, gpu_memory_utilization: float = 0.9, device: str = "cuda:0",
-                 use_cuda_graph: bool = True, max_capture_bs: int = 128):
+                 use_cuda_graph: bool = True, max_capture_bs: int = 128, kv_cache_dtype: str = "auto"):
         self.device = self._init_device(device)
         self.sm_count = self._sm_count()
         self.dtype = DTYPES[dtype]
@@ -319,18 +327,19 @@ class ModelRunner:
         finally:
             src.close()
         needs = self.model.cache_needs()
+        self.kv4 = self._wants_kv4(kv_cache_dtype, needs)
         if num_pages is None:
             torch.cuda.empty_cache()
             free, total = torch.cuda.mem_get_info(self.device)
             budget = int(total * gpu_memory_utilization) - (total - free)
-            per_page = max(kv_bytes_per_page(needs, page_size, self.dtype), 1)
+            per_page = max(kv_bytes_per_page(needs, page_size, self.dtype, self.kv4), 1)
             num_pages = max(budget // per_page, 0)
             num_pages = min(num_pages, max_reqs * (-(-self.max_context_len // page_size)))
             if num_pages < 1:
                 raise RuntimeError("no memory left for the cache; lower gpu_memory_utilization's complement or the model size")
         self.mgr = CacheManager(needs, page_size=page_size, num_pages=num_pages, max_reqs=max_reqs,
                                 max_context_len=self.max_context_len, max_step_tokens=max_step_tokens)
-        self.storage = CacheStorage(self.mgr, self.dtype, self.device)
+        self.storage = CacheStorage(self.mgr, self.dtype, self.device, self.kv4)
         self.workspace = Workspace(self.device)
         self.vocab_size = spec.vocab_size
         self._pinned = [None, None]
@@ -364,7 +373,7 @@ class ModelRunner:
             first, of_geom = len(self._plan_group), {}
             for cid in g.cache_ids:
                 need = needs[cid]
-                if need.library != "attention":
+                if need.library != "attention" or self.kv4:      # (attention over 4 bits deals out the keys by itself)
                     continue
                 G = max(need.q_heads // need.n_kv_heads, 1) if need.q_heads else 1
                 qt = ops.attention_tile_tokens(ops.VARIANT_MMA_DECODE, G, need.head_dim) if ops.mma_supported(need.head_dim, self.dtype) \
@@ -393,6 +402,24 @@ class ModelRunner:
                 ok = ok and ops.decode_even_ok(head_dim, self.dtype, G) and self.sm_count * per_sm >= n_kv
             if ok:
                 self._even_nb = [max(1, self.sm_count * per_sm // n_kv) for (n_kv, G, per_sm, _) in self._group_geom]
+
+    def _wants_kv4(self, kv_cache_dtype: str, needs: Dict[int, object]) -> bool:
+        """Whether keys and values are held in 4 bits ("int4") or in the activations' type ("auto"); a model that cannot have them so is refused."""
+        if kv_cache_dtype not in KV_CACHE_DTYPES:
+            raise ValueError(f"kv_cache_dtype {kv_cache_dtype!r}: one of {', '.join(KV_CACHE_DTYPES)}")
+        if kv_cache_dtype == "auto":
+            return False
+        paged = [n for n in needs.values() if isinstance(n, PagedKVNeed)]
+        if not paged:
+            raise ValueError("kv_cache_dtype int4: the model keeps no keys and values in pages")
+        for layer in self.model.layers:
+            need = layer.mixer.cache_need()
+            if any(isinstance(n, PagedKVNeed) for n in (need if isinstance(need, (tuple, list)) else (need,))) and not layer.mixer.takes_kv4:
+                raise ValueError(f"kv_cache_dtype int4: {type(layer.mixer).__name__} layers read caches of the activations' type only")
+        for n in paged:
+            if n.shared_kv or n.v_head_dim not in (None, n.head_dim) or n.chunk or n.keep_first or n.head_dim % 8 or n.head_dim > ops.KV4_MAX_HEAD_DIM:
+                raise ValueError(f"kv_cache_dtype int4: keys and values of one head size, in steps of 8 up to {ops.KV4_MAX_HEAD_DIM}, over all keys or a window; got {n}")
+        return True
 
     # -- device ------------------------------------------------------------------------------
     def _init_device(self, device: str) -> torch.device:
@@ -446,7 +473,7 @@ class ModelRunner:
         """Blocks of the whole-step decode kernel for a step of `tokens` single tokens with all logits wanted; 0 if the
         model or the size goes kernel by kernel."""
         fd = self.model.fused_decode
-        if fd is None or not 0 < tokens <= ops.FUSED_DECODE_MAX_TOKENS or len(self._plan_group) != 1:
+        if fd is None or not 0 < tokens <= ops.FUSED_DECODE_MAX_TOKENS or len(self._plan_group) != 1 or self.kv4:
             return 0
         return fd.blocks_for(tokens)
 
@@ -553,6 +580,8 @@ class ModelRunner:
         views: Dict[int, object] = {}
         for cid, (k, v) in self.storage.kv.items():
             views[cid] = KVCacheView(k, v, ctx.groups[self._plan_of_cache[cid]], self.page_size)
+        for cid, cache in self.storage.kv4.items():
+            views[cid] = KV4CacheView(cache, ctx.groups[self._plan_of_cache[cid]], self.page_size)
         for cid, st in self.storage.state.items():
             views[cid] = StateCacheView(st)
         # the caches of a mixer with several needs, (c, 0), (c, 1), ..., reach it as one tuple under the run's id c
@@ -648,9 +677,9 @@ class ModelRunner:
 
     # -- drafted tokens ------------------------------------------------------------------------
     def drafts_supported(self) -> bool:
-        """Whether `verify` takes this model: every mixer is one that takes drafts and attends to all keys of a paged cache (no windows, chunks or
+        """Whether `verify` takes this model: every mixer is one that takes drafts and attends to all keys of a paged cache of the activations' type (no windows, chunks or
         per-request states) with heads of up to 512."""
-        return bool(self.mgr.groups) and not self.mgr.state_ids and all(g.span is None for g in self.mgr.groups) and \
+        return bool(self.mgr.groups) and not self.kv4 and not self.mgr.state_ids and all(g.span is None for g in self.mgr.groups) and \
             all(layer.mixer.takes_drafts for layer in self.model.layers) and all((n.v_head_dim or n.head_dim) == n.head_dim <= 512 for n in self.mgr.needs.values())
 
     @torch.no_grad()
@@ -666,7 +695,7 @@ class ModelRunner:
         Every draft has a place in the cache during the step: a tree whose drafts and cached tokens together are beyond the context limit is refused
         (ValueError, naming the slot, before anything is taken for any entry), so callers bring smaller trees near the limit."""
         if not self.drafts_supported():
-            raise ValueError("drafted tokens need a model whose layers attend to all keys of a paged cache")
+            raise ValueError("drafted tokens need a model whose layers attend to all keys of a paged cache of the activations' type")
         entries = list(entries)
         if not entries:
             return []

@@ -8,7 +8,7 @@ from .. import ops
 from ..cache.manager import PagedKVNeed
 from ..weights.loader import TensorDecl
 from .base import Mixer, register_mixer
-from .context import KVCacheView, StepContext
+from .context import KV4CacheView, KVCacheView, StepContext
 
 
 @register_mixer("paged_attention")
@@ -28,6 +28,7 @@ class PagedAttention(Mixer):
 
     graph_safe = True
     takes_drafts = True
+    takes_kv4 = True
 
     def __init__(self, spec, prefix, env, position=None):
         super().__init__(spec, prefix, env)
@@ -90,6 +91,9 @@ class PagedAttention(Mixer):
     def forward(self, x: torch.Tensor, ctx: StepContext, cache: KVCacheView, writes_cache: bool = True) -> torch.Tensor:
         qkv = ops.linear(x, self.qkv, self.qkv_b)
         table = self.position.rotary_table() if self.position is not None else None
+        if isinstance(cache, KV4CacheView):
+            out = self.over_4_bits(qkv, table, ctx, cache, writes_cache)
+            return ops.linear(out.view(ctx.T, self.n_q * self.d), self.o)
         q = ops.qknorm_rope_kvwrite(
             qkv, ctx.positions, self.n_q, self.n_kv, self.d,
             q_weight=self.q_norm, k_weight=self.k_norm, eps=self.qk_norm_eps, rope_table=table,
@@ -99,6 +103,20 @@ class PagedAttention(Mixer):
         out = torch.empty_like(q)
         self.attend(q, out, ctx, cache)
         return ops.linear(out.view(ctx.T, self.n_q * self.d), self.o)
+
+    def over_4_bits(self, qkv: torch.Tensor, table: Optional[torch.Tensor], ctx: StepContext, cache: KV4CacheView, writes_cache: bool) -> torch.Tensor:
+        """The same over a cache in 4 bits: the new tokens' keys and values are coded as they are written, and read back from their codes like all others'."""
+        if ctx.drafts is not None:
+            raise ValueError("drafted tokens need a cache of the activations' type")
+        norm = dict(q_weight=self.q_norm, k_weight=self.k_norm, eps=self.qk_norm_eps, rope_table=table, interleaved=bool(getattr(self.position, "interleaved", False)))
+        if writes_cache:
+            q = ops.qknorm_rope_kv4write(qkv, ctx.positions, self.n_q, self.n_kv, self.d, out_loc=cache.group.out_loc, cache=cache.cache, **norm)
+        else:
+            q = ops.qknorm_rope_kvwrite(qkv, ctx.positions, self.n_q, self.n_kv, self.d, out_loc=None, k_cache=None, v_cache=None, page_size=cache.page_size, **norm)
+        out = torch.empty_like(q)
+        lens = {} if ctx.uniform_decode else dict(q_start=ctx.q_start, q_lens=ctx.host_q_lens, kv_lens=ctx.host_kv_lens)
+        ops.kv4_attention(q, out, cache.cache, kv_len=ctx.kv_len, block_table=cache.group.block_table, scale=self.scale, window=int(self.window or 0), workspace=ctx.workspace, **lens)
+        return out
 
     def attend(self, q: torch.Tensor, out: torch.Tensor, ctx: StepContext, cache: KVCacheView) -> None:
         paged_attend(q, out, ctx, cache, n_q=self.n_q, n_kv=self.n_kv, d=self.d, window=int(self.window or 0), scale=self.scale,

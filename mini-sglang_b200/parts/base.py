@@ -70,6 +70,8 @@ class Mixer(Part):
     # True if forward() takes a step of drafted tokens (ctx.drafts): over positions it reads only ctx.positions, over other
     # tokens only what `paged_attend` reads.
     takes_drafts = False
+    # True if forward() takes its cache with the keys and values in 4 bits (KV4CacheView) as well.
+    takes_kv4 = False
 
     def cache_need(self):
         return None

@@ -117,6 +117,14 @@ class KVCacheView:
 
 
 @dataclasses.dataclass
+class KV4CacheView:
+    """A cache whose keys and values are held in 4 bits (ops.KV4Cache), with the group context that addresses it."""
+    cache: Any
+    group: GroupContext
+    page_size: int
+
+
+@dataclasses.dataclass
 class StateCacheView:
     """A per-request state array [max requests + 1, ...]; row ctx.slots[r] belongs to request r."""
     state: torch.Tensor
