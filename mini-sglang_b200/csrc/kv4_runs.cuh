@@ -2,10 +2,10 @@
 //
 // A segment is up to 8 rows (token, query head) of one request under one kv head, and its keys in units of 32.  The units of all segments are dealt out
 // over the warps of one block an SM; every warp works out from the requests' lengths alone which are its own, and goes through them by itself.
-//   * few keys: a segment of u units has max(1, u / PIECE) equal pieces, a block a piece (or a block a whole segment, where that is nearly even), and a piece's
+//   * few keys: a segment of u units has u / PIECE equal pieces (one up to ALONE units), a block a piece (or a block a whole segment, where that is nearly even), and a piece's
 //     units are dealt out over the block's warps;
 //   * otherwise the units of all segments, each with HEAD units ahead for what a segment costs beside its keys, are laid end to end and cut into as many runs of
-//     equal length as there are warps; a cut within SNAP units of a segment's edge moves onto the edge.
+//     equal length as there are warps.
 // A segment within one warp's run is written out by it.  Of the others a warp leaves its part (it has at most two: one that its run starts with, and its last) in
 // shared memory; behind the only barrier after the cut, parts of one segment are added in the order of the keys.  Where other blocks hold parts too, the
 // sum goes to scratch memory, and the block that raises the segment's counter to the number of blocks adds them up and clears the counter.
@@ -28,9 +28,9 @@
 constexpr float KR_LAZY = 8.f;
 constexpr int KR_KEYS = 32;          // keys of a unit
 constexpr int KR_MAX_B = 256;        // requests of a launch, a thread each
-constexpr int KR_PIECE = 12;         // units of a block's piece at least, where segments are cut by themselves
-constexpr int KR_SNAP = 1;           // a cut this close to a segment's edge moves onto it
-constexpr int KR_HEAD = 2;           // what a segment costs beside its units, in units
+constexpr int KR_PIECE = 16;         // units of a block's piece at least, where segments are cut by themselves ...
+constexpr int KR_ALONE = 48;         // ... and none of up to this many units is
+constexpr int KR_HEAD = 1;           // what a segment costs beside its units, in units
 
 struct Kv4Runs {
     const __nv_bfloat16* q; __nv_bfloat16* out;
@@ -41,6 +41,7 @@ struct Kv4Runs {
     int* count;                      // a word a segment, zero before and after
     long long bt_stride;
     int B, T, n_q, n_kv, page_size, page_shift, pages, bt_width, window, max_q;
+    int beside;                      // all that is read here was written before the launch ahead of this one, which is waited for at the end
     float scale;
 };
 
@@ -97,6 +98,8 @@ __device__ __forceinline__ unsigned kr_half2(float lo, float hi) {
 // two rows of A (words wl, wh) times Q: elements 0 4, 1 5 (16 times their codes), 2 6, 3 7 (likewise) of the words
 constexpr unsigned KR_LOW = 0x000f000fu, KR_HIGH = 0x00f000f0u, KR_BYTE = 0x00ff00ffu;
 
+__device__ __forceinline__ int kr_pieces(int u) { return u <= KR_ALONE ? 1 : u / KR_PIECE; }
+
 struct KrCursor {
     int r, s, kvh, tile, c0, u;      // request, its segment, kv head and tile of rows; first unit of the segment among all, units
     int key0, keys;                  // (unit among all) * KR_KEYS + key0 is the unit's first key; keys of the request
@@ -134,7 +137,8 @@ __global__ void __launch_bounds__(NW * 32, 1) kv4_attn_runs_kernel(const Kv4Runs
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const int G = p.n_q / p.n_kv, NB = (int)gridDim.x, j = (int)blockIdx.x, W = NB * NW;      // W: warps of the launch
-    pdl_wait();
+    if (!p.beside) pdl_wait();
+    auto leave = [&]() { if (p.beside) pdl_wait(); };      // (whoever waits for this kernel counts on the one before it as well)
 
     // ---- the requests, a thread each; then one warp sums up their units, segments and pieces, neighbouring requests a lane, and cuts.  (Short code: it runs once, from a
     // cold instruction cache.)
@@ -159,7 +163,7 @@ __global__ void __launch_bounds__(NW * 32, 1) kv4_attn_runs_kernel(const Kv4Runs
             const int u = units[r], segs = pre_s[r];
             U += u * segs;
             S += segs;
-            P += max(1, u / KR_PIECE) * segs;
+            P += kr_pieces(u) * segs;
             longest = max(longest, u);
         }
         int at_u = -U, at_s = -S, at_p = -P;
@@ -177,7 +181,7 @@ __global__ void __launch_bounds__(NW * 32, 1) kv4_attn_runs_kernel(const Kv4Runs
         if (lane == 0) { sh_all[0] = U; sh_all[1] = S; sh_all[2] = by_piece; sh_all[3] = 1; pre_u[p.B] = U; pre_s[p.B] = S; }
 #pragma unroll 1
         for (int r = r0; r < r1; ++r) {
-            const int u = units[r], segs = pre_s[r], pc = whole ? 1 : max(1, u / KR_PIECE), in_r = j - at_p;
+            const int u = units[r], segs = pre_s[r], pc = whole ? 1 : kr_pieces(u), in_r = j - at_p;
             pre_u[r] = at_u; pre_s[r] = at_s;
             if (by_piece && in_r >= 0 && in_r < pc * segs) {      // the block's piece, dealt out over its warps
                 const int s = in_r / pc, piece = in_r - s * pc, a = (int)((long long)u * piece / pc), n = (int)((long long)u * (piece + 1) / pc) - a;
@@ -190,7 +194,7 @@ __global__ void __launch_bounds__(NW * 32, 1) kv4_attn_runs_kernel(const Kv4Runs
         }
         __syncwarp();
         if (!by_piece && lane <= NW) {
-            // cut i = floor(V i / W) falls into a request (the last whose V-sum before it is no larger), there into a segment, there onto an edge or a unit; a cut a lane
+            // cut i = floor(V i / W) falls into a request (the last whose V-sum before it is no larger), there into a segment, there onto a unit; a cut a lane
             const int V = U + KR_HEAD * S, V_per = V / W, i = j * NW + lane;
             int x = U;
             if (i < W) {
@@ -203,10 +207,10 @@ __global__ void __launch_bounds__(NW * 32, 1) kv4_attn_runs_kernel(const Kv4Runs
                 }
                 const int un = units[a], in_r = raw - pre_u[a] - KR_HEAD * pre_s[a];      // (requests without segments lie ahead of one with the same sum)
                 int s = in_r / (un + KR_HEAD);
-                const int off = in_r - s * (un + KR_HEAD) - KR_HEAD, unit = off <= KR_SNAP ? 0 : un - off <= KR_SNAP ? un : off;
+                const int off = in_r - s * (un + KR_HEAD) - KR_HEAD, unit = max(off, 0);
                 x = pre_u[a] + s * un + unit;
                 sh_r[lane] = a;
-                sh_s[lane] = unit == un ? s + 1 : s;      // a cut at the end: the run starts with the segment behind
+                sh_s[lane] = s;
             }
             sh_x[lane] = x;
         }
@@ -216,7 +220,7 @@ __global__ void __launch_bounds__(NW * 32, 1) kv4_attn_runs_kernel(const Kv4Runs
 
     // ---- this warp's run of units [lo, hi) of the segments laid end to end, and the segment it starts in
     const bool by_piece = sh_all[2];
-    if (sh_x[0] >= sh_x[NW]) return;                      // (the whole block)
+    if (sh_x[0] >= sh_x[NW]) { leave(); return; }         // (the whole block)
     auto settle = [&](KrCursor& c) {                      // from a request's end to the next segment; there is one
         while (c.s >= pre_s[c.r + 1] - pre_s[c.r]) { ++c.r; c.s = 0; }
         c.u = units[c.r];
@@ -567,7 +571,7 @@ __global__ void __launch_bounds__(NW * 32, 1) kv4_attn_runs_kernel(const Kv4Runs
     // the lane of a group's first slot its segment
     const int of_slot = lane < 2 * NW ? slot_seg[lane] : -1;
     const unsigned there = __ballot_sync(0xffffffffu, of_slot >= 0);
-    if (there == 0) return;                               // (all warps see the same)
+    if (there == 0) { leave(); return; }                  // (all warps see the same)
     const unsigned under = there & ((1u << lane) - 1u);
     const int before = __shfl_sync(0xffffffffu, of_slot, 31 - __clz(under | 1u));
     const bool leads = of_slot >= 0 && (under == 0 || before != of_slot);
@@ -586,10 +590,10 @@ __global__ void __launch_bounds__(NW * 32, 1) kv4_attn_runs_kernel(const Kv4Runs
         at_head = kvh * G;
         pieces = sh_all[3];
         mine = sh_mine;
-        if (!by_piece) {                                  // the cuts inside are those of c + SNAP < floor(V i / W) < c + u - SNAP; part k lies in warp first_cut - 1 + k
+        if (!by_piece) {                                  // the cuts inside are those of c < floor(V i / W) < c + u; part k lies in warp first_cut - 1 + k
             const long long at = pre_u[a] + (long long)s * units[a] + (long long)KR_HEAD * (of_slot + 1);
             const int V = sh_all[0] + KR_HEAD * sh_all[1];
-            const int first_cut = (int)(((at + KR_SNAP + 1) * W + V - 1) / V), last_cut = (int)(((at + units[a] - KR_SNAP) * W + V - 1) / V) - 1;
+            const int first_cut = (int)(((at + 1) * W + V - 1) / V), last_cut = (int)(((at + units[a]) * W + V - 1) / V) - 1;
             const int b0 = (first_cut - 1) / NW;
             pieces = last_cut / NW - b0 + 1;
             mine = j - b0;
@@ -639,7 +643,7 @@ __global__ void __launch_bounds__(NW * 32, 1) kv4_attn_runs_kernel(const Kv4Runs
     }
     // segments that other blocks hold parts of as well: one from before, one that goes on
     const unsigned open = __ballot_sync(0xffffffffu, pieces > 1);
-    if (open == 0) return;
+    if (open == 0) { leave(); return; }
     __syncthreads();
     if (warp == 0) {                                      // the fence behind the barrier covers what the block's other threads wrote
         if (pieces > 1) {
@@ -685,6 +689,7 @@ __global__ void __launch_bounds__(NW * 32, 1) kv4_attn_runs_kernel(const Kv4Runs
             if (lane < COLS) *reinterpret_cast<uint2*>(dst) = make_uint2(kr_pack(acc.x * inv, acc.y * inv), kr_pack(acc.z * inv, acc.w * inv));
         }
     }
+    leave();
 }
 
 #ifndef KR_WARPS
@@ -695,7 +700,7 @@ constexpr int KR_NW = KR_WARPS, KR_ST = KR_STAGES;
 
 // Requests with 1 .. max_q tokens; q_start null: request r has token r.  count: a word for every 8 rows of a request under a kv head, zero before and after.
 struct Kv4RunsArgs {
-    long long q, out, k, v, steps, q_start, kv_len, block_table, bt_stride, bt_width, part_o, part_ml, count, blocks, B, T, n_q, n_kv, d, page_size, pages, window, max_q, stream;
+    long long q, out, k, v, steps, q_start, kv_len, block_table, bt_stride, bt_width, part_o, part_ml, count, blocks, B, T, n_q, n_kv, d, page_size, pages, window, max_q, beside, stream;
     double scale;
 };
 
@@ -726,7 +731,7 @@ MSGL_API int msgl_kv4_attention_runs(const Kv4RunsArgs* x) {
         attr_set.mark();
     }
     Kv4Runs p = {(const __nv_bfloat16*)q, (__nv_bfloat16*)out, (const unsigned char*)k, (const unsigned char*)v, (const uint2*)steps, q_start, kv_len, block_table, part_o,
-                 part_ml, count, bt_stride, B, T, n_q, n_kv, page_size, -1, pages, bt_width, window, max_q, scale};
+                 part_ml, count, bt_stride, B, T, n_q, n_kv, page_size, -1, pages, bt_width, window, max_q, (int)x->beside, scale};
     if ((page_size & (page_size - 1)) == 0) { p.page_shift = 0; while ((1 << p.page_shift) < page_size) ++p.page_shift; }
     const bool whole = page_size % 16 == 0;
 #define KR_GO(DD, WW) if (d == DD && whole == WW) msgl_launch_pdl(kv4_attn_runs_kernel<DD, KR_NW, KR_ST, WW>, dim3(blocks), dim3(KR_NW * 32), kr_smem_bytes<DD, KR_NW, KR_ST>(), stream, p);

@@ -2704,7 +2704,13 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
 # a key/value cache held in 4 bits (csrc/kv4.cu)
 # ---------------------------------------------------------------------------------------
 KV4_MAX_HEAD_DIM = 512
-KV4_DIRECT_ROWS = 32              # (token, query head) rows of a request under a kv head up to which the codes are read directly; longer runs restore the keys first
+# (token, query head) rows of a request under a kv head up to which its codes are read directly; longer runs have the keys restored first.  On the tensor cores (bfloat16, head
+# sizes 64 and 128) reading codes costs 0.47 us of an SM for 8 rows and 128 keys, restoring 128 keys 2.5 and the prefill kernel's walk over them 2.6 for up to 256 rows: where
+# all SMs have work they are level at 86 rows (32 requests behind 2,000 keys, 32 on 8 heads, 16 tokens 111 / 151 us, 24: 161 / 151).  Up to KV4_MIDDLE_ROWS the two are estimated
+# (_kv4_middle): a few requests leave the prefill kernel with fewer blocks than SMs, each as long as its keys (one request of 64 tokens behind 4,000 keys 36 / 90 us, behind 500 16 / 27).
+# The float32 kernel reads 32 rows directly.
+KV4_DIRECT_ROWS, KV4_MIDDLE_ROWS, KV4_DIRECT_ROWS_F32 = 80, 512, 32
+KV4_US = 0.118, 2.5, 2.6          # SM microseconds: codes of 32 keys for 8 rows; restoring 128 keys; 128 keys of a tile of 256 rows of the prefill kernel
 _KV4_REQUESTS = 256               # requests of one launch that deals the keys out
 KV4_RESTORE_BYTES = 1 << 30       # of restored keys and values, what a step makes at a time
 _kv4 = None
@@ -2721,7 +2727,7 @@ def _kv4_lib():
 
 
 # The entry points take their arguments packed in one piece, 8 bytes each (ctypes takes 3 us to convert 25 of them one by one, which small steps wait for).
-_KV4_APPEND, _KV4_RESTORE, _KV4_ANY, _KV4_RUNS = (struct.Struct(f).pack for f in ("23qd", "23q", "23qd", "24qd"))
+_KV4_APPEND, _KV4_RESTORE, _KV4_ANY, _KV4_RUNS = (struct.Struct(f).pack for f in ("23qd", "23q", "23qd", "25qd"))
 
 
 class KV4Cache(NamedTuple):
@@ -2888,7 +2894,8 @@ def kv4_attention(q: torch.Tensor, out: torch.Tensor, cache: KV4Cache, *, kv_len
           and k.get_device() == v.get_device() == steps.get_device() == out.get_device() == kv_len.get_device() == block_table.get_device() == dev >= 0
           and dev == torch._C._cuda_getDevice())
     B, few, most = block_table.shape[0] if ok else 0, 1, 0
-    direct = max(1, KV4_DIRECT_ROWS * shape[1] // q.shape[1]) if ok else 1          # most tokens of a request that reads the codes directly
+    tensor = ok and dt is torch.bfloat16 and (shape[3] == 64 or shape[3] == 32)
+    direct = max(1, (KV4_DIRECT_ROWS if tensor else KV4_DIRECT_ROWS_F32) * shape[1] // q.shape[1]) if ok else 1          # most tokens of a request that reads the codes directly
     if ok and q_lens is None:
         ok = q.shape[0] == B
     elif ok:
@@ -2897,6 +2904,8 @@ def kv4_attention(q: torch.Tensor, out: torch.Tensor, cache: KV4Cache, *, kv_len
         if ok and B:
             few, most, places = 0, max(q_lens), block_table.shape[1] * shape[2]
             ok = min(q_lens) >= 0 and sum(q_lens) <= q.shape[0] and max(kv_lens) <= places and all(map(operator.le, q_lens, kv_lens))
+            if ok and tensor and most > direct:
+                direct = _kv4_middle(q_lens, kv_lens if not window else [min(kv, n + window) for n, kv in zip(q_lens, kv_lens)], direct, shape[1], q.shape[1] // shape[1], _sm(q))
             if most <= direct:
                 few = most
             elif ok:
@@ -2905,11 +2914,38 @@ def kv4_attention(q: torch.Tensor, out: torch.Tensor, cache: KV4Cache, *, kv_len
         _refuse_kv4_attention(q, out, cache, kv_len, block_table, scale, window, q_start, q_lens, kv_lens)
     if q.shape[0] == 0 or B == 0:
         return
-    if few:
-        _kv4_few(q, out, cache, kv_len, block_table, scale, window, q_start if q_lens is not None else None, few,
-                 None if q_lens is None else max(kv for n, kv in zip(q_lens, kv_lens) if 0 < n <= direct), workspace)
-    if most > direct:
-        _kv4_portions(q, out, cache, kv_len, block_table, scale, window, q_start, q_lens, kv_lens, direct + 1, workspace)
+    if most <= direct:
+        _kv4_few(q, out, cache, kv_len, block_table, scale, window, q_start if q_lens is not None else None, few, None if q_lens is None else max(kv_lens), workspace)
+        return
+
+    scratch = _kv4_scratch(q, cache, few, workspace) if few else None          # (ahead of the launch that the rest may run beside: it may have to be cleared)
+
+    def runs_of_few(beside: bool) -> None:
+        if few:
+            _kv4_few(q, out, cache, kv_len, block_table, scale, window, q_start, few, max(kv for n, kv in zip(q_lens, kv_lens) if 0 < n <= direct), workspace, beside, scratch)
+
+    _kv4_portions(q, out, cache, kv_len, block_table, scale, window, q_start, q_lens, kv_lens, direct + 1, workspace, runs_of_few)
+
+
+def _kv4_middle(q_lens, kv_lens, direct: int, n_kv: int, G: int, sms: int) -> int:
+    """Tokens up to which a request reads the codes directly, `direct` or KV4_MIDDLE_ROWS rows, whichever is estimated to be faster for the requests between; kv_lens: the keys that
+    they see."""
+    middle = max(direct, KV4_MIDDLE_ROWS // G)
+    mid = [(n, kv) for n, kv in zip(q_lens, kv_lens) if direct < n <= middle]
+    if not mid:
+        return direct
+    codes, restore, walk = (us * n_kv / sms for us in KV4_US)
+
+    def prefill(requests) -> float:
+        tiles = [(-(-n * G // 256), -(-kv // 128)) for n, kv in requests]
+        whole = sum(a * k for a, k in tiles)
+        # from 8 key tiles an SM on the prefill kernel cuts long tiles up, for some 20 us of merging
+        return whole * walk + 20.0 if whole * n_kv >= 8 * sms else max(whole * walk, max((k for _, k in tiles), default=0) * KV4_US[2])
+
+    large = [(n, kv) for n, kv in zip(q_lens, kv_lens) if n > middle]
+    by_codes = sum(-(-n * G // 8) * -(-kv // 32) for n, kv in mid) * codes + 9.0
+    restored = prefill(mid + large) - (prefill(large) if large else -8.0) + sum(-(-kv // 128) for _, kv in mid) * restore
+    return middle if by_codes < restored else direct
 
 
 def _refuse_kv4_attention(q, out, cache, kv_len, block_table, scale, window, q_start, q_lens, kv_lens) -> None:
@@ -2945,36 +2981,45 @@ def _refuse_kv4_attention(q, out, cache, kv_len, block_table, scale, window, q_s
     raise KernelError(f"{what}: arguments that do not go together")
 
 
-def _kv4_few(q, out, cache, kv_len, block_table, scale, window, q_start, max_q, longest, workspace) -> None:
-    """The requests with 1 to max_q tokens, from the codes; `longest` bounds their keys (None: the block table does)."""
+def _kv4_scratch(q, cache, max_q, workspace) -> torch.Tensor:
+    """Partial results of two segments a block, and behind them counters, one a segment and zero between launches, in one buffer that is laid out alike for both head sizes."""
+    words = 2 * 8 * _sm(q) * 130 + _KV4_REQUESTS * -(-max_q * q.shape[1] // cache.k.shape[1] // 8) * cache.k.shape[1]
+    scratch = workspace.counters("kv4_few", words) if workspace is not None else None
+    return scratch if scratch is not None else torch.zeros(words, dtype=torch.int32, device=q.device)          # (inside a stream capture the zeros are written by every replay)
+
+
+def _sm(q) -> int:
+    dev = q.get_device()
+    return _sms.get(dev) or _sms.setdefault(dev, sm_count(q.device))
+
+
+def _kv4_few(q, out, cache, kv_len, block_table, scale, window, q_start, max_q, longest, workspace, beside=False, scratch=None) -> None:
+    """The requests with 1 to max_q tokens, from the codes; `longest` bounds their keys (None: the block table does).  beside: the launch before this one is the prefill
+    kernel of the same call, which writes nothing that is read here and beside which it may run."""
     (T, n_q, d), (pages, n_kv, page_size, _), (B, width) = q.shape, cache.k.shape, block_table.shape
-    lib, G, dev = _kv4_lib(), n_q // n_kv, q.get_device()
-    sms = _sms.get(dev) or _sms.setdefault(dev, sm_count(q.device))
+    lib, G, sms = _kv4_lib(), n_q // n_kv, _sm(q)
     at_k, at_v, at_steps, at_q, at_out, at_kv, at_table, row = (cache.k.data_ptr(), cache.v.data_ptr(), cache.steps.data_ptr(), q.data_ptr(), out.data_ptr(), kv_len.data_ptr(),
                                                                 block_table.data_ptr(), block_table.stride(0))
     at_start = 0 if q_start is None else q_start.data_ptr()
     tiles = -(-max_q * G // 8)
     if q.dtype is torch.bfloat16 and (d == 128 or d == 64) and pages * n_kv * page_size < 0xffffffff and not (at_q | at_out | at_k | at_v | at_steps) & 15 \
             and min(B, _KV4_REQUESTS) * n_kv * tiles * (width * page_size // 32 + 5) < 1 << 31:
-        # partial results of two segments a block, and behind them counters, one a segment and zero between launches, in one buffer that is laid out alike for both head sizes
         n_part = 2 * 8 * sms
-        words = n_part * 130 + _KV4_REQUESTS * tiles * n_kv
-        scratch = workspace.counters("kv4_few", words) if workspace is not None else None
-        if scratch is None:          # (inside a stream capture the zeros are written by every replay)
-            scratch = torch.zeros(words, dtype=torch.int32, device=q.device)
+        if scratch is None:
+            scratch = _kv4_scratch(q, cache, max_q, workspace)
         at = scratch.data_ptr()
         for a in range(0, B, _KV4_REQUESTS):
             first = 0 if q_start is not None else a          # (without q_start token r is request r's)
             code = lib.msgl_kv4_attention_runs(_KV4_RUNS(
                 at_q + first * n_q * d * 2, at_out + first * n_q * d * 2, at_k, at_v, at_steps, at_start + 4 * a if at_start else 0, at_kv + 4 * a, at_table + 4 * a * row, row, width,
-                at, at + 4 * n_part * 128, at + 4 * n_part * 130, sms, min(B - a, _KV4_REQUESTS), T - first, n_q, n_kv, d, page_size, pages, window, max_q, _stream(), scale))
+                at, at + 4 * n_part * 128, at + 4 * n_part * 130, sms, min(B - a, _KV4_REQUESTS), T - first, n_q, n_kv, d, page_size, pages, window, max_q, beside and a == 0, _stream(), scale))
             if code:
                 _check(code, "kv4_attention")
             _count_launch()
         return
     tiles *= B * n_kv
     keys = width * page_size if longest is None else longest
-    splits = max(1, min(4 * sms // tiles, (min(keys, window + 8) if window else keys) // 128, 64))
+    splits = max(1, min(4 * sms // tiles, -(-(min(keys, window + max_q) if window else keys) // 128), 64))          # no fewer than 128 keys each, a unit of 32 a warp
     part = torch.empty(splits * T * n_q * (d + 2), dtype=torch.float32, device=q.device) if splits > 1 else None
     code = lib.msgl_kv4_attention_any(_KV4_ANY(at_q, at_out, at_k, at_v, at_steps, at_start, at_kv, at_table, row, width, 0 if part is None else part.data_ptr(), splits, B, T, n_q, n_kv, d,
                                                page_size, pages, window, max_q, _DT[q.dtype], _stream(), scale))
@@ -2983,15 +3028,16 @@ def _kv4_few(q, out, cache, kv_len, block_table, scale, window, q_start, max_q, 
         _count_launch()
 
 
-def _kv4_portions(q, out, cache, kv_len, block_table, scale, window, q_start, q_lens, kv_lens, min_q, workspace) -> None:
-    """The requests with at least min_q tokens: what they see is restored into pages of its own, which the prefill kernels then read."""
+def _kv4_portions(q, out, cache, kv_len, block_table, scale, window, q_start, q_lens, kv_lens, min_q, workspace, others) -> None:
+    """The requests with at least min_q tokens: what they see is restored into pages of its own, which the prefill kernels then read.  others(beside) launches the rest of the
+    step: beside the tiles of the tcgen05 kernel where that runs, whose last blocks leave SMs free."""
     (T, n_q, d), (pages, n_kv, page_size, _), width = q.shape, cache.k.shape, block_table.shape[1]
     lib, G, big = _kv4_lib(), n_q // n_kv, 1 << 30
     per = int(lib.msgl_kv4_restored_page())
     need = [0 if n < min_q else -(-kv // per) - (max(kv - n - window + 1, 0) // per if window else 0) for n, kv in zip(q_lens, kv_lens)]
     page_numel = n_kv * per * d
     most = max(1, KV4_RESTORE_BYTES // (2 * page_numel * q.element_size()))
-    a = 0
+    a, launched = 0, False
     while a < len(need):
         b, n = a, 0
         while b < len(need) and (n == 0 or n + need[b] <= most):
@@ -3008,12 +3054,17 @@ def _kv4_portions(q, out, cache, kv_len, block_table, scale, window, q_start, q_
             _check(code, "kv4_attention (keys restored)")
             k, v, table = k.view(n, n_kv, per, d), v.view(n, n_kv, per, d), table.view(b - a, t_width)
             common = dict(q_start=starts, kv_len=kv_part, block_table=table, n_kv=n_kv, page_size=per, window=window, scale=scale, qlen_min=min_q, qlen_max=big)
-            if not (tc_supported(d, q.dtype, G) and attention_tc(q, out, k, v, q_lens=lens, kv_lens=kvs, workspace=workspace, **common)):
+            beside = (lambda: others(True)) if not any(need[b:]) else None
+            if tc_supported(d, q.dtype, G) and attention_tc(q, out, k, v, q_lens=lens, kv_lens=kvs, workspace=workspace, beside=beside, **common):
+                launched = beside is not None
+            else:
                 variant = VARIANT_MMA_ROWS if mma_supported(d, q.dtype) else VARIANT_SIMT
                 qt = attention_tile_tokens(variant, G, d)
                 attention(q, out, k, v, nsplit=None, part_o=None, part_ml=None, max_split=1, uniform_decode=False, variant=variant,
                           grid_x=sum(-(-m // qt) for m in lens if m >= min_q), **common)
         a = b
+    if not launched:
+        others(False)
 
 
 # ---------------------------------------------------------------------------------------

@@ -150,9 +150,7 @@ def check(q_lens, kv_lens, *, n_q, n_kv, d, dtype, page=16, window=0, seed=0, ex
     want, facts = plain.attention(q, c, starts, q_lens, kv_lens, table, d ** -0.5, window)
     n = sum(q_lens)
     assert (out[n:] == 7.0).all()
-    longer = ops.KV4_DIRECT_ROWS // (n_q // n_kv)
-    restored = torch.tensor([m > max(1, longer) for m in q_lens for _ in range(m)], device="cuda")
-    tol = torch.where(restored[:, None, None], bound(facts[:n], max(kv_lens), d, dtype, True), bound(facts[:n], max(kv_lens), d, dtype, False))
+    tol = torch.maximum(bound(facts[:n], max(kv_lens), d, dtype, True), bound(facts[:n], max(kv_lens), d, dtype, False))          # (from codes or from restored keys)
     err = (out[:n].double() - want[:n]).abs()
     tol = tol + torch.finfo(dtype).eps / 2 * (want[:n].abs() + tol)
     assert (err <= tol).all(), (err - tol).max()

@@ -59,3 +59,13 @@ def test_drafts_are_refused():
     assert not r.drafts_supported()
     with pytest.raises(ValueError, match="activations' type"):
         r.verify([], None)
+
+
+def test_which_requests_read_codes_directly():
+    """The middle lengths go where they are estimated to be faster: few of them leave the prefill kernel without work for all SMs, many fill it."""
+    of = lambda n, kv, B=1, more=(): ops._kv4_middle([n] * B + [m for m, _ in more], [kv] * B + [k for _, k in more], 20, 8, 4, 148)      # noqa: E731
+    assert of(20, 4000) == 20                                     # none between
+    assert of(64, 4000) == 128 and of(96, 500) == 128             # one request: its codes
+    assert of(32, 2000, B=32) == 20 and of(64, 8000, B=8) == 20   # many: restored
+    assert of(64, 4000, more=[(4000, 4000)]) == 20                # beside a long portion's tiles
+    assert of(200, 4000) == 20                                    # longer than the middle
