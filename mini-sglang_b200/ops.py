@@ -436,7 +436,7 @@ def attention_tc(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_ca
             assert bias_log2.dtype == torch.float32 and bias_log2.dim() == 2 and bias_log2.shape[0] == n_q and bias_log2.is_contiguous()
     for version in versions:
         rows = TC_ROWS * version
-        qt = rows // group if group <= TC_ROWS else version
+        qt = (version * (TC_ROWS // group) if diff is None else rows // group) if group <= TC_ROWS else version          # (a query tile of 128 rows holds whole tokens)
         grid_x = sum(-(-n // qt) for n in q_lens if qlen_min <= n <= qlen_max)
         cut = None
         # the plan is made in Python: two bounds on the key tiles, the cheap one first, keep it out of launches that the rule leaves whole
