@@ -18,7 +18,9 @@
 //     q k = step 2^(24 - e) sum q^ (c 2^-24) + base sum q
 //     o   = sum_j p_j (base_j + step_j c_j) = 2^24 / F sum_j w_j (c_j 2^-24) + sum_j p_j base_j,   w_j = float16(p_j step_j F)
 // F is a power of two of the warp's own that keeps step F <= 64 (p is at most 2^8, see KR_LAZY): where a unit brings a larger step, F and the sums are scaled down.
-// w keeps 11 bits; below 2^-28 of the largest step it loses them one by one.
+// w keeps 11 bits; below 2^-28 of the largest step it loses them one by one.  The tensor core cuts its sums off rather than rounding them, and those of codes from
+// 0 up grow all the way while what they leave beside the bases is small (a mean of 16,000 values came out 1 % off); so every unit takes the middles of the codes times
+// its weights out of all sums by one more product, and they are added back at the end from float32 sums of their own.
 // Scores, p, sums and outputs are float32.  S^T = K Q^T with keys on the M dimension, the head's elements permuted so that a lane reads 16 bytes
 // of a row; P goes through movmatrix; V^T fragments come by ldmatrix.trans on 16-bit columns, four codes of two neighbouring keys a register.  The
 // exponentials' reference moves only where a score lies KR_LAZY above it.
@@ -97,6 +99,7 @@ __device__ __forceinline__ unsigned kr_half2(float lo, float hi) {
 }
 // two rows of A (words wl, wh) times Q: elements 0 4, 1 5 (16 times their codes), 2 6, 3 7 (likewise) of the words
 constexpr unsigned KR_LOW = 0x000f000fu, KR_HIGH = 0x00f000f0u, KR_BYTE = 0x00ff00ffu;
+constexpr unsigned KR_MID_BYTE = 0x80808080u, KR_MID_HIGH = 0x80788078u;      // -128 and -120, about the middles of a byte and of its upper code, as float16 subnormals
 
 __device__ __forceinline__ int kr_pieces(int u) { return u <= KR_ALONE ? 1 : u / KR_PIECE; }
 
@@ -374,6 +377,7 @@ __global__ void __launch_bounds__(NW * 32, 1) kv4_attn_runs_kernel(const Kv4Runs
             float m_c[2] = {-INFINITY, -INFINITY}, mu_c[2] = {0.f, 0.f}, l_c[2] = {0.f, 0.f}, z_c[2] = {0.f, 0.f};      // mu_c: the exponentials' reference (m_c, or 0 before a key)
             float lim_c[2] = {-INFINITY, -INFINITY};      // how far above it a score may lie (a first key lies above any)
             float F = 0.f;                                // 0: no step seen yet
+            float mid[4] = {0.f, 0.f, 0.f, 0.f};          // what the middles of the codes have been taken out by (KR_MID), rows and columns as o's
 
             for (; x < end; ++x) {
                 kr_wait<ST - 2>();
@@ -468,6 +472,8 @@ __global__ void __launch_bounds__(NW * 32, 1) kv4_attn_runs_kernel(const Kv4Runs
                         l_c[e] *= alpha[e];
                         z_c[e] *= alpha[e];
                         alpha[e] *= down;
+                        mid[e] *= alpha[e];
+                        mid[e + 2] *= alpha[e];
                         lim_c[e] = mn == -INFINITY ? -INFINITY : KR_LAZY;
                     }
 #pragma unroll
@@ -502,6 +508,18 @@ __global__ void __launch_bounds__(NW * 32, 1) kv4_attn_runs_kernel(const Kv4Runs
                         }
                         pb[m][h] = kr_trans(w);
                     }
+                // ---- the middles of the codes times the weights, out of all sums (the same for every element)
+                float d_mid[4];
+                kr_mma0(d_mid, KR_MID_BYTE, KR_MID_HIGH, KR_MID_BYTE, KR_MID_HIGH, pb[0][0], pb[0][1]);
+                kr_mma(d_mid, KR_MID_BYTE, KR_MID_HIGH, KR_MID_BYTE, KR_MID_HIGH, pb[1][0], pb[1][1]);
+                const F2 d_even = f2(d_mid[0], d_mid[1]), d_odd = f2(d_mid[2], d_mid[3]);
+                auto put = [&](float (&x)[4]) {
+                    f2_get(f2_add(f2(x[0], x[1]), d_even), x[0], x[1]);
+                    f2_get(f2_add(f2(x[2], x[3]), d_odd), x[2], x[3]);
+                };
+                put(mid);
+#pragma unroll
+                for (int mt = 0; mt < D / 16; ++mt) put(o[mt]);
                 // ---- O^T += C^T W^T; matrices: keys 0-7 and 8-15 of two neighbouring chunks.  Lane g gets codes 4 g .. 4 g + 3 of keys 2 t, 2 t + 1 of a chunk
                 kr_each<2>([&](auto mm) {
                     constexpr int m = mm.value;
@@ -525,6 +543,7 @@ __global__ void __launch_bounds__(NW * 32, 1) kv4_attn_runs_kernel(const Kv4Runs
             const float of = F > 0.f ? 16777216.f / F : 0.f, of16 = of * 0.0625f;
 #pragma unroll
             for (int mt = 0; mt < D / 16; ++mt) { o[mt][0] -= o[mt][2]; o[mt][1] -= o[mt][3]; }      // (even elements come with 16 times the odd one behind them)
+            const float even[2] = {mid[0] - mid[2], mid[1] - mid[3]}, odd[2] = {mid[2], mid[3]};
 #pragma unroll
             for (int e = 0; e < 2; ++e)
 #pragma unroll
@@ -540,11 +559,11 @@ __global__ void __launch_bounds__(NW * 32, 1) kv4_attn_runs_kernel(const Kv4Runs
                     if (row >= n) continue;
                     const int tok = row / G;
                     __nv_bfloat16* dst = p.out + ((size_t)(token[now.r] + tok) * p.n_q + (size_t)now.kvh * G + (row - tok * G)) * D + 4 * g;
-                    const float inv = l_c[e] != 0.f ? 1.f / l_c[e] : 0.f, a = of * inv, b = of16 * inv, z = z_c[e] * inv;
+                    const float inv = l_c[e] != 0.f ? 1.f / l_c[e] : 0.f, a = of * inv, b = of16 * inv, z0 = fmaf(-even[e], of, z_c[e]) * inv, z1 = fmaf(-odd[e], of16, z_c[e]) * inv;
 #pragma unroll
                     for (int c = 0; c < CH; ++c)
-                        *reinterpret_cast<uint2*>(dst + 32 * c) = make_uint2(kr_pack(fmaf(o[2 * c][e], a, z), fmaf(o[2 * c][e + 2], b, z)),
-                                                                             kr_pack(fmaf(o[2 * c + 1][e], a, z), fmaf(o[2 * c + 1][e + 2], b, z)));
+                        *reinterpret_cast<uint2*>(dst + 32 * c) = make_uint2(kr_pack(fmaf(o[2 * c][e], a, z0), fmaf(o[2 * c][e + 2], b, z1)),
+                                                                             kr_pack(fmaf(o[2 * c + 1][e], a, z0), fmaf(o[2 * c + 1][e + 2], b, z1)));
                 }
             } else {
                 const int slot = end == hi ? 1 : 0;
@@ -554,7 +573,7 @@ __global__ void __launch_bounds__(NW * 32, 1) kv4_attn_runs_kernel(const Kv4Runs
                 for (int mt = 0; mt < D / 16; ++mt)
 #pragma unroll
                     for (int e = 0; e < 2; ++e)
-                        *reinterpret_cast<float2*>(to + (2 * t + e) * OLD + (mt >> 1) * 32 + 4 * g + 2 * (mt & 1)) = make_float2(fmaf(o[mt][e], of, z_c[e]), fmaf(o[mt][e + 2], of16, z_c[e]));
+                        *reinterpret_cast<float2*>(to + (2 * t + e) * OLD + (mt >> 1) * 32 + 4 * g + 2 * (mt & 1)) = make_float2(fmaf(o[mt][e], of, fmaf(-even[e], of, z_c[e])), fmaf(o[mt][e + 2], of16, fmaf(-odd[e], of16, z_c[e])));
                 if (g == 0)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) *reinterpret_cast<float2*>(slot_ml + ((2 * warp + slot) * 8 + 2 * t + e) * 2) = make_float2(m_c[e], l_c[e]);
