@@ -105,7 +105,8 @@ __device__ __forceinline__ int kr_pieces(int u) { return u <= KR_ALONE ? 1 : u /
 
 struct KrCursor {
     int r, s, kvh, tile, c0, u;      // request, its segment, kv head and tile of rows; first unit of the segment among all, units
-    int key0, keys;                  // (unit among all) * KR_KEYS + key0 is the unit's first key; keys of the request
+    unsigned key0;                   // (unit among all) * KR_KEYS + key0 is the unit's first key, modulo 2^32
+    int keys;                        // of the request
 };
 
 template <int D, int NW, int ST>
@@ -148,7 +149,7 @@ __global__ void __launch_bounds__(NW * 32, 1) kv4_attn_runs_kernel(const Kv4Runs
     static_assert(NW * 32 >= KR_MAX_B || NW * 64 >= KR_MAX_B, "one or two requests a thread");
 #pragma unroll 1
     for (int r = tid; r < p.B; r += NW * 32) {
-        const int t0 = p.q_start != nullptr ? p.q_start[r] : r, n = p.q_start != nullptr ? p.q_start[r + 1] - t0 : 1, len = p.kv_len[r];
+        const int t0 = p.q_start != nullptr ? p.q_start[r] : r, n = p.q_start != nullptr ? p.q_start[r + 1] - t0 : 1, len = max(p.kv_len[r], 0);
         const int kv = max(min(len, p.bt_width * p.page_size), 0), f = (p.window > 0 ? max(len - n - p.window + 1, 0) : 0) / KR_KEYS;
         const bool taken = n >= 1 && n <= p.max_q && t0 >= 0 && t0 + n <= p.T;
         units[r] = taken ? max((kv + KR_KEYS - 1) / KR_KEYS - f, 1) : 0;
@@ -232,7 +233,7 @@ __global__ void __launch_bounds__(NW * 32, 1) kv4_attn_runs_kernel(const Kv4Runs
         c.tile = 0;
         if (tiles > 1) { c.kvh = c.s / tiles; c.tile = c.s - c.kvh * tiles; }
         c.c0 = pre_u[c.r] + c.s * c.u;
-        c.key0 = (first[c.r] - c.c0) * KR_KEYS;
+        c.key0 = (unsigned)(first[c.r] - c.c0) * KR_KEYS;
         c.keys = keys[c.r];
     };
     const int lo = sh_x[warp], hi = sh_x[warp + 1];
@@ -260,7 +261,7 @@ __global__ void __launch_bounds__(NW * 32, 1) kv4_attn_runs_kernel(const Kv4Runs
             Place w = {-1, -1, 0, 0};
             if (x >= hi) return w;
             while (x >= ld.c0 + ld.u) { ++ld.s; settle(ld); }
-            const int key = x * KR_KEYS + ld.key0;
+            const int key = (int)((unsigned)x * KR_KEYS + ld.key0);
             look_up(WHOLE ? key : key + lane, w.page0, w.add0);
             if (WHOLE) look_up(key + 16, w.page1, w.add1);
             return w;
@@ -385,7 +386,7 @@ __global__ void __launch_bounds__(NW * 32, 1) kv4_attn_runs_kernel(const Kv4Runs
                 if (x + ST - 1 < hi) load(st_load, next);
                 kr_commit();
                 next = place_of(x + ST);
-                const int key0 = x * KR_KEYS + seg.key0;
+                const int key0 = (int)((unsigned)x * KR_KEYS + seg.key0);
                 // ---- S^T = K Q^T, 16 keys a time; v: scores less their reference, log2 units
                 float v[2][4], s[2][2][4];
                 uint2 row_st[2][2];

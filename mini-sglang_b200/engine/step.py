@@ -318,7 +318,9 @@ class ModelRunner:
         self.model = DecoderModel(spec, env)
         head_dims = sorted({n.head_dim for n in self.model.cache_needs().values()
                             if isinstance(n, PagedKVNeed) and n.library == "attention"})
-        ops.warm_up(head_dims)
+        needs = self.model.cache_needs()
+        self.kv4 = self._wants_kv4(kv_cache_dtype, needs)
+        ops.warm_up(head_dims, kv4=self.kv4)
         expected = self.model.tensors()
         src = source_factory(expected, self.dtype, self.device)
         try:
@@ -326,8 +328,6 @@ class ModelRunner:
                 self.model.load(src)
         finally:
             src.close()
-        needs = self.model.cache_needs()
-        self.kv4 = self._wants_kv4(kv_cache_dtype, needs)
         if num_pages is None:
             torch.cuda.empty_cache()
             free, total = torch.cuda.mem_get_info(self.device)

@@ -138,9 +138,11 @@ def _attn_lib(head_dim: int):
     return lib
 
 
-def warm_up(head_dims=()) -> None:
-    """Build and load the libraries a model needs (compiles at the first call)."""
+def warm_up(head_dims=(), kv4: bool = False) -> None:
+    """Build and load the libraries a model needs (compiles at the first call); kv4: those of a cache in 4 bits too."""
     _lib()
+    if kv4:
+        _kv4_lib()
     for hd in head_dims:
         _attn_lib(hd)
 
@@ -2912,13 +2914,13 @@ def kv4_attention(q: torch.Tensor, out: torch.Tensor, cache: KV4Cache, *, kv_len
                 few = max((n for n in q_lens if n <= direct), default=0)
     if not ok:
         _refuse_kv4_attention(q, out, cache, kv_len, block_table, scale, window, q_start, q_lens, kv_lens)
-    if q.shape[0] == 0 or B == 0:
+    if q.shape[0] == 0 or B == 0 or few == most == 0:
         return
     if most <= direct:
         _kv4_few(q, out, cache, kv_len, block_table, scale, window, q_start if q_lens is not None else None, few, None if q_lens is None else max(kv_lens), workspace)
         return
 
-    scratch = _kv4_scratch(q, cache, few, workspace) if few else None          # (ahead of the launch that the rest may run beside: it may have to be cleared)
+    scratch = _kv4_scratch(q, cache, few, workspace) if few and tensor else None          # (ahead of the launch that the rest may run beside: it may have to be cleared)
 
     def runs_of_few(beside: bool) -> None:
         if few:

@@ -204,3 +204,13 @@ def test_long_portions_restored_a_few_requests_at_a_time(monkeypatch):
     near(whole, q, c, lens, kv, table)
     monkeypatch.setattr(ops, "KV4_RESTORE_BYTES", 4 * 2 * 128 * n_kv * d * 2)          # four pages of restored keys and values at a time, more where a request has more
     assert torch.equal(whole, attend(q, c, kv, table, **kw))
+
+
+def test_steps_without_tokens():
+    c, q = filled(21, 5, 2, 16, 128), normal(22, 3, 4, 128, dtype=BF)
+    out = attend(q, c, [9, 20], i32([1, 2, 3, 4]).view(2, 2), q_start=i32([0, 0, 0]), q_lens=[0, 0], kv_lens=[9, 20])
+    assert (out == 7.0).all()
+    empty = q[:0]
+    ops.kv4_attention(empty, empty, c, kv_len=i32([]), block_table=i32([]).view(0, 2), scale=1.0)
+    ops.kv4_attention(empty, empty, c, kv_len=i32([]), block_table=i32([]).view(0, 2), scale=1.0, q_start=i32([0]), q_lens=[], kv_lens=[])
+    assert ops.qknorm_rope_kv4write(normal(1, 0, 8 * 128), i32([]), 4, 2, 128, q_weight=None, k_weight=None, eps=1e-6, rope_table=None, out_loc=i32([]), cache=c).shape == (0, 4, 128)
