@@ -86,6 +86,7 @@ struct Kv4Append {
     unsigned char* k; unsigned char* v; unsigned* steps;  // steps: two words a row, keys' and values'
     long long slots;                                      // of the cache: page numbers beyond are left out
     int page_size, n_q, n_kv, d, T;
+    int early;                                            // the next launch may start while this one waits for the one ahead
     __device__ __forceinline__ long long row_of_slot(int slot, int kvh) const {      // -1: nowhere
         if (slot < 0 || slot >= slots) return -1;
         const int page = slot / page_size;
@@ -194,8 +195,9 @@ __global__ void __launch_bounds__(KV4_APPEND_THREADS, 9) kv4_append_vec_kernel(c
     const int token = (int)(unit / (unsigned)n_heads), head = (int)(unit - (unsigned)token * n_heads), t = min(token, p.T - 1);      // past the end: the last token again, not stored
     const bool is_q = head < p.n_q, is_k = !is_q && head < p.n_q + p.n_kv, turns = (is_q || is_k) && p.table != nullptr;
     const void* nw = is_q ? p.qw : (is_k ? p.kw : nullptr);
+    if (p.early) pdl_small();
     pdl_wait();
-    pdl_small();
+    if (!p.early) pdl_small();
     int pos = turns ? p.positions[t] : 0;
     const int slot = is_q ? 0 : p.out_loc[t];
     uint4 raw[2][N];
@@ -312,7 +314,7 @@ __global__ void __launch_bounds__(KV4_APPEND_THREADS, 9) kv4_append_vec_kernel(c
 
 // The entry points take their arguments in one piece, 8 bytes each in the order of these structs.
 struct Kv4AppendArgs {
-    long long qkv, stride, positions, out_loc, qw, kw, w_f32, table, rot, max_pos, interleaved, q_out, k, v, steps, slots, page_size, n_q, n_kv, d, T, dtype, stream;
+    long long qkv, stride, positions, out_loc, qw, kw, w_f32, table, rot, max_pos, interleaved, q_out, k, v, steps, slots, page_size, n_q, n_kv, d, T, dtype, early, stream;
     double eps;
 };
 
@@ -331,7 +333,7 @@ MSGL_API int msgl_kv4_append(const Kv4AppendArgs* x) {
     if (dtype != MSGL_F32 && dtype != MSGL_BF16) return MSGL_ERR_DTYPE;
     if (((uintptr_t)k | (uintptr_t)v | (uintptr_t)steps) & 15) return MSGL_ERR_ALIGN;
     Kv4Append p = {qkv, stride, positions, out_loc, qw, kw, w_f32, eps, table, rot, max_pos, interleaved, q_out, (unsigned char*)k, (unsigned char*)v, (unsigned*)steps,
-                   slots, page_size, n_q, n_kv, d, T};
+                   slots, page_size, n_q, n_kv, d, T, (int)x->early};
     const long long units = (long long)T * (n_q + 2 * n_kv);
     const int item = dtype == MSGL_F32 ? 4 : 2;
     const bool whole = table == nullptr || (rot == d && !interleaved && ((uintptr_t)table & 15) == 0);

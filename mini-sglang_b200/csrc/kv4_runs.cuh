@@ -43,7 +43,8 @@ struct Kv4Runs {
     int* count;                      // a word a segment, zero before and after
     long long bt_stride;
     int B, T, n_q, n_kv, page_size, page_shift, pages, bt_width, window, max_q;
-    int beside;                      // all that is read here was written before the launch ahead of this one, which is waited for at the end
+    int ahead;                       // what was written before the launch ahead of this one: 1: kv_len, q_start and block_table, which are read before it is waited for;
+                                     // 2: all that is read here: it is waited for at the end
     float scale;
 };
 
@@ -141,8 +142,8 @@ __global__ void __launch_bounds__(NW * 32, 1) kv4_attn_runs_kernel(const Kv4Runs
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const int G = p.n_q / p.n_kv, NB = (int)gridDim.x, j = (int)blockIdx.x, W = NB * NW;      // W: warps of the launch
-    if (!p.beside) pdl_wait();
-    auto leave = [&]() { if (p.beside) pdl_wait(); };      // (whoever waits for this kernel counts on the one before it as well)
+    if (p.ahead == 0) pdl_wait();
+    auto leave = [&]() { if (p.ahead != 0) pdl_wait(); };      // (whoever waits for this kernel counts on the one before it as well)
 
     // ---- the requests, a thread each; then one warp sums up their units, segments and pieces, neighbouring requests a lane, and cuts.  (Short code: it runs once, from a
     // cold instruction cache.)
@@ -351,13 +352,14 @@ __global__ void __launch_bounds__(NW * 32, 1) kv4_attn_runs_kernel(const Kv4Runs
             all_end = min(p0 + c.tile * 8 / G + 1, kv);
             all_from = p.window > 0 ? p0 + min(c.tile * 8 + 7, n - 1) / G - p.window + 1 : 0;
         };
-        fetch_q(seg);
+        if (p.ahead != 1) fetch_q(seg);
         Place next;
         {
             Place w[ST - 1];
 #pragma unroll
             for (int i = 0; i < ST - 1; ++i) w[i] = place_of(lo + i);
             next = place_of(lo + ST - 1);
+            if (p.ahead == 1) { pdl_wait(); fetch_q(seg); }
 #pragma unroll
             for (int i = 0; i < ST - 1; ++i) {
                 if (i < n_my) load(i * STAGE, w[i]);
@@ -720,7 +722,7 @@ constexpr int KR_NW = KR_WARPS, KR_ST = KR_STAGES;
 
 // Requests with 1 .. max_q tokens; q_start null: request r has token r.  count: a word for every 8 rows of a request under a kv head, zero before and after.
 struct Kv4RunsArgs {
-    long long q, out, k, v, steps, q_start, kv_len, block_table, bt_stride, bt_width, part_o, part_ml, count, blocks, B, T, n_q, n_kv, d, page_size, pages, window, max_q, beside, stream;
+    long long q, out, k, v, steps, q_start, kv_len, block_table, bt_stride, bt_width, part_o, part_ml, count, blocks, B, T, n_q, n_kv, d, page_size, pages, window, max_q, ahead, stream;
     double scale;
 };
 
@@ -751,7 +753,7 @@ MSGL_API int msgl_kv4_attention_runs(const Kv4RunsArgs* x) {
         attr_set.mark();
     }
     Kv4Runs p = {(const __nv_bfloat16*)q, (__nv_bfloat16*)out, (const unsigned char*)k, (const unsigned char*)v, (const uint2*)steps, q_start, kv_len, block_table, part_o,
-                 part_ml, count, bt_stride, B, T, n_q, n_kv, page_size, -1, pages, bt_width, window, max_q, (int)x->beside, scale};
+                 part_ml, count, bt_stride, B, T, n_q, n_kv, page_size, -1, pages, bt_width, window, max_q, (int)x->ahead, scale};
     if ((page_size & (page_size - 1)) == 0) { p.page_shift = 0; while ((1 << p.page_shift) < page_size) ++p.page_shift; }
     const bool whole = page_size % 16 == 0;
 #define KR_GO(DD, WW) if (d == DD && whole == WW) msgl_launch_pdl(kv4_attn_runs_kernel<DD, KR_NW, KR_ST, WW>, dim3(blocks), dim3(KR_NW * 32), kr_smem_bytes<DD, KR_NW, KR_ST>(), stream, p);

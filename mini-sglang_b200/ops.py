@@ -2729,7 +2729,7 @@ def _kv4_lib():
 
 
 # The entry points take their arguments packed in one piece, 8 bytes each (ctypes takes 3 us to convert 25 of them one by one, which small steps wait for).
-_KV4_APPEND, _KV4_RESTORE, _KV4_ANY, _KV4_RUNS = (struct.Struct(f).pack for f in ("23qd", "23q", "23qd", "25qd"))
+_KV4_APPEND, _KV4_RESTORE, _KV4_ANY, _KV4_RUNS = (struct.Struct(f).pack for f in ("24qd", "23q", "23qd", "25qd"))
 
 
 class KV4Cache(NamedTuple):
@@ -2771,11 +2771,12 @@ def _kv4_sizes(what: str, cache: KV4Cache) -> Tuple[int, int, int, int]:
 
 def qknorm_rope_kv4write(qkv: torch.Tensor, positions: torch.Tensor, n_q: int, n_kv: int, d: int, *, q_weight: Optional[torch.Tensor], k_weight: Optional[torch.Tensor],
                          eps: float, rope_table: Optional[torch.Tensor], out_loc: torch.Tensor, cache: KV4Cache, q_out: Optional[torch.Tensor] = None,
-                         interleaved: bool = False) -> torch.Tensor:
+                         interleaved: bool = False, attention_next: bool = False) -> torch.Tensor:
     """`qknorm_rope_kvwrite` for a cache in 4 bits: qkv [T, (n_q + 2 n_kv) d] float32 or bfloat16 (rows any distance apart), per-head RMSNorm of q and k (if weights
     are given), rotation from `rope_table` [max_pos, rot] float32 = cos | sin (if given), the rotated k and v put into 4 bits at token slots `out_loc` (int32; a
     slot outside the cache is left out), q returned as [T, n_q, d] in qkv's type.  Keys are coded from their float32 values, before any rounding to
-    qkv's type.  Two tokens with one slot leave one of the two rows or parts of both.  A row with a NaN or an infinity, or wider than bfloat16 reaches, stands for NaN."""
+    qkv's type.  Two tokens with one slot leave one of the two rows or parts of both.  A row with a NaN or an infinity, or wider than bfloat16 reaches, stands for NaN.
+    attention_next: as there, with `kv4_attention(fields_ahead=True)` as the next launch."""
     (k, v, steps), dt, dev = cache, qkv.dtype, qkv.get_device()
     shape, rot, max_pos = k.shape, 0, 0
     # every argument is looked at in one go, and told apart only where something is wrong: small steps wait for the host
@@ -2807,7 +2808,7 @@ def qknorm_rope_kv4write(qkv: torch.Tensor, positions: torch.Tensor, n_q: int, n
     code = _kv4_lib().msgl_kv4_append(_KV4_APPEND(
         qkv.data_ptr(), qkv.stride(0), positions.data_ptr(), out_loc.data_ptr(), 0 if q_weight is None else q_weight.data_ptr(), 0 if k_weight is None else k_weight.data_ptr(),
         q_weight is not None and q_weight.dtype is torch.float32, 0 if rope_table is None else rope_table.data_ptr(), rot, max_pos, bool(interleaved), q_out.data_ptr(),
-        k.data_ptr(), v.data_ptr(), steps.data_ptr(), shape[0] * shape[2], shape[2], n_q, n_kv, d, T, _DT[dt], _stream(), eps))
+        k.data_ptr(), v.data_ptr(), steps.data_ptr(), shape[0] * shape[2], shape[2], n_q, n_kv, d, T, _DT[dt], bool(attention_next), _stream(), eps))
     if code:
         _check(code, f"qknorm_rope_kv4write (head size {d})")
     _count_launch()
@@ -2873,7 +2874,8 @@ def kv4_restore(cache: KV4Cache, pages: torch.Tensor, dtype: torch.dtype) -> Tup
 
 
 def kv4_attention(q: torch.Tensor, out: torch.Tensor, cache: KV4Cache, *, kv_len: torch.Tensor, block_table: torch.Tensor, scale: float, window: int = 0,
-                  q_start: Optional[torch.Tensor] = None, q_lens: Optional[Sequence[int]] = None, kv_lens: Optional[Sequence[int]] = None, workspace=None) -> None:
+                  q_start: Optional[torch.Tensor] = None, q_lens: Optional[Sequence[int]] = None, kv_lens: Optional[Sequence[int]] = None, workspace=None,
+                  fields_ahead: bool = False) -> None:
     """Causal attention of a step's tokens over a paged cache in 4 bits: q and out [T, heads, head size] float32 or bfloat16, kv_len int32 [B] the tokens of every request in
     the cache with this step's, block_table int32 [B, pages].  Without q_lens every request brings one token, request r token r (the form that a graph
     captures); with it, the host's number of tokens of every request, which lie at q_start[r] .. q_start[r + 1] (int32 [B + 1]), and kv_lens, the host's copy of kv_len.
@@ -2881,7 +2883,9 @@ def kv4_attention(q: torch.Tensor, out: torch.Tensor, cache: KV4Cache, *, kv_len
     stay as they are, and so do all rows of a request without tokens.  A page number outside the cache reads as zeros.
 
     Requests with few tokens read the codes themselves; for longer runs the keys and values that they see are first put back into q's type, once a call, in scratch
-    memory of up to KV4_RESTORE_BYTES (more only where one request needs it).  workspace: where scratch memory is kept between calls (`parts.Workspace`); calls that share one run one after the other."""
+    memory of up to KV4_RESTORE_BYTES (more only where one request needs it).  workspace: where scratch memory is kept between calls (`parts.Workspace`); calls that share one run one after the other.
+    fields_ahead: kv_len, block_table and q_start were written three launches or more before this one (as a step's fields are in a model's layers): they are read while the launch
+    ahead of this one ends."""
     (k, v, steps), dt, dev = cache, q.dtype, q.get_device()
     shape, i32 = k.shape, torch.int32
     # every argument is looked at in one go, and told apart only where something is wrong: small steps wait for the host
@@ -2917,14 +2921,14 @@ def kv4_attention(q: torch.Tensor, out: torch.Tensor, cache: KV4Cache, *, kv_len
     if q.shape[0] == 0 or B == 0 or few == most == 0:
         return
     if most <= direct:
-        _kv4_few(q, out, cache, kv_len, block_table, scale, window, q_start if q_lens is not None else None, few, None if q_lens is None else max(kv_lens), workspace)
+        _kv4_few(q, out, cache, kv_len, block_table, scale, window, q_start if q_lens is not None else None, few, None if q_lens is None else max(kv_lens), workspace, 1 if fields_ahead else 0)
         return
 
     scratch = _kv4_scratch(q, cache, few, workspace) if few and tensor else None          # (ahead of the launch that the rest may run beside: it may have to be cleared)
 
     def runs_of_few(beside: bool) -> None:
         if few:
-            _kv4_few(q, out, cache, kv_len, block_table, scale, window, q_start, few, max(kv for n, kv in zip(q_lens, kv_lens) if 0 < n <= direct), workspace, beside, scratch)
+            _kv4_few(q, out, cache, kv_len, block_table, scale, window, q_start, few, max(kv for n, kv in zip(q_lens, kv_lens) if 0 < n <= direct), workspace, 2 if beside else 0, scratch)
 
     _kv4_portions(q, out, cache, kv_len, block_table, scale, window, q_start, q_lens, kv_lens, direct + 1, workspace, runs_of_few)
 
@@ -2995,9 +2999,9 @@ def _sm(q) -> int:
     return _sms.get(dev) or _sms.setdefault(dev, sm_count(q.device))
 
 
-def _kv4_few(q, out, cache, kv_len, block_table, scale, window, q_start, max_q, longest, workspace, beside=False, scratch=None) -> None:
-    """The requests with 1 to max_q tokens, from the codes; `longest` bounds their keys (None: the block table does).  beside: the launch before this one is the prefill
-    kernel of the same call, which writes nothing that is read here and beside which it may run."""
+def _kv4_few(q, out, cache, kv_len, block_table, scale, window, q_start, max_q, longest, workspace, ahead=0, scratch=None) -> None:
+    """The requests with 1 to max_q tokens, from the codes; `longest` bounds their keys (None: the block table does).  ahead: what was written before the launch
+    ahead of this one: 1, the fields of the step; 2, all that is read here (that launch is the prefill kernel of the same call, beside which this one may run)."""
     (T, n_q, d), (pages, n_kv, page_size, _), (B, width) = q.shape, cache.k.shape, block_table.shape
     lib, G, sms = _kv4_lib(), n_q // n_kv, _sm(q)
     at_k, at_v, at_steps, at_q, at_out, at_kv, at_table, row = (cache.k.data_ptr(), cache.v.data_ptr(), cache.steps.data_ptr(), q.data_ptr(), out.data_ptr(), kv_len.data_ptr(),
@@ -3014,7 +3018,7 @@ def _kv4_few(q, out, cache, kv_len, block_table, scale, window, q_start, max_q, 
             first = 0 if q_start is not None else a          # (without q_start token r is request r's)
             code = lib.msgl_kv4_attention_runs(_KV4_RUNS(
                 at_q + first * n_q * d * 2, at_out + first * n_q * d * 2, at_k, at_v, at_steps, at_start + 4 * a if at_start else 0, at_kv + 4 * a, at_table + 4 * a * row, row, width,
-                at, at + 4 * n_part * 128, at + 4 * n_part * 130, sms, min(B - a, _KV4_REQUESTS), T - first, n_q, n_kv, d, page_size, pages, window, max_q, beside and a == 0, _stream(), scale))
+                at, at + 4 * n_part * 128, at + 4 * n_part * 130, sms, min(B - a, _KV4_REQUESTS), T - first, n_q, n_kv, d, page_size, pages, window, max_q, ahead if a == 0 else 0, _stream(), scale))
             if code:
                 _check(code, "kv4_attention")
             _count_launch()

@@ -110,12 +110,12 @@ class PagedAttention(Mixer):
             raise ValueError("drafted tokens need a cache of the activations' type")
         norm = dict(q_weight=self.q_norm, k_weight=self.k_norm, eps=self.qk_norm_eps, rope_table=table, interleaved=bool(getattr(self.position, "interleaved", False)))
         if writes_cache:
-            q = ops.qknorm_rope_kv4write(qkv, ctx.positions, self.n_q, self.n_kv, self.d, out_loc=cache.group.out_loc, cache=cache.cache, **norm)
+            q = ops.qknorm_rope_kv4write(qkv, ctx.positions, self.n_q, self.n_kv, self.d, out_loc=cache.group.out_loc, cache=cache.cache, attention_next=ctx.uniform_decode, **norm)
         else:
             q = ops.qknorm_rope_kvwrite(qkv, ctx.positions, self.n_q, self.n_kv, self.d, out_loc=None, k_cache=None, v_cache=None, page_size=cache.page_size, **norm)
         out = torch.empty_like(q)
         lens = {} if ctx.uniform_decode else dict(q_start=ctx.q_start, q_lens=ctx.host_q_lens, kv_lens=ctx.host_kv_lens)
-        ops.kv4_attention(q, out, cache.cache, kv_len=ctx.kv_len, block_table=cache.group.block_table, scale=self.scale, window=int(self.window or 0), workspace=ctx.workspace, **lens)
+        ops.kv4_attention(q, out, cache.cache, kv_len=ctx.kv_len, block_table=cache.group.block_table, scale=self.scale, window=int(self.window or 0), workspace=ctx.workspace, fields_ahead=True, **lens)
         return out
 
     def attend(self, q: torch.Tensor, out: torch.Tensor, ctx: StepContext, cache: KVCacheView) -> None:

@@ -83,7 +83,7 @@ def test_every_layer_attends_to_what_it_wrote(name, dtype, window, monkeypatch):
     calls = dict(write=0, attend=0)
     write, attend = ops.qknorm_rope_kv4write, ops.kv4_attention
 
-    def checked_write(qkv, positions, n_q, n_kv, d, *, q_weight, k_weight, eps, rope_table, out_loc, cache, interleaved=False):
+    def checked_write(qkv, positions, n_q, n_kv, d, *, q_weight, k_weight, eps, rope_table, out_loc, cache, interleaved=False, attention_next=False):
         want = tuple(t.clone() for t in cache)
         q = write(qkv, positions, n_q, n_kv, d, q_weight=q_weight, k_weight=k_weight, eps=eps, rope_table=rope_table, out_loc=out_loc, cache=cache, interleaved=interleaved)
         q_plain = plain_kv4.append(qkv, positions, n_q, n_kv, d, q_weight, k_weight, eps, rope_table, out_loc, want, interleaved)
@@ -91,8 +91,9 @@ def test_every_layer_attends_to_what_it_wrote(name, dtype, window, monkeypatch):
         calls["write"] += 1
         return q
 
-    def checked_attend(q, out, cache, *, kv_len, block_table, scale, window=0, q_start=None, q_lens=None, kv_lens=None, workspace=None):
-        attend(q, out, cache, kv_len=kv_len, block_table=block_table, scale=scale, window=window, q_start=q_start, q_lens=q_lens, kv_lens=kv_lens, workspace=workspace)
+    def checked_attend(q, out, cache, *, kv_len, block_table, scale, window=0, q_start=None, q_lens=None, kv_lens=None, workspace=None, fields_ahead=False):
+        attend(q, out, cache, kv_len=kv_len, block_table=block_table, scale=scale, window=window, q_start=q_start, q_lens=q_lens, kv_lens=kv_lens, workspace=workspace,
+               fields_ahead=fields_ahead)
         lens, kvs = q_lens or [1] * len(kv_len), kv_len.tolist()
         assert kv_lens is None or kvs == list(kv_lens)
         starts = [sum(lens[:i]) for i in range(len(lens) + 1)]
