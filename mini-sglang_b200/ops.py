@@ -2714,6 +2714,7 @@ KV4_MAX_HEAD_DIM = 512
 KV4_DIRECT_ROWS, KV4_MIDDLE_ROWS, KV4_DIRECT_ROWS_F32 = 80, 512, 32
 KV4_US = 0.118, 2.5, 2.6          # SM microseconds: codes of 32 keys for 8 rows; restoring 128 keys; 128 keys of a tile of 256 rows of the prefill kernel
 _KV4_REQUESTS = 256               # requests of one launch that deals the keys out
+_KV4_PAGE = 128                   # keys of a restored page
 KV4_RESTORE_BYTES = 1 << 30       # of restored keys and values, what a step makes at a time
 _kv4 = None
 _sms = {}                        # SMs of the devices, by number
@@ -2724,6 +2725,7 @@ def _kv4_lib():
     if _kv4 is None:
         lib = _build.kv4_library()
         lib.msgl_kv4_append.argtypes = lib.msgl_kv4_restore.argtypes = lib.msgl_kv4_attention_any.argtypes = lib.msgl_kv4_attention_runs.argtypes = [ctypes.c_char_p]
+        assert lib.msgl_kv4_restored_page() == _KV4_PAGE
         _kv4 = lib
     return _kv4
 
@@ -3037,9 +3039,8 @@ def _kv4_few(q, out, cache, kv_len, block_table, scale, window, q_start, max_q, 
 def _kv4_portions(q, out, cache, kv_len, block_table, scale, window, q_start, q_lens, kv_lens, min_q, workspace, others) -> None:
     """The requests with at least min_q tokens: what they see is restored into pages of its own, which the prefill kernels then read.  others(beside) launches the rest of the
     step: beside the tiles of the tcgen05 kernel where that runs, whose last blocks leave SMs free."""
-    (T, n_q, d), (pages, n_kv, page_size, _), width = q.shape, cache.k.shape, block_table.shape[1]
+    (T, n_q, d), (pages, n_kv, page_size, _), width, per, dt = q.shape, cache.k.shape, block_table.shape[1], _KV4_PAGE, q.dtype
     lib, G, big = _kv4_lib(), n_q // n_kv, 1 << 30
-    per = int(lib.msgl_kv4_restored_page())
     need = [0 if n < min_q else -(-kv // per) - (max(kv - n - window + 1, 0) // per if window else 0) for n, kv in zip(q_lens, kv_lens)]
     page_numel = n_kv * per * d
     most = max(1, KV4_RESTORE_BYTES // (2 * page_numel * q.element_size()))
@@ -3050,21 +3051,24 @@ def _kv4_portions(q, out, cache, kv_len, block_table, scale, window, q_start, q_
             n += need[b]
             b += 1
         if n:
-            t_width = max(-(-kv // per) for kv in kv_lens[a:b])
-            sizes = (("kv4_keys", n * page_numel, q.dtype), ("kv4_values", n * page_numel, q.dtype), ("kv4_table", (b - a) * t_width, torch.int32))
-            k, v, table = (torch.empty(m, dtype=t, device=q.device) if workspace is None else workspace.get(name, m, t) for name, m, t in sizes)
-            lens, kvs, starts, kv_part = q_lens[a:b], kv_lens[a:b], q_start[a:b + 1], kv_len[a:b]
+            whole = b - a == len(need)
+            lens, kvs, starts, kv_part, rows = ((q_lens, kv_lens, q_start, kv_len, block_table) if whole else (q_lens[a:b], kv_lens[a:b], q_start[a:b + 1], kv_len[a:b], block_table[a:b]))
+            t_width = -(-max(kvs) // per)
+            if workspace is None:
+                kv, table = torch.empty(2 * n * page_numel, dtype=dt, device=q.device), torch.empty((b - a) * t_width, dtype=torch.int32, device=q.device)
+            else:
+                kv, table = workspace.get("kv4_restored", 2 * n * page_numel, dt), workspace.get("kv4_table", (b - a) * t_width, torch.int32)
+            (k, v), table = kv.view(2, n, n_kv, per, d).unbind(0), table.view(b - a, t_width)
             code = lib.msgl_kv4_restore(_KV4_RESTORE(cache.k.data_ptr(), cache.v.data_ptr(), cache.steps.data_ptr(), k.data_ptr(), v.data_ptr(), 0, n, starts.data_ptr(),
-                                                     kv_part.data_ptr(), block_table[a:b].data_ptr(), block_table.stride(0), width, table.data_ptr(), t_width, b - a, window, min_q,
-                                                     n_kv, page_size, pages, d, _DT[q.dtype], _stream()))
+                                                     kv_part.data_ptr(), rows.data_ptr(), block_table.stride(0), width, table.data_ptr(), t_width, b - a, window, min_q,
+                                                     n_kv, page_size, pages, d, _DT[dt], _stream()))
             _check(code, "kv4_attention (keys restored)")
-            k, v, table = k.view(n, n_kv, per, d), v.view(n, n_kv, per, d), table.view(b - a, t_width)
             common = dict(q_start=starts, kv_len=kv_part, block_table=table, n_kv=n_kv, page_size=per, window=window, scale=scale, qlen_min=min_q, qlen_max=big)
             beside = (lambda: others(True)) if not any(need[b:]) else None
-            if tc_supported(d, q.dtype, G) and attention_tc(q, out, k, v, q_lens=lens, kv_lens=kvs, workspace=workspace, beside=beside, **common):
+            if tc_supported(d, dt, G) and attention_tc(q, out, k, v, q_lens=lens, kv_lens=kvs, workspace=workspace, beside=beside, **common):
                 launched = beside is not None
             else:
-                variant = VARIANT_MMA_ROWS if mma_supported(d, q.dtype) else VARIANT_SIMT
+                variant = VARIANT_MMA_ROWS if mma_supported(d, dt) else VARIANT_SIMT
                 qt = attention_tile_tokens(variant, G, d)
                 attention(q, out, k, v, nsplit=None, part_o=None, part_ml=None, max_split=1, uniform_decode=False, variant=variant,
                           grid_x=sum(-(-m // qt) for m in lens if m >= min_q), **common)
