@@ -24,6 +24,14 @@
 // Scores, p, sums and outputs are float32.  S^T = K Q^T with keys on the M dimension, the head's elements permuted so that a lane reads 16 bytes
 // of a row; P goes through movmatrix; V^T fragments come by ldmatrix.trans on 16-bit columns, four codes of two neighbouring keys a register.  The
 // exponentials' reference moves only where a score lies KR_LAZY above it.
+//
+// What bounds it.  Where there is work for all SMs, the operations of a unit: 585 instructions a warp for 4.3 KB, 144 of them to take codes apart, on a pipe that takes half an instruction a
+// cycle; 64 requests of up to 16,000 keys (32 heads on 8, 794 MB) 152 us, 5.2 TB/s, 0.81 of copy.  Copies alone take 146 us so, arithmetic alone 147 (in blocks of 12 warps; together 195, then).  16 warps at
+// 128 registers 150, 12 at 152 with three units a ring 154, 8 at 159 with four 179.  Few keys: latency; 1 request of 1,000 keys 10.5 us: 1.5 until the warps know
+// their units, 1.4 for pages and queries, 2.5 for two units, 3 to add up and write.  16 requests of up to 4,096 keys 23 us (floor 8.4).
+// A block that handed units to its warps in turn, with a barrier and a merge a segment, took 195 us for the first case and 58 where this takes 32 (123 requests of up to 777 keys, 64 heads).  bfloat16 codes
+// 1 + c / 16 took 275 (two operations more a pair).  16 rows a segment, two products for every pair of codes, halve the codes' work but leave registers for 8 warps: 8 requests
+// of 32 tokens behind 8,000 keys 200 -> 177, 12 of 5 tokens behind 2,000 26 -> 30: not kept.
 #pragma once
 #include <type_traits>
 
