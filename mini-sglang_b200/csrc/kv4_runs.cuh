@@ -57,12 +57,14 @@ struct Kv4Runs {
 };
 
 __device__ __forceinline__ unsigned kr_smem(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
-// copies of 16 and 8 bytes, or of that many zeros (bytes = 0); offsets are compile-time numbers, so that they cost no additions
-template <int S, int G> __device__ __forceinline__ void kr_cp16(unsigned s, const void* g, int bytes) {
-    asm volatile("cp.async.cg.shared.global [%0 + %3], [%1 + %4], 16, %2;\n" ::"r"(s), "l"(g), "r"(bytes), "n"(S), "n"(G));
+// copies of 16 and 8 bytes; ZERO: or of that many zeros (there = false).  Offsets are compile-time numbers, so that they cost no additions
+template <int S, int G, bool ZERO> __device__ __forceinline__ void kr_cp16(unsigned s, const void* g, bool there) {
+    if (ZERO) asm volatile("{\n.reg .pred p;\nsetp.eq.u32 p, %2, 0;\ncp.async.cg.shared.global [%0 + %3], [%1 + %4], 16, p;\n}\n" ::"r"(s), "l"(g), "r"((unsigned)there), "n"(S), "n"(G));
+    else asm volatile("cp.async.cg.shared.global [%0 + %2], [%1 + %3], 16;\n" ::"r"(s), "l"(g), "n"(S), "n"(G));
 }
-__device__ __forceinline__ void kr_cp8(unsigned s, const void* g, int bytes) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;\n" ::"r"(s), "l"(g), "r"(bytes));
+template <bool ZERO> __device__ __forceinline__ void kr_cp8(unsigned s, const void* g, bool there) {
+    if (ZERO) asm volatile("{\n.reg .pred p;\nsetp.eq.u32 p, %2, 0;\ncp.async.ca.shared.global [%0], [%1], 8, p;\n}\n" ::"r"(s), "l"(g), "r"((unsigned)there));
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], 8;\n" ::"r"(s), "l"(g));
 }
 // f(0), f(1), ... with the number as a constant
 template <int N, int I = 0, typename F> __device__ __forceinline__ void kr_each(F f) {
@@ -253,23 +255,26 @@ __global__ void __launch_bounds__(NW * 32, 1) kv4_attn_runs_kernel(const Kv4Runs
     if (n_my > 0) {
         settle(seg);
 
-        // ---- the warp's loader.  WHOLE: a page holds whole runs of 16 keys, and all lanes know where the unit's two runs lie (rows behind the request's last key are
-        // copied as they are, and hidden); else a lane knows the row of key `lane`.  The pages are looked up a unit before they are asked for.
+        // ---- the warp's loader.  WHOLE: a page is a power of two of 16 keys or more, and all lanes know where the unit's two runs of 16 lie (rows behind the request's last
+        // key are copied as they are, and hidden); else a lane knows the row of key `lane`.  The pages are looked up a unit before they are asked for.
         KrCursor ld = seg;
+        const int* ld_table = p.block_table + ld.r * p.bt_stride;
         struct Place { int page0, page1, add0, add1; };      // row: page * n_kv * page_size + add
         const int page_rows = p.n_kv * p.page_size;
         auto look_up = [&](int key, int& page, int& add) {
             page = -1;
-            add = 0;
             if (key >= ld.keys) return;
-            const int at = p.page_shift >= 0 ? key >> p.page_shift : key / p.page_size;
-            add = ld.kvh * p.page_size + (key - at * p.page_size);
-            page = p.block_table[ld.r * p.bt_stride + at];
+            const int at = WHOLE ? key >> p.page_shift : key / p.page_size;
+            add = ld.kvh * p.page_size + (WHOLE ? key & (p.page_size - 1) : key - at * p.page_size);
+            page = ld_table[at];
         };
         auto place_of = [&](int x) -> Place {
             Place w = {-1, -1, 0, 0};
             if (x >= hi) return w;
-            while (x >= ld.c0 + ld.u) { ++ld.s; settle(ld); }
+            if (x >= ld.c0 + ld.u) {
+                do { ++ld.s; settle(ld); } while (x >= ld.c0 + ld.u);
+                ld_table = p.block_table + ld.r * p.bt_stride;
+            }
             const int key = (int)((unsigned)x * KR_KEYS + ld.key0);
             look_up(WHOLE ? key : key + lane, w.page0, w.add0);
             if (WHOLE) look_up(key + 16, w.page1, w.add1);
@@ -279,31 +284,38 @@ __global__ void __launch_bounds__(NW * 32, 1) kv4_attn_runs_kernel(const Kv4Runs
         const int l_row = lane / CH, l_ch = lane % CH;
         const unsigned l_dst = ring + l_row * ROW + ((l_ch ^ ((l_row >> SW) & (CH - 1))) << 4);
         static_assert(PER % (CH << SW) == 0, "one place for all copies");
+        const unsigned char *k_lane = p.k + lane * 16, *v_lane = p.v + lane * 16;
         auto load = [&](unsigned st, const Place& w) {    // st: the stage's offset in the ring
             if (WHOLE) {
-                const int b0 = (unsigned)w.page0 < (unsigned)p.pages ? 16 : 0, b1 = (unsigned)w.page1 < (unsigned)p.pages ? 16 : 0;
-                const unsigned r0 = b0 ? (unsigned)w.page0 * page_rows + w.add0 : 0u, r1 = b1 ? (unsigned)w.page1 * page_rows + w.add1 : 0u;
-                const size_t o0 = (size_t)r0 * ROW + lane * 16, o1 = (size_t)r1 * ROW + lane * 16;
-                const unsigned char *k0 = p.k + o0, *v0 = p.v + o0, *k1 = p.k + o1, *v1 = p.v + o1;
-                kr_each<CH>([&](auto m) {
-                    constexpr int R = m.value * PER, H = R / 16, S = R * ROW, O = (R - 16 * H) * ROW;
-                    kr_cp16<S, O>(l_dst + st, H ? k1 : k0, H ? b1 : b0);
-                    kr_cp16<S + KV_BYTES, O>(l_dst + st, H ? v1 : v0, H ? b1 : b0);
-                });
+                const bool t0 = (unsigned)w.page0 < (unsigned)p.pages, t1 = (unsigned)w.page1 < (unsigned)p.pages;
+                const unsigned r0 = t0 ? (unsigned)w.page0 * page_rows + w.add0 : 0u, r1 = t1 ? (unsigned)w.page1 * page_rows + w.add1 : 0u;
+                const unsigned char *k0 = k_lane + (size_t)r0 * ROW, *v0 = v_lane + (size_t)r0 * ROW, *k1 = k_lane + (size_t)r1 * ROW, *v1 = v_lane + (size_t)r1 * ROW;
                 const bool up = lane & 16;
-                kr_cp8(ring + st + 2 * KV_BYTES + lane * 8, p.steps + (up ? r1 : r0) + (lane & 15), up ? b1 >> 1 : b0 >> 1);
+                const uint2* s0 = p.steps + ((up ? r1 : r0) + (lane & 15));
+                auto copy = [&](auto zero) {
+                    constexpr bool ZERO = zero.value;
+                    kr_each<CH>([&](auto m) {
+                        constexpr int R = m.value * PER, H = R / 16, S = R * ROW, O = (R - 16 * H) * ROW;
+                        kr_cp16<S, O, ZERO>(l_dst + st, H ? k1 : k0, H ? t1 : t0);
+                        kr_cp16<S + KV_BYTES, O, ZERO>(l_dst + st, H ? v1 : v0, H ? t1 : t0);
+                    });
+                    kr_cp8<ZERO>(ring + st + 2 * KV_BYTES + lane * 8, s0, up ? t1 : t0);
+                };
+                if (t0 && t1) copy(std::false_type{});
+                else copy(std::true_type{});
             } else {
                 const unsigned row = (unsigned)w.page0 < (unsigned)p.pages ? (unsigned)w.page0 * page_rows + w.add0 : 0xffffffffu;
                 kr_each<CH>([&](auto m) {
                     constexpr int S = m.value * PER * ROW;
                     const unsigned src = __shfl_sync(0xffffffffu, row, m.value * PER + l_row);
                     const size_t off = src != 0xffffffffu ? (size_t)src * ROW + l_ch * 16 : 0;
-                    kr_cp16<S, 0>(l_dst + st, p.k + off, src != 0xffffffffu ? 16 : 0);
-                    kr_cp16<S + KV_BYTES, 0>(l_dst + st, p.v + off, src != 0xffffffffu ? 16 : 0);
+                    kr_cp16<S, 0, true>(l_dst + st, p.k + off, src != 0xffffffffu);
+                    kr_cp16<S + KV_BYTES, 0, true>(l_dst + st, p.v + off, src != 0xffffffffu);
                 });
-                kr_cp8(ring + st + 2 * KV_BYTES + lane * 8, p.steps + (row != 0xffffffffu ? row : 0u), row != 0xffffffffu ? 8 : 0);
+                kr_cp8<true>(ring + st + 2 * KV_BYTES + lane * 8, p.steps + (row != 0xffffffffu ? row : 0u), row != 0xffffffffu);
             }
         };
+
         // Q as B operand: lane (g, t) holds row g's elements e, e + 4 of each of its words of eight, e = 0..3
         const float sc = p.scale * 1.4426950408889634f;
         unsigned qf[QW][4];
@@ -437,16 +449,21 @@ __global__ void __launch_bounds__(NW * 32, 1) kv4_attn_runs_kernel(const Kv4Runs
 #pragma unroll
                         for (int e = 0; e < 2; ++e) v[m][2 * h + e] = fmaf(a * q_step[e], s[m][0][2 * h + e] + s[m][1][2 * h + e], fmaf(b, q_base[e], -mu_c[e]));
                     }
-                const bool edge = key0 + KR_KEYS > all_end || key0 < all_from;
-                unsigned hidden = 0;                      // bit 4 m + e: value e of part m is a key that its row does not see
-                if (edge) {
+                if (key0 + KR_KEYS > all_end || key0 < all_from) {      // keys that some row does not see
 #pragma unroll
                     for (int m = 0; m < 2; ++m)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int key = key0 + 16 * m + g + ((e & 2) ? 8 : 0);
-                            if (key >= c_end[e & 1] || key < c_from[e & 1]) { v[m][e] = -INFINITY; hidden |= 1u << (4 * m + e); }
-                            if (key >= seg.keys) row_st[m][e >> 1].y = 0u;      // (whatever lies behind the request's last key)
+                        for (int h = 0; h < 2; ++h) {
+                            const int key = key0 + 16 * m + 8 * h + g;
+                            // a value row that is no number shows through the scores of those who see it, and counts for nothing elsewhere; nor does what lies behind the last key
+                            const unsigned y = row_st[m][h].y;
+                            const bool number = (y & 0x7f800000u) != 0x7f800000u && (y & 0x7f80u) != 0x7f80u;
+                            if (!number || key >= seg.keys) row_st[m][h].y = 0u;
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                if (!number) v[m][2 * h + e] = CUDART_NAN_F;
+                                if (key >= c_end[e] || key < c_from[e]) v[m][2 * h + e] = -INFINITY;
+                            }
                         }
                 }
                 float st_f[2][2];                         // values' steps times F
@@ -507,17 +524,9 @@ __global__ void __launch_bounds__(NW * 32, 1) kv4_attn_runs_kernel(const Kv4Runs
                         const float p0 = kr_exp2(v[m][2 * h]), p1 = kr_exp2(v[m][2 * h + 1]);
                         l_c[0] += p0;
                         l_c[1] += p1;
-                        unsigned w = kr_half2(p0 * st_f[m][h], p1 * st_f[m][h]);
-                        if (edge) {                       // a key that a row does not see counts for nothing, whatever it holds
-                            const bool h0 = hidden >> (4 * m + 2 * h) & 1u, h1 = hidden >> (4 * m + 2 * h + 1) & 1u;
-                            if (!h0) z_c[0] = fmaf(p0, base, z_c[0]);
-                            if (!h1) z_c[1] = fmaf(p1, base, z_c[1]);
-                            w &= (h0 ? 0u : 0xffffu) | (h1 ? 0u : 0xffff0000u);
-                        } else {
-                            z_c[0] = fmaf(p0, base, z_c[0]);
-                            z_c[1] = fmaf(p1, base, z_c[1]);
-                        }
-                        pb[m][h] = kr_trans(w);
+                        z_c[0] = fmaf(p0, base, z_c[0]);
+                        z_c[1] = fmaf(p1, base, z_c[1]);
+                        pb[m][h] = kr_trans(kr_half2(p0 * st_f[m][h], p1 * st_f[m][h]));
                     }
                 // ---- the middles of the codes times the weights, out of all sums (the same for every element)
                 float d_mid[4];
@@ -763,7 +772,7 @@ MSGL_API int msgl_kv4_attention_runs(const Kv4RunsArgs* x) {
     Kv4Runs p = {(const __nv_bfloat16*)q, (__nv_bfloat16*)out, (const unsigned char*)k, (const unsigned char*)v, (const uint2*)steps, q_start, kv_len, block_table, part_o,
                  part_ml, count, bt_stride, B, T, n_q, n_kv, page_size, -1, pages, bt_width, window, max_q, (int)x->ahead, scale};
     if ((page_size & (page_size - 1)) == 0) { p.page_shift = 0; while ((1 << p.page_shift) < page_size) ++p.page_shift; }
-    const bool whole = page_size % 16 == 0;
+    const bool whole = page_size >= 16 && p.page_shift >= 0;
 #define KR_GO(DD, WW) if (d == DD && whole == WW) msgl_launch_pdl(kv4_attn_runs_kernel<DD, KR_NW, KR_ST, WW>, dim3(blocks), dim3(KR_NW * 32), kr_smem_bytes<DD, KR_NW, KR_ST>(), stream, p);
     KR_EACH(KR_GO)
 #undef KR_GO
