@@ -25,10 +25,11 @@
 // of a row; P goes through movmatrix; V^T fragments come by ldmatrix.trans on 16-bit columns, four codes of two neighbouring keys a register.  The
 // exponentials' reference moves only where a score lies KR_LAZY above it.
 //
-// What bounds it.  Where there is work for all SMs, the operations of a unit: 585 instructions a warp for 4.3 KB, 144 of them to take codes apart, on a pipe that takes half an instruction a
-// cycle; 64 requests of up to 16,000 keys (32 heads on 8, 794 MB) 152 us, 5.2 TB/s, 0.81 of copy.  Copies alone take 146 us so, arithmetic alone 147 (in blocks of 12 warps; together 195, then).  16 warps at
-// 128 registers 150, 12 at 152 with three units a ring 154, 8 at 159 with four 179.  Few keys: latency; 1 request of 1,000 keys 10.5 us: 1.5 until the warps know
-// their units, 1.4 for pages and queries, 2.5 for two units, 3 to add up and write.  16 requests of up to 4,096 keys 23 us (floor 8.4).
+// What bounds it.  Where there is work for all SMs, the operations of a unit: 530 instructions a warp for 4.3 KB, 144 of them to take codes apart, on a pipe that takes half an instruction a
+// cycle; 64 requests of up to 16,000 keys (32 heads on 8, 794 MB) 141 us, 5.6 TB/s, 0.87 of copy.  With nine copies a lane for every unit whose sizes are looked at one by one it took 152, with
+// selects for hidden keys in the inner loop 3 us more.  12 warps at 160 registers and three units a ring 141, 16 at 128 and two 145, 14 164, 8 with four 179 (before the last steps).  Few keys:
+// latency; 1 request of 1,000 keys 10 us: 1.5 until the warps know their units, 1.4 for pages and queries, 2.5 for two units, 3 to add up and write.  16 requests of up to 4,096 keys 22 us
+// (floor 8.4).
 // A block that handed units to its warps in turn, with a barrier and a merge a segment, took 195 us for the first case and 58 where this takes 32 (123 requests of up to 777 keys, 64 heads).  bfloat16 codes
 // 1 + c / 16 took 275 (two operations more a pair).  16 rows a segment, two products for every pair of codes, halve the codes' work but leave registers for 8 warps: 8 requests
 // of 32 tokens behind 8,000 keys 200 -> 177, 12 of 5 tokens behind 2,000 26 -> 30: not kept.
@@ -39,8 +40,8 @@ constexpr float KR_LAZY = 8.f;
 constexpr int KR_KEYS = 32;          // keys of a unit
 constexpr int KR_MAX_B = 256;        // requests of a launch, a thread each
 constexpr int KR_PIECE = 16;         // units of a block's piece at least, where segments are cut by themselves ...
-constexpr int KR_ALONE = 48;         // ... and none of up to this many units is
-constexpr int KR_HEAD = 1;           // what a segment costs beside its units, in units
+constexpr int KR_ALONE = 48;         // ... and none of up to this many units is (32 units, 1 request of 1,000 keys: whole 10.1 us, in two pieces 10.8)
+constexpr int KR_HEAD = 2;           // what a segment costs beside its units, in units (1: 12 of 5 tokens 26.4 us instead of 25.7; 3 and 4 are behind)
 
 struct Kv4Runs {
     const __nv_bfloat16* q; __nv_bfloat16* out;
@@ -731,11 +732,7 @@ __global__ void __launch_bounds__(NW * 32, 1) kv4_attn_runs_kernel(const Kv4Runs
     leave();
 }
 
-#ifndef KR_WARPS
-#define KR_WARPS 16
-#define KR_STAGES 2
-#endif
-constexpr int KR_NW = KR_WARPS, KR_ST = KR_STAGES;
+constexpr int KR_NW = 12, KR_ST = 3;      // warps of a block, units of a warp's ring
 
 // Requests with 1 .. max_q tokens; q_start null: request r has token r.  count: a word for every 8 rows of a request under a kv head, zero before and after.
 struct Kv4RunsArgs {
