@@ -87,6 +87,7 @@ struct Kv4Append {
     long long slots;                                      // of the cache: page numbers beyond are left out
     int page_size, n_q, n_kv, d, T;
     int early;                                            // the next launch may start while this one waits for the one ahead
+    unsigned magic; int shift;                            // for quotients by the number of heads of a token, at least 2: (h + (x - h) / 2) >> shift with h = x magic >> 32 (Granlund and Montgomery)
     __device__ __forceinline__ long long row_of_slot(int slot, int kvh) const {      // -1: nowhere
         if (slot < 0 || slot >= slots) return -1;
         const int page = slot / page_size;
@@ -195,7 +196,8 @@ __global__ void __launch_bounds__(KV4_APPEND_THREADS, 9) kv4_append_vec_kernel(c
     constexpr int d = 16 * L, half = 8 * L, V = 16 / sizeof(T), N = 8 / V;          // elements of a 16-byte piece, pieces of eight elements
     const int l = threadIdx.x & (L - 1), n_heads = p.n_q + 2 * p.n_kv;
     const unsigned unit = blockIdx.x * (KV4_APPEND_THREADS / L) + threadIdx.x / L;
-    const int token = (int)(unit / (unsigned)n_heads), head = (int)(unit - (unsigned)token * n_heads), t = min(token, p.T - 1);      // past the end: the last token again, not stored
+    const unsigned high = __umulhi(unit, p.magic);
+    const int token = (int)((high + ((unit - high) >> 1)) >> p.shift), head = (int)(unit - (unsigned)token * n_heads), t = min(token, p.T - 1);      // past the end: the last token again, not stored
     const bool is_q = head < p.n_q, is_k = !is_q && head < p.n_q + p.n_kv, turns = (is_q || is_k) && p.table != nullptr;
     const void* nw = is_q ? p.qw : (is_k ? p.kw : nullptr);
     if (p.early) pdl_small();
@@ -257,13 +259,14 @@ __global__ void __launch_bounds__(KV4_APPEND_THREADS, 9) kv4_append_vec_kernel(c
     if (turns) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            float a[2], b[2], c[2], s[2];                 // (one by one: packed products and sums are contracted)
-            f2_get(x[k], a[0], a[1]);
-            f2_get(x[4 + k], b[0], b[1]);
-            f2_get(ang[k], c[0], c[1]);
-            f2_get(ang[4 + k], s[0], s[1]);
-            x[k] = f2(rot_sub(a[0], c[0], b[0], s[0]), rot_sub(a[1], c[1], b[1], s[1]));
-            x[4 + k] = f2(rot_add(a[0], s[0], b[0], c[0]), rot_add(a[1], s[1], b[1], c[1]));
+            const F2 a = x[k], b = x[4 + k], c = ang[k], s = ang[4 + k];
+            float ac[2], bs[2], as[2], bc[2];             // (sums one by one: packed sums of packed products are contracted)
+            f2_get(f2_mul(a, c), ac[0], ac[1]);
+            f2_get(f2_mul(b, s), bs[0], bs[1]);
+            f2_get(f2_mul(a, s), as[0], as[1]);
+            f2_get(f2_mul(b, c), bc[0], bc[1]);
+            x[k] = f2(__fsub_rn(ac[0], bs[0]), __fsub_rn(ac[1], bs[1]));
+            x[4 + k] = f2(__fadd_rn(as[0], bc[0]), __fadd_rn(as[1], bc[1]));
         }
     }
     if (is_q) {
@@ -336,7 +339,10 @@ MSGL_API int msgl_kv4_append(const Kv4AppendArgs* x) {
     if (dtype != MSGL_F32 && dtype != MSGL_BF16) return MSGL_ERR_DTYPE;
     if (((uintptr_t)k | (uintptr_t)v | (uintptr_t)steps) & 15) return MSGL_ERR_ALIGN;
     Kv4Append p = {qkv, stride, positions, out_loc, qw, kw, w_f32, eps, table, rot, max_pos, interleaved, q_out, (unsigned char*)k, (unsigned char*)v, (unsigned*)steps,
-                   slots, page_size, n_q, n_kv, d, T, (int)x->early};
+                   slots, page_size, n_q, n_kv, d, T, (int)x->early, 0u, 0};
+    const unsigned n_heads = (unsigned)(n_q + 2 * n_kv);
+    while ((2ull << p.shift) < n_heads) ++p.shift;      // 2^(shift + 1) is the power of two from n_heads on
+    p.magic = (unsigned)((((2ull << p.shift) - n_heads) << 32) / n_heads + 1);
     const long long units = (long long)T * (n_q + 2 * n_kv);
     const int item = dtype == MSGL_F32 ? 4 : 2;
     const bool whole = table == nullptr || (rot == d && !interleaved && ((uintptr_t)table & 15) == 0);
