@@ -561,10 +561,14 @@ __global__ void __launch_bounds__(NW * 32, 1) kv4_attn_runs_kernel(const Kv4Runs
             }
             // ---- the segment's result, or this warp's part of it
             const KrCursor now = seg;
-            const float of = F > 0.f ? 16777216.f / F : 0.f, of16 = of * 0.0625f;
+            const float of = F > 0.f ? 1.f / F : 0.f, of16 = of * 0.0625f;
+            constexpr float UP = 16777216.f;              // (by itself: UP / F is beyond float32 for steps above 2^109)
 #pragma unroll
-            for (int mt = 0; mt < D / 16; ++mt) { o[mt][0] -= o[mt][2]; o[mt][1] -= o[mt][3]; }      // (even elements come with 16 times the odd one behind them)
-            const float even[2] = {mid[0] - mid[2], mid[1] - mid[3]}, odd[2] = {mid[2], mid[3]};
+            for (int mt = 0; mt < D / 16; ++mt) {         // even elements come with 16 times the odd one behind them
+                o[mt][0] = (o[mt][0] - o[mt][2]) * UP; o[mt][1] = (o[mt][1] - o[mt][3]) * UP;
+                o[mt][2] *= UP; o[mt][3] *= UP;
+            }
+            const float even[2] = {(mid[0] - mid[2]) * UP, (mid[1] - mid[3]) * UP}, odd[2] = {mid[2] * UP, mid[3] * UP};
 #pragma unroll
             for (int e = 0; e < 2; ++e)
 #pragma unroll

@@ -82,6 +82,17 @@ def test_steps_and_bases_of_all_sizes(n_q, n_kv, d, dtype):
 
 
 @pytest.mark.parametrize("n_q,n_kv,d,dtype", SHAPES)
+@pytest.mark.parametrize("power", [111, -90])
+def test_values_of_either_end_of_the_range(n_q, n_kv, d, dtype, power):
+    """All values times 2^111 (their steps are above 2^109; sums of 40 products with weights up to 2^8 stay below 2^128) or 2^-90 (their steps above 2^-100)."""
+    B, n = 3, 40
+    c, table = filled(10, 3 * 3 + 1, n_kv, 16, d), table_of(B, 3)
+    c.steps[..., 2:] *= 2.0 ** power
+    q = normal(11, B, n_q, d, dtype=dtype)
+    assert torch.isfinite(near(attend(q, c, [n] * B, table), q, c, [1] * B, [n] * B, table)).all()
+
+
+@pytest.mark.parametrize("n_q,n_kv,d,dtype", SHAPES)
 @pytest.mark.parametrize("kept", [True, False])
 def test_a_captured_call_reads_what_is_there_when_it_is_replayed(n_q, n_kv, d, dtype, kept):
     B, width = 5, 40
