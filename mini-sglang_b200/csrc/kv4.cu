@@ -174,9 +174,9 @@ __global__ void kv4_append_kernel(const Kv4Append p) {
 // Head sizes 32, 64, 128, 256 whose rotation (if any) covers the whole head in halves: L = d / 16 lanes own one head of a token, a lane eight
 // elements of the lower half and the eight that they are rotated with, so that every copy is 16 bytes, every word of codes one lane's, and only the sum
 // and the extremes take shuffles.  All that a lane reads but the weights is asked for before it works on any of it.
-// Bound by its operations (350 instructions a warp of four heads) and by how few warps wait on memory meanwhile: 8,192 tokens of 32 + 8 heads (176 MB, floor 27 us) 52 us, 3.4 TB/s; one
-// token 2.4, 128 3.0 (the 16-bit cache's kernel: 47, 1.6, 2.0).  Blocks of 256 threads 59, scalar arithmetic and a division an element 65; two tokens a lane at once 79 (registers spill), one
-// after the other with the second's loads ahead 49, but 12.2 for 11.5 where there is less (3 x 637 tokens).  The squares' sum in 32 bits would save 4 us.
+// Bound by its operations (330 instructions a warp of four heads) and by how few warps wait on memory meanwhile: 8,192 tokens of 32 + 8 heads (176 MB, floor 27 us) 50.5 us, 3.5 TB/s; one
+// token 2.4, 128 2.9 (the 16-bit cache's kernel: 47, 1.5, 2.0).  Blocks of 256 threads 59, scalar arithmetic and a division an element 65; two tokens a lane at once 79 (registers spill), one
+// after the other with the second's loads ahead 49 and 12.2 for 3 x 637 tokens, where one took 52 and 11.5.  The squares' sum in 32 bits would save 4 us.
 constexpr int KV4_APPEND_THREADS = 128;
 __device__ __forceinline__ void kv4_weights(const void* w, int at, int f32, F2 (&out)[4]) {      // eight of them, 16 bytes a load
     if (f32) {
@@ -372,7 +372,7 @@ MSGL_API int msgl_kv4_append(const Kv4AppendArgs* x) {
 // Two uses.  By pages: pages[i] of the cache becomes page i of the results, [n][kv heads][page][d].  By requests: the keys that the requests with
 // at least min_q tokens see are packed into pages of KV4_RESTORED keys, request after request, and `table` names those pages as a block table does
 // (the tensor-core prefill kernel then fetches whole tiles of keys; a key's place in its page is that of its position).  Keys behind a request's
-// last one are zeros.  bfloat16 results are rounded once, as a bfloat16 cache would hold them.  8,192 keys of 8 heads (42 MB) 8.4 us, 5.0 TB/s.
+// last one are zeros.  bfloat16 results are rounded once, as a bfloat16 cache would hold them.  8,192 keys of 8 heads (42 MB) 8.6 us, 4.9 TB/s.
 constexpr int KV4_RESTORED = 128;
 
 struct Kv4Restore {

@@ -25,7 +25,7 @@
 // of a row; P goes through movmatrix; V^T fragments come by ldmatrix.trans on 16-bit columns, four codes of two neighbouring keys a register.  The
 // exponentials' reference moves only where a score lies KR_LAZY above it.
 //
-// What bounds it.  Where there is work for all SMs, the operations of a unit: 530 instructions a warp for 4.3 KB, 144 of them to take codes apart, on a pipe that takes half an instruction a
+// What bounds it.  Where there is work for all SMs, the operations of a unit: 500 instructions a warp for 4.3 KB, 144 of them to take codes apart, on a pipe that takes half an instruction a
 // cycle; 64 requests of up to 16,000 keys (32 heads on 8, 794 MB) 141 us, 5.6 TB/s, 0.87 of copy.  With nine copies a lane for every unit whose sizes are looked at one by one it took 152, with
 // selects for hidden keys in the inner loop 3 us more.  12 warps at 160 registers and three units a ring 141, 16 at 128 and two 145, 14 164, 8 with four 179 (before the last steps).  Few keys:
 // latency; 1 request of 1,000 keys 10 us: 1.5 until the warps know their units, 1.4 for pages and queries, 2.5 for two units, 3 to add up and write.  16 requests of up to 4,096 keys 22 us
