@@ -87,7 +87,8 @@ struct Kv4Append {
     long long slots;                                      // of the cache: page numbers beyond are left out
     int page_size, n_q, n_kv, d, T;
     int early;                                            // the next launch may start while this one waits for the one ahead
-    unsigned magic; int shift;                            // for quotients by the number of heads of a token, at least 2: (h + (x - h) / 2) >> shift with h = x magic >> 32 (Granlund and Montgomery)
+    int parts;                                            // parts that a token's heads are dealt out over
+    unsigned magic; int less, shift;                      // a quotient by it: (h + ((x - h) >> less)) >> shift with h = x magic >> 32 (Granlund and Montgomery)
     __device__ __forceinline__ long long row_of_slot(int slot, int kvh) const {      // -1: nowhere
         if (slot < 0 || slot >= slots) return -1;
         const int page = slot / page_size;
@@ -171,13 +172,17 @@ __global__ void kv4_append_kernel(const Kv4Append p) {
     if (lane == 0) p.steps[2 * row + (is_k ? 0 : 1)] = sc.bits;
 }
 
-// Head sizes 32, 64, 128, 256 whose rotation (if any) covers the whole head in halves: L = d / 16 lanes own one head of a token, a lane eight
+// Head sizes 32, 64, 128, 256 whose rotation (if any) covers the whole head in halves: L = d / 16 lanes work on one head of a token, a lane on eight
 // elements of the lower half and the eight that they are rotated with, so that every copy is 16 bytes, every word of codes one lane's, and only the sum
 // and the extremes take shuffles.  All that a lane reads but the weights is asked for before it works on any of it.
-// Bound by its operations (330 instructions a warp of four heads) and by how few warps wait on memory meanwhile: 8,192 tokens of 32 + 8 heads (176 MB, floor 27 us) 50.5 us, 3.5 TB/s; one
-// token 2.4, 128 2.9 (the 16-bit cache's kernel: 47, 1.5, 2.0).  Blocks of 256 threads 59, scalar arithmetic and a division an element 65; two tokens a lane at once 79 (registers spill), one
-// after the other with the second's loads ahead 49 and 12.2 for 3 x 637 tokens, where one took 52 and 11.5.  The squares' sum in 32 bits would save 4 us.
+// Bound by its operations and by how few warps wait on memory meanwhile.  Where there is much to do, lanes therefore go through several heads of their token (LOOP): the cosines, the slot and its
+// page are looked up once, and the next head is asked for while they work on one.  8,192 tokens of 32 + 8 heads (176 MB, floor 27 us) 40 us, 4.4 TB/s; with one head
+// a lane 50.4 (330 instructions a warp of four heads), the 16-bit cache's kernel 46.7; 16,000 tokens 79 and 93.5.  The loop's registers leave 28 warps an SM for 36, so that up to KV4_APPEND_ROUNDS times
+// what runs at a time one head a lane is quicker (1,500 tokens 9.9 us and 11.0, 400 3.9 and 5.1; level at 2,500); where all run at once the loop's kernel is again, without its loop (1 token 2.35 and 2.5; 128 2.9;
+// the 16-bit cache's kernel 1.5, 2.0).  Blocks of 256 threads 59 (where these took 52), scalar arithmetic and a division an element 65; the next head not asked for ahead 48 (where these took 41).
 constexpr int KV4_APPEND_THREADS = 128;
+constexpr int KV4_APPEND_ROUNDS = 4;      // one head a lane up to so many times what runs at a time
+template <typename T, bool LOOP> constexpr int KV4_APPEND_BLOCKS = !LOOP ? 9 : sizeof(T) == 2 ? 7 : 6;      // an SM: 56, 72 and 80 registers a thread
 __device__ __forceinline__ void kv4_weights(const void* w, int at, int f32, F2 (&out)[4]) {      // eight of them, 16 bytes a load
     if (f32) {
         const ulonglong2* p = reinterpret_cast<const ulonglong2*>(reinterpret_cast<const float*>(w) + at);
@@ -191,37 +196,34 @@ __device__ __forceinline__ void kv4_weights(const void* w, int at, int f32, F2 (
     }
 }
 
+// 8 elements of either half of the rotation, asked for
 template <typename T, int L>
-__global__ void __launch_bounds__(KV4_APPEND_THREADS, 9) kv4_append_vec_kernel(const Kv4Append p) {
-    constexpr int d = 16 * L, half = 8 * L, V = 16 / sizeof(T), N = 8 / V;          // elements of a 16-byte piece, pieces of eight elements
-    const int l = threadIdx.x & (L - 1), n_heads = p.n_q + 2 * p.n_kv;
-    const unsigned unit = blockIdx.x * (KV4_APPEND_THREADS / L) + threadIdx.x / L;
-    const unsigned high = __umulhi(unit, p.magic);
-    const int token = (int)((high + ((unit - high) >> 1)) >> p.shift), head = (int)(unit - (unsigned)token * n_heads), t = min(token, p.T - 1);      // past the end: the last token again, not stored
-    const bool is_q = head < p.n_q, is_k = !is_q && head < p.n_q + p.n_kv, turns = (is_q || is_k) && p.table != nullptr;
-    const void* nw = is_q ? p.qw : (is_k ? p.kw : nullptr);
-    if (p.early) pdl_small();
-    pdl_wait();
-    if (!p.early) pdl_small();
-    int pos = turns ? p.positions[t] : 0;
-    const int slot = is_q ? 0 : p.out_loc[t];
-    uint4 raw[2][N];
-    const T* src = reinterpret_cast<const T*>(p.qkv) + (size_t)t * p.stride + (size_t)head * d + 8 * l;
+__device__ __forceinline__ void kv4_append_ask(const T* src, uint4 (&raw)[2][sizeof(T) / 2]) {
+    constexpr int V = 16 / sizeof(T);
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int k = 0; k < N; ++k) raw[h][k] = *reinterpret_cast<const uint4*>(src + h * half + k * V);
-    F2 ang[8];                                            // cosines and sines of the lower half's elements
-    if (turns) {
-        pos = pos < 0 ? 0 : (pos >= p.max_pos ? p.max_pos - 1 : pos);
-        const ulonglong2* cs = reinterpret_cast<const ulonglong2*>(p.table + (size_t)pos * d + 8 * l);
+        for (int k = 0; k < sizeof(T) / 2; ++k) raw[h][k] = *reinterpret_cast<const uint4*>(src + h * 8 * L + k * V);
+}
+// cosines and sines of the lower half's elements at a position
+template <int L>
+__device__ __forceinline__ void kv4_append_angles(const Kv4Append& p, int pos, int l, F2 (&ang)[8]) {
+    pos = pos < 0 ? 0 : (pos >= p.max_pos ? p.max_pos - 1 : pos);
+    const ulonglong2* cs = reinterpret_cast<const ulonglong2*>(p.table + (size_t)pos * (16 * L) + 8 * l);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const ulonglong2 a = cs[(k & 1) + (k >> 1) * (half / 4)];
-            ang[2 * k] = a.x;
-            ang[2 * k + 1] = a.y;
-        }
+    for (int k = 0; k < 4; ++k) {
+        const ulonglong2 a = cs[(k & 1) + (k >> 1) * (8 * L / 4)];
+        ang[2 * k] = a.x;
+        ang[2 * k + 1] = a.y;
     }
+}
+// one head of a token; row_of(kv head): its row in the cache, -1: nowhere
+template <typename T, int L, typename Row>
+__device__ __forceinline__ void kv4_append_head(const Kv4Append& p, const uint4 (&raw)[2][sizeof(T) / 2], const F2 (&ang)[8], int l, int token, int head, Row row_of) {
+    constexpr int d = 16 * L, half = 8 * L, V = 16 / sizeof(T), N = 8 / V;          // elements of a 16-byte piece, pieces of eight elements
+    const bool is_q = head < p.n_q, is_k = !is_q && head < p.n_q + p.n_kv, turns = (is_q || is_k) && p.table != nullptr;
+    const void* nw = is_q ? p.qw : (is_k ? p.kw : nullptr);
+    const unsigned group = (unsigned)(((1ull << L) - 1) << (threadIdx.x & 31 & ~(L - 1)));
     F2 x[8];                                              // the lower half's elements and the upper half's
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -235,7 +237,6 @@ __global__ void __launch_bounds__(KV4_APPEND_THREADS, 9) kv4_append_vec_kernel(c
             for (int k = 0; k < 4; ++k) x[4 * h + k] = f2(__uint_as_float(y[k] << 16), __uint_as_float(y[k] & 0xffff0000u));
         }
     }
-    const unsigned group = (unsigned)(((1ull << L) - 1) << (threadIdx.x & 31 & ~(L - 1)));
     if (nw != nullptr) {
         double ss = 0.0;
 #pragma unroll
@@ -270,7 +271,6 @@ __global__ void __launch_bounds__(KV4_APPEND_THREADS, 9) kv4_append_vec_kernel(c
         }
     }
     if (is_q) {
-        if (token >= p.T) return;
         T* dst = reinterpret_cast<T*>(p.q_out) + ((size_t)token * p.n_q + head) * d + 8 * l;
 #pragma unroll
         for (int h = 0; h < 2; ++h)
@@ -309,13 +309,56 @@ __global__ void __launch_bounds__(KV4_APPEND_THREADS, 9) kv4_append_vec_kernel(c
         hi = max_nan(hi, __shfl_xor_sync(group, hi, o));
     }
     const Kv4Scale sc(lo, hi);
-    const long long row = token < p.T ? p.row_of_slot(slot, is_k ? head - p.n_q : head - p.n_q - p.n_kv) : -1;
+    const long long row = row_of(is_k ? head - p.n_q : head - p.n_q - p.n_kv);
     if (row < 0) return;
     unsigned* dst = reinterpret_cast<unsigned*>((is_k ? p.k : p.v) + row * (d / 2)) + l;
     const F2 x0[4] = {x[0], x[1], x[2], x[3]}, x1[4] = {x[4], x[5], x[6], x[7]};
     dst[0] = sc.codes(x0);
     dst[L] = sc.codes(x1);
     if (l == 0) p.steps[2 * row + (is_k ? 0 : 1)] = sc.bits;
+}
+
+// L lanes take every `parts`-th head of a token; LOOP: that may be several
+template <typename T, int L, bool LOOP>
+__global__ void __launch_bounds__(KV4_APPEND_THREADS, KV4_APPEND_BLOCKS<T, LOOP>) kv4_append_vec_kernel(const Kv4Append p) {
+    const int l = threadIdx.x & (L - 1), n_heads = p.n_q + 2 * p.n_kv;
+    const unsigned group = blockIdx.x * (KV4_APPEND_THREADS / L) + threadIdx.x / L;
+    const unsigned high = __umulhi(group, p.magic);
+    const int token = (int)((high + ((group - high) >> p.less)) >> p.shift);
+    int head = (int)(group - (unsigned)token * p.parts);
+    if (p.early) pdl_small();
+    pdl_wait();
+    if (!p.early) pdl_small();
+    if (token >= p.T) return;
+    const bool turns = p.table != nullptr && head < p.n_q + p.n_kv, stores = head >= p.n_q || p.parts < n_heads;
+    const int pos = turns ? p.positions[token] : 0, slot = stores ? p.out_loc[token] : 0;
+    const T* src = reinterpret_cast<const T*>(p.qkv) + (size_t)token * p.stride + (size_t)head * (16 * L) + 8 * l;
+    uint4 raw[2][sizeof(T) / 2];
+    kv4_append_ask<T, L>(src, raw);
+    F2 ang[8];
+    if (turns) kv4_append_angles<L>(p, pos, l, ang);
+    if (!LOOP) {
+        kv4_append_head<T, L>(p, raw, ang, l, token, head, [&](int kvh) { return p.row_of_slot(slot, kvh); });
+        return;
+    }
+    const long long row0 = stores ? p.row_of_slot(slot, 0) : -1;
+    auto row_of = [&](int kvh) { return row0 < 0 ? -1 : row0 + (long long)kvh * p.page_size; };
+    if (p.parts == n_heads) {
+        kv4_append_head<T, L>(p, raw, ang, l, token, head, row_of);
+        return;
+    }
+    while (true) {
+        uint4 next[2][sizeof(T) / 2];
+        src += (size_t)p.parts * (16 * L);
+        if (head + p.parts < n_heads) kv4_append_ask<T, L>(src, next);
+        kv4_append_head<T, L>(p, raw, ang, l, token, head, row_of);
+        head += p.parts;
+        if (head >= n_heads) return;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int k = 0; k < sizeof(T) / 2; ++k) raw[h][k] = next[h][k];
+    }
 }
 
 // The entry points take their arguments in one piece, 8 bytes each in the order of these structs.
@@ -339,18 +382,30 @@ MSGL_API int msgl_kv4_append(const Kv4AppendArgs* x) {
     if (dtype != MSGL_F32 && dtype != MSGL_BF16) return MSGL_ERR_DTYPE;
     if (((uintptr_t)k | (uintptr_t)v | (uintptr_t)steps) & 15) return MSGL_ERR_ALIGN;
     Kv4Append p = {qkv, stride, positions, out_loc, qw, kw, w_f32, eps, table, rot, max_pos, interleaved, q_out, (unsigned char*)k, (unsigned char*)v, (unsigned*)steps,
-                   slots, page_size, n_q, n_kv, d, T, (int)x->early, 0u, 0};
-    const unsigned n_heads = (unsigned)(n_q + 2 * n_kv);
-    while ((2ull << p.shift) < n_heads) ++p.shift;      // 2^(shift + 1) is the power of two from n_heads on
-    p.magic = (unsigned)((((2ull << p.shift) - n_heads) << 32) / n_heads + 1);
-    const long long units = (long long)T * (n_q + 2 * n_kv);
+                   slots, page_size, n_q, n_kv, d, T, (int)x->early, n_q + 2 * n_kv, 0u, 0, 0};
+    const int n_heads = n_q + 2 * n_kv;
+    const long long units = (long long)T * n_heads;
     const int item = dtype == MSGL_F32 ? 4 : 2;
     const bool whole = table == nullptr || (rot == d && !interleaved && ((uintptr_t)table & 15) == 0);
     if (whole && (d == 32 || d == 64 || d == 128 || d == 256) && (((uintptr_t)qkv | (uintptr_t)q_out | (uintptr_t)qw | (uintptr_t)kw) & 15) == 0 && (stride * item) % 16 == 0) {
         const int L = d / 16, per = KV4_APPEND_THREADS / L;
-        const long long blocks = (units + per - 1) / per;
         if (units > 0x7fffffffLL) return MSGL_ERR_SIZE;
-#define KV4_VEC(TT, LL) msgl_launch_pdl(kv4_append_vec_kernel<TT, LL>, dim3((unsigned)blocks), dim3(KV4_APPEND_THREADS), 0, stream, p)
+        const long long sms = msgl_sm_count(), at_a_time = sms * (dtype == MSGL_F32 ? KV4_APPEND_BLOCKS<float, true> : KV4_APPEND_BLOCKS<__nv_bfloat16, true>) * per;
+        const bool much = units > sms * KV4_APPEND_BLOCKS<float, false> * per * KV4_APPEND_ROUNDS, loop = much || units <= at_a_time / 2;
+        if (much) {          // the number of parts with the least rounds of them times heads of a part (starting a part costs 0.8 of a head's time)
+            double least = 1e300;
+            for (int c = n_heads; c >= 1; --c) {
+                const double cost = (double)((T * (long long)c + at_a_time - 1) / at_a_time) * ((n_heads + c - 1) / c + 0.8);
+                if (cost < least) { least = cost; p.parts = c; }
+            }
+        }
+        if (p.parts > 1) {
+            p.less = 1;
+            while ((2ull << p.shift) < (unsigned)p.parts) ++p.shift;      // 2^(shift + 1) is the power of two from p.parts on
+            p.magic = (unsigned)((((2ull << p.shift) - p.parts) << 32) / p.parts + 1);
+        }
+        const long long blocks = ((long long)T * p.parts + per - 1) / per;
+#define KV4_VEC(TT, LL) msgl_launch_pdl(loop ? kv4_append_vec_kernel<TT, LL, true> : kv4_append_vec_kernel<TT, LL, false>, dim3((unsigned)blocks), dim3(KV4_APPEND_THREADS), 0, stream, p)
 #define KV4_VEC_L(TT) do { if (L == 2) KV4_VEC(TT, 2); else if (L == 4) KV4_VEC(TT, 4); else if (L == 8) KV4_VEC(TT, 8); else KV4_VEC(TT, 16); } while (0)
         if (dtype == MSGL_F32) KV4_VEC_L(float); else KV4_VEC_L(__nv_bfloat16);
 #undef KV4_VEC_L
