@@ -230,7 +230,7 @@ def _append(s):
 
 
 def _attention(s):
-    case, q = s["case"], s["q"]
+    case, q, table = s["case"], s["q"], s["table"].long()
     T, n_q, _ = q.shape
     n_kv, P, W, scale = HEADS[case["heads"]][1], case["page"], case["window"], D ** -0.5
     if own:
@@ -239,7 +239,6 @@ def _attention(s):
         ops.kv4_attention(q, out, ops.KV4Cache(*s["kv"], s["steps"]), q_start=s["q_start"], kv_len=s["kv_len"], block_table=s["table"], scale=scale, window=W,
                           q_lens=s["q_lens"], kv_lens=s["kv_lens"], workspace=_workspace())
         return out
-    table = s["table"].long()
     B, G, L, N = table.shape[0], n_q // n_kv, table.shape[1] * P, case["tokens"]
     keys, values = (_values(s["kv"][i][table], s["steps"][table][..., 2 * i], s["steps"][table][..., 2 * i + 1]).permute(0, 2, 1, 3, 4).reshape(B, n_kv, L, D) for i in range(2))
     first, kv = s["q_start"][:-1].long(), s["kv_len"].long()
