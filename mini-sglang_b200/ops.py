@@ -407,20 +407,24 @@ def attention_tc(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_ca
                  window: int, scale: float, qlen_min: int, qlen_max: int, q_lens: Sequence[int], keep_first: int = 0,
                  bias_log2: Optional[torch.Tensor] = None, null_log2: Optional[torch.Tensor] = None,
                  gate: Optional[torch.Tensor] = None, chunk: int = 0, diff: Optional[Tuple[float, float, float]] = None,
-                 kv_lens: Optional[Sequence[int]] = None, workspace=None, beside=None) -> bool:
+                 kv_lens: Optional[Sequence[int]] = None, workspace=None, beside=None, first_token: Optional[int] = None) -> bool:
     """Prefill attention on tcgen05 tensor cores for the requests with q_len in [qlen_min, qlen_max];
     q_lens: the host's copy of every request's number of query tokens (to size the grid).  keep_first, bias_log2: as in
     `attention`; they are taken by the kernel on pairs of query tiles only (TMA page sizes), and the call returns False,
     having launched nothing, where that kernel cannot run.  null_log2, gate, chunk: as in `attention`, taken by both kernels;
     diff: as there, by the kernel on pairs of query tiles only.  With kv_lens (the host's copy of kv_len) and a workspace
     query tiles with far more keys than the launch's mean are cut into pieces (`plan_tc_pieces`) and merged here.
-    beside: called behind the tiles' launch, ahead of the merges: for launches that run beside the tiles."""
+    beside: called behind the tiles' launch, ahead of the merges: for launches that run beside the tiles.
+    first_token: for a launch over some of a step's requests in a row (q_start, kv_len, block_table and the host's lengths are theirs, q and out the whole
+    step's, and q_start counts the whole step's tokens), the token that the first of them starts at."""
     global _tc2_usable
     gate_stride = _attention_extras(q, null_log2, gate)
     _need_cuda(q, out, k_cache, v_cache, q_start, kv_len, block_table)
     T, n_q, d = q.shape
     B = kv_len.numel()
+    tokens = T if first_token is None else sum(q_lens)          # of the requests that the lengths are of
     assert q.is_contiguous() and out.is_contiguous() and block_table.stride(1) == 1 and q.dtype == torch.bfloat16
+    assert first_token is None or (first_token >= 0 and first_token + tokens <= T and len(q_lens) == B)
     assert tuple(out.shape) == (T, n_q if diff is None else n_q // 2, d) and q_start.numel() == B + 1 and block_table.shape[0] == B
     status = _status_tensor(q.device)
     group = n_q // n_kv
@@ -444,14 +448,15 @@ def attention_tc(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_ca
         # the plan is made in Python: two bounds on the key tiles, the cheap one first, keep it out of launches that the rule leaves whole
         if version == 2 and kv_lens is not None and workspace is not None and not (window or chunk or ext) and \
                 (longest := max(kv_lens)) > 128 * (TC_PIECE_MIN + TC_PIECE_GAIN - 1) and \
-                (T // qt + B) * (longest // 128 + 1) * n_kv >= (enough := TC_PIECE_MEAN * sm_count(q.device)) and \
+                (tokens // qt + B) * (longest // 128 + 1) * n_kv >= (enough := TC_PIECE_MEAN * sm_count(q.device)) and \
                 sum((n // qt + 1) * (kv // 128 + 1) for n, kv in zip(q_lens, kv_lens) if n >= qlen_min) * n_kv >= enough:
             cut = plan_tc_pieces(q_lens, kv_lens, qlen_min=qlen_min, qlen_max=qlen_max, tile_tokens=qt, heads=n_kv * (1 if group <= TC_ROWS else -(-group // TC_ROWS)),
-                                 sms=sm_count(q.device), bytes_per_piece=T * n_q * d * 4)
+                                 sms=sm_count(q.device), bytes_per_piece=tokens * n_q * d * 4)
         part_o = part_ml = tok_pieces = None
         lo = plane = 0
         if cut is not None:                   # rows for the tokens from the first cut one to the last, in buffers that no decode graph knows
-            lo, plane = cut[2][0][0], cut[2][-1][0] + cut[2][-1][1] - cut[2][0][0]
+            runs = [(tok0 + (first_token or 0), n) for tok0, n in cut[2]]          # (the plan counts tokens from the first length's on, the kernels the step's)
+            lo, plane = runs[0][0], runs[-1][0] + runs[-1][1] - runs[0][0]
             part_o = workspace.get("attn_piece_o", cut[1] * plane * n_q * d, torch.float32)
             part_ml = workspace.get("attn_piece_ml", cut[1] * plane * n_q * 2, torch.float32)
             tok_pieces = workspace.get("attn_tok_pieces", T, torch.int32)
@@ -469,7 +474,7 @@ def attention_tc(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_ca
         _check(code, "attention_tc")
         if beside is not None:
             beside()
-        for tok0, n in cut[2] if cut is not None else ():
+        for tok0, n in runs if cut is not None else ():
             _check(_attn_lib(d).msgl_attention_combine_range(_ptr(part_o), _ptr(part_ml), _ptr(tok_pieces), _ptr(out), T, lo, plane, tok0, n, n_q, d, cut[1],
                                                              _dt(out), _ptr(null_log2), _ptr(gate), gate_stride, _stream()), "attention_combine_range")
         return True
@@ -3066,7 +3071,7 @@ def _kv4_portions(q, out, cache, kv_len, block_table, scale, window, q_start, q_
             _check(code, "kv4_attention (keys restored)")
             common = dict(q_start=starts, kv_len=kv_part, block_table=table, n_kv=n_kv, page_size=per, window=window, scale=scale, qlen_min=min_q, qlen_max=big)
             beside = (lambda: others(True)) if not any(need[b:]) else None
-            if tc_supported(d, dt, G) and attention_tc(q, out, k, v, q_lens=lens, kv_lens=kvs, workspace=workspace, beside=beside, **common):
+            if tc_supported(d, dt, G) and attention_tc(q, out, k, v, q_lens=lens, kv_lens=kvs, workspace=workspace, beside=beside, first_token=None if whole else sum(q_lens[:a]), **common):
                 launched = beside is not None
             else:
                 variant = VARIANT_MMA_ROWS if mma_supported(d, dt) else VARIANT_SIMT
