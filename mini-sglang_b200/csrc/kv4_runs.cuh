@@ -170,6 +170,7 @@ __global__ void __launch_bounds__(NW * 32, 1) kv4_attn_runs_kernel(const Kv4Runs
     }
     if (lane < 2) slot_seg[2 * warp + lane] = -1;
     if (tid <= NW) sh_x[tid] = 0;
+    if (tid == 0) sh_all[3] = 1;                          // (ahead of the barrier: the lane that finds the block's piece writes over it)
     __syncthreads();
     if (warp == 0) {
         const int per = (p.B + 31) >> 5, r0 = lane * per, r1 = min(r0 + per, p.B);
@@ -194,7 +195,7 @@ __global__ void __launch_bounds__(NW * 32, 1) kv4_attn_runs_kernel(const Kv4Runs
         const bool whole = P > NB && S <= NB && 3ll * longest * NB <= 4ll * U;      // a block a segment is nearly even, and nothing is left to merge
         const bool by_piece = whole || P <= NB;
         if (whole) at_p = at_s;
-        if (lane == 0) { sh_all[0] = U; sh_all[1] = S; sh_all[2] = by_piece; sh_all[3] = 1; pre_u[p.B] = U; pre_s[p.B] = S; }
+        if (lane == 0) { sh_all[0] = U; sh_all[1] = S; sh_all[2] = by_piece; pre_u[p.B] = U; pre_s[p.B] = S; }
 #pragma unroll 1
         for (int r = r0; r < r1; ++r) {
             const int u = units[r], segs = pre_s[r], pc = whole ? 1 : kr_pieces(u), in_r = j - at_p;
