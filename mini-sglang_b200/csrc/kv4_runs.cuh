@@ -18,7 +18,11 @@
 //     q k = step 2^(24 - e) sum q^ (c 2^-24) + base sum q
 //     o   = sum_j p_j (base_j + step_j c_j) = 2^24 / F sum_j w_j (c_j 2^-24) + sum_j p_j base_j,   w_j = float16(p_j step_j F)
 // F is a power of two of the warp's own that keeps step F <= 64 (p is at most 2^8, see KR_LAZY): where a unit brings a larger step, F and the sums are scaled down.
-// w keeps 11 bits; below 2^-28 of the largest step it loses them one by one.  The tensor core cuts its sums off rather than rounding them, and those of codes from
+// That step may be of a key which a row does not see or gives no weight.  A row whose largest weight p step F then lies below KR_FLOOR takes its exponentials' reference g powers of two
+// below its largest score: its p are up to 2^g and its w large enough again.  All sums of a row are against the same reference, so nothing else changes, but that every unit is
+// looked at while g > 0.  w keeps 11 bits; below 2^-11 of the row's largest weight (2^-20 where steps are alike) it loses them one by one, and so it does where an unseen step
+// is more than KR_LIFT powers of two above those that count.  (64 requests of up to 16,000 keys take 0.7 % longer for it; with a factor a row, and weights looked at in every unit
+// whose steps grow, 4 %.)  The tensor core cuts its sums off rather than rounding them, and those of codes from
 // 0 up grow all the way while what they leave beside the bases is small (a mean of 16,000 values came out 1 % off); so every unit takes the middles of the codes times
 // its weights out of all sums by one more product, and they are added back at the end from float32 sums of their own.
 // Scores, p, sums and outputs are float32.  S^T = K Q^T with keys on the M dimension, the head's elements permuted so that a lane reads 16 bytes
@@ -37,6 +41,7 @@
 #include <type_traits>
 
 constexpr float KR_LAZY = 8.f;
+constexpr int KR_FLOOR = -3, KR_LIFT = 100;      // powers of two: where a row's largest weight lies at least; how far its reference goes below its largest score at most
 constexpr int KR_KEYS = 32;          // keys of a unit
 constexpr int KR_MAX_B = 256;        // requests of a launch, a thread each
 constexpr int KR_PIECE = 16;         // units of a block's piece at least, where segments are cut by themselves ...
@@ -123,7 +128,7 @@ struct KrCursor {
 
 template <int D, int NW, int ST>
 constexpr size_t kr_smem_bytes() {
-    return (size_t)NW * ST * (KR_KEYS * (D + 8)) + (size_t)NW * 8 * (D + 4) * 4 + (size_t)NW * 2 * (16 + 1) * 4 + (8 * KR_MAX_B + 4) * 4;
+    return (size_t)NW * ST * (KR_KEYS * (D + 8)) + (size_t)NW * 8 * (D + 4) * 4 + (size_t)NW * 2 * (16 + 1) * 4 + (8 * KR_MAX_B + 4) * 4 + (size_t)NW * 16 * 4;
 }
 
 template <int D, int NW, int ST, bool WHOLE>
@@ -146,6 +151,7 @@ __global__ void __launch_bounds__(NW * 32, 1) kv4_attn_runs_kernel(const Kv4Runs
     int* token = keys + KR_MAX_B;
     int* tokens = token + KR_MAX_B;
     int* ends = tokens + KR_MAX_B;
+    float* lifts = reinterpret_cast<float*>(ends + KR_MAX_B + 2) + (threadIdx.x >> 5) * 16;      // [8][2] a warp's rows: largest p step (p against the largest score), g; since the first key
     __shared__ int sh_all[4];                             // units and segments of all requests; whether segments are cut by themselves; (by_piece) blocks of this block's segment
     __shared__ int sh_mine;                               // by_piece: this block's number among them
     __shared__ int sh_x[NW + 1], sh_r[NW + 1], sh_s[NW + 1];      // the warps' runs: where they start among all units, the request, its segment
@@ -493,18 +499,34 @@ __global__ void __launch_bounds__(NW * 32, 1) kv4_attn_runs_kernel(const Kv4Runs
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-                        const float mn = fmaxf(m_c[e], mx + mu_c[e]), mu = mn == -INFINITY ? 0.f : mn;
+                        float* lift = lifts + 4 * t + 2 * e;
+                        const bool first = m_c[e] == -INFINITY;
+                        const float old = m_c[e] + (first ? 0.f : lift[1]), mn = fmaxf(old, mx + mu_c[e]), at = mn == -INFINITY ? 0.f : mn;
+                        float top = 0.f;                  // the unit's largest p step
+#pragma unroll
+                        for (int m = 0; m < 2; ++m)
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) top = fmaxf(top, kr_exp2(v[m][2 * h + e] + (mu_c[e] - at)) * __uint_as_float(row_st[m][h].y << 16));
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                        if (!first) top = fmaxf(top, lift[0] * kr_exp2(old - at));
+                        const int g = top > 0.f ? min(max(KR_FLOOR + 127 - (int)(__float_as_uint(top * F) >> 23), 0), KR_LIFT) : 0;
+                        const float mu = at - (float)g;
+                        __syncwarp();                     // (eight lanes have the same rows)
+                        lift[0] = top;
+                        lift[1] = (float)g;
                         alpha[e] = kr_exp2(m_c[e] - mu);
 #pragma unroll
                         for (int m = 0; m < 2; ++m) { v[m][e] -= mu - mu_c[e]; v[m][e + 2] -= mu - mu_c[e]; }
-                        m_c[e] = mn;
+                        m_c[e] = mn == -INFINITY ? -INFINITY : mu;
                         mu_c[e] = mu;
                         l_c[e] *= alpha[e];
                         z_c[e] *= alpha[e];
                         alpha[e] *= down;
                         mid[e] *= alpha[e];
                         mid[e + 2] *= alpha[e];
-                        lim_c[e] = mn == -INFINITY ? -INFINITY : KR_LAZY;
+                        lim_c[e] = mn == -INFINITY || g > 0 ? -INFINITY : KR_LAZY;
                     }
 #pragma unroll
                     for (int m = 0; m < 2; ++m)
