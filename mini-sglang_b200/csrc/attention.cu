@@ -1405,8 +1405,8 @@ __global__ void __launch_bounds__(SIMT_THREADS) attn_simt_kernel(const AttnParam
         const size_t tok = (size_t)(ti.q_base + ti.t0 + tl);
         const int head = kvh * G + hg;
         if (ns == 1) {
-            const float l = Ls[r] + null_weight(p.null_log2, head, Ms[r]);
-            og[(tok * p.n_q + head) * D + c] = from_f32<T>((l > 0.f ? Os[idx] / l : 0.f) * gate_factor<T>(p.gate, p.gate_stride, tok, head * D + c));
+            const float l = Ls[r] + null_weight(p.null_log2, head, Ms[r]);      // (0: no key is seen; a NaN stays one)
+            og[(tok * p.n_q + head) * D + c] = from_f32<T>((l != 0.f ? Os[idx] / l : 0.f) * gate_factor<T>(p.gate, p.gate_stride, tok, head * D + c));
         } else {
             const size_t prow = ((size_t)split * p.T + tok) * p.n_q + head;
             p.part_o[prow * D + c] = Os[idx];
@@ -1644,7 +1644,7 @@ __global__ void __launch_bounds__(F32_THREADS, D <= 128 ? 2 : 1) attn_f32_kernel
             float y[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-                y[k] = ns == 1 ? (l > 0.f ? o[v][r][k] / l : 0.f) * gate_factor<float>(p.gate, p.gate_stride, tok, head * D + e + k) : o[v][r][k];
+                y[k] = ns == 1 ? (l != 0.f ? o[v][r][k] / l : 0.f) * gate_factor<float>(p.gate, p.gate_stride, tok, head * D + e + k) : o[v][r][k];
             *reinterpret_cast<float4*>((ns == 1 ? og : p.part_o) + at * D + e) = make_float4(y[0], y[1], y[2], y[3]);
         }
     }

@@ -1,0 +1,59 @@
+"""Rows of a cache in 4 bits that are no numbers, in portions (keys and values restored for the prefill kernels): they show in the tokens that see them, and in no other."""
+import math
+
+import pytest
+import torch
+
+from mini_sglang_b200 import ops
+from mini_sglang_b200.parts import Workspace
+from test_kv4_edges_gpu import attend, table_of
+from test_kv4_gpu import BF, F32, filled, i32, normal
+
+pytestmark = pytest.mark.gpu
+#         one of every prefill kernel: tcgen05, mma, scalar in bfloat16 and float32, tiles of float32
+SHAPES = [(8, 2, 128, BF), (4, 2, 64, BF), (4, 4, 40, BF), (2, 1, 512, BF), (4, 2, 128, F32), (3, 1, 40, F32)]
+LENS, KV = [150, 1, 60, 3], [200, 77, 300, 9]
+
+
+def portions(monkeypatch, q, c, table, window):
+    """The step's attention, its two long requests as portions."""
+    taken, restored = [], ops._kv4_portions
+    monkeypatch.setattr(ops, "_kv4_middle", lambda q_lens, kv_lens, direct, *a: direct)
+    monkeypatch.setattr(ops, "_kv4_portions", lambda *a: taken.append(a[10]) or restored(*a))
+    starts = [sum(LENS[:i]) for i in range(5)]
+    out = attend(q, c, KV, table, window=window, q_start=i32(starts), q_lens=LENS, kv_lens=KV, workspace=Workspace("cuda"))
+    ops.check_kernel_status()
+    assert len(taken) == 1 and taken[0] <= 60
+    return out
+
+
+def check(monkeypatch, shape, which, window, keys):
+    n_q, n_kv, d, dtype = shape
+    table = table_of(4, 19)
+    c, q = filled(71, 77, n_kv, 16, d), normal(72, sum(LENS) + 1, n_q, d, dtype=dtype)
+    clean = portions(monkeypatch, q, c, table, window)
+    assert torch.isfinite(clean).all()
+    shown, t = [], 0
+    for r, (n, kv) in enumerate(zip(LENS, KV)):
+        for pos in range(kv - n, kv):
+            shown.append(any(key <= pos and (not window or key > pos - window) for key in keys[r]))
+        for key in keys[r]:
+            c.steps[int(table[r, key // 16]), :, key % 16, which] = math.nan
+    out = portions(monkeypatch, q, c, table, window)
+    shown = torch.tensor(shown + [False], device="cuda")
+    assert 0 < shown[:150].sum() < 150 and 0 < shown[151:211].sum() < 60          # some tokens of either portion
+    assert torch.equal(out.isnan().flatten(1).all(1), shown) and torch.equal(out.isnan().flatten(1).any(1), shown)
+    # the others are as without those rows, up to the order of a few sums
+    torch.testing.assert_close(out[~shown].float(), clean[~shown].float(), rtol=2.0 ** -7 if dtype == BF else 1e-5, atol=2.0 ** -7 if dtype == BF else 1e-5)
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("window", [0, 40])
+def test_keys(monkeypatch, shape, window):
+    check(monkeypatch, shape, 1, window, [[120, 121], [], [250, 299], []])
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+def test_a_key_alone_in_its_tile(monkeypatch, shape):
+    """Position 192 starts a tile of 64 or 128 keys: the token there sees that key alone of it."""
+    check(monkeypatch, shape, 1, 0, [[192], [], [256], []])
