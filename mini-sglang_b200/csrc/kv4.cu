@@ -427,7 +427,8 @@ MSGL_API int msgl_kv4_append(const Kv4AppendArgs* x) {
 // Two uses.  By pages: pages[i] of the cache becomes page i of the results, [n][kv heads][page][d].  By requests: the keys that the requests with
 // at least min_q tokens see are packed into pages of KV4_RESTORED keys, request after request, and `table` names those pages as a block table does
 // (the tensor-core prefill kernel then fetches whole tiles of keys; a key's place in its page is that of its position).  Keys behind a request's
-// last one are zeros.  bfloat16 results are rounded once, as a bfloat16 cache would hold them.  8,192 keys of 8 heads (42 MB) 8.6 us, 4.9 TB/s.
+// last one are zeros.  A value row that is no number becomes a key row that is none beside values of 0: it then shows through the scores of those who see it, where as a value it would
+// meet the weights of 0 that others have for it as well.  bfloat16 results are rounded once, as a bfloat16 cache would hold them.  8,192 keys of 8 heads (42 MB) 8.6 us, 4.9 TB/s.
 constexpr int KV4_RESTORED = 128;
 
 struct Kv4Restore {
@@ -537,6 +538,10 @@ __global__ void __launch_bounds__(256) kv4_restore_kernel(const Kv4Restore p) {
             kw = reinterpret_cast<const unsigned*>(p.k)[src * words + w];
             vw = reinterpret_cast<const unsigned*>(p.v)[src * words + w];
             st = p.steps[src];
+            if (p.pages_in == nullptr && ((st.y & 0x7f800000u) == 0x7f800000u || (st.y & 0x7f80u) == 0x7f80u)) {
+                kw = vw = 0;
+                st = make_uint2(0x7fc00000u, 0u);
+            }
         }
         kv4_put<WIDE>(p.k_out, to + 8ll * i, kw, bf16_of(st.x & 0xffffu), bf16_of(st.x >> 16));
         kv4_put<WIDE>(p.v_out, to + 8ll * i, vw, bf16_of(st.y & 0xffffu), bf16_of(st.y >> 16));

@@ -54,6 +54,20 @@ def test_keys(monkeypatch, shape, window):
 
 
 @pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("window", [0, 40])
+def test_values(monkeypatch, shape, window):
+    """Earlier tokens of the same query tile have weights of 0 for such a row, and so have those whose window has passed it."""
+    check(monkeypatch, shape, 3, window, [[120, 121], [], [250, 299], []])
+
+
+def test_pages_read_back_as_they_are():
+    c = filled(73, 3, 2, 16, 64)
+    c.steps[1, :, 5, 3] = math.nan
+    k, v = ops.kv4_restore(c, i32([1]), F32)
+    assert torch.isfinite(k).all() and v[0, :, 5].isnan().all() and torch.isfinite(v[0, :, :5]).all()
+
+
+@pytest.mark.parametrize("shape", SHAPES)
 def test_a_key_alone_in_its_tile(monkeypatch, shape):
     """Position 192 starts a tile of 64 or 128 keys: the token there sees that key alone of it."""
     check(monkeypatch, shape, 1, 0, [[192], [], [256], []])
