@@ -647,9 +647,10 @@ __global__ void __launch_bounds__(KV4_ANY_WARPS * 32) kv4_attn_any_kernel(const 
         }
         const uint2 st = src >= 0 ? p.steps[src] : make_uint2(0u, 0u);
         const float ks = bf16_of(st.x & 0xffffu), kb = bf16_of(st.x >> 16);
+        const float none = (st.y & 0x7f800000u) == 0x7f800000u || (st.y & 0x7f80u) == 0x7f80u ? CUDART_NAN_F : 0.f;      // a value row that is no number: its score is none, whatever its weight
         float s[R];
 #pragma unroll
-        for (int r = 0; r < R; ++r) s[r] = 0.f;
+        for (int r = 0; r < R; ++r) s[r] = none;
         const unsigned* k_row = reinterpret_cast<const unsigned*>(p.k) + (src >= 0 ? src : 0ll) * words;      // (a key that is not there: step and base 0)
 #pragma unroll 8
         for (int w = 0; w < words; ++w) {

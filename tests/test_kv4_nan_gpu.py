@@ -6,7 +6,7 @@ import torch
 
 from mini_sglang_b200 import ops
 from mini_sglang_b200.parts import Workspace
-from test_kv4_edges_gpu import attend, table_of
+from test_kv4_edges_gpu import SHAPES as FEW, attend, table_of
 from test_kv4_gpu import BF, F32, filled, i32, normal
 
 pytestmark = pytest.mark.gpu
@@ -71,3 +71,20 @@ def test_pages_read_back_as_they_are():
 def test_a_key_alone_in_its_tile(monkeypatch, shape):
     """Position 192 starts a tile of 64 or 128 keys: the token there sees that key alone of it."""
     check(monkeypatch, shape, 1, 0, [[192], [], [256], []])
+
+
+@pytest.mark.parametrize("n_q,n_kv,d,dtype", FEW)
+@pytest.mark.parametrize("at", [3, 40, 99])
+def test_rows_of_next_to_no_weight(n_q, n_kv, d, dtype, at):
+    """A value row that is no number shows where it is seen, however small its weight (200 below the other scores): from codes and in portions."""
+    c, table = filled(74, 2 * 7 + 1, n_kv, 16, d), table_of(2, 7)
+    q = normal(75, 2, n_q, d, dtype=dtype) * 0.125 + 1
+    page = int(table[0, at // 16])
+    c.steps[page, :, at % 16, 0] = 0.0
+    c.steps[page, :, at % 16, 1] = -200.0 / d ** 0.5
+    c.steps[page, :, at % 16, 3] = math.nan
+    out = attend(q, c, [100, 100], table)
+    assert out[0].isnan().all() and torch.isfinite(out[1]).all()
+    q = normal(76, 100, n_q, d, dtype=dtype) * 0.125 + 1
+    out = attend(q, c, [100], table[:1], q_start=i32([0, 100]), q_lens=[100], kv_lens=[100])
+    assert out[at:].isnan().all() and torch.isfinite(out[:at]).all()
