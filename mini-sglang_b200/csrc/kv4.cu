@@ -691,7 +691,7 @@ __global__ void __launch_bounds__(KV4_ANY_WARPS * 32) kv4_attn_any_kernel(const 
                 float x[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) x[e] = fmaf((float)((word >> (4 * e)) & 15u), step, base);
-                const bool number = fabsf(base) <= FLT_MAX;      // (a row that is no number counts only where it is seen)
+                const bool number = fabsf(base) <= FLT_MAX && step <= FLT_MAX;      // (a row that is no number counts only where it is seen)
 #pragma unroll
                 for (int r = 0; r < R; ++r) {
                     const float pr = pw[r * 32 + j];

@@ -88,3 +88,15 @@ def test_rows_of_next_to_no_weight(n_q, n_kv, d, dtype, at):
     q = normal(76, 100, n_q, d, dtype=dtype) * 0.125 + 1
     out = attend(q, c, [100], table[:1], q_start=i32([0, 100]), q_lens=[100], kv_lens=[100])
     assert out[at:].isnan().all() and torch.isfinite(out[:at]).all()
+
+
+@pytest.mark.parametrize("n_q,n_kv,d,dtype", FEW)
+@pytest.mark.parametrize("which,value", [(2, math.inf), (2, math.nan), (3, math.inf), (3, -math.inf)])
+def test_steps_and_bases_that_are_none_ahead_of_a_window(n_q, n_kv, d, dtype, which, value):
+    """What no append writes: such rows count for nothing where they are not seen."""
+    c, table = filled(77, 8, n_kv, 16, d), table_of(1, 7)
+    for key in (60, 70, 90):
+        c.steps[int(table[0, key // 16]), :, key % 16, which] = value
+    q = normal(78, 3, n_q, d, dtype=dtype)
+    out = attend(q, c, [100], table, window=8, q_start=i32([0, 3]), q_lens=[3], kv_lens=[100])          # positions 97 to 99: keys from 90, 91 and 92 on
+    assert out[0].isfinite().flatten().tolist().count(True) == 0 and out[1:].isfinite().all()
