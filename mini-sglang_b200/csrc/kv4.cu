@@ -573,6 +573,7 @@ MSGL_API int msgl_kv4_restore(const Kv4RestoreArgs* x) {
     if (n <= 0) return MSGL_OK;
     if (d < 8 || d > KV4_MAX_D || d % 8 || n_kv < 1 || n_kv > 65535 || page_size < 1 || pages < 1) return MSGL_ERR_SIZE;
     if (dtype != MSGL_F32 && dtype != MSGL_BF16) return MSGL_ERR_DTYPE;
+    if (pages_in != nullptr && (long long)page_size * (d >> 3) >= 1LL << 30) return MSGL_ERR_SIZE;
     if (((uintptr_t)k | (uintptr_t)v | (uintptr_t)steps | (uintptr_t)k_out | (uintptr_t)v_out) & 15) return MSGL_ERR_ALIGN;
     if (pages_in == nullptr && (q_start == nullptr || kv_len == nullptr || block_table == nullptr || table == nullptr || B < 1 || t_width < 1)) return MSGL_ERR_SIZE;
     Kv4Restore p = {(const unsigned char*)k, (const unsigned char*)v, (const uint2*)steps, k_out, v_out, pages_in, q_start, kv_len, block_table, table, bt_stride, B, bt_width,

@@ -2860,13 +2860,15 @@ def kv4_restore(cache: KV4Cache, pages: torch.Tensor, dtype: torch.dtype) -> Tup
     if not (len(shape) == 4 and shape[0] >= 1 and shape[1] >= 1 and shape[2] >= 1 and shape[3] % 4 == 0 and 4 <= shape[3] <= KV4_MAX_HEAD_DIM // 2
             and k.dtype is v.dtype is torch.uint8 and v.shape == shape and steps.dtype is torch.bfloat16 and steps.shape == (*shape[:3], 4)
             and k.is_contiguous() and v.is_contiguous() and steps.is_contiguous() and shape[0] * shape[2] <= 0x7fffffff
-            and dtype in _DT and pages.dtype is torch.int32 and pages.is_contiguous()
+            and dtype in _DT and pages.dtype is torch.int32 and pages.is_contiguous() and shape[2] * shape[3] < 1 << 32
             and k.get_device() == v.get_device() == steps.get_device() == dev >= 0 and dev == torch._C._cuda_getDevice()):
         what = "kv4_restore"
         _kv4_sizes(what, cache)
         if dtype not in _DT:
             raise KernelError(f"{what}: results are float32 or bfloat16; got {dtype}")
         _index(what, "pages", pages)
+        if shape[2] * shape[3] >= 1 << 32:          # (a block counts a page's words of eight codes in 32 bits)
+            raise KernelError(f"{what}: pages of {shape[2]} tokens: up to 2^33 elements a page and kv head")
         _same_device(what, *cache, pages)
         raise KernelError(f"{what}: arguments that do not go together")
     n, d = pages.numel(), 2 * shape[3]
