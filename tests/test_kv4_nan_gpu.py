@@ -100,3 +100,27 @@ def test_steps_and_bases_that_are_none_ahead_of_a_window(n_q, n_kv, d, dtype, wh
     q = normal(78, 3, n_q, d, dtype=dtype)
     out = attend(q, c, [100], table, window=8, q_start=i32([0, 3]), q_lens=[3], kv_lens=[100])          # positions 97 to 99: keys from 90, 91 and 92 on
     assert out[0].isfinite().flatten().tolist().count(True) == 0 and out[1:].isfinite().all()
+
+
+def test_values_beyond_the_range_where_they_are_not_seen(monkeypatch):
+    """Codes whose value passes the largest float32, ahead of windows and in later tokens: finite steps and bases, as append writes them for rows that reach the end of the range."""
+    def place(c, table, r, keys):
+        for key in keys:
+            c.steps[int(table[r, key // 16]), :, key % 16, 2] = 1.5e37
+            c.steps[int(table[r, key // 16]), :, key % 16, 3] = 1.5e38          # 15 steps above: 3.75e38
+
+    for n_q, n_kv, d, dtype in FEW:
+        c, table = filled(79, 8, n_kv, 16, d), table_of(1, 7)
+        place(c, table, 0, (60, 70, 90, 99))
+        out = attend(normal(80, 3, n_q, d, dtype=dtype), c, [100], table, window=8, q_start=i32([0, 3]), q_lens=[3], kv_lens=[100])
+        assert out[1].isfinite().all() and (out[[0, 2]].abs().amax(-1) > 1e30).all(), (n_q, d, dtype)
+    for n_q, n_kv, d, dtype in SHAPES:
+        table = table_of(4, 19)
+        c, q = filled(81, 77, n_kv, 16, d), normal(82, sum(LENS) + 1, n_q, d, dtype=dtype)
+        place(c, table, 0, (120,))
+        place(c, table, 2, (250, 299))
+        for window in (0, 40):
+            with monkeypatch.context() as m:
+                out = portions(m, q, c, table, window)
+            seen = torch.tensor([any(k <= pos and (not window or k > pos - window) for k in keys) for n, kv, keys in zip(LENS, KV, ((120,), (), (250, 299), ())) for pos in range(kv - n, kv)] + [False])
+            assert torch.equal(out.isfinite().flatten(1).all(1).cpu(), ~seen), (n_q, d, dtype, window)
