@@ -20,9 +20,10 @@
 // F is a power of two of the warp's own that keeps step F <= 64 (p is at most 2^8, see KR_LAZY): where a unit brings a larger step, F and the sums are scaled down.
 // That step may be of a key which a row does not see or gives no weight.  A row whose largest weight p step F then lies below KR_FLOOR takes its exponentials' reference g powers of two
 // below its largest score: its p are up to 2^g and its w large enough again.  All sums of a row are against the same reference, so nothing else changes, but that every unit is
-// looked at while g > 0.  w keeps 11 bits; below 2^-11 of the row's largest weight (2^-20 where steps are alike) it loses them one by one, and so it does where an unseen step
-// is more than KR_LIFT powers of two above those that count.  (64 requests of up to 16,000 keys take 0.7 % longer for it; with a factor a row, and weights looked at in every unit
-// whose steps grow, 4 %.)  The tensor core cuts its sums off rather than rounding them, and those of codes from
+// looked at while g > 0.  w keeps 11 bits; below 2^-8 of the row's largest weight (2^-20 where steps are alike) it loses them one by one, and so it does where an unseen step
+// is more than KR_LIFT powers of two above those that count.  64 requests of up to 16,000 keys take 0.7 % longer for it (with a factor a row, and weights looked at in every unit
+// whose steps grow, 4 %); with g > 0 for all rows 64 of 8,000 take 124 us instead of 104.  So KR_FLOOR leaves g at 0 where a first key has nearly all weight and a value 1/500 of the
+// others' size (2^-3 did not).  The tensor core cuts its sums off rather than rounding them, and those of codes from
 // 0 up grow all the way while what they leave beside the bases is small (a mean of 16,000 values came out 1 % off); so every unit takes the middles of the codes times
 // its weights out of all sums by one more product, and they are added back at the end from float32 sums of their own.
 // Scores, p, sums and outputs are float32.  S^T = K Q^T with keys on the M dimension, the head's elements permuted so that a lane reads 16 bytes
@@ -41,7 +42,7 @@
 #include <type_traits>
 
 constexpr float KR_LAZY = 8.f;
-constexpr int KR_FLOOR = -3, KR_LIFT = 100;      // powers of two: where a row's largest weight lies at least; how far its reference goes below its largest score at most
+constexpr int KR_FLOOR = -6, KR_LIFT = 100;      // powers of two: where a row's largest weight lies at least; how far its reference goes below its largest score at most
 constexpr int KR_KEYS = 32;          // keys of a unit
 constexpr int KR_MAX_B = 256;        // requests of a launch, a thread each
 constexpr int KR_PIECE = 16;         // units of a block's piece at least, where segments are cut by themselves ...

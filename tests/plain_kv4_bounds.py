@@ -4,8 +4,8 @@ Every path: float32 sums of d products leave a score off by (d + 8) 2^-24 of its
 e^(2 x) - 1 of themselves; float32 sums of weights and values over n keys add 2 (n + 64) 2^-24 of the sum of p |v|.
   float32      nothing else.
   codes        (mma on float16) A score's sum of q c, cut off by 2^-22 of up to 16 sum |q| in each of d / 16 + 1 additions; queries kept to 2^-35 of the largest, 15 codes a product.
-               A weight p step is rounded to float16, half a step being 2^-11 of it, or 2^-25 of the unit that the row's largest weight lies at 2^-3 of or above: 2^-22 of that;
-               both count by codes up to 15.  Sums of weights times codes less the middles (128 at most, a byte at a time), cut off by 2^-22 in each addition of 16 keys.
+               A weight p step is rounded to float16, half a step being 2^-11 of it, or 2^-25 where that is more; the row's largest weight lies at 2^-6 or above, so that this is
+               2^-19 of the largest weight; both count by codes up to 15.  Sums of weights times codes less the middles (128 at most, a byte at a time), cut off by 2^-22 in each addition of 16 keys.
   restored     keys rounded to bfloat16, half a step being 2^-8 of a key (2^-8 of the score's terms), values likewise, weights likewise.
 The result's own rounding is apart."""
 import torch
@@ -42,7 +42,7 @@ def attention(q, cache, starts, q_lens, kv_lens, block_table, scale, window, pat
             Q = (rows.abs().sum(-1, keepdim=True) * st[:, None, None, :, 0] * scale).masked_fill(hidden, 0.0)
             ds = ds + Q * (16 * (d / 16 + 1) * 2.0 ** -22 + 15 * d * 2.0 ** -35)
             w = p * st[:, None, None, :, 2]
-            sizes = sizes + (15 * (2.0 ** -11 * w + torch.minimum(w, 2.0 ** -22 * w.amax(-1, keepdim=True))).sum(-1, keepdim=True)
+            sizes = sizes + (15 * (2.0 ** -11 * w + torch.minimum(w, 2.0 ** -19 * w.amax(-1, keepdim=True))).sum(-1, keepdim=True)
                              + (kv / 16 + 8) * 2.0 ** -22 * 128 * w.sum(-1, keepdim=True))
         if path == "restored":
             ds = ds + 2.0 ** -8 * S
