@@ -428,7 +428,7 @@ MSGL_API int msgl_kv4_append(const Kv4AppendArgs* x) {
 // at least min_q tokens see are packed into pages of KV4_RESTORED keys, request after request, and `table` names those pages as a block table does
 // (the tensor-core prefill kernel then fetches whole tiles of keys; a key's place in its page is that of its position).  Keys behind a request's
 // last one are zeros.  A value row that is no number, or reaches beyond them, becomes a key row that is none beside values of 0: it then shows through the scores of those who see it, where as a value it would
-// meet the weights of 0 that others have for it as well.  bfloat16 results are rounded once, as a bfloat16 cache would hold them.  8,192 keys of 8 heads (42 MB) 8.6 us, 4.9 TB/s.
+// meet the weights of 0 that others have for it as well.  bfloat16 results are rounded once, as a bfloat16 cache would hold them.  8,192 keys of 8 heads (42 MB) 8.8 us, 4.8 TB/s.
 constexpr int KV4_RESTORED = 128;
 
 struct Kv4Restore {

@@ -31,9 +31,9 @@
 // exponentials' reference moves only where a score lies KR_LAZY above it.
 //
 // What bounds it.  Where there is work for all SMs, the operations of a unit: 500 instructions a warp for 4.3 KB, 144 of them to take codes apart, on a pipe that takes half an instruction a
-// cycle; 64 requests of up to 16,000 keys (32 heads on 8, 794 MB) 141 us, 5.6 TB/s, 0.87 of copy.  With nine copies a lane for every unit whose sizes are looked at one by one it took 152, with
+// cycle; 64 requests of up to 16,000 keys (32 heads on 8, 794 MB) 142 us, 5.6 TB/s, 0.86 of copy.  With nine copies a lane for every unit whose sizes are looked at one by one it took 152, with
 // selects for hidden keys in the inner loop 3 us more.  12 warps at 160 registers and three units a ring 141, 16 at 128 and two 145, 14 164, 8 with four 179 (before the last steps).  Few keys:
-// latency; 1 request of 1,000 keys 10 us: 1.5 until the warps know their units, 1.4 for pages and queries, 2.5 for two units, 3 to add up and write.  16 requests of up to 4,096 keys 22 us
+// latency; 1 request of 1,000 keys 10.5 us: 1.5 until the warps know their units, 1.4 for pages and queries, 2.5 for two units, 3 to add up and write.  16 requests of up to 4,096 keys 22.6 us
 // (floor 8.4).
 // A block that handed units to its warps in turn, with a barrier and a merge a segment, took 195 us for the first case and 58 where this takes 32 (123 requests of up to 777 keys, 64 heads).  bfloat16 codes
 // 1 + c / 16 took 275 (two operations more a pair).  16 rows a segment, two products for every pair of codes, halve the codes' work but leave registers for 8 warps: 8 requests

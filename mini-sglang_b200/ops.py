@@ -2891,10 +2891,13 @@ def kv4_attention(q: torch.Tensor, out: torch.Tensor, cache: KV4Cache, *, kv_len
     A token at position p sees the keys 0 .. p, with a window the last `window` of them; one that sees none gets 0.  Rows of out behind the last request
     stay as they are, and so do all rows of a request without tokens.  A page number outside the cache reads as zeros.  Scores and
     sums are float32: what passes its range on the way (queries above 2^115, steps of keys above 2^117, values near 2^128) comes out as an infinity or NaN.
-    Values may differ in size as they like, whether they are seen, carry weight or neither, up to 2^100 times between a request's steps.
+    Values may differ in size as they like, whether they are seen, carry weight or neither, up to 2^100 times between a request's steps.  A row that stands for NaN shows in the
+    tokens that see it and in no other.
 
     Requests with few tokens read the codes themselves; for longer runs the keys and values that they see are first put back into q's type, once a call, in scratch
-    memory of up to KV4_RESTORE_BYTES (more only where one request needs it).  workspace: where scratch memory is kept between calls (`parts.Workspace`); calls that share one run one after the other.
+    memory of up to KV4_RESTORE_BYTES (more only where one request needs it).  Restored to bfloat16 they are rounded to it, as the prefill kernels' weights are: results are then some
+    3.7e-3 of their size off, and 1.8e-3 from the codes.  Between 80 and 512 rows (token, query head of a kv head) a request may come by either, as is estimated to be faster for
+    the step, so its last digits can change with the requests beside it.  workspace: where scratch memory is kept between calls (`parts.Workspace`); calls that share one run one after the other.
     fields_ahead: kv_len, block_table and q_start were written three launches or more before this one (as a step's fields are in a model's layers): they are read while the launch
     ahead of this one ends."""
     (k, v, steps), dt, dev = cache, q.dtype, q.get_device()
